@@ -13,9 +13,18 @@ the C ABI of ``include/imq.h`` (``aestrix_amd/libimq.so``):
 ``qmm_postscale`` / ``qmm_gate_add`` / ``qmm_swiglu`` fold the reference's
 post-qmm glue kernels into the MFMA kernel's epilogue; ``cast_prescale`` and
 ``apply_linear`` are the f16 sandwich around them (x / 16 to f16, qmm, x 16).
+``ln_mod``, ``rope`` and ``attention`` (``include/imq_core.h``) are the work of
+a block between its projections.
 """
 
 from ._lib import ImqError, ImqInvalid, ImqLibraryMissing, ImqUnsupported  # noqa: F401
+from .core import (  # noqa: F401
+    attention,
+    attention_plan,
+    ln_mod,
+    rope,
+    rope_frequencies,
+)
 from .ops import (  # noqa: F401
     BITS,
     GROUP_SIZE,

@@ -144,6 +144,13 @@ SIGNATURES = {
     "imq_cond_sinusoid": ([_p, _i, _i, _p], _i),
     "imq_cond_destroy": ([_p], _i),
     "imq_dit_step_destroy": ([_p], _i),
+    # imq_core.h
+    "imq_ln_mod": ([_p, _p, _i, _p, _p, _p, _i, _p, _i, _i, _i, ctypes.c_float, ctypes.c_float, _p],
+                   _i),
+    "imq_rope": ([_p, _p, _i, _i, _i, _i, _i, _p, _i, _p, _p, ctypes.c_float, ctypes.c_float, _i,
+                  _p], _i),
+    "imq_attention": ([_p, _p, _p], _i),
+    "imq_attention_plan": ([_p, _p, _p], _i),
 }
 
 

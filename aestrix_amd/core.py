@@ -1,0 +1,306 @@
+"""What stands between the quantized projections of a block (include/imq_core.h).
+
+* ``ln_mod``    -- LayerNorm with the block's modulation (``lnMod``,
+  ``Sources/ImarelloDirect/DirectDiTKernels.swift:16-59``);
+* ``rope``      -- per-head RMSNorm and rotary positions of queries and keys
+  (``DirectDiTKernels.swift:61-122``, ``DirectGlueKernels.swift:14-75``), and
+  ``rope_frequencies`` for the frequencies, scaled for long contexts or not;
+* ``attention`` -- softmax attention over padded batches, packed documents and
+  caches (``DirectDiTStep.swift:457-488``, ``DirectTEEncoder.swift:159-202``).
+
+Calls run on torch's current HIP stream; tensors may be strided views (columns
+of a projection's output, rows of a cache) whose last dimension is contiguous.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Sequence
+
+import torch
+
+from . import _lib
+from .ops import _DTYPES, _require, context, raw_stream, run_on
+
+_i32 = torch.int32
+
+
+def _device_of(x: torch.Tensor, what: str) -> int:
+    if not x.is_cuda:
+        raise ValueError(f"{what} must be on a HIP device")
+    return x.get_device()
+
+
+def _side(t: torch.Tensor | None, idx: int, dtype: torch.dtype, shape, what: str) -> int:
+    """Pointer of a contiguous side tensor (0 where it is not given)."""
+    if t is None:
+        return 0
+    if not (t.dtype == dtype and t.is_cuda and t.get_device() == idx and t.is_contiguous() and
+            tuple(t.shape) == tuple(shape)):
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on "
+                         f"the inputs' device")
+    return t.data_ptr()
+
+
+def ln_mod(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
+           sets: torch.Tensor | None = None, eps: float = 1e-6, post_scale: float = 1.0,
+           out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """T(((x - mean) * rsqrt(var + eps) * (1 + scale) + shift) * post_scale) over x's last dim.
+
+    x: contiguous float32 or T [..., cols]; shift, scale: float32 [cols] or [n, cols];
+    sets: int32, x's leading shape: the modulation each row takes (text and image rows of
+    a joint residual in one launch), row 0's where it is not given.  T: ``out_dtype``,
+    float16 or bfloat16 (default: x's own type, or float16 for float32)."""
+    idx = _device_of(x, "x")
+    _require(x.dim() >= 1 and x.is_contiguous(), "x must be contiguous [..., cols]")
+    lead, cols = x.shape[:-1], x.shape[-1]
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else \
+            torch.float16 if x.dtype == torch.float32 else x.dtype
+    n = 1 if shift.dim() == 1 else shift.shape[0]
+    shape = (cols,) if shift.dim() == 1 else (n, cols)
+    psh = _side(shift, idx, torch.float32, shape, "shift")
+    psc = _side(scale, idx, torch.float32, shape, "scale")
+    pse = _side(sets, idx, _i32, lead, "sets")
+    if out is None:
+        out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    _require(out.dtype == out_dtype and out.shape == x.shape and out.is_contiguous() and
+             out.is_cuda and out.get_device() == idx,
+             "out must be a contiguous tensor of out_dtype shaped like x")
+    rows = x.numel() // cols if cols else 0
+    ctx = context(idx)
+    _lib.check(run_on(idx, _lib.load().imq_ln_mod, ctx, x.data_ptr(), _DTYPES.get(x.dtype, -1),
+                      psh, psc, pse, n, out.data_ptr(), _DTYPES.get(out_dtype, -1), rows, cols,
+                      float(eps), float(post_scale), raw_stream(idx)), ctx)
+    return out
+
+
+def rope_frequencies(rot_dim: int, base: float = 1e6, *, scaling: str | None = None,
+                     factor: float = 1.0, original_len: int = 32768, beta_fast: float = 32.0,
+                     beta_slow: float = 1.0, device=None) -> tuple[torch.Tensor, float]:
+    """(inv_freq, amplitude) of ``rope``: float64 [rot_dim / 2] radians a position,
+    base^(-2 j / rot_dim), and the factor on cos and sin (1 without YaRN).
+
+    ``scaling`` for contexts ``factor`` times ``original_len``:
+
+    * ``"linear"``: every frequency divided by factor (position interpolation);
+    * ``"ntk"``: base * factor^(rot_dim / (rot_dim - 2)), which divides the slowest
+      frequency by factor and keeps the fastest;
+    * ``"yarn"``: pairs that turn more than beta_fast times over original_len are kept,
+      those under beta_slow divided by factor, a linear ramp over the pair's index
+      between; amplitude 0.1 ln(factor) + 1 (Peng et al., YaRN, 2023)."""
+    _require(rot_dim >= 2 and rot_dim % 2 == 0, "rot_dim must be even and positive")
+    _require(base > 1.0 and factor >= 1.0, "base must be above 1 and factor at least 1")
+    amplitude = 1.0
+    if scaling == "ntk":
+        _require(rot_dim > 2, "ntk scaling needs rot_dim above 2")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    j = torch.arange(rot_dim // 2, dtype=torch.float64)
+    f = base ** (-2.0 * j / rot_dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        _require(beta_fast > beta_slow > 0.0 and original_len > 0,
+                 "yarn needs beta_fast > beta_slow > 0 and a positive original_len")
+
+        def pair_of(turns: float) -> float:
+            return rot_dim * math.log(original_len / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+        lo = max(math.floor(pair_of(beta_fast)), 0)
+        hi = min(math.ceil(pair_of(beta_slow)), rot_dim // 2 - 1)
+        slow = ((j - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+        f = f * (1.0 - slow) + f / factor * slow
+        amplitude = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"scaling {scaling!r}: None, 'linear', 'ntk' or 'yarn'")
+    return (f if device is None else f.to(device)), amplitude
+
+
+class RopeHeads(ctypes.Structure):
+    """imq_rope_heads."""
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("heads", ctypes.c_int),
+                ("x_row", ctypes.c_int64), ("x_head", ctypes.c_int64),
+                ("y_row", ctypes.c_int64), ("y_head", ctypes.c_int64), ("weight", ctypes.c_void_p)]
+
+
+def _rope_group(x, out, weight, rows, dim, dtype, idx, what):
+    if not (x.dim() == 3 and x.shape[0] == rows and x.shape[2] == dim and x.dtype == dtype and
+            x.is_cuda and x.get_device() == idx):
+        raise ValueError(f"{what} must be a {dtype} [{rows}, heads, {dim}] tensor on one device "
+                         "with the others")
+    if out is None:
+        out = torch.empty(x.shape, dtype=dtype, device=x.device)
+    elif not (out.shape == x.shape and out.dtype == dtype and out.is_cuda and
+              out.get_device() == idx):
+        raise ValueError(f"{what}_out must be a {dtype} tensor shaped like {what}")
+    if x.numel() and not (x.stride(2) == 1 and out.stride(2) == 1):
+        raise ValueError(f"{what} and {what}_out must be contiguous in the head dim")
+    w = _side(weight, idx, torch.float32, (dim,), f"{what}_weight")
+    return out, RopeHeads(x.data_ptr(), out.data_ptr(), x.shape[1], x.stride(0), x.stride(1),
+                          out.stride(0), out.stride(1), w)
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Tensor,
+         inv_freq: torch.Tensor, sections: Sequence[int] | None = None, interleaved: bool = False,
+         amplitude: float = 1.0, q_weight: torch.Tensor | None = None,
+         k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+         q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Per-head RMSNorm (where a weight is given) and rotary positions, one launch.
+
+    q [rows, heads, dim] and k [rows, kv_heads, dim], strided views allowed; the first
+    2 * len(inv_freq) elements of a head are turned (``rot_dim``), the rest only normed.
+    positions: int32 [rows] or [rows, axes]; inv_freq: float64 [rot_dim / 2] on the
+    device (``rope_frequencies``); sections: pairs an axis, where there are more than one.
+    interleaved False pairs j with j + rot_dim / 2, True 2j with 2j + 1.  q_out / k_out:
+    where the results go (``q_out=q`` in place, ``k_out`` the rows of a cache), else new
+    contiguous tensors.  Returns q's result, or (q's, k's) where k is given."""
+    idx = _device_of(q, "q")
+    _require(q.dim() == 3, "q must be [rows, heads, dim]")
+    rows, dim = q.shape[0], q.shape[2]
+    dtype = q.dtype
+    if not (inv_freq.dtype == torch.float64 and inv_freq.dim() == 1):
+        raise ValueError("inv_freq must be a float64 [rot_dim / 2] tensor")
+    half = inv_freq.shape[0]
+    pf = _side(inv_freq, idx, torch.float64, (half,), "inv_freq")
+    axes = 1 if positions.dim() == 1 else positions.shape[1] if positions.dim() == 2 else 0
+    pp = _side(positions, idx, _i32, (rows,) if positions.dim() == 1 else (rows, axes), "positions")
+    if sections is not None:
+        _require(len(sections) == axes, f"{len(sections)} sections for {axes} axes of positions")
+        sec = (ctypes.c_int * axes)(*sections)
+    else:
+        sec = None
+    groups = (RopeHeads * 2)()
+    q_out, groups[0] = _rope_group(q, q_out, q_weight, rows, dim, dtype, idx, "q")
+    n = 1
+    if k is not None:
+        k_out, groups[1] = _rope_group(k, k_out, k_weight, rows, dim, dtype, idx, "k")
+        n = 2
+    else:
+        _require(k_out is None and k_weight is None, "k_out and k_weight need k")
+    ctx = context(idx)
+    _lib.check(run_on(idx, _lib.load().imq_rope, ctx, groups, n, rows, dim, 2 * half,
+                      int(bool(interleaved)), pp, axes, sec, pf, float(amplitude), float(eps),
+                      _DTYPES.get(dtype, -1), raw_stream(idx)), ctx)
+    return q_out if k is None else (q_out, k_out)
+
+
+class AttentionArgs(ctypes.Structure):
+    """imq_attention_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out")] +
+                [(f"{t}_{d}", ctypes.c_int64) for t in ("q", "k", "v", "out")
+                 for d in ("seq", "row", "head")] +
+                [(n, ctypes.c_int) for n in ("n_seq", "heads", "kv_heads", "dim", "max_q", "max_k",
+                                             "q_rows", "k_rows")] +
+                [(n, ctypes.c_void_p) for n in ("q_offsets", "k_offsets", "q_lens", "k_lens",
+                                                "prefix_lens", "slopes")] +
+                [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("causal", ctypes.c_int),
+                 ("dtype", ctypes.c_int)])
+
+
+class AttentionPlanInfo(ctypes.Structure):
+    """imq_attention_plan_info."""
+    _fields_ = [("kernel", ctypes.c_int), ("tile_rows", ctypes.c_int), ("splits", ctypes.c_int),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+ATTENTION_KERNELS = {0: "rows", 1: "tiles", 2: "few"}
+
+
+def _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens, prefix_lens,
+                    q_offsets, k_offsets, max_q, max_k, out):
+    idx = _device_of(q, "q")
+    dtype = q.dtype
+    nd = q.dim()
+    if not (nd == k.dim() == v.dim() and nd in (3, 4)):
+        raise ValueError("q, k and v must be all [rows, heads, dim] or all [seqs, rows, heads, dim]")
+    if not (k.dtype == v.dtype == dtype and k.is_cuda and v.is_cuda and
+            k.get_device() == v.get_device() == idx):
+        raise ValueError("q, k and v must share a dtype and a device")
+    qs, ks = q.shape, k.shape
+    heads, dim, kv = qs[-2], qs[-1], ks[-2]
+    if not (ks == v.shape and ks[-1] == dim):
+        raise ValueError(f"k and v must be [..., kv_heads, {dim}] of one shape, "
+                         f"got {tuple(ks)} and {tuple(v.shape)}")
+    packed = q_offsets is not None
+    if packed or k_offsets is not None:
+        if nd != 3 or q_offsets is None or k_offsets is None:
+            raise ValueError("packed documents are [rows, heads, dim] with q_offsets and k_offsets")
+        if max_q is None or max_k is None:
+            raise ValueError("packed documents need max_q and max_k, the longest document's rows")
+        if q_lens is not None or k_lens is not None:
+            raise ValueError("offsets and lengths exclude each other")
+        n = q_offsets.shape[0] - 1 if q_offsets.dim() == 1 else -1
+        if n < 0:
+            raise ValueError("q_offsets must be int32 [n + 1]")
+    else:
+        if max_q is not None or max_k is not None:
+            raise ValueError("max_q and max_k are for packed documents")
+        n = qs[0] if nd == 4 else 1
+        if nd == 4 and ks[0] != n:
+            raise ValueError(f"q has {n} sequences, k and v {ks[0]}")
+        max_q, max_k = qs[-3], ks[-3]
+    if out is None:
+        out = torch.empty(qs, dtype=dtype, device=q.device)
+    elif not (out.shape == qs and out.dtype == dtype and out.is_cuda and out.get_device() == idx):
+        raise ValueError("out must be shaped like q, of its dtype and device")
+    if q.numel() and not (q.stride(-1) == 1 and out.stride(-1) == 1) or \
+            k.numel() and not (k.stride(-1) == 1 and v.stride(-1) == 1):
+        raise ValueError("q, k, v and out must be contiguous in the head dim")
+    if scale is None:
+        scale = dim ** -0.5 if dim else 1.0
+    s = [0, 0, 0, 0] if nd == 3 else [q.stride(0), k.stride(0), v.stride(0), out.stride(0)]
+    return idx, out, AttentionArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+        s[0], q.stride(-3), q.stride(-2), s[1], k.stride(-3), k.stride(-2),
+        s[2], v.stride(-3), v.stride(-2), s[3], out.stride(-3), out.stride(-2),
+        n, heads, kv, dim, max_q, max_k, qs[-3], ks[-3],
+        _side(q_offsets, idx, _i32, (n + 1,), "q_offsets"),
+        _side(k_offsets, idx, _i32, (n + 1,), "k_offsets"),
+        _side(q_lens, idx, _i32, (n,), "q_lens"), _side(k_lens, idx, _i32, (n,), "k_lens"),
+        _side(prefix_lens, idx, _i32, (n,), "prefix_lens"),
+        _side(slopes, idx, torch.float32, (heads,), "slopes"),
+        scale, softcap, 1 if causal else 0, _DTYPES.get(dtype, -1))
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None,
+              causal: bool = False, softcap: float = 0.0, slopes: torch.Tensor | None = None,
+              q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None,
+              prefix_lens: torch.Tensor | None = None, q_offsets: torch.Tensor | None = None,
+              k_offsets: torch.Tensor | None = None, max_q: int | None = None,
+              max_k: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scores) v with heads sharing key heads in whole groups, bf16 or f16.
+
+    Scores are scale * q . k (scale: 1 / sqrt(dim) by default), then capped to
+    softcap * tanh(score / softcap) where softcap > 0, then lowered by slopes[head] times
+    the distance.  The last query stands at the last key; ``causal`` hides later keys but
+    for the first prefix_lens[s] of a sequence.  A query that sees nothing gives zeros.
+
+    * one sequence: q [rows, heads, dim], k and v [keys, kv_heads, dim];
+    * a batch, or a cache: q [n, rows, heads, dim], k and v [n, keys, kv_heads, dim], of
+      which sequence s uses the first q_lens[s] rows and k_lens[s] keys (int32 [n]);
+    * packed documents: q, k, v [rows, ...], document s in rows q_offsets[s] to
+      q_offsets[s + 1] (int32 [n + 1]), max_q and max_k the longest one's rows.
+
+    Views with a contiguous last dim are taken as they are.  Rows of ``out`` that are no
+    query's are left as they were (in a new tensor: undefined)."""
+    idx, out, args = _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens,
+                                     prefix_lens, q_offsets, k_offsets, max_q, max_k, out)
+    ctx = context(idx)
+    _lib.check(run_on(idx, _lib.load().imq_attention, ctx, ctypes.byref(args), raw_stream(idx)),
+               ctx)
+    return out
+
+
+def attention_plan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale=None, causal=False,
+                   softcap=0.0, slopes=None, q_lens=None, k_lens=None, prefix_lens=None,
+                   q_offsets=None, k_offsets=None, max_q=None, max_k=None, out=None) -> dict:
+    """The kernel ("rows", "tiles" or "few"), tile height and key splits that
+    ``attention`` with these arguments would run, without launching anything."""
+    idx, _, args = _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens,
+                                   prefix_lens, q_offsets, k_offsets, max_q, max_k, out)
+    ctx = context(idx)
+    info = AttentionPlanInfo()
+    _lib.check(_lib.load().imq_attention_plan(ctx, ctypes.byref(args), ctypes.byref(info)), ctx)
+    return {"kernel": ATTENTION_KERNELS[info.kernel], "tile_rows": info.tile_rows,
+            "splits": info.splits, "workspace_bytes": info.workspace_bytes}

@@ -118,6 +118,31 @@ int bind_device(imq_ctx* ctx) {
   return e == hipSuccess ? IMQ_OK : hip_fail(ctx, e, "hipSetDevice");
 }
 
+// The split-K workspace of stream st, at least `need` bytes; empty (run
+// unsplit) when it would have to grow during stream capture or the
+// allocation fails.  A workspace that is outgrown is retired, not freed: a
+// graph captured earlier on this stream still addresses it, and so may the
+// stream's queued work; retired buffers are freed with the context.
+SplitWs split_ws(imq_ctx* ctx, hipStream_t st, size_t need) {
+  if (need == 0) return {};
+  std::lock_guard<std::mutex> lk(ctx->ws_mu);
+  auto& e = ctx->split_ws[st];
+  if (e.second >= need) return {static_cast<float*>(e.first), e.second};
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) {
+    (void)hipGetLastError();
+    return {};
+  }
+  void* p = nullptr;
+  if (hipMalloc(&p, need) != hipSuccess) {
+    (void)hipGetLastError();
+    return {};
+  }
+  if (e.first) ctx->retired_ws.push_back(e.first);
+  e = {p, need};
+  return {static_cast<float*>(p), need};
+}
+
 }  // namespace detail
 }  // namespace imq
 
@@ -155,31 +180,6 @@ int check_qmm(imq_ctx* ctx, const char* fn, const uint32_t* w, const void* s, co
 // the split-K partial sums in the library's static scratch
 // (imq_qmm_t_noalloc); kGemv / kGemm: one kernel family alone.
 enum class Regime { kAuto, kAutoNoAlloc, kGemv, kGemm };
-
-// The split-K workspace of stream st, at least `need` bytes; empty (run
-// unsplit) when it would have to grow during stream capture or the
-// allocation fails.  A workspace that is outgrown is retired, not freed: a
-// graph captured earlier on this stream still addresses it, and so may the
-// stream's queued work; retired buffers are freed with the context.
-imq::SplitWs split_ws(imq_ctx* ctx, hipStream_t st, size_t need) {
-  if (need == 0) return {};
-  std::lock_guard<std::mutex> lk(ctx->ws_mu);
-  auto& e = ctx->split_ws[st];
-  if (e.second >= need) return {static_cast<float*>(e.first), e.second};
-  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(st, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) {
-    (void)hipGetLastError();
-    return {};
-  }
-  void* p = nullptr;
-  if (hipMalloc(&p, need) != hipSuccess) {
-    (void)hipGetLastError();
-    return {};
-  }
-  if (e.first) ctx->retired_ws.push_back(e.first);
-  e = {p, need};
-  return {static_cast<float*>(p), need};
-}
 
 // Orders an allocation-free call that uses the static scratch after the
 // previous such call on the same GPU, whatever stream or thread made it, so
@@ -355,6 +355,8 @@ int imq_create(int device, imq_ctx** out) {
   auto* c = new (std::nothrow) imq_ctx;
   if (!c) return fail(nullptr, IMQ_ENOMEM, "imq_create: out of host memory");
   c->device = device;
+  if (hipDeviceGetAttribute(&c->cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess)
+    c->cus = 256;
   c->static_scratch = scratch;
   *out = c;
   return IMQ_OK;

@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "imq.h"
+#include "imq_kernels.hpp"
 
 namespace imq {
 
@@ -46,6 +47,7 @@ struct imq_ctx {
   static constexpr size_t kStagingBytes = 32u << 20;
 
   int device = 0;
+  int cus = 0;  // compute units of the device, looked up at imq_create
   mutable std::mutex mu;
   std::string err;
   // Pinned bounce buffers of imq_upload (allocated on first use), each with
@@ -79,6 +81,8 @@ int hip_fail(imq_ctx* ctx, hipError_t e, const char* what);
 bool aligned(const void* p, size_t a);
 size_t elem_size(imq_dtype dtype);
 int bind_device(imq_ctx* ctx);
+// The split workspace of stream st, at least `need` bytes, or empty.
+SplitWs split_ws(imq_ctx* ctx, hipStream_t st, size_t need);
 
 }  // namespace detail
 }  // namespace imq
