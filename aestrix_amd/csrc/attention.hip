@@ -1,6 +1,9 @@
 // attention.hip -- softmax attention (include/imq_core.h): plans and launches.
 #include "attention.hpp"
+#include "attention_tiles.hpp"
 #include "imq_core.h"
+
+#include <algorithm>
 
 namespace imq {
 namespace {
@@ -32,26 +35,84 @@ hipError_t launch_rows(const AttnArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <int T, int D, int NW, bool kCap, bool kSlope>
+hipError_t launch_tiles(const AttnArgs& a, const AttnPlan& plan, float* ws, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
+  const int tiles = (int)((rows + NW * 32 - 1) / (NW * 32));
+  const int64_t blocks = (int64_t)a.n_seq * a.kv_heads * tiles;
+  if (plan.splits > 1) {
+    hipLaunchKernelGGL((attn_tiles_kernel<T, D, NW, kCap, kSlope, true>),
+                       dim3((unsigned)(blocks * plan.splits)), dim3(NW * 64), 0, stream, a, tiles,
+                       plan.splits, plan.chunk, ws);
+    const int64_t all = blocks * NW * 32;
+    hipLaunchKernelGGL((attn_join_kernel<T, D, kCap, kSlope>), dim3((unsigned)((all + 15) / 16)),
+                       dim3(256), 0, stream, a, NW * 32, tiles, plan.splits, ws);
+  } else {
+    hipLaunchKernelGGL((attn_tiles_kernel<T, D, NW, kCap, kSlope, false>), dim3((unsigned)blocks),
+                       dim3(NW * 64), 0, stream, a, tiles, 1, 0, nullptr);
+  }
+  return hipGetLastError();
+}
+
+template <int T, bool kCap, bool kSlope>
+hipError_t launch_scored(const AttnArgs& a, const AttnPlan& plan, float* ws, hipStream_t stream) {
+  if (plan.kernel == IMQ_ATTENTION_ROWS) return launch_rows<T, kCap, kSlope>(a, stream);
+  const bool wide = plan.tile_rows == 128;
+  if (a.dim > 64)
+    return wide ? launch_tiles<T, 128, 4, kCap, kSlope>(a, plan, ws, stream)
+                : launch_tiles<T, 128, 2, kCap, kSlope>(a, plan, ws, stream);
+  return wide ? launch_tiles<T, 64, 4, kCap, kSlope>(a, plan, ws, stream)
+              : launch_tiles<T, 64, 2, kCap, kSlope>(a, plan, ws, stream);
+}
+
 template <int T>
-hipError_t launch_t(const AttnArgs& a, hipStream_t stream) {
+hipError_t launch_t(const AttnArgs& a, const AttnPlan& plan, float* ws, hipStream_t stream) {
   const bool cap = a.softcap > 0.f, slope = a.slopes != nullptr;
-  if (cap && slope) return launch_rows<T, true, true>(a, stream);
-  if (cap) return launch_rows<T, true, false>(a, stream);
-  if (slope) return launch_rows<T, false, true>(a, stream);
-  return launch_rows<T, false, false>(a, stream);
+  if (cap && slope) return launch_scored<T, true, true>(a, plan, ws, stream);
+  if (cap) return launch_scored<T, true, false>(a, plan, ws, stream);
+  if (slope) return launch_scored<T, false, true>(a, plan, ws, stream);
+  return launch_scored<T, false, false>(a, plan, ws, stream);
+}
+
+// Whole 16-byte pieces everywhere, and a 64-row tile within 31-bit offsets.
+bool tiles_fit(const AttnArgs& a) {
+  const int64_t strides = a.q_seq | a.q_row | a.q_head | a.k_seq | a.k_row | a.k_head | a.v_seq |
+                          a.v_row | a.v_head | a.out_seq | a.out_row | a.out_head;
+  const uintptr_t ptrs = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out;
+  const int64_t far = (int64_t)1 << 24;  // elements of a row: 64 rows stay under 2^31 bytes
+  return a.dim % 8 == 0 && a.dim <= 128 && strides % 8 == 0 && ptrs % 16 == 0 && a.k_row <= far - 128 &&
+         a.v_row <= far - 128;
 }
 
 }  // namespace
 
-AttnPlan attention_plan(const AttnArgs&, int) {
-  return AttnPlan{IMQ_ATTENTION_ROWS, 1, 1, 0, 0};
+AttnPlan attention_plan(const AttnArgs& a, int cus) {
+  const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
+  const int64_t hs = (int64_t)a.n_seq * a.kv_heads;
+  if (!tiles_fit(a) || rows > (1 << 30) || a.max_k > (1 << 30) || hs > (1 << 20))
+    return AttnPlan{IMQ_ATTENTION_ROWS, 1, 1, 0, 0};
+  AttnPlan p{IMQ_ATTENTION_TILES, rows > 64 ? 128 : 64, 1, 0, 0};
+  const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  const int64_t blocks = hs * tiles;
+  if (blocks > ((int64_t)1 << 31) / 64) return AttnPlan{IMQ_ATTENTION_ROWS, 1, 1, 0, 0};
+  const int64_t key_tiles = (a.max_k + kAttnKeys - 1) / kAttnKeys;
+  const int64_t want = std::min<int64_t>((2 * cus + blocks - 1) / std::max<int64_t>(blocks, 1), key_tiles / 4);
+  if (want > 1) {
+    const int64_t per = (key_tiles + want - 1) / want;
+    p.chunk = (int)(per * kAttnKeys);
+    p.splits = (int)((key_tiles + per - 1) / per);
+    const int d = a.dim > 64 ? 128 : 64;
+    p.bytes = (size_t)p.splits * blocks * p.tile_rows * (d + 2) * 4;
+    if (p.splits == 1) p.chunk = 0, p.bytes = 0;
+  }
+  return p;
 }
 
-hipError_t launch_attention(const AttnArgs& a, const AttnPlan&, float*, int dtype,
+hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, float* ws, int dtype,
                             hipStream_t stream) {
   switch (dtype) {
-    case kBf16: return launch_t<kBf16>(a, stream);
-    case kF16: return launch_t<kF16>(a, stream);
+    case kBf16: return launch_t<kBf16>(a, plan, ws, stream);
+    case kF16: return launch_t<kF16>(a, plan, ws, stream);
     default: return hipErrorInvalidValue;
   }
 }

@@ -1,0 +1,394 @@
+// attention_tiles.hpp -- the matrix-core attention kernel and the kernel that
+// joins its key ranges.
+//
+// A workgroup of NW waves holds NW * 32 rows of one sequence and key head,
+// 32 a wave: row m is query m / G of head m % G of the G heads that share the
+// key head, so keys and values are staged once for the whole group, and a few
+// queries of many heads still fill a tile.  It walks the keys 64 at a time:
+//
+//   S^T [64 keys][32 rows] = K Q^T        2 * D/16 MFMAs of 32 x 32 x 16
+//   P^T = exp2(S^T - max)                 32 values a lane, one row a lane pair
+//   O^T [D][32 rows] += V^T P^T           4 * D/32 MFMAs
+//
+// The products are transposed so that a lane holds scores of one row only: the
+// row's maximum and sum are a lane's own (joined with the lane 32 away), and
+// the accumulator layout of S^T is, with the keys of a 16-key slice taken in
+// the order 8 (e / 4) + 4 h + e % 4, the operand layout of P^T: the weights
+// never leave their registers.  K and V tiles go straight from memory to LDS
+// (16 bytes a lane, no registers), one tile ahead of the one in use; V's
+// operand is read through the LDS transpose loads, 4 keys of 16 columns each.
+// 16-byte pieces of a row are swizzled (XOR with the row) at their source, so
+// the row-per-lane reads of K and the 4-row reads of V touch every bank evenly.
+#pragma once
+
+#include "attention.hpp"
+
+namespace imq {
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+constexpr int kAttnKeys = 64;  // keys of a tile
+
+template <int T>
+__device__ __forceinline__ f32x16_t attn_mfma(s16x8_t a, s16x8_t b, f32x16_t c) {
+  if constexpr (T == kBf16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// A lane's value and that of the lane 32 away, in the same order in both.
+// (The halves are taken as rvalues: bit-casting a vector's element in place
+// reads element 0.)
+__device__ __forceinline__ void lane_pair(float v, float& lo, float& hi) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned a = r[0], b = r[1];
+  lo = __builtin_bit_cast(float, a);
+  hi = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float pair_max(float v) {
+  float a, b;
+  lane_pair(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  float a, b;
+  lane_pair(v, a, b);
+  return a + b;
+}
+
+// Where in a row the 16-byte piece `piece` of row `row` lies in LDS.
+template <int D>
+__device__ __forceinline__ int k_piece(int row, int piece) {
+  return D == 128 ? piece ^ (row & 15) : piece ^ ((row >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int v_piece(int row, int piece) {
+  return D == 128 ? piece ^ (2 * (row & 7)) : piece ^ (2 * ((row >> 1) & 3));
+}
+
+template <int D>
+struct AttnStage {
+  uint4 k[kAttnKeys * D / 8];
+  uint4 v[kAttnKeys * D / 8];
+};
+
+// One tile of `rows` (up to 64) rows of K or V into LDS: NW waves, D / (8 NW)
+// loads each.  Pieces past the tensor's rows or the head's dim read as zero.
+template <int D, int NW>
+__device__ __forceinline__ void attn_load(const char* base, int64_t row_bytes, int rows, int dim,
+                                          const uint32_t (&off)[D / (8 * NW)], uint4* lds, int wave) {
+  const __amdgpu_buffer_rsrc_t rs =
+      make_rsrc(base, (uint32_t)((rows - 1) * row_bytes + dim * 2));
+#pragma unroll
+  for (int i = 0; i < D / (8 * NW); ++i) load_lds16(rs, off[i], 0, lds + (i * NW + wave) * 64);
+}
+
+template <int T, int D, int NW, bool kCap, bool kSlope, bool kSplit>
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(AttnArgs a, int tiles, int splits,
+                                                               int chunk, float* ws) {
+  using S = typename Elem<T>::S;
+  constexpr int kLoads = D / (8 * NW);
+  __shared__ AttnStage<D> st0, st1;
+  __shared__ float qs[NW][D];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hs_n = a.n_seq * a.kv_heads;
+  const int hs = blockIdx.x % hs_n, rest = blockIdx.x / hs_n;
+  const int split = kSplit ? rest % splits : 0;
+  // The last rows of a causal sequence have the most keys: they start first.
+  const int tile = tiles - 1 - (kSplit ? rest / splits : rest);
+  const int kh = hs % a.kv_heads;
+  AttnSeq s = attn_seq(a, hs / a.kv_heads);
+  const int group = a.heads / a.kv_heads;
+  const int rows = s.nq * group;  // checked on the host to fit
+  const int m0 = tile * NW * 32;
+  if (m0 >= rows) return;
+  // Rows past the last repeat it; they are not stored.
+  const int mw = m0 + wave * 32;
+  const int m = min(mw + c, rows - 1);
+  const int t = m / group, head = kh * group + m % group;
+  const int seen = attn_seen(a, s, t);
+  const int seen_wg = __builtin_amdgcn_readfirstlane(
+      attn_seen(a, s, min(m0 + NW * 32 - 1, rows - 1) / group));
+  const int seen_hi = mw >= rows ? 0 : __builtin_amdgcn_readfirstlane(
+      attn_seen(a, s, min(mw + 31, rows - 1) / group));
+  const int seen_lo = __builtin_amdgcn_readfirstlane(attn_seen(a, s, min(mw, rows - 1) / group));
+  const int begin = kSplit ? split * chunk : 0;
+  const int end = kSplit ? min(seen_wg, begin + chunk) : seen_wg;
+
+  // Sources of this thread's pieces in a tile.
+  const int64_t kb = a.k_row * 2, vb = a.v_row * 2;
+  uint32_t k_off[kLoads], v_off[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int at = (i * NW + wave) * 64 + lane, row = at / (D / 8), piece = at % (D / 8);
+    const int kp = k_piece<D>(row, piece), vp = v_piece<D>(row, piece);
+    k_off[i] = kp * 8 < a.dim ? (uint32_t)(row * kb + kp * 16) : 0x80000000u;
+    v_off[i] = vp * 8 < a.dim ? (uint32_t)(row * vb + vp * 16) : 0x80000000u;
+  }
+  const char* kbase = reinterpret_cast<const char*>(static_cast<const S*>(a.k) + s.k_at + kh * a.k_head);
+  const char* vbase = reinterpret_cast<const char*>(static_cast<const S*>(a.v) + s.v_at + kh * a.v_head);
+  auto issue = [&](AttnStage<D>& st, int j0) {
+    const int n = min(kAttnKeys, s.nk - j0);
+    attn_load<D, NW>(kbase + j0 * kb, kb, n, a.dim, k_off, st.k, wave);
+    attn_load<D, NW>(vbase + j0 * vb, vb, n, a.dim, v_off, st.v, wave);
+  };
+  if (begin < end) issue(st0, begin);
+
+  // Q^T fragments: row m, elements 16 i + 8 h .. + 8.
+  s16x8_t qf[D / 16];
+  {
+    const S* q = static_cast<const S*>(a.q) + s.q_at + t * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const int d = 16 * i + 8 * h;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (d < a.dim) v = *reinterpret_cast<const uint4*>(q + d);
+      qf[i] = __builtin_bit_cast(s16x8_t, v);
+    }
+  }
+  const AttnScore<kCap, kSlope> score(a, head);
+  const int p = t + s.nk - s.nq;
+  // Read addresses in a stage: K row c of a 32-key half, V rows 4 h + (lane % 16) / 4.
+  const int kf = D == 128 ? (c & 15) : ((c >> 1) & 7);
+  const int vr = 4 * h + ((lane & 15) >> 2);
+  const int vf = D == 128 ? 2 * (vr & 7) : 2 * ((vr >> 1) & 3);
+  const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);  // 16-byte piece in 32 columns
+  const int vhalf = lane & 1;
+
+  f32x16_t o[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+  float top = -INFINITY, sum = 0.f;
+
+  auto step = [&](const AttnStage<D>& st, int j0) {
+    f32x16_t sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const s16x8_t kv = __builtin_bit_cast(
+            s16x8_t, st.k[(u * 32 + c) * (D / 8) + ((2 * i + h) ^ kf)]);
+        sc[u] = attn_mfma<T>(kv, qf[i], sc[u]);
+      }
+    }
+    // Scores to exponents where they are more than a multiple of the product.
+    if constexpr (kCap || kSlope) {
+      const float away = (float)(p - j0 - 4 * h);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sc[u][e] = score(sc[u][e], away - (float)(u * 32 + 8 * (e / 4) + e % 4));
+    }
+    if (j0 + kAttnKeys > seen_lo) {
+      const int lim = seen - j0 - 4 * h;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sc[u][e] = u * 32 + 8 * (e / 4) + e % 4 < lim ? sc[u][e] : -INFINITY;
+    }
+    float mx = sc[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
+    mx = pair_max(mx);
+    constexpr bool kRaw = !kCap && !kSlope;
+    if constexpr (kRaw) mx *= score.mul;
+    // The sums move to a new maximum only where a row's has grown by 2^8: until
+    // then weights are up to 2^8, which costs no precision in either type.
+    if (__builtin_amdgcn_ballot_w64(mx > top + 8.f)) {
+      const float next = fmaxf(top, mx);
+      const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
+      top = next;
+      sum *= keep;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] *= keep;
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+    s16x8_t pf[4];
+    float add = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float x0 = sc[u][half * 8 + e], x1 = sc[u][half * 8 + e + 1];
+          const float p0 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x0, score.mul, -base) : x0 - base);
+          const float p1 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x1, score.mul, -base) : x1 - base);
+          add += p0 + p1;
+          w[e / 2] = Elem<T>::pack2(p0, p1);
+        }
+        pf[u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+      }
+    sum += add;
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        s16x4_t part[2];
+#pragma unroll
+        for (int e4 = 0; e4 < 2; ++e4) {
+          const int at = ((16 * kc + 8 * e4 + vr) * (D / 8) + ((4 * i + vc) ^ vf)) * 2 + vhalf;
+          part[e4] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4_t*)(reinterpret_cast<const uint2*>(st.v) + at));
+        }
+        const s16x8_t vv = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        o[i] = attn_mfma<T>(vv, pf[kc], o[i]);
+      }
+  };
+
+  // A tile in use, the next in flight.  Every wave's loads of a stage have
+  // landed, and its reads of the other are done, once all have met.
+  auto meet = [&] {
+    __builtin_amdgcn_sched_barrier(0);
+    IMQ_WAIT_VM_LGKM_0();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int j0 = begin; j0 < end; j0 += 2 * kAttnKeys) {
+    meet();
+    if (j0 + kAttnKeys < end) issue(st1, j0 + kAttnKeys);
+    if (j0 < seen_hi) step(st0, j0);
+    if (j0 + kAttnKeys >= end) break;
+    meet();
+    if (j0 + 2 * kAttnKeys < end) issue(st0, j0 + 2 * kAttnKeys);
+    if (j0 + kAttnKeys < seen_hi) step(st1, j0 + kAttnKeys);
+  }
+
+  sum = pair_sum(sum);
+  if constexpr (kSplit) {
+    // [split][row of all tiles][D], then (top, sum) of each.
+    const int64_t all = (int64_t)hs_n * tiles * (NW * 32);
+    const int64_t row = ((int64_t)hs * tiles + tile) * (NW * 32) + wave * 32 + c;
+    if (mw + c < rows) {
+      float* po = ws + ((int64_t)split * all + row) * D;
+      if (begin < end)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(po + i * 32 + 2 * e + 4 * h) =
+                make_float4(o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]);
+      if (h == 0)
+        *reinterpret_cast<float2*>(ws + (int64_t)splits * all * D +
+                                   ((int64_t)split * all + row) * 2) = make_float2(top, sum);
+    }
+  } else {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        o[i][e] *= inv;
+        finite = finite && __builtin_fabsf(o[i][e]) < INFINITY;
+      }
+    if (mw + c < rows)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int d = i * 32 + 2 * e + 4 * h;
+          if (d < a.dim)
+            *reinterpret_cast<uint2*>(out + d) = make_uint2(Elem<T>::pack2(o[i][e], o[i][e + 1]),
+                                                            Elem<T>::pack2(o[i][e + 2], o[i][e + 3]));
+        }
+    // A tile multiplies what it hides by zero, which a NaN or an infinity
+    // outlives: such rows again, from the keys they see alone.
+    uint64_t again = __builtin_amdgcn_ballot_w64(!finite && mw + c < rows);
+    again = (again | again >> 32) & 0xFFFFFFFFu;
+    while (again) {
+      const int r = __builtin_ctzll(again);
+      again &= again - 1;
+      const int tr = (mw + r) / group;
+      attn_row<T, kCap, kSlope>(a, s, kh * group + (mw + r) % group, tr, attn_seen(a, s, tr), qs[wave]);
+    }
+  }
+}
+
+// Joins the key ranges of a split plan: 16 lanes a row, D / 16 columns each,
+// the ranges in order.
+template <int T, int D, bool kCap, bool kSlope>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_rows, int tiles,
+                                                        int splits, const float* ws) {
+  using S = typename Elem<T>::S;
+  __shared__ float qs[4][D];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t all = (int64_t)a.n_seq * a.kv_heads * tiles * tile_rows;
+  const int64_t row = (int64_t)blockIdx.x * 16 + wave * 4 + lane / 16;
+  const int group = a.heads / a.kv_heads;
+  bool live = row < all;
+  const int64_t hs = (live ? row : 0) / ((int64_t)tiles * tile_rows);
+  const int m = (int)((live ? row : 0) % ((int64_t)tiles * tile_rows));
+  const AttnSeq s = attn_seq(a, (int)(hs / a.kv_heads));
+  const int kh = (int)(hs % a.kv_heads);
+  live = live && m < s.nq * group;
+  const int t = m / group, head = kh * group + m % group;
+  bool finite = true;
+  if (live) {
+    const float* ml = ws + (int64_t)splits * all * D;
+    float top = -INFINITY;
+    for (int i = 0; i < splits; ++i) top = fmaxf(top, ml[((int64_t)i * all + row) * 2]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float acc[D / 16] = {}, sum = 0.f;
+    const int d0 = (lane & 15) * (D / 16);
+    for (int i = 0; i < splits; ++i) {
+      const float2 v = *reinterpret_cast<const float2*>(ml + ((int64_t)i * all + row) * 2);
+      if (v.y == 0.f) continue;  // a range without a key this row sees; its sums were not written
+      const float keep = __builtin_amdgcn_exp2f(v.x - base);
+      sum = __builtin_fmaf(v.y, keep, sum);
+      const float4* po = reinterpret_cast<const float4*>(ws + ((int64_t)i * all + row) * D + d0);
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) {
+        const float4 w = po[e];
+        acc[4 * e] = __builtin_fmaf(w.x, keep, acc[4 * e]);
+        acc[4 * e + 1] = __builtin_fmaf(w.y, keep, acc[4 * e + 1]);
+        acc[4 * e + 2] = __builtin_fmaf(w.z, keep, acc[4 * e + 2]);
+        acc[4 * e + 3] = __builtin_fmaf(w.w, keep, acc[4 * e + 3]);
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) {
+      acc[e] *= inv;
+      finite = finite && __builtin_fabsf(acc[e]) < INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < D / 16; e += 4)
+      if (d0 + e < a.dim)
+        *reinterpret_cast<uint2*>(out + d0 + e) =
+            make_uint2(Elem<T>::pack2(acc[e], acc[e + 1]), Elem<T>::pack2(acc[e + 2], acc[e + 3]));
+  }
+  uint64_t again = __builtin_amdgcn_ballot_w64(!finite);
+  while (again) {
+    const int l = __builtin_ctzll(again) & ~15;
+    again &= ~(0xFFFFull << l);
+    // The row's place from the lanes that hold it.
+    const int mr = __builtin_amdgcn_readlane(m, l), hr = __builtin_amdgcn_readlane((int)hs, l);
+    const AttnSeq sr = attn_seq(a, hr / a.kv_heads);
+    const int tr = mr / group;
+    attn_row<T, kCap, kSlope>(a, sr, (hr % a.kv_heads) * group + mr % group, tr,
+                              attn_seen(a, sr, tr), qs[wave]);
+  }
+}
+
+}  // namespace imq
