@@ -95,12 +95,196 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
   }
 }
 
+// 8 consecutive elements: 16 bytes (two pieces of 16 in f32).
+template <int T>
+struct Piece8 {
+  uint4 v[T == kF32 ? 2 : 1];
+};
+
+template <int T>
+__device__ __forceinline__ Piece8<T> load8(const typename Elem<T>::S* p) {
+  Piece8<T> r;
+  const uint4* q = reinterpret_cast<const uint4*>(p);
+  r.v[0] = q[0];
+  if constexpr (T == kF32) r.v[1] = q[1];
+  return r;
+}
+
+template <int T>
+__device__ __forceinline__ void unpack8(const Piece8<T>& p, float f[8]) {
+  const uint32_t w[4] = {p.v[0].x, p.v[0].y, p.v[0].z, p.v[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T == kF32) {
+      const uint32_t w1[4] = {p.v[1].x, p.v[1].y, p.v[1].z, p.v[1].w};
+      f[i] = __uint_as_float(w[i]);
+      f[4 + i] = __uint_as_float(w1[i]);
+    } else {
+      f[2 * i] = Elem<T>::param((uint16_t)(w[i] & 0xFFFFu));
+      f[2 * i + 1] = Elem<T>::param((uint16_t)(w[i] >> 16));
+    }
+  }
+}
+
+template <int T>
+__device__ __forceinline__ void store8(typename Elem<T>::S* p, const float f[8]) {
+  uint4* q = reinterpret_cast<uint4*>(p);
+  if constexpr (T == kF32) {
+    q[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                      __float_as_uint(f[3]));
+    q[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
+                      __float_as_uint(f[7]));
+  } else {
+    q[0] = make_uint4(Elem<T>::pack2(f[0], f[1]), Elem<T>::pack2(f[2], f[3]),
+                      Elem<T>::pack2(f[4], f[5]), Elem<T>::pack2(f[6], f[7]));
+  }
+}
+
+constexpr int kMaxVecDim = 512;
+constexpr int kBatch = 3;  // head groups a wave holds at once: their loads are in flight together
+
+// The vector form: a lane holds 16 elements of a head (the two 8-element sides
+// of 8 pairs in the half layout, 16 consecutive ones interleaved or not
+// turned), 2^lanes_log2 lanes a head.  The angles of a row are computed once,
+// a pair per thread, and every lane keeps the cos and sin of its 8 pairs in
+// registers over all heads.  kRows rows a workgroup: 4, a wave each, where
+// there are many; 1, its heads over the four waves, where there are few.
+template <int T, bool kInterleaved, int kRows>
+__global__ __launch_bounds__(kThreads) void rope_vec_kernel(RopeArgs a, int lanes_log2) {
+  using S = typename Elem<T>::S;
+  __shared__ float2 cs[kRows][kMaxVecDim / 2];
+  const int half = a.rot / 2;
+  const int row0 = blockIdx.x * kRows;
+  for (int i = threadIdx.x; i < kRows * half; i += kThreads) {
+    const int r = i / half, j = i % half;
+    if (row0 + r < a.rows)
+      cs[r][j] = cos_sin(a.positions[(int64_t)(row0 + r) * a.axes + axis_of(a, j)], a.inv_freq[j],
+                         a.amplitude);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = row0 + (kRows == 4 ? wave : 0);
+  if (row >= a.rows) return;
+  const int unit = lane & ((1 << lanes_log2) - 1), sub = lane >> lanes_log2;
+  const int per = 64 >> lanes_log2;  // heads of a wave's group
+  const bool turned = 16 * unit < a.rot, used = 16 * unit < a.dim;
+  const int e0 = !kInterleaved && turned ? 8 * unit : 16 * unit;
+  const int e1 = !kInterleaved && turned ? 8 * unit + half : 16 * unit + 8;
+  float2 t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    t[i] = turned ? cs[kRows == 4 ? wave : 0][8 * unit + i] : make_float2(1.f, 0.f);
+#pragma unroll 1
+  for (int gi = 0; gi < a.groups; ++gi) {
+    const RopeGroup g = a.g[gi];
+    const S* x = static_cast<const S*>(g.x) + row * g.x_row;
+    S* y = static_cast<S*>(g.y) + row * g.y_row;
+    float w0[8], w1[8];
+    if (g.weight && used) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 u = *reinterpret_cast<const float4*>(g.weight + e0 + 4 * i);
+        const float4 v = *reinterpret_cast<const float4*>(g.weight + e1 + 4 * i);
+        w0[4 * i] = u.x, w0[4 * i + 1] = u.y, w0[4 * i + 2] = u.z, w0[4 * i + 3] = u.w;
+        w1[4 * i] = v.x, w1[4 * i + 1] = v.y, w1[4 * i + 2] = v.z, w1[4 * i + 3] = v.w;
+      }
+    }
+    const int step = kRows == 4 ? per : 4 * per;
+    for (int h0 = (kRows == 4 ? 0 : wave * per) + sub; h0 - sub < g.heads; h0 += kBatch * step) {
+      Piece8<T> p0[kBatch], p1[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int h = h0 + b * step;
+        if (used && h < g.heads) {
+          p0[b] = load8<T>(x + h * g.x_head + e0);
+          p1[b] = load8<T>(x + h * g.x_head + e1);
+        } else {
+          p0[b] = p1[b] = Piece8<T>{};
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int h = h0 + b * step;
+        if (h - sub >= g.heads) break;  // for the whole wave
+        float u[8], v[8];
+        unpack8<T>(p0[b], u);
+        unpack8<T>(p1[b], v);
+        if (g.weight) {
+          float acc = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            acc = __builtin_fmaf(u[i], u[i], acc);
+            acc = __builtin_fmaf(v[i], v[i], acc);
+          }
+          for (int off = (1 << lanes_log2) >> 1; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
+          const float inv = __frsqrt_rn(acc / (float)a.dim + a.eps);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            u[i] *= inv * w0[i];
+            v[i] *= inv * w1[i];
+          }
+        }
+        if (turned) {
+          if constexpr (kInterleaved) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              const float2 c0 = t[i / 2], c1 = t[4 + i / 2];
+              const float u0 = u[i], u1 = u[i + 1], v0 = v[i], v1 = v[i + 1];
+              u[i] = u0 * c0.x - u1 * c0.y;
+              u[i + 1] = u1 * c0.x + u0 * c0.y;
+              v[i] = v0 * c1.x - v1 * c1.y;
+              v[i + 1] = v1 * c1.x + v0 * c1.y;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float u0 = u[i], v0 = v[i];
+              u[i] = u0 * t[i].x - v0 * t[i].y;
+              v[i] = v0 * t[i].x + u0 * t[i].y;
+            }
+          }
+        }
+        if (used && h < g.heads) {
+          store8<T>(y + h * g.y_head + e0, u);
+          store8<T>(y + h * g.y_head + e1, v);
+        }
+      }
+    }
+  }
+}
+
+bool vec_fits(const RopeArgs& a, int es) {
+  if (a.dim % 16 != 0 || a.rot % 16 != 0 || a.dim > kMaxVecDim) return false;
+  for (int i = 0; i < a.groups; ++i) {
+    const RopeGroup& g = a.g[i];
+    if (((uintptr_t)g.x | (uintptr_t)g.y | (uintptr_t)g.weight) % 16 != 0) return false;
+    if ((g.x_row | g.x_head | g.y_row | g.y_head) * es % 16 != 0) return false;
+  }
+  return true;
+}
+
 template <int T>
 hipError_t launch_t(const RopeArgs& a, bool interleaved, hipStream_t stream) {
   const int64_t heads = (int64_t)a.g[0].heads + (a.groups > 1 ? a.g[1].heads : 0);
   const int64_t blocks = (a.rows * heads + kThreads / 64 - 1) / (kThreads / 64);
   if (blocks == 0) return hipSuccess;
-  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20))), block(kThreads);
+  const dim3 block(kThreads);
+  if (vec_fits(a, Elem<T>::kBytes)) {
+    int log2 = 0;
+    while ((16 << log2) < a.dim) ++log2;
+    const bool many = a.rows >= 1024;
+    const dim3 grid((unsigned)(many ? (a.rows + 3) / 4 : a.rows));
+    if (interleaved && many)
+      hipLaunchKernelGGL((rope_vec_kernel<T, true, 4>), grid, block, 0, stream, a, log2);
+    else if (interleaved)
+      hipLaunchKernelGGL((rope_vec_kernel<T, true, 1>), grid, block, 0, stream, a, log2);
+    else if (many)
+      hipLaunchKernelGGL((rope_vec_kernel<T, false, 4>), grid, block, 0, stream, a, log2);
+    else
+      hipLaunchKernelGGL((rope_vec_kernel<T, false, 1>), grid, block, 0, stream, a, log2);
+    return hipGetLastError();
+  }
+  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)));
   if (interleaved)
     hipLaunchKernelGGL((rope_kernel<T, true>), grid, block, 0, stream, a);
   else
