@@ -16,14 +16,19 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Sequence
 
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _require, context, raw_stream, run_on
+from .ops import _DTYPES, _require, context, new_out, raw_stream, run_on
 
 _i32 = torch.int32
+
+# Calls of one row cost mostly what happens here: shapes and strides are read
+# once, a C struct is packed as bytes (a ctypes.Structure of as many fields
+# takes three times as long), messages are only formatted when a check fails.
 
 
 def _device_of(x: torch.Tensor, what: str) -> int:
@@ -32,15 +37,23 @@ def _device_of(x: torch.Tensor, what: str) -> int:
     return x.get_device()
 
 
-def _side(t: torch.Tensor | None, idx: int, dtype: torch.dtype, shape, what: str) -> int:
+def _side(t: torch.Tensor | None, idx: int, dtype: torch.dtype, shape: tuple, what: str) -> int:
     """Pointer of a contiguous side tensor (0 where it is not given)."""
     if t is None:
         return 0
-    if not (t.dtype == dtype and t.is_cuda and t.get_device() == idx and t.is_contiguous() and
-            tuple(t.shape) == tuple(shape)):
+    if not (t.dtype == dtype and t.is_cuda and t.get_device() == idx and t.shape == shape and
+            t.is_contiguous()):
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on "
                          f"the inputs' device")
     return t.data_ptr()
+
+
+def _packed(fields: struct.Struct, *values) -> bytes:
+    """values as a C struct."""
+    try:
+        return fields.pack(*values)
+    except (struct.error, OverflowError) as e:  # a size past 32 bits, a float past float32
+        raise ValueError(f"an argument does not fit its C type: {e}") from None
 
 
 def ln_mod(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
@@ -53,26 +66,29 @@ def ln_mod(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
     a joint residual in one launch), row 0's where it is not given.  T: ``out_dtype``,
     float16 or bfloat16 (default: x's own type, or float16 for float32)."""
     idx = _device_of(x, "x")
-    _require(x.dim() >= 1 and x.is_contiguous(), "x must be contiguous [..., cols]")
-    lead, cols = x.shape[:-1], x.shape[-1]
+    shape = x.shape
+    if not (len(shape) >= 1 and x.is_contiguous()):
+        raise ValueError("x must be contiguous [..., cols]")
+    cols = shape[-1]
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else \
             torch.float16 if x.dtype == torch.float32 else x.dtype
     n = 1 if shift.dim() == 1 else shift.shape[0]
-    shape = (cols,) if shift.dim() == 1 else (n, cols)
-    psh = _side(shift, idx, torch.float32, shape, "shift")
-    psc = _side(scale, idx, torch.float32, shape, "scale")
-    pse = _side(sets, idx, _i32, lead, "sets")
+    side = (cols,) if shift.dim() == 1 else (n, cols)
+    psh = _side(shift, idx, torch.float32, side, "shift")
+    psc = _side(scale, idx, torch.float32, side, "scale")
+    pse = _side(sets, idx, _i32, shape[:-1], "sets")
     if out is None:
-        out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    _require(out.dtype == out_dtype and out.shape == x.shape and out.is_contiguous() and
-             out.is_cuda and out.get_device() == idx,
-             "out must be a contiguous tensor of out_dtype shaped like x")
-    rows = x.numel() // cols if cols else 0
+        out = torch.empty(shape, dtype=out_dtype, device=x.device)
+    elif not (out.dtype == out_dtype and out.shape == shape and out.is_contiguous() and
+              out.is_cuda and out.get_device() == idx):
+        raise ValueError("out must be a contiguous tensor of out_dtype shaped like x")
     ctx = context(idx)
-    _lib.check(run_on(idx, _lib.load().imq_ln_mod, ctx, x.data_ptr(), _DTYPES.get(x.dtype, -1),
-                      psh, psc, pse, n, out.data_ptr(), _DTYPES.get(out_dtype, -1), rows, cols,
-                      float(eps), float(post_scale), raw_stream(idx)), ctx)
+    rc = run_on(idx, _lib.load().imq_ln_mod, ctx, x.data_ptr(), _DTYPES.get(x.dtype, -1), psh, psc,
+                pse, n, out.data_ptr(), _DTYPES.get(out_dtype, -1), x.numel() // cols if cols else 0,
+                cols, eps, post_scale, raw_stream(idx))
+    if rc:
+        _lib.check(rc, ctx)
     return out
 
 
@@ -117,28 +133,28 @@ def rope_frequencies(rot_dim: int, base: float = 1e6, *, scaling: str | None = N
     return (f if device is None else f.to(device)), amplitude
 
 
-class RopeHeads(ctypes.Structure):
-    """imq_rope_heads."""
-    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("heads", ctypes.c_int),
-                ("x_row", ctypes.c_int64), ("x_head", ctypes.c_int64),
-                ("y_row", ctypes.c_int64), ("y_head", ctypes.c_int64), ("weight", ctypes.c_void_p)]
+# imq_rope_heads: x, y, heads, strides, weight.
+_ROPE_HEADS = struct.Struct("@PPi4x4qP")
 
 
 def _rope_group(x, out, weight, rows, dim, dtype, idx, what):
-    if not (x.dim() == 3 and x.shape[0] == rows and x.shape[2] == dim and x.dtype == dtype and
+    """(out, the packed imq_rope_heads) of one group of heads."""
+    shape = x.shape
+    if not (len(shape) == 3 and shape[0] == rows and shape[2] == dim and x.dtype == dtype and
             x.is_cuda and x.get_device() == idx):
         raise ValueError(f"{what} must be a {dtype} [{rows}, heads, {dim}] tensor on one device "
                          "with the others")
     if out is None:
-        out = torch.empty(x.shape, dtype=dtype, device=x.device)
-    elif not (out.shape == x.shape and out.dtype == dtype and out.is_cuda and
+        out = new_out(x, shape)
+    elif not (out.shape == shape and out.dtype == dtype and out.is_cuda and
               out.get_device() == idx):
         raise ValueError(f"{what}_out must be a {dtype} tensor shaped like {what}")
-    if x.numel() and not (x.stride(2) == 1 and out.stride(2) == 1):
+    xr, xh, xd = x.stride()
+    yr, yh, yd = out.stride()
+    if not (xd == 1 and yd == 1) and x.numel():
         raise ValueError(f"{what} and {what}_out must be contiguous in the head dim")
     w = _side(weight, idx, torch.float32, (dim,), f"{what}_weight")
-    return out, RopeHeads(x.data_ptr(), out.data_ptr(), x.shape[1], x.stride(0), x.stride(1),
-                          out.stride(0), out.stride(1), w)
+    return out, _packed(_ROPE_HEADS, x.data_ptr(), out.data_ptr(), shape[1], xr, xh, yr, yh, w)
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Tensor,
@@ -156,8 +172,9 @@ def rope(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Ten
     where the results go (``q_out=q`` in place, ``k_out`` the rows of a cache), else new
     contiguous tensors.  Returns q's result, or (q's, k's) where k is given."""
     idx = _device_of(q, "q")
-    _require(q.dim() == 3, "q must be [rows, heads, dim]")
-    rows, dim = q.shape[0], q.shape[2]
+    if q.dim() != 3:
+        raise ValueError("q must be [rows, heads, dim]")
+    rows, _, dim = q.shape
     dtype = q.dtype
     if not (inv_freq.dtype == torch.float64 and inv_freq.dim() == 1):
         raise ValueError("inv_freq must be a float64 [rot_dim / 2] tensor")
@@ -165,37 +182,30 @@ def rope(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Ten
     pf = _side(inv_freq, idx, torch.float64, (half,), "inv_freq")
     axes = 1 if positions.dim() == 1 else positions.shape[1] if positions.dim() == 2 else 0
     pp = _side(positions, idx, _i32, (rows,) if positions.dim() == 1 else (rows, axes), "positions")
+    sec = None
     if sections is not None:
-        _require(len(sections) == axes, f"{len(sections)} sections for {axes} axes of positions")
-        sec = (ctypes.c_int * axes)(*sections)
-    else:
-        sec = None
-    groups = (RopeHeads * 2)()
-    q_out, groups[0] = _rope_group(q, q_out, q_weight, rows, dim, dtype, idx, "q")
+        if len(sections) != axes:
+            raise ValueError(f"{len(sections)} sections for {axes} axes of positions")
+        sec = _packed(struct.Struct(f"@{axes}i"), *sections)
+    q_out, groups = _rope_group(q, q_out, q_weight, rows, dim, dtype, idx, "q")
     n = 1
     if k is not None:
-        k_out, groups[1] = _rope_group(k, k_out, k_weight, rows, dim, dtype, idx, "k")
+        k_out, group = _rope_group(k, k_out, k_weight, rows, dim, dtype, idx, "k")
+        groups += group
         n = 2
-    else:
-        _require(k_out is None and k_weight is None, "k_out and k_weight need k")
+    elif k_out is not None or k_weight is not None:
+        raise ValueError("k_out and k_weight need k")
     ctx = context(idx)
-    _lib.check(run_on(idx, _lib.load().imq_rope, ctx, groups, n, rows, dim, 2 * half,
-                      int(bool(interleaved)), pp, axes, sec, pf, float(amplitude), float(eps),
-                      _DTYPES.get(dtype, -1), raw_stream(idx)), ctx)
+    rc = run_on(idx, _lib.load().imq_rope, ctx, groups, n, rows, dim, 2 * half,
+                1 if interleaved else 0, pp, axes, sec, pf, amplitude, eps, _DTYPES.get(dtype, -1),
+                raw_stream(idx))
+    if rc:
+        _lib.check(rc, ctx)
     return q_out if k is None else (q_out, k_out)
 
 
-class AttentionArgs(ctypes.Structure):
-    """imq_attention_args."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out")] +
-                [(f"{t}_{d}", ctypes.c_int64) for t in ("q", "k", "v", "out")
-                 for d in ("seq", "row", "head")] +
-                [(n, ctypes.c_int) for n in ("n_seq", "heads", "kv_heads", "dim", "max_q", "max_k",
-                                             "q_rows", "k_rows")] +
-                [(n, ctypes.c_void_p) for n in ("q_offsets", "k_offsets", "q_lens", "k_lens",
-                                                "prefix_lens", "slopes")] +
-                [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("causal", ctypes.c_int),
-                 ("dtype", ctypes.c_int)])
+# imq_attention_args: pointers, strides, sizes, side arrays, scale, softcap, causal, dtype.
+_ATTENTION_ARGS = struct.Struct("@4P12q8i6P2f2i")
 
 
 class AttentionPlanInfo(ctypes.Structure):
@@ -211,19 +221,19 @@ def _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens, pre
                     q_offsets, k_offsets, max_q, max_k, out):
     idx = _device_of(q, "q")
     dtype = q.dtype
-    nd = q.dim()
-    if not (nd == k.dim() == v.dim() and nd in (3, 4)):
-        raise ValueError("q, k and v must be all [rows, heads, dim] or all [seqs, rows, heads, dim]")
-    if not (k.dtype == v.dtype == dtype and k.is_cuda and v.is_cuda and
-            k.get_device() == v.get_device() == idx):
-        raise ValueError("q, k and v must share a dtype and a device")
     qs, ks = q.shape, k.shape
-    heads, dim, kv = qs[-2], qs[-1], ks[-2]
-    if not (ks == v.shape and ks[-1] == dim):
+    nd = len(qs)
+    if not (nd == len(ks) and (nd == 3 or nd == 4)):
+        raise ValueError("q, k and v must be all [rows, heads, dim] or all [seqs, rows, heads, dim]")
+    if not (k.dtype == dtype and v.dtype == dtype and k.is_cuda and v.is_cuda and
+            k.get_device() == idx and v.get_device() == idx):
+        raise ValueError("q, k and v must share a dtype and a device")
+    q_rows, heads, dim = qs[-3:]
+    k_rows, kv, kd = ks[-3:]
+    if not (ks == v.shape and kd == dim):
         raise ValueError(f"k and v must be [..., kv_heads, {dim}] of one shape, "
                          f"got {tuple(ks)} and {tuple(v.shape)}")
-    packed = q_offsets is not None
-    if packed or k_offsets is not None:
+    if q_offsets is not None or k_offsets is not None:
         if nd != 3 or q_offsets is None or k_offsets is None:
             raise ValueError("packed documents are [rows, heads, dim] with q_offsets and k_offsets")
         if max_q is None or max_k is None:
@@ -239,28 +249,28 @@ def _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens, pre
         n = qs[0] if nd == 4 else 1
         if nd == 4 and ks[0] != n:
             raise ValueError(f"q has {n} sequences, k and v {ks[0]}")
-        max_q, max_k = qs[-3], ks[-3]
+        max_q, max_k = q_rows, k_rows
     if out is None:
-        out = torch.empty(qs, dtype=dtype, device=q.device)
+        out = new_out(q, qs)
     elif not (out.shape == qs and out.dtype == dtype and out.is_cuda and out.get_device() == idx):
         raise ValueError("out must be shaped like q, of its dtype and device")
-    if q.numel() and not (q.stride(-1) == 1 and out.stride(-1) == 1) or \
-            k.numel() and not (k.stride(-1) == 1 and v.stride(-1) == 1):
+    if nd == 3:
+        sq, sk, sv, so = (0, *q.stride()), (0, *k.stride()), (0, *v.stride()), (0, *out.stride())
+    else:
+        sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
+    if not (sq[3] == 1 and sk[3] == 1 and sv[3] == 1 and so[3] == 1) and \
+            (q.numel() and not sq[3] == so[3] == 1 or k.numel() and not sk[3] == sv[3] == 1):
         raise ValueError("q, k, v and out must be contiguous in the head dim")
-    if scale is None:
-        scale = dim ** -0.5 if dim else 1.0
-    s = [0, 0, 0, 0] if nd == 3 else [q.stride(0), k.stride(0), v.stride(0), out.stride(0)]
-    return idx, out, AttentionArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-        s[0], q.stride(-3), q.stride(-2), s[1], k.stride(-3), k.stride(-2),
-        s[2], v.stride(-3), v.stride(-2), s[3], out.stride(-3), out.stride(-2),
-        n, heads, kv, dim, max_q, max_k, qs[-3], ks[-3],
+    return idx, out, _packed(
+        _ATTENTION_ARGS, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *sq[:3], *sk[:3], *sv[:3],
+        *so[:3], n, heads, kv, dim, max_q, max_k, q_rows, k_rows,
         _side(q_offsets, idx, _i32, (n + 1,), "q_offsets"),
         _side(k_offsets, idx, _i32, (n + 1,), "k_offsets"),
         _side(q_lens, idx, _i32, (n,), "q_lens"), _side(k_lens, idx, _i32, (n,), "k_lens"),
         _side(prefix_lens, idx, _i32, (n,), "prefix_lens"),
         _side(slopes, idx, torch.float32, (heads,), "slopes"),
-        scale, softcap, 1 if causal else 0, _DTYPES.get(dtype, -1))
+        scale if scale is not None else dim ** -0.5 if dim else 1.0, softcap, 1 if causal else 0,
+        _DTYPES.get(dtype, -1))
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None,
@@ -287,8 +297,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
     idx, out, args = _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens,
                                      prefix_lens, q_offsets, k_offsets, max_q, max_k, out)
     ctx = context(idx)
-    _lib.check(run_on(idx, _lib.load().imq_attention, ctx, ctypes.byref(args), raw_stream(idx)),
-               ctx)
+    rc = run_on(idx, _lib.load().imq_attention, ctx, args, raw_stream(idx))
+    if rc:
+        _lib.check(rc, ctx)
     return out
 
 
@@ -301,6 +312,6 @@ def attention_plan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale=N
                                    prefix_lens, q_offsets, k_offsets, max_q, max_k, out)
     ctx = context(idx)
     info = AttentionPlanInfo()
-    _lib.check(_lib.load().imq_attention_plan(ctx, ctypes.byref(args), ctypes.byref(info)), ctx)
+    _lib.check(_lib.load().imq_attention_plan(ctx, args, ctypes.byref(info)), ctx)
     return {"kernel": ATTENTION_KERNELS[info.kernel], "tile_rows": info.tile_rows,
             "splits": info.splits, "workspace_bytes": info.workspace_bytes}
