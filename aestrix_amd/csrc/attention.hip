@@ -1,5 +1,6 @@
 // attention.hip -- softmax attention (include/imq_core.h): plans and launches.
 #include "attention.hpp"
+#include "attention_few.hpp"
 #include "attention_tiles.hpp"
 #include "imq_core.h"
 
@@ -46,7 +47,7 @@ hipError_t launch_tiles(const AttnArgs& a, const AttnPlan& plan, float* ws, hipS
                        plan.splits, plan.chunk, ws);
     const int64_t all = blocks * NW * 32;
     hipLaunchKernelGGL((attn_join_kernel<T, D, kCap, kSlope>), dim3((unsigned)((all + 15) / 16)),
-                       dim3(256), 0, stream, a, NW * 32, tiles, plan.splits, ws);
+                       dim3(256), 0, stream, a, NW * 32, tiles, plan.splits, plan.chunk, ws);
   } else {
     hipLaunchKernelGGL((attn_tiles_kernel<T, D, NW, kCap, kSlope, false>), dim3((unsigned)blocks),
                        dim3(NW * 64), 0, stream, a, tiles, 1, 0, nullptr);
@@ -54,9 +55,29 @@ hipError_t launch_tiles(const AttnArgs& a, const AttnPlan& plan, float* ws, hipS
   return hipGetLastError();
 }
 
+template <int T, int D, bool kCap, bool kSlope>
+hipError_t launch_few(const AttnArgs& a, const AttnPlan& plan, float* ws, hipStream_t stream) {
+  const int rows = a.max_q * (a.heads / a.kv_heads);
+  const unsigned hs = (unsigned)(a.n_seq * a.kv_heads);
+  const dim3 block(kFewWaves * 64);
+  if (plan.splits > 1) {
+    hipLaunchKernelGGL((attn_few_kernel<T, D, kCap, kSlope, true>), dim3(hs * plan.splits), block, 0,
+                       stream, a, rows, plan.splits, plan.chunk, ws);
+    hipLaunchKernelGGL((attn_join_kernel<T, D, kCap, kSlope>), dim3((hs * rows + 15) / 16), dim3(256), 0,
+                       stream, a, rows, 1, plan.splits, plan.chunk, ws);
+  } else {
+    hipLaunchKernelGGL((attn_few_kernel<T, D, kCap, kSlope, false>), dim3(hs), block, 0, stream, a,
+                       rows, 1, 0, nullptr);
+  }
+  return hipGetLastError();
+}
+
 template <int T, bool kCap, bool kSlope>
 hipError_t launch_scored(const AttnArgs& a, const AttnPlan& plan, float* ws, hipStream_t stream) {
   if (plan.kernel == IMQ_ATTENTION_ROWS) return launch_rows<T, kCap, kSlope>(a, stream);
+  if (plan.kernel == IMQ_ATTENTION_FEW)
+    return a.dim > 64 ? launch_few<T, 128, kCap, kSlope>(a, plan, ws, stream)
+                      : launch_few<T, 64, kCap, kSlope>(a, plan, ws, stream);
   const bool wide = plan.tile_rows == 128;
   if (a.dim > 64)
     return wide ? launch_tiles<T, 128, 4, kCap, kSlope>(a, plan, ws, stream)
@@ -91,6 +112,20 @@ AttnPlan attention_plan(const AttnArgs& a, int cus) {
   const int64_t hs = (int64_t)a.n_seq * a.kv_heads;
   if (!tiles_fit(a) || rows > (1 << 30) || a.max_k > (1 << 30) || hs > (1 << 20))
     return AttnPlan{IMQ_ATTENTION_ROWS, 1, 1, 0, 0};
+  const int d = a.dim > 64 ? 128 : 64;
+  if (rows <= 32) {
+    AttnPlan p{IMQ_ATTENTION_FEW, (int)rows, 1, 0, 0};
+    constexpr int kRound = kFewWaves * kFewKeys;
+    const int64_t rounds = (a.max_k + kRound - 1) / kRound;  // tiles of each wave
+    const int64_t want = std::min<int64_t>((2 * cus + hs - 1) / hs, rounds);
+    if (want > 1) {
+      const int64_t per = (rounds + want - 1) / want;
+      p.chunk = (int)(per * kRound);
+      p.splits = (int)((rounds + per - 1) / per);
+      p.bytes = (size_t)p.splits * hs * rows * (d + 2) * 4;
+    }
+    return p;
+  }
   AttnPlan p{IMQ_ATTENTION_TILES, rows > 64 ? 128 : 64, 1, 0, 0};
   const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t blocks = hs * tiles;
@@ -101,7 +136,6 @@ AttnPlan attention_plan(const AttnArgs& a, int cus) {
     const int64_t per = (key_tiles + want - 1) / want;
     p.chunk = (int)(per * kAttnKeys);
     p.splits = (int)((key_tiles + per - 1) / per);
-    const int d = a.dim > 64 ? 128 : 64;
     p.bytes = (size_t)p.splits * blocks * p.tile_rows * (d + 2) * 4;
     if (p.splits == 1) p.chunk = 0, p.bytes = 0;
   }

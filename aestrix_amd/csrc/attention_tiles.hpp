@@ -72,6 +72,123 @@ __device__ __forceinline__ int v_piece(int row, int piece) {
   return D == 128 ? piece ^ (2 * (row & 7)) : piece ^ (2 * ((row >> 1) & 3));
 }
 
+// The scores of 32 U keys (S^T accumulators) to weights: capped, lowered and
+// masked, the running maximum and sum moved on, P^T fragments out.  j0: the
+// first key; seen: the keys this lane's row sees; seen_lo: the fewest that any
+// row of the wave sees; away0: p - j0 of the row.
+template <int T, int D, int U, bool kCap, bool kSlope>
+__device__ __forceinline__ void attn_softmax(const AttnScore<kCap, kSlope>& score, f32x16_t (&sc)[U],
+                                             f32x16_t (&o)[D / 32], float& top, float& sum,
+                                             s16x8_t (&pf)[2 * U], int j0, int h, int seen,
+                                             int seen_lo, int away0) {
+  if constexpr (kCap || kSlope) {
+    const float away = (float)(away0 - 4 * h);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        sc[u][e] = score(sc[u][e], away - (float)(u * 32 + 8 * (e / 4) + e % 4));
+  }
+  if (j0 + 32 * U > seen_lo) {
+    const int lim = seen - j0 - 4 * h;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        sc[u][e] = u * 32 + 8 * (e / 4) + e % 4 < lim ? sc[u][e] : -INFINITY;
+  }
+  float mx = sc[0][0];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
+  mx = pair_max(mx);
+  constexpr bool kRaw = !kCap && !kSlope;  // scores are products still: a positive factor is due
+  if constexpr (kRaw) mx *= score.mul;
+  // The sums move to a new maximum only where a row's has grown by 2^8: until
+  // then weights are up to 2^8, which costs no precision in either type.
+  if (__builtin_amdgcn_ballot_w64(mx > top + 8.f)) {
+    const float next = fmaxf(top, mx);
+    const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
+    top = next;
+    sum *= keep;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] *= keep;
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+  float add = 0.f;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float x0 = sc[u][half * 8 + e], x1 = sc[u][half * 8 + e + 1];
+        const float p0 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x0, score.mul, -base) : x0 - base);
+        const float p1 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x1, score.mul, -base) : x1 - base);
+        add += p0 + p1;
+        w[e / 2] = Elem<T>::pack2(p0, p1);
+      }
+      pf[u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+    }
+  sum += add;
+}
+
+// S^T of 32 keys: K rows from LDS (row c of the 32 at `lds`), Q^T from registers.
+template <int T, int D>
+__device__ __forceinline__ f32x16_t attn_qk(const uint4* lds, const s16x8_t (&qf)[D / 16], int c,
+                                            int h) {
+  const int kf = D == 128 ? (c & 15) : ((c >> 1) & 7);  // k_piece's
+  f32x16_t sc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+    sc = attn_mfma<T>(__builtin_bit_cast(s16x8_t, lds[c * (D / 8) + ((2 * i + h) ^ kf)]), qf[i], sc);
+  return sc;
+}
+
+// O^T += V^T P^T over 16 N keys: the rows at `lds` through the transpose loads.
+template <int T, int D, int N>
+__device__ __forceinline__ void attn_pv(const uint4* lds, const s16x8_t (&pf)[N],
+                                        f32x16_t (&o)[D / 32], int lane) {
+  const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2);           // of 8 rows
+  const int vf = D == 128 ? 2 * (vr & 7) : 2 * ((vr >> 1) & 3);  // v_piece's
+  const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);      // 16-byte piece of 32 columns
+#pragma unroll
+  for (int kc = 0; kc < N; ++kc)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      s16x4_t part[2];
+#pragma unroll
+      for (int e4 = 0; e4 < 2; ++e4) {
+        const int at = ((16 * kc + 8 * e4 + vr) * (D / 8) + ((4 * i + vc) ^ vf)) * 2 + (lane & 1);
+        part[e4] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4_t*)(reinterpret_cast<const uint2*>(lds) + at));
+      }
+      o[i] = attn_mfma<T>(__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7), pf[kc],
+                          o[i]);
+    }
+}
+
+// Q^T fragments of this lane's row: elements 16 i + 8 h to 16 i + 8 h + 8, zero past dim.
+template <int T, int D>
+__device__ __forceinline__ void attn_load_q(const AttnArgs& a, const AttnSeq& s, int t, int head,
+                                            int h, s16x8_t (&qf)[D / 16]) {
+  using S = typename Elem<T>::S;
+  const S* q = static_cast<const S*>(a.q) + s.q_at + t * a.q_row + head * a.q_head;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const int d = 16 * i + 8 * h;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (d < a.dim) v = *reinterpret_cast<const uint4*>(q + d);
+    qf[i] = __builtin_bit_cast(s16x8_t, v);
+  }
+}
+
 template <int D>
 struct AttnStage {
   uint4 k[kAttnKeys * D / 8];
@@ -121,6 +238,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   const int seen_lo = __builtin_amdgcn_readfirstlane(attn_seen(a, s, min(mw, rows - 1) / group));
   const int begin = kSplit ? split * chunk : 0;
   const int end = kSplit ? min(seen_wg, begin + chunk) : seen_wg;
+  if (kSplit && begin >= end) return;  // the join reads the ranges up to seen_wg only
 
   // Sources of this thread's pieces in a tile.
   const int64_t kb = a.k_row * 2, vb = a.v_row * 2;
@@ -141,27 +259,10 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   };
   if (begin < end) issue(st0, begin);
 
-  // Q^T fragments: row m, elements 16 i + 8 h .. + 8.
   s16x8_t qf[D / 16];
-  {
-    const S* q = static_cast<const S*>(a.q) + s.q_at + t * a.q_row + head * a.q_head;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const int d = 16 * i + 8 * h;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (d < a.dim) v = *reinterpret_cast<const uint4*>(q + d);
-      qf[i] = __builtin_bit_cast(s16x8_t, v);
-    }
-  }
+  attn_load_q<T, D>(a, s, t, head, h, qf);
   const AttnScore<kCap, kSlope> score(a, head);
   const int p = t + s.nk - s.nq;
-  // Read addresses in a stage: K row c of a 32-key half, V rows 4 h + (lane % 16) / 4.
-  const int kf = D == 128 ? (c & 15) : ((c >> 1) & 7);
-  const int vr = 4 * h + ((lane & 15) >> 2);
-  const int vf = D == 128 ? 2 * (vr & 7) : 2 * ((vr >> 1) & 3);
-  const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);  // 16-byte piece in 32 columns
-  const int vhalf = lane & 1;
-
   f32x16_t o[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
@@ -172,86 +273,10 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   auto step = [&](const AttnStage<D>& st, int j0) {
     f32x16_t sc[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const s16x8_t kv = __builtin_bit_cast(
-            s16x8_t, st.k[(u * 32 + c) * (D / 8) + ((2 * i + h) ^ kf)]);
-        sc[u] = attn_mfma<T>(kv, qf[i], sc[u]);
-      }
-    }
-    // Scores to exponents where they are more than a multiple of the product.
-    if constexpr (kCap || kSlope) {
-      const float away = (float)(p - j0 - 4 * h);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          sc[u][e] = score(sc[u][e], away - (float)(u * 32 + 8 * (e / 4) + e % 4));
-    }
-    if (j0 + kAttnKeys > seen_lo) {
-      const int lim = seen - j0 - 4 * h;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          sc[u][e] = u * 32 + 8 * (e / 4) + e % 4 < lim ? sc[u][e] : -INFINITY;
-    }
-    float mx = sc[0][0];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
-    mx = pair_max(mx);
-    constexpr bool kRaw = !kCap && !kSlope;
-    if constexpr (kRaw) mx *= score.mul;
-    // The sums move to a new maximum only where a row's has grown by 2^8: until
-    // then weights are up to 2^8, which costs no precision in either type.
-    if (__builtin_amdgcn_ballot_w64(mx > top + 8.f)) {
-      const float next = fmaxf(top, mx);
-      const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
-      top = next;
-      sum *= keep;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] *= keep;
-    }
-    const float base = top == -INFINITY ? 0.f : top;
+    for (int u = 0; u < 2; ++u) sc[u] = attn_qk<T, D>(st.k + u * 32 * (D / 8), qf, c, h);
     s16x8_t pf[4];
-    float add = 0.f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float x0 = sc[u][half * 8 + e], x1 = sc[u][half * 8 + e + 1];
-          const float p0 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x0, score.mul, -base) : x0 - base);
-          const float p1 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x1, score.mul, -base) : x1 - base);
-          add += p0 + p1;
-          w[e / 2] = Elem<T>::pack2(p0, p1);
-        }
-        pf[u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
-      }
-    sum += add;
-#pragma unroll
-    for (int kc = 0; kc < 4; ++kc)
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        s16x4_t part[2];
-#pragma unroll
-        for (int e4 = 0; e4 < 2; ++e4) {
-          const int at = ((16 * kc + 8 * e4 + vr) * (D / 8) + ((4 * i + vc) ^ vf)) * 2 + vhalf;
-          part[e4] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_s16x4_t*)(reinterpret_cast<const uint2*>(st.v) + at));
-        }
-        const s16x8_t vv = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        o[i] = attn_mfma<T>(vv, pf[kc], o[i]);
-      }
+    attn_softmax<T, D, 2, kCap, kSlope>(score, sc, o, top, sum, pf, j0, h, seen, seen_lo, p - j0);
+    attn_pv<T, D, 4>(st.v, pf, o, lane);
   };
 
   // A tile in use, the next in flight.  Every wave's loads of a stage have
@@ -279,13 +304,12 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
     const int64_t row = ((int64_t)hs * tiles + tile) * (NW * 32) + wave * 32 + c;
     if (mw + c < rows) {
       float* po = ws + ((int64_t)split * all + row) * D;
-      if (begin < end)
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4*>(po + i * 32 + 2 * e + 4 * h) =
-                make_float4(o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]);
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<float4*>(po + i * 32 + 2 * e + 4 * h) =
+              make_float4(o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]);
       if (h == 0)
         *reinterpret_cast<float2*>(ws + (int64_t)splits * all * D +
                                    ((int64_t)split * all + row) * 2) = make_float2(top, sum);
@@ -324,45 +348,67 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   }
 }
 
-// Joins the key ranges of a split plan: 16 lanes a row, D / 16 columns each,
-// the ranges in order.
+// Joins the key ranges of a split plan, in order: 16 lanes a row, D / 16 columns
+// each.  tile_rows rows a tile; a tile's ranges up to the last key that its
+// last row sees are written, the others not.
 template <int T, int D, bool kCap, bool kSlope>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_rows, int tiles,
-                                                        int splits, const float* ws) {
+                                                        int splits, int chunk, const float* ws) {
   using S = typename Elem<T>::S;
   __shared__ float qs[4][D];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t all = (int64_t)a.n_seq * a.kv_heads * tiles * tile_rows;
   const int64_t row = (int64_t)blockIdx.x * 16 + wave * 4 + lane / 16;
   const int group = a.heads / a.kv_heads;
+  const int64_t of_seq = (int64_t)tiles * tile_rows;
   bool live = row < all;
-  const int64_t hs = (live ? row : 0) / ((int64_t)tiles * tile_rows);
-  const int m = (int)((live ? row : 0) % ((int64_t)tiles * tile_rows));
-  const AttnSeq s = attn_seq(a, (int)(hs / a.kv_heads));
-  const int kh = (int)(hs % a.kv_heads);
-  live = live && m < s.nq * group;
+  const int hs = (int)((live ? row : 0) / of_seq);
+  const int m = (int)((live ? row : 0) % of_seq);
+  const AttnSeq s = attn_seq(a, hs / a.kv_heads);
+  const int kh = hs % a.kv_heads;
+  const int rows = s.nq * group;
+  live = live && m < rows;
   const int t = m / group, head = kh * group + m % group;
   bool finite = true;
   if (live) {
-    const float* ml = ws + (int64_t)splits * all * D;
-    float top = -INFINITY;
-    for (int i = 0; i < splits; ++i) top = fmaxf(top, ml[((int64_t)i * all + row) * 2]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float acc[D / 16] = {}, sum = 0.f;
+    const int last = min(m / tile_rows * tile_rows + tile_rows, rows) - 1;
+    const int used = (int)(((int64_t)attn_seen(a, s, last / group) + chunk - 1) / chunk);
+    const float2* ml = reinterpret_cast<const float2*>(ws + (int64_t)splits * all * D) + row;
     const int d0 = (lane & 15) * (D / 16);
-    for (int i = 0; i < splits; ++i) {
-      const float2 v = *reinterpret_cast<const float2*>(ml + ((int64_t)i * all + row) * 2);
-      if (v.y == 0.f) continue;  // a range without a key this row sees; its sums were not written
-      const float keep = __builtin_amdgcn_exp2f(v.x - base);
-      sum = __builtin_fmaf(v.y, keep, sum);
-      const float4* po = reinterpret_cast<const float4*>(ws + ((int64_t)i * all + row) * D + d0);
+    const float* po = ws + row * D + d0;
+    float acc[D / 16] = {}, top = -INFINITY, sum = 0.f;
+    // Four ranges at a time, their loads in flight together.
+    for (int i = 0; i < used; i += 4) {
+      float2 v[4];
+      float4 w[4][D / 64];
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) {
-        const float4 w = po[e];
-        acc[4 * e] = __builtin_fmaf(w.x, keep, acc[4 * e]);
-        acc[4 * e + 1] = __builtin_fmaf(w.y, keep, acc[4 * e + 1]);
-        acc[4 * e + 2] = __builtin_fmaf(w.z, keep, acc[4 * e + 2]);
-        acc[4 * e + 3] = __builtin_fmaf(w.w, keep, acc[4 * e + 3]);
+      for (int b = 0; b < 4; ++b) {
+        const int64_t at = (int64_t)min(i + b, used - 1) * all;
+        v[b] = ml[at];
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) w[b][e] = reinterpret_cast<const float4*>(po + at * D)[e];
+      }
+      float next = top;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) next = fmaxf(next, v[b].x);
+      const float base = next == -INFINITY ? 0.f : next;
+      const float old = __builtin_amdgcn_exp2f(top - base);
+      top = next;
+      sum *= old;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) acc[e] *= old;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (i + b >= used) break;
+        const float keep = __builtin_amdgcn_exp2f(v[b].x - base);
+        sum = __builtin_fmaf(v[b].y, keep, sum);
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) {
+          acc[4 * e] = __builtin_fmaf(w[b][e].x, keep, acc[4 * e]);
+          acc[4 * e + 1] = __builtin_fmaf(w[b][e].y, keep, acc[4 * e + 1]);
+          acc[4 * e + 2] = __builtin_fmaf(w[b][e].z, keep, acc[4 * e + 2]);
+          acc[4 * e + 3] = __builtin_fmaf(w[b][e].w, keep, acc[4 * e + 3]);
+        }
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -378,12 +424,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
         *reinterpret_cast<uint2*>(out + d0 + e) =
             make_uint2(Elem<T>::pack2(acc[e], acc[e + 1]), Elem<T>::pack2(acc[e + 2], acc[e + 3]));
   }
+  // Rows that are not finite again, from the keys they see alone (attn_tiles_kernel).
   uint64_t again = __builtin_amdgcn_ballot_w64(!finite);
   while (again) {
     const int l = __builtin_ctzll(again) & ~15;
     again &= ~(0xFFFFull << l);
-    // The row's place from the lanes that hold it.
-    const int mr = __builtin_amdgcn_readlane(m, l), hr = __builtin_amdgcn_readlane((int)hs, l);
+    const int mr = __builtin_amdgcn_readlane(m, l), hr = __builtin_amdgcn_readlane(hs, l);
     const AttnSeq sr = attn_seq(a, hr / a.kv_heads);
     const int tr = mr / group;
     attn_row<T, kCap, kSlope>(a, sr, (hr % a.kv_heads) * group + mr % group, tr,

@@ -197,6 +197,8 @@ __device__ __forceinline__ u32x4_t load_b128(__amdgpu_buffer_rsrc_t rs, uint32_t
 // s_waitcnt vmcnt(n) leaving expcnt and lgkmcnt unconstrained (gfx9 encoding).
 #define IMQ_WAIT_VMCNT(n) \
   __builtin_amdgcn_s_waitcnt(((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
+// s_waitcnt lgkmcnt(0): every LDS read of this wave has completed.
+#define IMQ_WAIT_LGKM_0() __builtin_amdgcn_s_waitcnt((15 | 3 << 14) | (7 << 4))
 // s_waitcnt vmcnt(0) lgkmcnt(0): every load of this wave, to registers or LDS,
 // and every LDS read has completed.
 #define IMQ_WAIT_VM_LGKM_0() __builtin_amdgcn_s_waitcnt(7 << 4)
