@@ -36,6 +36,18 @@ hipError_t launch_rows(const AttnArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// all: rows of all tiles.
+template <int T, int D, bool kCap, bool kSlope>
+void launch_join(const AttnArgs& a, const AttnPlan& plan, int tile_rows, int tiles, int64_t all,
+                 const float* ws, hipStream_t stream) {
+  if (plan.splits > 4)
+    hipLaunchKernelGGL((attn_join_kernel<T, D, 16, kCap, kSlope>), dim3((unsigned)all), dim3(256), 0,
+                       stream, a, tile_rows, tiles, plan.splits, plan.chunk, ws);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<T, D, 1, kCap, kSlope>), dim3((unsigned)((all + 15) / 16)),
+                       dim3(256), 0, stream, a, tile_rows, tiles, plan.splits, plan.chunk, ws);
+}
+
 template <int T, int D, int NW, bool kCap, bool kSlope>
 hipError_t launch_tiles(const AttnArgs& a, const AttnPlan& plan, float* ws, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
@@ -45,9 +57,7 @@ hipError_t launch_tiles(const AttnArgs& a, const AttnPlan& plan, float* ws, hipS
     hipLaunchKernelGGL((attn_tiles_kernel<T, D, NW, kCap, kSlope, true>),
                        dim3((unsigned)(blocks * plan.splits)), dim3(NW * 64), 0, stream, a, tiles,
                        plan.splits, plan.chunk, ws);
-    const int64_t all = blocks * NW * 32;
-    hipLaunchKernelGGL((attn_join_kernel<T, D, kCap, kSlope>), dim3((unsigned)((all + 15) / 16)),
-                       dim3(256), 0, stream, a, NW * 32, tiles, plan.splits, plan.chunk, ws);
+    launch_join<T, D, kCap, kSlope>(a, plan, NW * 32, tiles, blocks * NW * 32, ws, stream);
   } else {
     hipLaunchKernelGGL((attn_tiles_kernel<T, D, NW, kCap, kSlope, false>), dim3((unsigned)blocks),
                        dim3(NW * 64), 0, stream, a, tiles, 1, 0, nullptr);
@@ -63,8 +73,7 @@ hipError_t launch_few(const AttnArgs& a, const AttnPlan& plan, float* ws, hipStr
   if (plan.splits > 1) {
     hipLaunchKernelGGL((attn_few_kernel<T, D, kCap, kSlope, true>), dim3(hs * plan.splits), block, 0,
                        stream, a, rows, plan.splits, plan.chunk, ws);
-    hipLaunchKernelGGL((attn_join_kernel<T, D, kCap, kSlope>), dim3((hs * rows + 15) / 16), dim3(256), 0,
-                       stream, a, rows, 1, plan.splits, plan.chunk, ws);
+    launch_join<T, D, kCap, kSlope>(a, plan, rows, 1, (int64_t)hs * rows, ws, stream);
   } else {
     hipLaunchKernelGGL((attn_few_kernel<T, D, kCap, kSlope, false>), dim3(hs), block, 0, stream, a,
                        rows, 1, 0, nullptr);
@@ -117,7 +126,10 @@ AttnPlan attention_plan(const AttnArgs& a, int cus) {
     AttnPlan p{IMQ_ATTENTION_FEW, (int)rows, 1, 0, 0};
     constexpr int kRound = kFewWaves * kFewKeys;
     const int64_t rounds = (a.max_k + kRound - 1) / kRound;  // tiles of each wave
-    const int64_t want = std::min<int64_t>((2 * cus + hs - 1) / hs, rounds);
+    // One workgroup a CU: 131072 keys of 8 key heads 92.8 us (5.8 TB/s), two a
+    // CU 100.1, four 95.3; 8 x up to 2048 keys 9.1 / 10.0 / 11.8 (with the
+    // join's 5.2 / 5.7 / 7.7 and 4.0 / 4.3 / 4.0).
+    const int64_t want = std::min<int64_t>(cus / hs, rounds);
     if (want > 1) {
       const int64_t per = (rounds + want - 1) / want;
       p.chunk = (int)(per * kRound);

@@ -104,7 +104,8 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
     if constexpr (kMore) load(kbase, kb, k_off, kl, j0 + kStep);
     __builtin_amdgcn_sched_barrier(0);
     s16x8_t pf[2];
-    attn_softmax<T, D, 1, kCap, kSlope>(score, sc, o, top, sum, pf, j0, h, seen, seen_lo, p - j0);
+    attn_top<D>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0), o, top, sum);
+    attn_weights<T, 1, kCap, kSlope>(score, sc, top, sum, pf);
     __builtin_amdgcn_sched_barrier(0);
     IMQ_WAIT_VMCNT(kMore ? kLoads : 0);  // V has landed (the next K is in flight)
     __builtin_amdgcn_sched_barrier(0);

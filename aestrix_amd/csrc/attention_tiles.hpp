@@ -69,17 +69,27 @@ __device__ __forceinline__ int k_piece(int row, int piece) {
 }
 template <int D>
 __device__ __forceinline__ int v_piece(int row, int piece) {
-  return D == 128 ? piece ^ (2 * (row & 7)) : piece ^ (2 * ((row >> 1) & 3));
+  return D == 128 ? piece ^ (4 * (row & 3)) : piece ^ (4 * ((row >> 1) & 1));
 }
 
-// The scores of 32 U keys (S^T accumulators) to weights: capped, lowered and
-// masked, the running maximum and sum moved on, P^T fragments out.  j0: the
-// first key; seen: the keys this lane's row sees; seen_lo: the fewest that any
-// row of the wave sees; away0: p - j0 of the row.
-template <int T, int D, int U, bool kCap, bool kSlope>
-__device__ __forceinline__ void attn_softmax(const AttnScore<kCap, kSlope>& score, f32x16_t (&sc)[U],
-                                             f32x16_t (&o)[D / 32], float& top, float& sum,
-                                             s16x8_t (&pf)[2 * U], int j0, int h, int seen,
+// The largest of a lane's scores and of the lane 32 away: the row's.
+template <int U>
+__device__ __forceinline__ float attn_max(const f32x16_t (&sc)[U]) {
+  float mx = sc[0][0];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
+  return pair_max(mx);
+}
+
+// The scores of 32 U keys (S^T accumulators) capped, lowered and masked; their
+// row's largest.
+// j0: the first key; seen: the keys this lane's row sees; seen_lo: the fewest
+// that any row of the wave sees; away0: p - j0 of the row.
+template <int U, bool kCap, bool kSlope>
+__device__ __forceinline__ float attn_scores(const AttnScore<kCap, kSlope>& score,
+                                             f32x16_t (&sc)[U], int j0, int h, int seen,
                                              int seen_lo, int away0) {
   if constexpr (kCap || kSlope) {
     const float away = (float)(away0 - 4 * h);
@@ -97,16 +107,16 @@ __device__ __forceinline__ void attn_softmax(const AttnScore<kCap, kSlope>& scor
       for (int e = 0; e < 16; ++e)
         sc[u][e] = u * 32 + 8 * (e / 4) + e % 4 < lim ? sc[u][e] : -INFINITY;
   }
-  float mx = sc[0][0];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
-  mx = pair_max(mx);
-  constexpr bool kRaw = !kCap && !kSlope;  // scores are products still: a positive factor is due
-  if constexpr (kRaw) mx *= score.mul;
-  // The sums move to a new maximum only where a row's has grown by 2^8: until
-  // then weights are up to 2^8, which costs no precision in either type.
+  float mx = attn_max(sc);
+  if constexpr (!kCap && !kSlope) mx *= score.mul;  // products still: a positive factor is due
+  return mx;
+}
+
+// Moves the running maximum on, and the sums with it: only where a row's has
+// grown by 2^8, until then weights are up to 2^8, which costs no precision in
+// either type.
+template <int D>
+__device__ __forceinline__ void attn_top(float mx, f32x16_t (&o)[D / 32], float& top, float& sum) {
   if (__builtin_amdgcn_ballot_w64(mx > top + 8.f)) {
     const float next = fmaxf(top, mx);
     const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
@@ -117,6 +127,27 @@ __device__ __forceinline__ void attn_softmax(const AttnScore<kCap, kSlope>& scor
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[i][e] *= keep;
   }
+}
+
+// Two weights to T.  In f16 by the instruction itself: among the sums of the
+// same values the compiler converts one at a time and packs (three for one).
+template <int T>
+__device__ __forceinline__ uint32_t attn_pack2(float lo, float hi) {
+  if constexpr (T == kF16) {
+    uint32_t r;
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
+    return r;
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
+
+// Scores to weights, exp2(score - top): P^T fragments, and their sum.
+template <int T, int U, bool kCap, bool kSlope>
+__device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& score,
+                                             const f32x16_t (&sc)[U], float top, float& sum,
+                                             s16x8_t (&pf)[2 * U]) {
+  constexpr bool kRaw = !kCap && !kSlope;
   const float base = top == -INFINITY ? 0.f : top;
   float add = 0.f;
 #pragma unroll
@@ -130,7 +161,7 @@ __device__ __forceinline__ void attn_softmax(const AttnScore<kCap, kSlope>& scor
         const float p0 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x0, score.mul, -base) : x0 - base);
         const float p1 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x1, score.mul, -base) : x1 - base);
         add += p0 + p1;
-        w[e / 2] = Elem<T>::pack2(p0, p1);
+        w[e / 2] = attn_pack2<T>(p0, p1);
       }
       pf[u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
     }
@@ -156,7 +187,7 @@ template <int T, int D, int N>
 __device__ __forceinline__ void attn_pv(const uint4* lds, const s16x8_t (&pf)[N],
                                         f32x16_t (&o)[D / 32], int lane) {
   const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2);           // of 8 rows
-  const int vf = D == 128 ? 2 * (vr & 7) : 2 * ((vr >> 1) & 3);  // v_piece's
+  const int vf = D == 128 ? 4 * (vr & 3) : 4 * ((vr >> 1) & 1);  // v_piece's
   const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);      // 16-byte piece of 32 columns
 #pragma unroll
   for (int kc = 0; kc < N; ++kc)
@@ -275,7 +306,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
 #pragma unroll
     for (int u = 0; u < 2; ++u) sc[u] = attn_qk<T, D>(st.k + u * 32 * (D / 8), qf, c, h);
     s16x8_t pf[4];
-    attn_softmax<T, D, 2, kCap, kSlope>(score, sc, o, top, sum, pf, j0, h, seen, seen_lo, p - j0);
+    attn_top<D>(attn_scores<2, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0), o, top, sum);
+    attn_weights<T, 2, kCap, kSlope>(score, sc, top, sum, pf);
     attn_pv<T, D, 4>(st.v, pf, o, lane);
   };
 
@@ -348,17 +380,22 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   }
 }
 
-// Joins the key ranges of a split plan, in order: 16 lanes a row, D / 16 columns
-// each.  tile_rows rows a tile; a tile's ranges up to the last key that its
-// last row sees are written, the others not.
-template <int T, int D, bool kCap, bool kSlope>
+// Joins the key ranges of a split plan: 16 lanes a row, D / 16 columns each,
+// kParts such groups a row that take the ranges in turn (range i is group
+// i % kParts's) and are joined through LDS in order.  tile_rows rows a tile; a
+// tile's ranges up to the last key that its last row sees are written, the
+// others not.  Bound by the latency of its loads: four ranges a group are in
+// flight together.
+template <int T, int D, int kParts, bool kCap, bool kSlope>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_rows, int tiles,
                                                         int splits, int chunk, const float* ws) {
   using S = typename Elem<T>::S;
   __shared__ float qs[4][D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float sums[kParts > 1 ? 16 : 1][D + 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slot = threadIdx.x / 16;
   const int64_t all = (int64_t)a.n_seq * a.kv_heads * tiles * tile_rows;
-  const int64_t row = (int64_t)blockIdx.x * 16 + wave * 4 + lane / 16;
+  const int64_t row = (int64_t)blockIdx.x * (16 / kParts) + slot / kParts;
+  const int part = slot % kParts;
   const int group = a.heads / a.kv_heads;
   const int64_t of_seq = (int64_t)tiles * tile_rows;
   bool live = row < all;
@@ -369,21 +406,19 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
   const int rows = s.nq * group;
   live = live && m < rows;
   const int t = m / group, head = kh * group + m % group;
-  bool finite = true;
+  const int d0 = (lane & 15) * (D / 16);
+  float acc[D / 16] = {}, top = -INFINITY, sum = 0.f;
   if (live) {
     const int last = min(m / tile_rows * tile_rows + tile_rows, rows) - 1;
     const int used = (int)(((int64_t)attn_seen(a, s, last / group) + chunk - 1) / chunk);
     const float2* ml = reinterpret_cast<const float2*>(ws + (int64_t)splits * all * D) + row;
-    const int d0 = (lane & 15) * (D / 16);
     const float* po = ws + row * D + d0;
-    float acc[D / 16] = {}, top = -INFINITY, sum = 0.f;
-    // Four ranges at a time, their loads in flight together.
-    for (int i = 0; i < used; i += 4) {
+    for (int i = part; i < used; i += 4 * kParts) {
       float2 v[4];
       float4 w[4][D / 64];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int64_t at = (int64_t)min(i + b, used - 1) * all;
+        const int64_t at = (int64_t)min(i + b * kParts, used - 1) * all;
         v[b] = ml[at];
 #pragma unroll
         for (int e = 0; e < D / 64; ++e) w[b][e] = reinterpret_cast<const float4*>(po + at * D)[e];
@@ -399,7 +434,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
       for (int e = 0; e < D / 16; ++e) acc[e] *= old;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        if (i + b >= used) break;
+        if (i + b * kParts >= used) break;
         const float keep = __builtin_amdgcn_exp2f(v[b].x - base);
         sum = __builtin_fmaf(v[b].y, keep, sum);
 #pragma unroll
@@ -411,6 +446,35 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
         }
       }
     }
+  }
+  if constexpr (kParts > 1) {
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) sums[slot][d0 + e] = acc[e];
+    if ((lane & 15) == 0) {
+      sums[slot][D] = top;
+      sums[slot][D + 1] = sum;
+    }
+    __syncthreads();
+    const int s0 = slot - part;
+    live = live && part == 0;
+    if (live) {
+#pragma unroll
+      for (int b = 1; b < kParts; ++b) top = fmaxf(top, sums[s0 + b][D]);
+      const float base = top == -INFINITY ? 0.f : top;
+      sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int b = 0; b < kParts; ++b) {
+        const float keep = __builtin_amdgcn_exp2f(sums[s0 + b][D] - base);
+        sum = __builtin_fmaf(sums[s0 + b][D + 1], keep, sum);
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) acc[e] = __builtin_fmaf(sums[s0 + b][d0 + e], keep, acc[e]);
+      }
+    }
+  }
+  bool finite = true;
+  if (live) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
 #pragma unroll
