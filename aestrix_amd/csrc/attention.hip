@@ -48,19 +48,20 @@ void launch_join(const AttnArgs& a, const AttnPlan& plan, int tile_rows, int til
                        dim3(256), 0, stream, a, tile_rows, tiles, plan.splits, plan.chunk, ws);
 }
 
-template <int T, int D, int NW, bool kCap, bool kSlope>
+template <int T, int D, int WM, bool kCap, bool kSlope>
 hipError_t launch_tiles(const AttnArgs& a, const AttnPlan& plan, float* ws, hipStream_t stream) {
+  constexpr int kRows = WM * 32;
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
-  const int tiles = (int)((rows + NW * 32 - 1) / (NW * 32));
+  const int tiles = (int)((rows + kRows - 1) / kRows);
   const int64_t blocks = (int64_t)a.n_seq * a.kv_heads * tiles;
   if (plan.splits > 1) {
-    hipLaunchKernelGGL((attn_tiles_kernel<T, D, NW, kCap, kSlope, true>),
-                       dim3((unsigned)(blocks * plan.splits)), dim3(NW * 64), 0, stream, a, tiles,
+    hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, kSlope, true>),
+                       dim3((unsigned)(blocks * plan.splits)), dim3(256), 0, stream, a, tiles,
                        plan.splits, plan.chunk, ws);
-    launch_join<T, D, kCap, kSlope>(a, plan, NW * 32, tiles, blocks * NW * 32, ws, stream);
+    launch_join<T, D, kCap, kSlope>(a, plan, kRows, tiles, blocks * kRows, ws, stream);
   } else {
-    hipLaunchKernelGGL((attn_tiles_kernel<T, D, NW, kCap, kSlope, false>), dim3((unsigned)blocks),
-                       dim3(NW * 64), 0, stream, a, tiles, 1, 0, nullptr);
+    hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, kSlope, false>), dim3((unsigned)blocks),
+                       dim3(256), 0, stream, a, tiles, 1, 0, nullptr);
   }
   return hipGetLastError();
 }
@@ -117,39 +118,51 @@ bool tiles_fit(const AttnArgs& a) {
 }  // namespace
 
 AttnPlan attention_plan(const AttnArgs& a, int cus) {
+  const AttnPlan by_rows{IMQ_ATTENTION_ROWS, 1, 1, 0, 0};
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
   const int64_t hs = (int64_t)a.n_seq * a.kv_heads;
-  if (!tiles_fit(a) || rows > (1 << 30) || a.max_k > (1 << 30) || hs > (1 << 20))
-    return AttnPlan{IMQ_ATTENTION_ROWS, 1, 1, 0, 0};
+  if (!tiles_fit(a) || rows > (1 << 30) || a.max_k > (1 << 30) || hs > (1 << 20) ||
+      rows * hs == 0)
+    return by_rows;
   const int d = a.dim > 64 ? 128 : 64;
+  AttnPlan p{};
+  int64_t blocks, ranges, unit;  // workgroups unsplit, ranges of keys wanted, keys of the least range
   if (rows <= 32) {
-    AttnPlan p{IMQ_ATTENTION_FEW, (int)rows, 1, 0, 0};
-    constexpr int kRound = kFewWaves * kFewKeys;
-    const int64_t rounds = (a.max_k + kRound - 1) / kRound;  // tiles of each wave
+    p.kernel = IMQ_ATTENTION_FEW;
+    p.tile_rows = (int)rows;
+    blocks = hs;
+    unit = kFewWaves * kFewKeys;  // a tile for each wave
     // One workgroup a CU: 131072 keys of 8 key heads 92.8 us (5.8 TB/s), two a
     // CU 100.1, four 95.3; 8 x up to 2048 keys 9.1 / 10.0 / 11.8 (with the
     // join's 5.2 / 5.7 / 7.7 and 4.0 / 4.3 / 4.0).
-    const int64_t want = std::min<int64_t>(cus / hs, rounds);
-    if (want > 1) {
-      const int64_t per = (rounds + want - 1) / want;
-      p.chunk = (int)(per * kRound);
-      p.splits = (int)((rounds + per - 1) / per);
-      p.bytes = (size_t)p.splits * hs * rows * (d + 2) * 4;
-    }
-    return p;
+    ranges = cus / blocks;
+  } else {
+    p.kernel = IMQ_ATTENTION_TILES;
+    // 64 rows where that gives no CU a second workgroup: the waves share the
+    // keys then, and a tile of 64 keys takes 0.71 us against 0.92 (512 causal
+    // rows of 32 / 8 heads 11.8 us against 13.7).  More workgroups than that
+    // only load K and V more often (2048 rows of 64 heads on 1024 keys 102 us
+    // against 90, 1024 image rows of 24 heads 28 against 25).
+    p.tile_rows = hs * ((rows + 63) / 64) > cus ? 128 : 64;
+    blocks = hs * ((rows + p.tile_rows - 1) / p.tile_rows);
+    unit = 4 * kAttnKeys;
+    ranges = cus / blocks;
+    // Two a CU from 4096 keys a range: 65 rows on 100000 keys 222 us against
+    // 288, 512 on 8192 98 against 105; but 256 on 2048 36 against 21.
+    const int64_t two = 2 * cus / blocks;
+    if (two > 1 && a.max_k / two >= 4096) ranges = two;
   }
-  AttnPlan p{IMQ_ATTENTION_TILES, rows > 64 ? 128 : 64, 1, 0, 0};
-  const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-  const int64_t blocks = hs * tiles;
-  if (blocks > ((int64_t)1 << 31) / 64) return AttnPlan{IMQ_ATTENTION_ROWS, 1, 1, 0, 0};
-  const int64_t key_tiles = (a.max_k + kAttnKeys - 1) / kAttnKeys;
-  const int64_t want = std::min<int64_t>((2 * cus + blocks - 1) / std::max<int64_t>(blocks, 1), key_tiles / 4);
-  if (want > 1) {
-    const int64_t per = (key_tiles + want - 1) / want;
-    p.chunk = (int)(per * kAttnKeys);
-    p.splits = (int)((key_tiles + per - 1) / per);
-    p.bytes = (size_t)p.splits * blocks * p.tile_rows * (d + 2) * 4;
-    if (p.splits == 1) p.chunk = 0, p.bytes = 0;
+  if (blocks * 64 > ((int64_t)1 << 31)) return by_rows;
+  ranges = std::min<int64_t>(ranges, (a.max_k + unit - 1) / unit);
+  p.splits = 1;
+  if (ranges > 1) {
+    const int64_t step = p.kernel == IMQ_ATTENTION_FEW ? unit : kAttnKeys;
+    const int64_t steps = (a.max_k + step - 1) / step, per = (steps + ranges - 1) / ranges;
+    if (per < steps) {
+      p.chunk = (int)(per * step);
+      p.splits = (int)((steps + per - 1) / per);
+      p.bytes = (size_t)p.splits * blocks * p.tile_rows * (d + 2) * 4;
+    }
   }
   return p;
 }

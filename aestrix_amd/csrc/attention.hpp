@@ -65,12 +65,12 @@ struct AttnScore {
     top = kCap ? a.softcap * kLog2e : 0.f;
     fall = kSlope ? a.slopes[head] * kLog2e : 0.f;
   }
+  __device__ __forceinline__ float capped(float dot) const {
+    const float z = __builtin_amdgcn_exp2f(dot * mul);
+    return top - 2.f * top * __builtin_amdgcn_rcpf(z + 1.f);
+  }
   __device__ __forceinline__ float operator()(float dot, float away) const {
-    float e = dot * mul;
-    if constexpr (kCap) {
-      const float z = __builtin_amdgcn_exp2f(e);
-      e = top - 2.f * top * __builtin_amdgcn_rcpf(z + 1.f);
-    }
+    float e = kCap ? capped(dot) : dot * mul;
     if constexpr (kSlope) e = __builtin_fmaf(-fall, __builtin_fabsf(away), e);
     return e;
   }

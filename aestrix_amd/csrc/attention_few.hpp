@@ -80,6 +80,8 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
   __builtin_amdgcn_sched_barrier(0);
   const AttnScore<kCap, kSlope> score(a, head);
   const int p = t + s.nk - s.nq;
+  // Keys below `near` are at or before every row's p, or hidden behind it.
+  const int near = a.causal && !a.prefix_lens ? INT_MAX : s.nk - s.nq + 1;
   f32x16_t o[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
@@ -104,8 +106,10 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
     if constexpr (kMore) load(kbase, kb, k_off, kl, j0 + kStep);
     __builtin_amdgcn_sched_barrier(0);
     s16x8_t pf[2];
-    attn_top<D>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0), o, top, sum);
-    attn_weights<T, 1, kCap, kSlope>(score, sc, top, sum, pf);
+    float shift;
+    attn_top<D>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
+                                             j0 + kFewKeys <= near, shift), o, top, sum);
+    attn_weights<T, 1, kCap, kSlope>(score, sc, shift, top, sum, pf);
     __builtin_amdgcn_sched_barrier(0);
     IMQ_WAIT_VMCNT(kMore ? kLoads : 0);  // V has landed (the next K is in flight)
     __builtin_amdgcn_sched_barrier(0);

@@ -21,6 +21,8 @@
 // the row-per-lane reads of K and the 4-row reads of V touch every bank evenly.
 #pragma once
 
+#include <climits>
+
 #include "attention.hpp"
 
 namespace imq {
@@ -72,32 +74,42 @@ __device__ __forceinline__ int v_piece(int row, int piece) {
   return D == 128 ? piece ^ (4 * (row & 3)) : piece ^ (4 * ((row >> 1) & 1));
 }
 
-// The largest of a lane's scores and of the lane 32 away: the row's.
-template <int U>
-__device__ __forceinline__ float attn_max(const f32x16_t (&sc)[U]) {
-  float mx = sc[0][0];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
-  return pair_max(mx);
-}
-
 // The scores of 32 U keys (S^T accumulators) capped, lowered and masked; their
-// row's largest.
-// j0: the first key; seen: the keys this lane's row sees; seen_lo: the fewest
-// that any row of the wave sees; away0: p - j0 of the row.
+// row's largest, in units of log2.  j0: the first key; seen: the keys this
+// lane's row sees; seen_lo: the fewest that any row of the wave sees; away0:
+// p - j0 of the row.  What is left in sc is such that a key's exponent is
+// sc * score.mul + shift without cap and slope, sc + shift with them.
+// A slope's fall is linear in the key before p: one fma a score, and the part
+// that all keys of the tile share goes into shift.  Tiles that reach past p
+// (none where causal hides those keys) take the distance itself.
 template <int U, bool kCap, bool kSlope>
 __device__ __forceinline__ float attn_scores(const AttnScore<kCap, kSlope>& score,
                                              f32x16_t (&sc)[U], int j0, int h, int seen,
-                                             int seen_lo, int away0) {
-  if constexpr (kCap || kSlope) {
+                                             int seen_lo, int away0, bool linear, float& shift) {
+  shift = 0.f;
+  if constexpr (kSlope) {
     const float away = (float)(away0 - 4 * h);
+    if (linear) {
+      shift = -score.fall * away;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = kCap ? score.capped(sc[u][e]) : sc[u][e] * score.mul;
+          sc[u][e] = __builtin_fmaf(score.fall, (float)(u * 32 + 8 * (e / 4) + e % 4), x);
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sc[u][e] = score(sc[u][e], away - (float)(u * 32 + 8 * (e / 4) + e % 4));
+    }
+  } else if constexpr (kCap) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        sc[u][e] = score(sc[u][e], away - (float)(u * 32 + 8 * (e / 4) + e % 4));
+      for (int e = 0; e < 16; ++e) sc[u][e] = score.capped(sc[u][e]);
   }
   if (j0 + 32 * U > seen_lo) {
     const int lim = seen - j0 - 4 * h;
@@ -107,9 +119,14 @@ __device__ __forceinline__ float attn_scores(const AttnScore<kCap, kSlope>& scor
       for (int e = 0; e < 16; ++e)
         sc[u][e] = u * 32 + 8 * (e / 4) + e % 4 < lim ? sc[u][e] : -INFINITY;
   }
-  float mx = attn_max(sc);
-  if constexpr (!kCap && !kSlope) mx *= score.mul;  // products still: a positive factor is due
-  return mx;
+  float mx = sc[0][0];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
+  if constexpr (kSlope) mx += shift;
+  else if constexpr (!kCap) mx *= score.mul;  // a positive factor
+  return pair_max(mx);
 }
 
 // Moves the running maximum on, and the sums with it: only where a row's has
@@ -129,27 +146,35 @@ __device__ __forceinline__ void attn_top(float mx, f32x16_t (&o)[D / 32], float&
   }
 }
 
-// Two weights to T.  In f16 by the instruction itself: among the sums of the
-// same values the compiler converts one at a time and packs (three for one).
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+// Two weights to T.  In f16 as a vector: of two scalar conversions, among the
+// sums of the same values, the compiler makes three instructions for one.
 template <int T>
 __device__ __forceinline__ uint32_t attn_pack2(float lo, float hi) {
-  if constexpr (T == kF16) {
-    uint32_t r;
-    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
-    return r;
-  } else {
+  if constexpr (T == kF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo, hi}), f16x2_t));
+  else
     return pack_bf16x2(lo, hi);
-  }
 }
 
-// Scores to weights, exp2(score - top): P^T fragments, and their sum.
+// x + the sum of the two T values of w, exactly added up in 32 bits.
+template <int T>
+__device__ __forceinline__ float attn_add2(uint32_t w, float x) {
+  if constexpr (T == kF16) return dot2_f16(w, 0x3C003C00u, x);
+  else return dot2_bf16(w, 0x3F803F80u, x);
+}
+
+// Scores to weights, exp2(score - top): P^T fragments, and their sum.  The sum
+// is that of the weights as rounded to T, which are what V is multiplied by;
+// two a dot2 instruction.
 template <int T, int U, bool kCap, bool kSlope>
 __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& score,
-                                             const f32x16_t (&sc)[U], float top, float& sum,
-                                             s16x8_t (&pf)[2 * U]) {
+                                             const f32x16_t (&sc)[U], float shift, float top,
+                                             float& sum, s16x8_t (&pf)[2 * U]) {
   constexpr bool kRaw = !kCap && !kSlope;
-  const float base = top == -INFINITY ? 0.f : top;
-  float add = 0.f;
+  const float base = (top == -INFINITY ? 0.f : top) - shift;
+  float add[2] = {sum, 0.f};
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -160,12 +185,12 @@ __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& scor
         const float x0 = sc[u][half * 8 + e], x1 = sc[u][half * 8 + e + 1];
         const float p0 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x0, score.mul, -base) : x0 - base);
         const float p1 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x1, score.mul, -base) : x1 - base);
-        add += p0 + p1;
         w[e / 2] = attn_pack2<T>(p0, p1);
+        add[(e / 2) & 1] = attn_add2<T>(w[e / 2], add[(e / 2) & 1]);
       }
       pf[u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
     }
-  sum += add;
+  sum = add[0] + add[1];
 }
 
 // S^T of 32 keys: K rows from LDS (row c of the 32 at `lds`), Q^T from registers.
@@ -231,16 +256,19 @@ struct AttnStage {
 template <int D, int NW>
 __device__ __forceinline__ void attn_load(const char* base, int64_t row_bytes, int rows, int dim,
                                           const uint32_t (&off)[D / (8 * NW)], uint4* lds, int wave) {
+  // No rows: every read gives zero.
   const __amdgpu_buffer_rsrc_t rs =
-      make_rsrc(base, (uint32_t)((rows - 1) * row_bytes + dim * 2));
+      make_rsrc(base, rows > 0 ? (uint32_t)((rows - 1) * row_bytes + dim * 2) : 0u);
 #pragma unroll
   for (int i = 0; i < D / (8 * NW); ++i) load_lds16(rs, off[i], 0, lds + (i * NW + wave) * 64);
 }
 
-template <int T, int D, int NW, bool kCap, bool kSlope, bool kSplit>
-__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(AttnArgs a, int tiles, int splits,
+template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
+__global__ __launch_bounds__(256, 2) void attn_tiles_kernel(AttnArgs a, int tiles, int splits,
                                                                int chunk, float* ws) {
   using S = typename Elem<T>::S;
+  // WM waves on rows of their own, WK on a part of every tile's keys each.
+  constexpr int NW = 4, WK = NW / WM, U = 2 / WK, kRows = WM * 32;
   constexpr int kLoads = D / (8 * NW);
   __shared__ AttnStage<D> st0, st1;
   __shared__ float qs[NW][D];
@@ -255,15 +283,16 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   AttnSeq s = attn_seq(a, hs / a.kv_heads);
   const int group = a.heads / a.kv_heads;
   const int rows = s.nq * group;  // checked on the host to fit
-  const int m0 = tile * NW * 32;
+  const int m0 = tile * kRows;
   if (m0 >= rows) return;
   // Rows past the last repeat it; they are not stored.
-  const int mw = m0 + wave * 32;
+  const int wm = wave % WM, wk = wave / WM;
+  const int mw = m0 + wm * 32;
   const int m = min(mw + c, rows - 1);
   const int t = m / group, head = kh * group + m % group;
   const int seen = attn_seen(a, s, t);
   const int seen_wg = __builtin_amdgcn_readfirstlane(
-      attn_seen(a, s, min(m0 + NW * 32 - 1, rows - 1) / group));
+      attn_seen(a, s, min(m0 + kRows - 1, rows - 1) / group));
   const int seen_hi = mw >= rows ? 0 : __builtin_amdgcn_readfirstlane(
       attn_seen(a, s, min(mw + 31, rows - 1) / group));
   const int seen_lo = __builtin_amdgcn_readfirstlane(attn_seen(a, s, min(mw, rows - 1) / group));
@@ -284,7 +313,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   const char* kbase = reinterpret_cast<const char*>(static_cast<const S*>(a.k) + s.k_at + kh * a.k_head);
   const char* vbase = reinterpret_cast<const char*>(static_cast<const S*>(a.v) + s.v_at + kh * a.v_head);
   auto issue = [&](AttnStage<D>& st, int j0) {
-    const int n = min(kAttnKeys, s.nk - j0);
+    // Nothing past the last tile: rows below 1.
+    const int n = j0 < end ? min(kAttnKeys, s.nk - j0) : 0;
     attn_load<D, NW>(kbase + j0 * kb, kb, n, a.dim, k_off, st.k, wave);
     attn_load<D, NW>(vbase + j0 * vb, vb, n, a.dim, v_off, st.v, wave);
   };
@@ -294,6 +324,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   attn_load_q<T, D>(a, s, t, head, h, qf);
   const AttnScore<kCap, kSlope> score(a, head);
   const int p = t + s.nk - s.nq;
+  // Keys below `near` are at or before every row's p, or hidden behind it.
+  const int near = a.causal && !a.prefix_lens ? INT_MAX : min(mw, rows - 1) / group + s.nk - s.nq + 1;
   f32x16_t o[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
@@ -301,14 +333,41 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
     for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
   float top = -INFINITY, sum = 0.f;
 
-  auto step = [&](const AttnStage<D>& st, int j0) {
-    f32x16_t sc[2];
+  // The wave's keys of the tile that begins at j0.
+  // The next tile's loads go out among the score's MFMAs: before them they
+  // would hold up the wave that has everyone wait.
+  auto step = [&](const AttnStage<D>& st, AttnStage<D>& to, int j0) __attribute__((always_inline)) {
+    const int j1 = j0 + kAttnKeys;
+    j0 += wk * (32 * U);
+    if (j0 >= seen_hi) {
+      issue(to, j1);
+      return;
+    }
+    const uint4* k = st.k + wk * U * 32 * (D / 8);
+    f32x16_t sc[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) sc[u] = attn_qk<T, D>(st.k + u * 32 * (D / 8), qf, c, h);
-    s16x8_t pf[4];
-    attn_top<D>(attn_scores<2, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0), o, top, sum);
-    attn_weights<T, 2, kCap, kSlope>(score, sc, top, sum, pf);
-    attn_pv<T, D, 4>(st.v, pf, o, lane);
+    for (int u = 0; u < U; ++u) sc[u] = attn_qk<T, D>(k + u * 32 * (D / 8), qf, c, h);
+    issue(to, j1);
+    // K of eight MFMAs is read ahead: one read an MFMA, as the compiler has
+    // it, leaves most of an LDS read's 100 to 200 cycles exposed.
+    constexpr int kReads = U * D / 16, kAhead = kReads < 8 ? kReads : 8;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < kReads - kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+    }
+    s16x8_t pf[2 * U];
+    float shift;
+    attn_top<D>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
+                                             j0 + 32 * U <= near, shift), o, top, sum);
+    attn_weights<T, U, kCap, kSlope>(score, sc, shift, top, sum, pf);
+    attn_pv<T, D, 2 * U>(st.v + wk * U * 32 * (D / 8), pf, o, lane);
   };
 
   // A tile in use, the next in flight.  Every wave's loads of a stage have
@@ -321,19 +380,52 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void attn_tiles_kernel(At
   };
   for (int j0 = begin; j0 < end; j0 += 2 * kAttnKeys) {
     meet();
-    if (j0 + kAttnKeys < end) issue(st1, j0 + kAttnKeys);
-    if (j0 < seen_hi) step(st0, j0);
+    step(st0, st1, j0);
     if (j0 + kAttnKeys >= end) break;
     meet();
-    if (j0 + 2 * kAttnKeys < end) issue(st0, j0 + 2 * kAttnKeys);
-    if (j0 + kAttnKeys < seen_hi) step(st1, j0 + kAttnKeys);
+    step(st1, st0, j0 + kAttnKeys);
   }
+  IMQ_WAIT_VMCNT(0);  // the loads past the last tile (of nothing), before their LDS is used again
+  __builtin_amdgcn_sched_barrier(0);
 
   sum = pair_sum(sum);
+  if constexpr (WK == 2) {
+    // The second half's sums through the stages' LDS, lane for lane.
+    static_assert(sizeof(AttnStage<D>) >= WM * 64 * (D / 2) * 4, "a wave's sums fit half a stage");
+    float4* po = reinterpret_cast<float4*>(&st0) + wm * (D / 8) * 64 + lane;
+    float2* pt = reinterpret_cast<float2*>(&st1) + wm * 64 + lane;
+    meet();
+    if (wk == 1) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          po[(i * 4 + e / 4) * 64] = make_float4(o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]);
+      *pt = make_float2(top, sum);
+    }
+    meet();
+    if (wk == 1) return;
+    const float2 other = *pt;
+    const float next = fmaxf(top, other.x);
+    const float base = next == -INFINITY ? 0.f : next;
+    const float keep0 = __builtin_amdgcn_exp2f(top - base), keep1 = __builtin_amdgcn_exp2f(other.x - base);
+    top = next;
+    sum = sum * keep0 + other.y * keep1;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const float4 v = po[(i * 4 + e / 4) * 64];
+        o[i][e] = o[i][e] * keep0 + v.x * keep1;
+        o[i][e + 1] = o[i][e + 1] * keep0 + v.y * keep1;
+        o[i][e + 2] = o[i][e + 2] * keep0 + v.z * keep1;
+        o[i][e + 3] = o[i][e + 3] * keep0 + v.w * keep1;
+      }
+  }
   if constexpr (kSplit) {
     // [split][row of all tiles][D], then (top, sum) of each.
-    const int64_t all = (int64_t)hs_n * tiles * (NW * 32);
-    const int64_t row = ((int64_t)hs * tiles + tile) * (NW * 32) + wave * 32 + c;
+    const int64_t all = (int64_t)hs_n * tiles * kRows;
+    const int64_t row = ((int64_t)hs * tiles + tile) * kRows + wm * 32 + c;
     if (mw + c < rows) {
       float* po = ws + ((int64_t)split * all + row) * D;
 #pragma unroll
