@@ -34,7 +34,7 @@ int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, i
   if (!p) return fail(ctx, IMQ_EINVAL, "%s: null arguments", fn);
   if (p->dtype != IMQ_BF16 && p->dtype != IMQ_F16)
     return fail(ctx, IMQ_EUNSUPPORTED, "%s: dtype %d (bf16 and f16 are provided)", fn,
-                (int)p->dtype);
+                p->dtype);
   if (p->n_seq < 0 || p->max_q < 0 || p->max_k < 0 || p->q_rows < 0 || p->k_rows < 0)
     return fail(ctx, IMQ_EINVAL, "%s: n_seq %d, max_q %d, max_k %d, q_rows %d, k_rows %d", fn,
                 p->n_seq, p->max_q, p->max_k, p->q_rows, p->k_rows);
@@ -220,7 +220,7 @@ int imq_attention(imq_ctx* ctx, const imq_attention_args* args, imq_stream strea
       plan.bytes = 0;
     }
   }
-  const hipError_t e = imq::launch_attention(a, plan, ws, (int)args->dtype, st);
+  const hipError_t e = imq::launch_attention(a, plan, ws, args->dtype, st);
   return e == hipSuccess ? IMQ_OK : hip_fail(ctx, e, fn);
 }
 

@@ -133,7 +133,7 @@ typedef struct imq_attention_args {
     float scale;                  /* finite, > 0 */
     float softcap;                /* finite, >= 0; 0: none */
     int causal;
-    imq_dtype dtype;
+    int dtype;                    /* an imq_dtype */
 } imq_attention_args;
 
 int imq_attention(imq_ctx* ctx, const imq_attention_args* args, imq_stream stream);
