@@ -65,10 +65,10 @@ struct AttnScore {
     top = kCap ? a.softcap * kLog2e : 0.f;
     fall = kSlope ? a.slopes[head] * kLog2e : 0.f;
   }
-  __device__ __forceinline__ float capped(float dot) const {
-    const float z = __builtin_amdgcn_exp2f(dot * mul);
-    return top - 2.f * top * __builtin_amdgcn_rcpf(z + 1.f);
+  __device__ __forceinline__ float rest(float dot) const {
+    return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * mul) + 1.f);
   }
+  __device__ __forceinline__ float capped(float dot) const { return top - 2.f * top * rest(dot); }
   __device__ __forceinline__ float operator()(float dot, float away) const {
     float e = kCap ? capped(dot) : dot * mul;
     if constexpr (kSlope) e = __builtin_fmaf(-fall, __builtin_fabsf(away), e);

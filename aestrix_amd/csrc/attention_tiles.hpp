@@ -78,7 +78,9 @@ __device__ __forceinline__ int v_piece(int row, int piece) {
 // row's largest, in units of log2.  j0: the first key; seen: the keys this
 // lane's row sees; seen_lo: the fewest that any row of the wave sees; away0:
 // p - j0 of the row.  What is left in sc is such that a key's exponent is
-// sc * score.mul + shift without cap and slope, sc + shift with them.
+// sc * score.mul without cap and slope; with a cap alone, top - 2 top sc, as sc
+// is the 1 / (exp(2 z) + 1) of the tanh (the exponent is one fma from it, made
+// with the subtraction of the maximum); with a slope, sc + shift.
 // A slope's fall is linear in the key before p: one fma a score, and the part
 // that all keys of the tile share goes into shift.  Tiles that reach past p
 // (none where causal hides those keys) take the distance itself.
@@ -109,23 +111,25 @@ __device__ __forceinline__ float attn_scores(const AttnScore<kCap, kSlope>& scor
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[u][e] = score.capped(sc[u][e]);
+      for (int e = 0; e < 16; ++e) sc[u][e] = score.rest(sc[u][e]);
   }
+  constexpr bool kRest = kCap && !kSlope;  // falls with the score: a hidden key's is infinite
   if (j0 + 32 * U > seen_lo) {
     const int lim = seen - j0 - 4 * h;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        sc[u][e] = u * 32 + 8 * (e / 4) + e % 4 < lim ? sc[u][e] : -INFINITY;
+        sc[u][e] = u * 32 + 8 * (e / 4) + e % 4 < lim ? sc[u][e] : kRest ? INFINITY : -INFINITY;
   }
   float mx = sc[0][0];
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
-  if constexpr (kSlope) mx += shift;
-  else if constexpr (!kCap) mx *= score.mul;  // a positive factor
+    for (int e = 0; e < 16; ++e) mx = kRest ? fminf(mx, sc[u][e]) : fmaxf(mx, sc[u][e]);
+  if constexpr (kRest) mx = __builtin_fmaf(-2.f * score.top, mx, score.top);
+  else if constexpr (kSlope) mx += shift;
+  else mx *= score.mul;  // a positive factor
   return pair_max(mx);
 }
 
@@ -172,8 +176,9 @@ template <int T, int U, bool kCap, bool kSlope>
 __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& score,
                                              const f32x16_t (&sc)[U], float shift, float top,
                                              float& sum, s16x8_t (&pf)[2 * U]) {
-  constexpr bool kRaw = !kCap && !kSlope;
-  const float base = (top == -INFINITY ? 0.f : top) - shift;
+  // The exponent as one fma of what attn_scores left.
+  const float by = kSlope ? 1.f : kCap ? -2.f * score.top : score.mul;
+  const float base = (top == -INFINITY ? 0.f : top) - (kSlope ? shift : kCap ? score.top : 0.f);
   float add[2] = {sum, 0.f};
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -183,8 +188,8 @@ __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& scor
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const float x0 = sc[u][half * 8 + e], x1 = sc[u][half * 8 + e + 1];
-        const float p0 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x0, score.mul, -base) : x0 - base);
-        const float p1 = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x1, score.mul, -base) : x1 - base);
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x0, by, -base));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x1, by, -base));
         w[e / 2] = attn_pack2<T>(p0, p1);
         add[(e / 2) & 1] = attn_add2<T>(w[e / 2], add[(e / 2) & 1]);
       }
