@@ -269,8 +269,8 @@ __device__ __forceinline__ void attn_load(const char* base, int64_t row_bytes, i
 }
 
 template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
-__global__ __launch_bounds__(256, 2) void attn_tiles_kernel(AttnArgs a, int tiles, int splits,
-                                                               int chunk, float* ws) {
+__global__ __launch_bounds__(256, 2) void attn_tiles_kernel(AttnArgs a, int tiles, int first,
+                                                               int splits, int chunk, float* ws) {
   using S = typename Elem<T>::S;
   // WM waves on rows of their own, WK on a part of every tile's keys each.
   constexpr int NW = 4, WK = NW / WM, U = 2 / WK, kRows = WM * 32;
@@ -283,7 +283,11 @@ __global__ __launch_bounds__(256, 2) void attn_tiles_kernel(AttnArgs a, int tile
   const int hs = blockIdx.x % hs_n, rest = blockIdx.x / hs_n;
   const int split = kSplit ? rest % splits : 0;
   // The last rows of a causal sequence have the most keys: they start first.
-  const int tile = tiles - 1 - (kSplit ? rest / splits : rest);
+  // Where every workgroup is resident from the start, two a CU, those behind
+  // the first `first` ranks, which get a CU's second place, go from the least
+  // keys up instead, so that a long one shares its CU with a short one.
+  const int rank = kSplit ? rest / splits : rest;
+  const int tile = rank < first ? tiles - 1 - rank : rank - first;
   const int kh = hs % a.kv_heads;
   AttnSeq s = attn_seq(a, hs / a.kv_heads);
   const int group = a.heads / a.kv_heads;
