@@ -25,6 +25,10 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
                                                                     int splits, int chunk, float* ws) {
   using S = typename Elem<T>::S;
   constexpr int kPieces = kFewKeys * D / 8, kLoads = kPieces / 64;
+  // bf16 weights carry 8 bits; what a rounding to them loses, up to 2^-9 of a
+  // weight, is multiplied with V as well: the matrix cores have the time.  (f16
+  // weights lose 2^-12.)
+  constexpr bool kRest = T == kBf16;
   __shared__ uint4 kbuf[kFewWaves][kPieces];
   __shared__ uint4 vbuf[kFewWaves][kPieces];
   __shared__ float2 ml[kFewWaves][32];
@@ -105,15 +109,15 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
     IMQ_WAIT_LGKM_0();  // K has been read
     if constexpr (kMore) load(kbase, kb, k_off, kl, j0 + kStep);
     __builtin_amdgcn_sched_barrier(0);
-    s16x8_t pf[2];
+    s16x8_t pf[kRest ? 4 : 2];
     float shift;
     attn_top<D>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
                                              j0 + kFewKeys <= near, shift), o, top, sum);
-    attn_weights<T, 1, kCap, kSlope>(score, sc, shift, top, sum, pf);
+    attn_weights<T, 1, kCap, kSlope, kRest>(score, sc, shift, top, sum, pf);
     __builtin_amdgcn_sched_barrier(0);
     IMQ_WAIT_VMCNT(kMore ? kLoads : 0);  // V has landed (the next K is in flight)
     __builtin_amdgcn_sched_barrier(0);
-    attn_pv<T, D, 2>(vl, pf, o, lane);
+    attn_pv<T, D, 2, kRest>(vl, pf, o, lane);
     __builtin_amdgcn_sched_barrier(0);
     IMQ_WAIT_LGKM_0();  // V has been read
     if constexpr (kMore) load(vbase, vb, v_off, vl, j0 + kStep);

@@ -171,11 +171,12 @@ __device__ __forceinline__ float attn_add2(uint32_t w, float x) {
 
 // Scores to weights, exp2(score - top): P^T fragments, and their sum.  The sum
 // is that of the weights as rounded to T, which are what V is multiplied by;
-// two a dot2 instruction.
-template <int T, int U, bool kCap, bool kSlope>
+// two a dot2 instruction.  kRest: the weights' remainders after that rounding
+// as fragments of their own, for a second product with V.
+template <int T, int U, bool kCap, bool kSlope, bool kRest = false>
 __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& score,
                                              const f32x16_t (&sc)[U], float shift, float top,
-                                             float& sum, s16x8_t (&pf)[2 * U]) {
+                                             float& sum, s16x8_t (&pf)[2 * U * (kRest ? 2 : 1)]) {
   // The exponent as one fma of what attn_scores left.
   const float by = kSlope ? 1.f : kCap ? -2.f * score.top : score.mul;
   const float base = (top == -INFINITY ? 0.f : top) - (kSlope ? shift : kCap ? score.top : 0.f);
@@ -184,7 +185,7 @@ __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& scor
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      uint32_t w[4];
+      uint32_t w[4], rest[4];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const float x0 = sc[u][half * 8 + e], x1 = sc[u][half * 8 + e + 1];
@@ -192,8 +193,15 @@ __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& scor
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x1, by, -base));
         w[e / 2] = attn_pack2<T>(p0, p1);
         add[(e / 2) & 1] = attn_add2<T>(w[e / 2], add[(e / 2) & 1]);
+        if constexpr (kRest) {
+          rest[e / 2] = attn_pack2<T>(p0 - Elem<T>::param((uint16_t)(w[e / 2] & 0xFFFFu)),
+                                      p1 - Elem<T>::param((uint16_t)(w[e / 2] >> 16)));
+          add[(e / 2) & 1] = attn_add2<T>(rest[e / 2], add[(e / 2) & 1]);
+        }
       }
       pf[u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+      if constexpr (kRest)
+        pf[2 * U + u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(rest[0], rest[1], rest[2], rest[3]));
     }
   sum = add[0] + add[1];
 }
@@ -212,9 +220,10 @@ __device__ __forceinline__ f32x16_t attn_qk(const uint4* lds, const s16x8_t (&qf
   return sc;
 }
 
-// O^T += V^T P^T over 16 N keys: the rows at `lds` through the transpose loads.
-template <int T, int D, int N>
-__device__ __forceinline__ void attn_pv(const uint4* lds, const s16x8_t (&pf)[N],
+// O^T += V^T P^T over 16 N keys: the rows at `lds` through the transpose loads
+// (kRest: and the weights' remainders, N fragments behind the weights').
+template <int T, int D, int N, bool kRest = false>
+__device__ __forceinline__ void attn_pv(const uint4* lds, const s16x8_t (&pf)[N * (kRest ? 2 : 1)],
                                         f32x16_t (&o)[D / 32], int lane) {
   const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2);           // of 8 rows
   const int vf = D == 128 ? 4 * (vr & 3) : 4 * ((vr >> 1) & 1);  // v_piece's
@@ -230,8 +239,9 @@ __device__ __forceinline__ void attn_pv(const uint4* lds, const s16x8_t (&pf)[N]
         part[e4] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (lds_s16x4_t*)(reinterpret_cast<const uint2*>(lds) + at));
       }
-      o[i] = attn_mfma<T>(__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7), pf[kc],
-                          o[i]);
+      const s16x8_t vv = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      o[i] = attn_mfma<T>(vv, pf[kc], o[i]);
+      if constexpr (kRest) o[i] = attn_mfma<T>(vv, pf[N + kc], o[i]);
     }
 }
 

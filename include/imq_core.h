@@ -91,7 +91,8 @@ int imq_rope(imq_ctx* ctx, const imq_rope_heads* groups, int n_groups, int rows,
  * and a whole prompt are the same call.  Keys that a query does not see do
  * not touch its output, whatever they hold (NaN and infinities included).
  * T: bf16 or f16; scores, softmax and sums in fp32, the softmax's weights
- * rounded to T before the product with v.
+ * rounded to T before the product with v (up to 32 rows in bf16 with the
+ * remainders of that rounding multiplied too; by rows, not rounded).
  *
  * A sequence's rows:
  *   q_offsets NULL: its queries are rows 0.. of q + s * q_seq (max_q rows are
