@@ -54,15 +54,18 @@ hipError_t launch_tiles(const AttnArgs& a, const AttnPlan& plan, float* ws, hipS
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
   const int tiles = (int)((rows + kRows - 1) / kRows);
   const int64_t blocks = (int64_t)a.n_seq * a.kv_heads * tiles;
-  if (plan.splits > 1) {
-    hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, kSlope, true>),
-                       dim3((unsigned)(blocks * plan.splits)), dim3(256), 0, stream, a, tiles,
-                       plan.first, plan.splits, plan.chunk, ws);
-    launch_join<T, D, kCap, kSlope>(a, plan, kRows, tiles, blocks * kRows, ws, stream);
-  } else {
-    hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, kSlope, false>), dim3((unsigned)blocks),
-                       dim3(256), 0, stream, a, tiles, plan.first, 1, 0, nullptr);
+  const dim3 block(attn_waves(WM) * 64);
+  if constexpr (WM < 8) {  // the plan splits no keys of 256 rows
+    if (plan.splits > 1) {
+      hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, kSlope, true>),
+                         dim3((unsigned)(blocks * plan.splits)), block, 0, stream, a, tiles,
+                         plan.first, plan.splits, plan.chunk, ws);
+      launch_join<T, D, kCap, kSlope>(a, plan, kRows, tiles, blocks * kRows, ws, stream);
+      return hipGetLastError();
+    }
   }
+  hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, kSlope, false>), dim3((unsigned)blocks),
+                     block, 0, stream, a, tiles, plan.first, 1, 0, nullptr);
   return hipGetLastError();
 }
 
@@ -88,12 +91,15 @@ hipError_t launch_scored(const AttnArgs& a, const AttnPlan& plan, float* ws, hip
   if (plan.kernel == IMQ_ATTENTION_FEW)
     return a.dim > 64 ? launch_few<T, 128, kCap, kSlope>(a, plan, ws, stream)
                       : launch_few<T, 64, kCap, kSlope>(a, plan, ws, stream);
-  const bool wide = plan.tile_rows == 128;
-  if (a.dim > 64)
-    return wide ? launch_tiles<T, 128, 4, kCap, kSlope>(a, plan, ws, stream)
-                : launch_tiles<T, 128, 2, kCap, kSlope>(a, plan, ws, stream);
-  return wide ? launch_tiles<T, 64, 4, kCap, kSlope>(a, plan, ws, stream)
-              : launch_tiles<T, 64, 2, kCap, kSlope>(a, plan, ws, stream);
+  switch (a.dim > 64 ? plan.tile_rows : -plan.tile_rows) {
+    case 256: return launch_tiles<T, 128, 8, kCap, kSlope>(a, plan, ws, stream);
+    case 128: return launch_tiles<T, 128, 4, kCap, kSlope>(a, plan, ws, stream);
+    case 64: return launch_tiles<T, 128, 2, kCap, kSlope>(a, plan, ws, stream);
+    case -256: return launch_tiles<T, 64, 8, kCap, kSlope>(a, plan, ws, stream);
+    case -128: return launch_tiles<T, 64, 4, kCap, kSlope>(a, plan, ws, stream);
+    case -64: return launch_tiles<T, 64, 2, kCap, kSlope>(a, plan, ws, stream);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 template <int T>
@@ -144,19 +150,32 @@ AttnPlan attention_plan(const AttnArgs& a, int cus) {
     // only load K and V more often (2048 rows of 64 heads on 1024 keys 102 us
     // against 90, 1024 image rows of 24 heads 28 against 25).
     p.tile_rows = hs * ((rows + 63) / 64) > cus ? 128 : 64;
+    // 256 rows where they fill the card: a workgroup of eight waves on one stage
+    // of keys then writes LDS half as often as two of four.  4608 rows of 24
+    // heads 279 us against 294 (64 elements 155 / 169), 1536 53 / 55, 8192 causal
+    // rows of 32 / 8 heads 532 / 543, 32768 8.03 ms / 8.24.  Not where half of the
+    // CUs would have none in the last round: two small ones share a CU, one alone
+    // is quicker (9216 rows 1056 us against 1014); nor short causal rows, whose
+    // tiles differ most (2048 62 us against 48, 4 x 2048 155 / 152).
+    const int64_t wide = hs * ((rows + 255) / 256), last = wide % cus;
+    if ((last == 0 || last > cus / 2) &&
+        (a.causal ? rows >= 4096 && wide >= 2 * cus : rows >= 1024))
+      p.tile_rows = 256;
     const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
     blocks = hs * tiles;
     // (attn_tiles_kernel; four prompts of 512, 316, 121 and 437 rows, 32 / 8 heads:
     // 18.0 us against 19.4.)
-    p.first = (int)(blocks <= 2 * cus && blocks > cus ? cus / hs : tiles);
+    p.first = (int)(p.tile_rows < 256 && blocks <= 2 * cus && blocks > cus ? cus / hs : tiles);
     unit = 4 * kAttnKeys;
     ranges = cus / blocks;
     // Two a CU from 4096 keys a range: 65 rows on 100000 keys 222 us against
     // 288, 512 on 8192 98 against 105; but 256 on 2048 36 against 21.
     const int64_t two = 2 * cus / blocks;
-    if (two > 1 && a.max_k / two >= 4096) ranges = two;
+    if (p.tile_rows == 256)
+      ranges = 1;  // more than cus / 2 workgroups already, and one a CU
+    else if (two > 1 && a.max_k / two >= 4096) ranges = two;
   }
-  if (blocks * 64 > ((int64_t)1 << 31)) return by_rows;
+  if (blocks * 512 >= ((int64_t)1 << 32)) return by_rows;
   ranges = std::min<int64_t>(ranges, (a.max_k + unit - 1) / unit);
   p.splits = 1;
   if (ranges > 1) {

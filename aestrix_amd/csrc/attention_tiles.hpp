@@ -18,7 +18,22 @@
 // (16 bytes a lane, no registers), one tile ahead of the one in use; V's
 // operand is read through the LDS transpose loads, 4 keys of 16 columns each.
 // 16-byte pieces of a row are swizzled (XOR with the row) at their source, so
-// the row-per-lane reads of K and the 4-row reads of V touch every bank evenly.
+// the row-per-lane reads of K and the 4-row reads of V touch every bank evenly
+// (no conflicts counted).
+//
+// Two workgroups of four waves share a CU (64 KB of LDS and up to 256 registers a
+// lane each), or one of eight has it, so that one wave of a SIMD multiplies while
+// the other weighs: a tile of 64 keys is 32 MFMAs
+// of 32 cycles a wave and some 130 VALU instructions, 32 of them exponentials
+// (8 cycles).  Measured, D = 128: 4608 x 4608 of 24 heads in f16 255-285 us
+// (870-970 TFLOP/s, the clock at 1.8 GHz; a large hipBLASLt product 1467), 16384 causal
+// rows of 32 / 8 heads in bf16 1.97 ms (1114), with slopes 2.08-2.11.  The matrix cores
+// are busy for half of the cycles.  With parts left out, the last took 2.05 ms of four
+// waves a workgroup, 1.88 without the loads, 1.60 without the LDS reads, 1.65
+// without the weighing: LDS, written and read, is what the rest waits for.
+// Tried and slower: 256 rows in two groups of waves that take turns by
+// barriers, the next scores' MFMAs among one wave's own exponentials, 64 rows of
+// a workgroup where a CU gets more than one, V and K lines read ahead into L2.
 #pragma once
 
 #include <climits>
@@ -278,12 +293,15 @@ __device__ __forceinline__ void attn_load(const char* base, int64_t row_bytes, i
   for (int i = 0; i < D / (8 * NW); ++i) load_lds16(rs, off[i], 0, lds + (i * NW + wave) * 64);
 }
 
+// Waves of a workgroup with WM of them on rows of their own.
+constexpr int attn_waves(int wm) { return wm < 4 ? 4 : wm; }
+
 template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
-__global__ __launch_bounds__(256, 2) void attn_tiles_kernel(AttnArgs a, int tiles, int first,
-                                                               int splits, int chunk, float* ws) {
+__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
+    AttnArgs a, int tiles, int first, int splits, int chunk, float* ws) {
   using S = typename Elem<T>::S;
   // WM waves on rows of their own, WK on a part of every tile's keys each.
-  constexpr int NW = 4, WK = NW / WM, U = 2 / WK, kRows = WM * 32;
+  constexpr int NW = attn_waves(WM), WK = NW / WM, U = 2 / WK, kRows = WM * 32;
   constexpr int kLoads = D / (8 * NW);
   __shared__ AttnStage<D> st0, st1;
   __shared__ float qs[NW][D];

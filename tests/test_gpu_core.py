@@ -255,6 +255,36 @@ def test_attention_documents(dim, dtype, causal):
         packed(lens, lens, 6, 3, dim, dtype, True, prefix=[1, 0, 30, 64, 100, 0, 0, 5], softcap=20.0)
 
 
+@pytest.mark.parametrize("softcap,slope", [(0.0, False), (30.0, False), (0.0, True), (5.0, True)])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, F16), (72, F16)])
+def test_attention_wide_tiles(dim, dtype, softcap, slope):
+    """256 rows a workgroup: its last tile partly, one key and keys past a tile, prompts of all lengths."""
+    rows = lambda n, nq, nk, heads, kv, causal: imq.attention_plan(
+        *(torch.empty((n, a, b, dim), dtype=dtype, device="cuda") for a, b in ((nq, heads), (nk, kv), (nk, kv))),
+        causal=causal)["tile_rows"]
+    kw = dict(softcap=softcap, slope=slope)
+    if rows(1, 1100, 65, 32, 32, False) == rows(10, 1031, 1100, 16, 4, True) == 256:  # as on 256 CUs
+        run_batch(1100, 65, 32, 32, dim, dtype, **kw)
+        run_batch(1026, 1, 32, 32, dim, dtype, **kw)
+        run_batch(1031, 1100, 16, 4, dim, dtype, causal=True, qn=[1031, 1, 0, 1030, 65, 700, 1031, 257, 64, 1031],
+                  kn=[1100, 9, 70, 3, 1030, 700, 1031, 257, 64, 0], **kw)
+    else:
+        pytest.skip("this card's plan takes other tiles")
+
+
+def test_attention_wide_tiles_hidden_keys():
+    """NaN and infinities behind a sequence's keys and behind the diagonal, 256 rows a workgroup."""
+    g = gen(18)
+    q, k, v = (randn(g, 10, 1040, h, 128, dtype=BF16) for h in (16, 4, 4))
+    kn = [1040 - 9 * s for s in range(10)]
+    for s, b in enumerate(kn):
+        k[s, b:], v[s, b - 3:, 1], v[s, b:, 2] = float("nan"), float("inf"), float("nan")
+    got = imq.attention(q, k, v, causal=True, k_lens=torch.tensor(kn, dtype=torch.int32, device="cuda"))
+    for s, b in enumerate(kn):  # the queries that see none of the last three keys
+        want, bound = attention_sequence(q[s, :1037], k[s, :b - 3], v[s, :b - 3], scale=128 ** -0.5, causal=True)
+        check(got[s, :1037], want, bound, f"sequence {s}")
+
+
 def test_attention_views_of_a_projection_and_of_a_cache():
     """q, k, v as columns of one product, the output a column block, the cache [n, kv, rows, dim]."""
     g = gen(12)
