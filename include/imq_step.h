@@ -20,8 +20,9 @@
  * created with (zeros).  Their output is therefore NOT the model's: they
  * time and check the quantized-linear work of a step at its real shapes.
  * A caller that runs the real model drives the block halves further down
- * (imq_dit_double_attn_in ... imq_dit_head_out) with its own attention core
- * and LayerNorm modulation between them; run and denoise are exactly those
+ * (imq_dit_double_attn_in ... imq_dit_head_out) with the attention core and
+ * the LayerNorm modulation between them (imq_ln_mod, imq_rope and
+ * imq_attention of imq_core.h, or its own); run and denoise are exactly those
  * halves with the stand-ins (same kernels, same bits).
  *
  * Data flow per double block (img rows = the l_img rows after the l_txt text

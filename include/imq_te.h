@@ -7,8 +7,8 @@
  * encodes RMSNorm, q/k/v qmm, the per-head norms, RoPE and masked attention,
  * o_proj qmm, dq_add, RMSNorm, gate and up qmm, dq_silu_mul, down qmm and
  * dq_add: 7 qmm and 5 glue dispatches.  Here a layer is two calls around the
- * attention core (per-head norms, RoPE, attention: not quantized-linear work,
- * left to the caller):
+ * attention core (per-head norms, RoPE, attention: imq_rope and imq_attention
+ * of imq_core.h, or the caller's own):
  *
  *   imq_te_attn_in:       h1 = RMSNorm(x); qkv = h1 . [Wq; Wk; Wv]^T      (2 launches)
  *   imq_te_attn_out_mlp:  r = T(x + T(attn_o . Wo^T))                     (fused dq_add)
