@@ -5,7 +5,7 @@
 // reference's dd_ln_mod_prescale (Sources/ImarelloDirect/DirectDiTKernels.swift:16-59),
 // a row picking its modulation s by an index.  Bound by HBM: x is read once into
 // registers, y written once; the modulations stay in the caches.  4608 x 3072
-// fp32 to f16: 16.3 us (5.2 TB/s, a 1 GiB copy reaches 5.18; a kernel that reads
+// fp32 to f16: 15.8 us (5.4 TB/s, part of it cached; a 1 GiB copy reaches 5.18; a kernel that reads
 // x three times 31.5); 1536 rows 8.0.
 #include "core_kernels.hpp"
 #include "imq_device.hpp"
@@ -31,7 +31,7 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
 // squares would cancel where a row's mean is large against its spread.
 template <int TX, int TY>
 __global__ __launch_bounds__(kThreads) void ln_mod_kernel(
-    const typename Elem<TX>::S* __restrict__ x, const float* __restrict__ shift,
+    const typename Elem<TX>::S* x, const float* __restrict__ shift,
     const float* __restrict__ scale, const int32_t* __restrict__ sets, int n_sets,
     typename Elem<TY>::S* y, int cols, float eps, float post) {
   __shared__ float part[2][kThreads / 64];
@@ -70,10 +70,10 @@ __device__ __forceinline__ float4 load4(const typename Elem<T>::S* p) {
 
 // cols % 4 == 0: the row is read once and kept in registers, V float4 a lane,
 // kWaves waves a row (1: four rows a workgroup, no barrier; 4: one row, whose
-// loads are in flight together, where there are too few rows to fill the CUs).
+// loads are in flight together).
 template <int TX, int TY, int kWaves, int V>
 __global__ __launch_bounds__(kThreads) void ln_mod_vec_kernel(
-    const typename Elem<TX>::S* __restrict__ x, const float* __restrict__ shift,
+    const typename Elem<TX>::S* x, const float* __restrict__ shift,
     const float* __restrict__ scale, const int32_t* __restrict__ sets, int n_sets,
     typename Elem<TY>::S* y, int rows, int cols, float eps, float post) {
   __shared__ float part[2][kThreads / 64];
@@ -138,11 +138,11 @@ hipError_t launch_t(const void* x, const float* shift, const float* scale, const
 #define IMQ_LN_VEC(W, V)                                                                         \
   hipLaunchKernelGGL((ln_mod_vec_kernel<TX, TY, W, V>), dim3(W == 4 ? rows : (rows + 3) / 4), \
                      block, 0, stream, xx, shift, scale, sets, n_sets, yy, rows, cols, eps, post)
-  if (vec && rows >= 2048 && cols <= 5120) {
-    if (cols <= 1024) IMQ_LN_VEC(1, 4);
-    else if (cols <= 2048) IMQ_LN_VEC(1, 8);
-    else if (cols <= 3072) IMQ_LN_VEC(1, 12);
-    else IMQ_LN_VEC(1, 20);
+  // A wave a row for many short rows: 16384 x 512 12.6 us against 18.1, x 1024 22.8 /
+  // 24.2, 4096 x 1024 6.9 / 7.2; but x 1280 26.8 / 27.5 and x 2048 43.0 / 37.7, 4608 x 3072
+  // 21.6 / 19.6, 2048 x 1024 5.2 / 4.8 (in a captured graph over 500 MB of rows).
+  if (vec && rows >= 4096 && cols <= 1024) {
+    IMQ_LN_VEC(1, 4);
   } else if (vec && cols <= 8192) {
     if (cols <= 1024) IMQ_LN_VEC(4, 1);
     else if (cols <= 2048) IMQ_LN_VEC(4, 2);
@@ -162,7 +162,19 @@ hipError_t launch_t(const void* x, const float* shift, const float* scale, const
 hipError_t launch_ln_mod(const void* x, int x_dtype, const float* shift, const float* scale,
                          const int32_t* sets, int n_sets, void* y, int y_dtype, int rows, int cols,
                          float eps, float post, hipStream_t stream) {
+  constexpr int kMost = 1 << 23;  // rows of a launch: its threads stay under 2^32
   if (rows <= 0) return hipSuccess;
+  if (rows > kMost) {
+    for (int64_t r = 0; r < rows; r += kMost) {
+      const size_t at = (size_t)r * cols;
+      const hipError_t e = launch_ln_mod(
+          static_cast<const char*>(x) + at * (x_dtype == kF32 ? 4 : 2), x_dtype, shift, scale,
+          sets ? sets + r : nullptr, n_sets, static_cast<char*>(y) + at * 2, y_dtype,
+          (int)(rows - r < kMost ? rows - r : kMost), cols, eps, post, stream);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
 #define IMQ_LN_MOD(TX, TY) \
   return launch_t<TX, TY>(x, shift, scale, sets, n_sets, y, rows, cols, eps, post, stream)
   if (x_dtype == kF32 && y_dtype == kBf16) IMQ_LN_MOD(kF32, kBf16);

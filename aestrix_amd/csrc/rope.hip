@@ -152,8 +152,8 @@ constexpr int kBatch = 3;  // head groups a wave holds at once: their loads are 
 // a pair per thread, and every lane keeps the cos and sin of its 8 pairs in
 // registers over all heads: the angle in fp64 and its sine are some 60
 // instructions, against 16 elements of a head.  kRows rows a workgroup: 4, a
-// wave each, where there are 1024 rows or more (a row's heads then share one
-// set of angles); 1, its heads over the four waves, where there are few.
+// wave each (a row's heads then share one set of angles), where there are many;
+// 1, its heads over the four waves, where there are few.
 template <int T, bool kInterleaved, int kRows>
 __global__ __launch_bounds__(kThreads) void rope_vec_kernel(RopeArgs a, int lanes_log2) {
   using S = typename Elem<T>::S;
@@ -277,7 +277,10 @@ hipError_t launch_t(const RopeArgs& a, bool interleaved, hipStream_t stream) {
   if (vec_fits(a, Elem<T>::kBytes)) {
     int log2 = 0;
     while ((16 << log2) < a.dim) ++log2;
-    const bool many = a.rows >= 1024;
+    // Many rows against a row's width: 4096 rows of 5 heads of 128 6.3 us against
+    // 11.2, 2048 of 20 8.1 / 9.7, 3072 of 48 15.3 / 15.9; but 1024 of 48 9.8 / 7.7,
+    // 2048 of 48 12.5 / 11.9, 2048 of 32 of 256 16.7 / 14.3; 16384 rows level.
+    const bool many = 5 * (int64_t)a.rows >= 2 * heads * a.dim;
     const dim3 grid((unsigned)(many ? (a.rows + 3) / 4 : a.rows));
     if (interleaved && many)
       hipLaunchKernelGGL((rope_vec_kernel<T, true, 4>), grid, block, 0, stream, a, log2);
@@ -300,6 +303,22 @@ hipError_t launch_t(const RopeArgs& a, bool interleaved, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_rope(const RopeArgs& a, bool interleaved, int dtype, hipStream_t stream) {
+  constexpr int kMost = 1 << 23;  // rows of a launch: its threads stay under 2^32
+  if (a.rows > kMost) {
+    const int64_t es = dtype == kF32 ? 4 : 2;
+    for (int64_t r = 0; r < a.rows; r += kMost) {
+      RopeArgs part = a;
+      part.rows = (int)(a.rows - r < kMost ? a.rows - r : kMost);
+      if (a.positions) part.positions = a.positions + r * a.axes;
+      for (int i = 0; i < a.groups; ++i) {
+        part.g[i].x = static_cast<const char*>(a.g[i].x) + r * a.g[i].x_row * es;
+        part.g[i].y = static_cast<char*>(a.g[i].y) + r * a.g[i].y_row * es;
+      }
+      const hipError_t e = launch_rope(part, interleaved, dtype, stream);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   switch (dtype) {
     case kBf16: return launch_t<kBf16>(a, interleaved, stream);
     case kF16: return launch_t<kF16>(a, interleaved, stream);

@@ -34,7 +34,8 @@ def randn(g, *shape, dtype=F32):
 @pytest.mark.parametrize("rows,cols,sets,xt,yt", [
     (1, 64, 0, F32, F16), (3, 1, 0, F32, BF16), (5, 333, 2, F32, F16), (17, 2560, 0, BF16, BF16),
     (9, 3072, 3, F32, BF16), (300, 1000, 4, F16, F16), (1, 8192, 1, F32, F16), (1025, 264, 5, F32, F16),
-    (33, 5120, 2, F32, F16), (7, 20000, 2, F32, BF16), (2050, 2052, 2, BF16, BF16)])
+    (33, 5120, 2, F32, F16), (7, 20000, 2, F32, BF16), (2050, 2052, 2, BF16, BF16),
+    (4101, 1000, 3, F32, F16), (4096, 516, 2, BF16, BF16)])
 def test_ln_mod(rows, cols, sets, xt, yt):
     g = gen(rows + cols)
     n = max(sets, 1)
@@ -58,6 +59,34 @@ def test_ln_mod_means_and_constant_rows():
     got = imq.ln_mod(x, shift, scale, eps=1e-6, out_dtype=BF16)
     want, bound = ln_mod(x, shift, scale, None, 1e-6, 1.0, BF16)
     check(got, want, bound, "ln_mod odd rows")
+
+
+@pytest.mark.parametrize("cols", [4, 3])
+def test_ln_mod_of_more_rows_than_a_launch(cols):
+    rows = (1 << 24) + 7
+    g = gen(cols)
+    x, sh, sc = randn(g, rows, cols, dtype=F16), randn(g, 2, cols), randn(g, 2, cols)
+    sets = (torch.arange(rows, device="cuda") % 3 == 0).int()
+    got = imq.ln_mod(x, sh, sc, sets=sets)
+    for a in (0, (1 << 23) - 64, (1 << 24) - 64, rows - 64):
+        b = min(a + 128, rows)
+        want, bound = ln_mod(x[a:b], sh, sc, sets[a:b], 1e-6, 1.0, F16)
+        check(got[a:b], want, bound, f"rows from {a}")
+
+
+@pytest.mark.parametrize("dim", [16, 6])
+def test_rope_of_more_rows_than_a_launch(dim):
+    rows = (1 << 23) + 77
+    g = gen(dim)
+    x, k = randn(g, rows, 1, dim, dtype=BF16), randn(g, rows, 2, dim, dtype=BF16)
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda") % 100003
+    f, _ = imq.rope_frequencies(dim, device="cuda")
+    out = imq.rope(x, k, positions=pos, inv_freq=f)
+    for t, got in zip((x, k), out):
+        for a in (0, (1 << 23) - 64, rows - 64):
+            b = min(a + 128, rows)
+            want, bound = rope(t[a:b], pos[a:b], f, None, False, 1.0, None, 1e-6)
+            check(got[a:b], want, bound, f"rows from {a}")
 
 
 def test_ln_mod_in_place_and_clamped_sets():
