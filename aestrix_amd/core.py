@@ -48,6 +48,12 @@ def _side(t: torch.Tensor | None, idx: int, dtype: torch.dtype, shape: tuple, wh
     return t.data_ptr()
 
 
+def _int32(n: int, what: str) -> int:
+    if not 0 <= n < 1 << 31:
+        raise ValueError(f"{n} {what}: fewer than 2^31 are taken")
+    return n
+
+
 def _packed(fields: struct.Struct, *values) -> bytes:
     """values as a C struct."""
     try:
@@ -73,8 +79,8 @@ def ln_mod(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else \
             torch.float16 if x.dtype == torch.float32 else x.dtype
-    n = 1 if shift.dim() == 1 else shift.shape[0]
-    side = (cols,) if shift.dim() == 1 else (n, cols)
+    n = shift.shape[0] if shift.dim() == 2 else 1
+    side = (n, cols) if shift.dim() == 2 else (cols,)
     psh = _side(shift, idx, torch.float32, side, "shift")
     psc = _side(scale, idx, torch.float32, side, "scale")
     pse = _side(sets, idx, _i32, shape[:-1], "sets")
@@ -85,8 +91,9 @@ def ln_mod(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
         raise ValueError("out must be a contiguous tensor of out_dtype shaped like x")
     ctx = context(idx)
     rc = run_on(idx, _lib.load().imq_ln_mod, ctx, x.data_ptr(), _DTYPES.get(x.dtype, -1), psh, psc,
-                pse, n, out.data_ptr(), _DTYPES.get(out_dtype, -1), x.numel() // cols if cols else 0,
-                cols, eps, post_scale, raw_stream(idx))
+                pse, n, out.data_ptr(), _DTYPES.get(out_dtype, -1),
+                _int32(x.numel() // cols if cols else 0, "rows"), _int32(cols, "columns"), eps,
+                post_scale, raw_stream(idx))
     if rc:
         _lib.check(rc, ctx)
     return out
@@ -175,6 +182,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Ten
     if q.dim() != 3:
         raise ValueError("q must be [rows, heads, dim]")
     rows, _, dim = q.shape
+    _int32(rows, "rows")
     dtype = q.dtype
     if not (inv_freq.dtype == torch.float64 and inv_freq.dim() == 1):
         raise ValueError("inv_freq must be a float64 [rot_dim / 2] tensor")
@@ -282,7 +290,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
     """softmax(scores) v with heads sharing key heads in whole groups, bf16 or f16.
 
     Scores are scale * q . k (scale: 1 / sqrt(dim) by default), then capped to
-    softcap * tanh(score / softcap) where softcap > 0, then lowered by slopes[head] times
+    softcap * tanh(score / softcap) where softcap > 0 (up to 4096), then lowered by slopes[head] times
     the distance.  The last query stands at the last key; ``causal`` hides later keys but
     for the first prefix_lens[s] of a sequence.  A query that sees nothing gives zeros.
 
@@ -292,7 +300,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
     * packed documents: q, k, v [rows, ...], document s in rows q_offsets[s] to
       q_offsets[s + 1] (int32 [n + 1]), max_q and max_k the longest one's rows.
 
-    Views with a contiguous last dim are taken as they are.  Rows of ``out`` that are no
+    Views with a contiguous last dim are taken as they are; ``out`` overlaps none of
+    q, k and v.  Rows of ``out`` that are no
     query's are left as they were (in a new tensor: undefined)."""
     idx, out, args = _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens,
                                      prefix_lens, q_offsets, k_offsets, max_q, max_k, out)

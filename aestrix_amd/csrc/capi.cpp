@@ -355,8 +355,10 @@ int imq_create(int device, imq_ctx** out) {
   auto* c = new (std::nothrow) imq_ctx;
   if (!c) return fail(nullptr, IMQ_ENOMEM, "imq_create: out of host memory");
   c->device = device;
-  if (hipDeviceGetAttribute(&c->cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess)
+  if (hipDeviceGetAttribute(&c->cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) {
+    (void)hipGetLastError();
     c->cus = 256;
+  }
   c->static_scratch = scratch;
   *out = c;
   return IMQ_OK;

@@ -49,6 +49,12 @@ int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, i
   if (!std::isfinite(p->softcap) || p->softcap < 0.f)
     return fail(ctx, IMQ_EINVAL, "%s: softcap %g must be finite and not negative", fn,
                 (double)p->softcap);
+  // A capped score is a difference of numbers of the cap's size.
+  if (p->softcap > 4096.f)
+    return fail(ctx, IMQ_EUNSUPPORTED, "%s: softcap %g (up to 4096)", fn, (double)p->softcap);
+  if (!std::isfinite((p->softcap > 0.f ? 2.f * p->scale / p->softcap : p->scale) * 1.5f))
+    return fail(ctx, IMQ_EINVAL, "%s: scale %g over softcap %g leaves fp32", fn, (double)p->scale,
+                (double)p->softcap);
   if (p->causal != 0 && p->causal != 1)
     return fail(ctx, IMQ_EINVAL, "%s: causal %d (0 or 1)", fn, p->causal);
   if (p->prefix_lens && !p->causal)
@@ -74,6 +80,8 @@ int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, i
     if (!p->q || !p->out || (p->max_k > 0 && (!p->k || !p->v)))
       return fail(ctx, IMQ_EINVAL, "%s: null device pointer (q=%p k=%p v=%p out=%p)", fn, p->q, p->k,
                   p->v, p->out);
+    if (p->out == p->q || (p->max_k > 0 && (p->out == p->k || p->out == p->v)))
+      return fail(ctx, IMQ_EINVAL, "%s: out is q, k or v", fn);
     if (!aligned(p->q, 2) || !aligned(p->k, 2) || !aligned(p->v, 2) || !aligned(p->out, 2))
       return fail(ctx, IMQ_EINVAL, "%s: q, k, v and out must be 2-byte aligned", fn);
   }

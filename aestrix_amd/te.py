@@ -124,6 +124,8 @@ class TextEncoderLayers:
         dims = [ctypes.c_int() for _ in range(4)]
         _lib.check(self._L.imq_te_dims(self._h, *[ctypes.byref(d) for d in dims]), self._ctx)
         self.hidden, self.nq, self.nkv, self.inter = (d.value for d in dims)
+        if self.nq % HEAD_DIM == 0 and self.nkv % HEAD_DIM == 0:
+            self.set_rope()  # here, so that a first attn_core may be captured
 
     def close(self) -> None:
         if self._h:
@@ -173,7 +175,8 @@ class TextEncoderLayers:
 
     def set_rope(self, head_dim: int = HEAD_DIM, base: float = ROPE_BASE, **scaling) -> None:
         """Head size and rotary frequencies of ``attn_core`` (``rope_frequencies``' scaling
-        for windows past the trained length); without a call, the Qwen3 encoder's."""
+        for windows past the trained length); without a call, the Qwen3 encoder's, where the
+        columns are heads of its size."""
         _require(head_dim > 0 and self.nq % head_dim == 0 and self.nkv % head_dim == 0,
                  f"q and k / v of {self.nq} and {self.nkv} columns are not heads of {head_dim}")
         self.head_dim = head_dim
@@ -192,8 +195,8 @@ class TextEncoderLayers:
         each window."""
         rows = self._rows(qkv, self.nq + 2 * self.nkv, "qkv")
         _require(prompts >= 1 and rows % prompts == 0, f"{rows} rows are not {prompts} windows")
-        if not hasattr(self, "freq"):
-            self.set_rope()
+        _require(hasattr(self, "freq"), f"q and k / v of {self.nq} and {self.nkv} columns are not "
+                 f"heads of {HEAD_DIM}: set_rope first")
         if positions is None:
             positions = torch.arange(rows // prompts, dtype=torch.int32, device=self.device)
             if prompts > 1:

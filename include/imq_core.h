@@ -89,7 +89,8 @@ int imq_rope(imq_ctx* ctx, const imq_rope_heads* groups, int n_groups, int rows,
  *   o[t][h][d] = T( sum_j softmax_j(e)_j v[j][h'][d] ) over the keys seen; 0 where none is.
  * The last query stands at the last key (p), so a few queries over a cache
  * and a whole prompt are the same call.  Keys that a query does not see do
- * not touch its output, whatever they hold (NaN and infinities included).
+ * not touch its output, whatever they hold (NaN and infinities included); an
+ * output that comes out not finite is made a second time, by the slower kernel.
  * T: bf16 or f16; scores, softmax and sums in fp32, the softmax's weights
  * rounded to T before the product with v (up to 32 rows in bf16 with the
  * remainders of that rounding multiplied too; by rows, not rounded).
@@ -117,7 +118,7 @@ typedef struct imq_attention_args {
     const void* q;
     const void* k;
     const void* v;
-    void* out; /* overlaps no input */
+    void* out; /* overlaps no input (out at q, k or v itself is refused) */
     int64_t q_seq, q_row, q_head; /* element strides: sequence, row, head; dims are contiguous */
     int64_t k_seq, k_row, k_head;
     int64_t v_seq, v_row, v_head;
@@ -132,7 +133,8 @@ typedef struct imq_attention_args {
     const int32_t* prefix_lens;   /* [n_seq], or NULL; only with causal */
     const float* slopes;          /* [heads], or NULL */
     float scale;                  /* finite, > 0 */
-    float softcap;                /* finite, >= 0; 0: none */
+    float softcap;                /* 0: none; else up to 4096: a capped score is right to some
+                                     2^-21 of it */
     int causal;
     int dtype;                    /* an imq_dtype */
 } imq_attention_args;

@@ -106,6 +106,12 @@ void attention_checks() {
   attention(IMQ_EINVAL, "5 heads of 2", [](A& a) { a.heads = 5, a.kv_heads = 2; });
   for (float bad : {0.f, -1.f, kNan, kInf, -kInf}) attention(IMQ_EINVAL, "scale", [&](A& a) { a.scale = bad; });
   for (float bad : {-1.f, kNan, kInf}) attention(IMQ_EINVAL, "softcap", [&](A& a) { a.softcap = bad; });
+  attention(IMQ_EHIP, "largest softcap", [](A& a) { a.softcap = 4096.f; });
+  for (float bad : {4097.f, 3e38f}) attention(IMQ_EUNSUPPORTED, "softcap", [&](A& a) { a.softcap = bad; });
+  attention(IMQ_EINVAL, "scale past fp32", [](A& a) { a.scale = 3e38f; });
+  attention(IMQ_EINVAL, "scale over softcap", [](A& a) { a.scale = 1e20f, a.softcap = 1e-20f; });
+  attention(IMQ_EINVAL, "out is q", [](A& a) { a.out = const_cast<void*>(a.q); });
+  attention(IMQ_EINVAL, "out is v", [](A& a) { a.q = mem + 1024, a.k = mem + 512, a.out = const_cast<void*>(a.v); });
   attention(IMQ_EINVAL, "prefix without causal", [&](A& a) { a.prefix_lens = i32; });
   attention(IMQ_EINVAL, "q_offsets and q_lens", [&](A& a) { a.q_offsets = a.q_lens = i32, a.q_rows = 4; });
   attention(IMQ_EINVAL, "k_offsets and k_lens", [&](A& a) { a.k_offsets = a.k_lens = i32, a.k_rows = 4; });

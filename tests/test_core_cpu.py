@@ -110,3 +110,11 @@ def test_host_tensors_are_refused():
         imq.rope(z, positions=pos, inv_freq=f)
     with pytest.raises(ValueError):
         imq.ln_mod(z, torch.zeros(64), torch.zeros(64))
+
+
+def test_rows_past_32_bits_are_refused():
+    """They would be passed on modulo 2^32."""
+    from aestrix_amd.core import _int32
+    assert _int32((1 << 31) - 1, "rows") == (1 << 31) - 1 and _int32(0, "rows") == 0
+    with pytest.raises(ValueError, match="2147483648 rows"):
+        _int32(1 << 31, "rows")

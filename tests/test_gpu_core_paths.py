@@ -147,6 +147,24 @@ def test_te_padding_leaves_prompts_alone():
     assert torch.equal(one[:63], two[:63])
 
 
+def test_te_first_core_in_a_graph():
+    """A layer's core captured before any eager call of it."""
+    plan = te(BF16)
+    qkv = randn(gen(15), 48, plan.nq + 2 * plan.nkv, dtype=BF16)
+    start, out = qkv.clone(), torch.zeros((48, plan.nq), dtype=BF16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.attn_core(0, qkv, 2, out=out)
+    qkv.copy_(start)
+    want = plan.attn_core(0, qkv, 2)
+    for _ in range(3):
+        qkv.copy_(start)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_te_without_head_norms_and_refusals():
     plan = te(BF16, norms=False)
     x = randn(gen(5), 6, plan.hidden, dtype=BF16)
@@ -444,6 +462,10 @@ def test_refusals():
               (q, k.half(), k.half()), (q.cpu(), k, k), (q, k.cpu(), k.cpu())):
         with pytest.raises(ValueError):
             imq.attention(*a)
+    with pytest.raises(ValueError, match="out is q"):
+        imq.attention(q, k, k, out=q)
+    with pytest.raises(NotImplementedError, match="softcap"):
+        imq.attention(q, k, k, softcap=1e4)
     p = q.flatten(0, 1), k.flatten(0, 1), k.flatten(0, 1)
     for kw in (dict(q_offsets=i32(0, 5, 10)), dict(q_offsets=i32(0, 5, 10), k_offsets=i32(0, 9, 18)),
                dict(q_offsets=i32(0, 5, 10), k_offsets=i32(0, 18), max_q=5, max_k=9),
@@ -479,7 +501,7 @@ def test_refusals():
                dict(sets=i32(*[0] * 6).long()), dict(out=z(6, 64, t=F32)[:, :32])):
         with pytest.raises(ValueError):
             imq.ln_mod(y, s, s, **kw)
-    for a in ((y, s[:32], s[:32]), (y, s, s.half()), (y, torch.stack([s, s]), torch.stack([s, s])), (y.T, s[:6], s[:6]),
+    for a in ((y, s[0], s[0]), (y, s[:32], s[:32]), (y, s, s.half()), (y, torch.stack([s, s]), torch.stack([s, s])), (y.T, s[:6], s[:6]),
               (y.cpu(), s, s)):
         with pytest.raises(ValueError):
             imq.ln_mod(*a)
