@@ -59,13 +59,13 @@ hipError_t launch_tiles(const AttnArgs& a, const AttnPlan& plan, float* ws, hipS
     if (plan.splits > 1) {
       hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, kSlope, true>),
                          dim3((unsigned)(blocks * plan.splits)), block, 0, stream, a, tiles,
-                         plan.first, plan.splits, plan.chunk, ws);
+                         plan.first, 1, plan.splits, plan.chunk, ws);
       launch_join<T, D, kCap, kSlope>(a, plan, kRows, tiles, blocks * kRows, ws, stream);
       return hipGetLastError();
     }
   }
   hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, kSlope, false>), dim3((unsigned)blocks),
-                     block, 0, stream, a, tiles, plan.first, 1, 0, nullptr);
+                     block, 0, stream, a, tiles, plan.first, plan.near_hs, 1, 0, nullptr);
   return hipGetLastError();
 }
 
@@ -124,7 +124,7 @@ bool tiles_fit(const AttnArgs& a) {
 }  // namespace
 
 AttnPlan attention_plan(const AttnArgs& a, int cus) {
-  const AttnPlan by_rows{IMQ_ATTENTION_ROWS, 1, 1, 0, 0, 0};
+  const AttnPlan by_rows{IMQ_ATTENTION_ROWS, 1, 1, 0, 0, 0, 0};
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
   const int64_t hs = (int64_t)a.n_seq * a.kv_heads;
   if (!tiles_fit(a) || rows > (1 << 30) || a.max_k > (1 << 30) || hs > (1 << 20) ||
@@ -166,6 +166,14 @@ AttnPlan attention_plan(const AttnArgs& a, int cus) {
     // (attn_tiles_kernel; four prompts of 512, 316, 121 and 437 rows, 32 / 8 heads:
     // 18.0 us against 19.4.)
     p.first = (int)(p.tile_rows < 256 && blocks <= 2 * cus && blocks > cus ? cus / hs : tiles);
+    // 32 sequences and key heads at a time, so that the L2s hold what is being read
+    // of K and V, where that gives 16 rounds of workgroups of one size: 128 prompts of 512
+    // rows, 32 / 8 heads, 530 us against 623, 64 x 1024 of 16 655 / 762, 32 x 1024 of 32 / 8
+    // 406 / 420, 256 x 512 of 12 of 64 305 / 430.  Otherwise all, tile by tile, so that the longest start first: 61 documents of
+    // up to 777 rows 82 us against 102, 16 x 4096 of 8 heads of 64 306 / 326.
+    const int64_t places = p.tile_rows == 256 ? cus : 2 * cus;
+    const bool even = !a.q_offsets && !a.q_lens && !a.k_offsets && !a.k_lens;
+    p.near_hs = (int)(even && blocks >= 16 * places ? std::min<int64_t>(hs, 32) : hs);
     unit = 4 * kAttnKeys;
     ranges = cus / blocks;
     // Two a CU from 4096 keys a range: 65 rows on 100000 keys 222 us against

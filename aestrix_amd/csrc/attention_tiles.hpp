@@ -298,7 +298,7 @@ constexpr int attn_waves(int wm) { return wm < 4 ? 4 : wm; }
 
 template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
 __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
-    AttnArgs a, int tiles, int first, int splits, int chunk, float* ws) {
+    AttnArgs a, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
   using S = typename Elem<T>::S;
   // WM waves on rows of their own, WK on a part of every tile's keys each.
   constexpr int NW = attn_waves(WM), WK = NW / WM, U = 2 / WK, kRows = WM * 32;
@@ -308,7 +308,11 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hs_n = a.n_seq * a.kv_heads;
-  const int hs = blockIdx.x % hs_n, rest = blockIdx.x / hs_n;
+  // near_hs sequences and key heads (all, where keys are split) at a time.
+  const int hs0 = kSplit ? 0 : blockIdx.x / (near_hs * tiles) * near_hs;
+  const int hs_now = kSplit ? hs_n : min(near_hs, hs_n - hs0);
+  const int at = blockIdx.x - hs0 * tiles;
+  const int hs = hs0 + at % hs_now, rest = at / hs_now;
   const int split = kSplit ? rest % splits : 0;
   // The last rows of a causal sequence have the most keys: they start first.
   // Where every workgroup is resident from the start, two a CU, those behind

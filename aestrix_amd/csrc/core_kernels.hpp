@@ -49,6 +49,7 @@ struct AttnPlan {
   int tile_rows;  // query rows (queries x heads a key head) of a workgroup
   int splits;     // key ranges
   int first;      // ranks of tiles that go from the last rows back (attn_tiles_kernel)
+  int near_hs;    // sequences and key heads taken at a time (attn_tiles_kernel)
   int chunk;      // keys of a range, whole key tiles
   size_t bytes;   // workspace of the partial sums (0: not split)
 };

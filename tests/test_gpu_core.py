@@ -183,9 +183,9 @@ def sequences(q, k, qn, kn):
 
 
 def run_batch(nq, nk, heads, kv, dim, dtype, *, causal=False, softcap=0.0, slope=False, qn=None,
-              kn=None, prefix=None, seed=0, scale=None):
+              kn=None, prefix=None, seed=0, scale=None, n=None):
     g = gen(seed + nq + 3 * nk + dim)
-    n = len(kn) if kn else len(qn) if qn else 1
+    n = len(kn) if kn else len(qn) if qn else n or 1
     q = randn(g, n, nq, heads, dim, dtype=dtype)
     k, v = randn(g, n, nk, kv, dim, dtype=dtype), randn(g, n, nk, kv, dim, dtype=dtype)
     slopes = torch.exp2(-8.0 * torch.arange(1, heads + 1, device="cuda") / heads).float() if slope else None
@@ -299,6 +299,13 @@ def test_attention_wide_tiles(dim, dtype, softcap, slope):
                   kn=[1100, 9, 70, 3, 1030, 700, 1031, 257, 64, 0], **kw)
     else:
         pytest.skip("this card's plan takes other tiles")
+
+
+@pytest.mark.parametrize("n,nq,nk,heads,kv,causal", [(150, 1000, 40, 7, 7, False), (45, 4000, 33, 6, 6, False),
+                                                     (301, 150, 150, 24, 8, True)])
+def test_attention_many_sequences(n, nq, nk, heads, kv, causal):
+    """So many tiles that a few sequences' and key heads' run at a time, the last few fewer."""
+    run_batch(nq, nk, heads, kv, 64, BF16, causal=causal, seed=n, n=n)
 
 
 def test_attention_wide_tiles_hidden_keys():
