@@ -85,6 +85,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
   load(vbase, vb, v_off, vl, max(min(first, end - 1), 0));
   __builtin_amdgcn_sched_barrier(0);
   const AttnScore<kCap, kSlope> score(a, head);
+  const f32x16_t c0 = attn_start(score);
   const int p = t + s.nk - s.nq;
   // Keys below `near` are at or before every row's p, or hidden behind it.
   const int near = a.causal && !a.prefix_lens ? INT_MAX : s.nk - s.nq + 1;
@@ -106,13 +107,13 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
     IMQ_WAIT_VMCNT(kLoads);
     __builtin_amdgcn_sched_barrier(0);
     f32x16_t sc[1];
-    sc[0] = attn_qk<T, D>(kl, qf, c, h);
+    sc[0] = attn_qk<T, D>(kl, qf, c, h, c0);
     __builtin_amdgcn_sched_barrier(0);
     IMQ_WAIT_LGKM_0();  // K has been read
     if constexpr (kMore) load(kbase, kb, k_off, kl, j0 + kStep);
     __builtin_amdgcn_sched_barrier(0);
     s16x8_t pf[kRest ? 4 : 2];
-    float shift;
+    float shift[1];
     attn_top<D>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
                                              j0 + kFewKeys <= near, shift), o, top, sum);
     attn_weights<T, 1, kCap, kSlope, kRest>(score, sc, shift, top, sum, pf);

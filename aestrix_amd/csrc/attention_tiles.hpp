@@ -89,38 +89,59 @@ __device__ __forceinline__ int v_piece(int row, int piece) {
   return D == 128 ? piece ^ (4 * (row & 3)) : piece ^ (4 * ((row >> 1) & 1));
 }
 
-// The scores of 32 U keys (S^T accumulators) capped, lowered and masked; their
-// row's largest, in units of log2.  j0: the first key; seen: the keys this
-// lane's row sees; seen_lo: the fewest that any row of the wave sees; away0:
+// What S^T accumulators of 32 keys start from.  A slope's fall is linear in the
+// key before p: what it gives the keys of a tile apart from their first one is put
+// there, divided by the factor that the scores take later, so that it costs nothing
+// a score.  (A capped score is capped before it falls.)
+template <bool kCap, bool kSlope>
+__device__ __forceinline__ f32x16_t attn_start(const AttnScore<kCap, kSlope>& score) {
+  f32x16_t c0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    c0[e] = kSlope && !kCap ? score.fall / score.mul * (float)(8 * (e / 4) + e % 4) : 0.f;
+  return c0;
+}
+
+// The scores of 32 U keys (S^T accumulators, from attn_start) capped, lowered and
+// masked; their row's largest, in units of log2.  j0: the first key; seen: the keys
+// this lane's row sees; seen_lo: the fewest that any row of the wave sees; away0:
 // p - j0 of the row.  What is left in sc is such that a key's exponent is
-// sc * score.mul without cap and slope; with a cap alone, top - 2 top sc, as sc
-// is the 1 / (exp(2 z) + 1) of the tanh (the exponent is one fma from it, made
-// with the subtraction of the maximum); with a slope, sc + shift.
-// A slope's fall is linear in the key before p: one fma a score, and the part
-// that all keys of the tile share goes into shift.  Tiles that reach past p
-// (none where causal hides those keys) take the distance itself.
+// sc * score.mul without a cap; with a cap alone, top - 2 top sc, as sc is the
+// 1 / (exp(2 z) + 1) of the tanh (the exponent is one fma from it, made with the
+// subtraction of the maximum); with cap and slope, sc; and with a slope, + shift[u],
+// the part that 32 keys share.  Tiles that reach past p (none where causal hides
+// those keys) take the distance itself.
 template <int U, bool kCap, bool kSlope>
 __device__ __forceinline__ float attn_scores(const AttnScore<kCap, kSlope>& score,
                                              f32x16_t (&sc)[U], int j0, int h, int seen,
-                                             int seen_lo, int away0, bool linear, float& shift) {
-  shift = 0.f;
+                                             int seen_lo, int away0, bool linear,
+                                             float (&shift)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) shift[u] = 0.f;
   if constexpr (kSlope) {
     const float away = (float)(away0 - 4 * h);
     if (linear) {
-      shift = -score.fall * away;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        shift[u] = -score.fall * (away - (float)(u * 32));
+        if constexpr (kCap)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = kCap ? score.capped(sc[u][e]) : sc[u][e] * score.mul;
-          sc[u][e] = __builtin_fmaf(score.fall, (float)(u * 32 + 8 * (e / 4) + e % 4), x);
-        }
+          for (int e = 0; e < 16; ++e)
+            sc[u][e] = __builtin_fmaf(score.fall, (float)(8 * (e / 4) + e % 4), score.capped(sc[u][e]));
+      }
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          sc[u][e] = score(sc[u][e], away - (float)(u * 32 + 8 * (e / 4) + e % 4));
+        for (int e = 0; e < 16; ++e) {
+          const float key = (float)(8 * (e / 4) + e % 4), from = away - (float)(u * 32) - key;
+          if constexpr (kCap) {
+            sc[u][e] = score(sc[u][e], from);
+          } else {
+            const float x = __builtin_fmaf(-score.fall, key, sc[u][e] * score.mul);
+            sc[u][e] = __builtin_fmaf(-score.fall, __builtin_fabsf(from), x) * (1.f / score.mul);
+          }
+        }
     }
   } else if constexpr (kCap) {
 #pragma unroll
@@ -137,14 +158,18 @@ __device__ __forceinline__ float attn_scores(const AttnScore<kCap, kSlope>& scor
       for (int e = 0; e < 16; ++e)
         sc[u][e] = u * 32 + 8 * (e / 4) + e % 4 < lim ? sc[u][e] : kRest ? INFINITY : -INFINITY;
   }
-  float mx = sc[0][0];
+  float mx;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int u = 0; u < U; ++u) {
+    float m = sc[u][0];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) mx = kRest ? fminf(mx, sc[u][e]) : fmaxf(mx, sc[u][e]);
+    for (int e = 1; e < 16; ++e) m = kRest ? fminf(m, sc[u][e]) : fmaxf(m, sc[u][e]);
+    // mul is positive.
+    if constexpr (kSlope) m = kCap ? m + shift[u] : __builtin_fmaf(m, score.mul, shift[u]);
+    mx = u == 0 ? m : kRest ? fminf(mx, m) : fmaxf(mx, m);
+  }
   if constexpr (kRest) mx = __builtin_fmaf(-2.f * score.top, mx, score.top);
-  else if constexpr (kSlope) mx += shift;
-  else mx *= score.mul;  // a positive factor
+  else if constexpr (!kSlope) mx *= score.mul;
   return pair_max(mx);
 }
 
@@ -190,14 +215,14 @@ __device__ __forceinline__ float attn_add2(uint32_t w, float x) {
 // as fragments of their own, for a second product with V.
 template <int T, int U, bool kCap, bool kSlope, bool kRest = false>
 __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& score,
-                                             const f32x16_t (&sc)[U], float shift, float top,
-                                             float& sum, s16x8_t (&pf)[2 * U * (kRest ? 2 : 1)]) {
+                                             const f32x16_t (&sc)[U], const float (&shift)[U],
+                                             float top, float& sum, s16x8_t (&pf)[2 * U * (kRest ? 2 : 1)]) {
   // The exponent as one fma of what attn_scores left.
-  const float by = kSlope ? 1.f : kCap ? -2.f * score.top : score.mul;
-  const float base = (top == -INFINITY ? 0.f : top) - (kSlope ? shift : kCap ? score.top : 0.f);
+  const float by = !kCap ? score.mul : kSlope ? 1.f : -2.f * score.top;
   float add[2] = {sum, 0.f};
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int u = 0; u < U; ++u) {
+    const float base = (top == -INFINITY ? 0.f : top) - (kSlope ? shift[u] : kCap ? score.top : 0.f);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       uint32_t w[4], rest[4];
@@ -218,17 +243,16 @@ __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& scor
       if constexpr (kRest)
         pf[2 * U + u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(rest[0], rest[1], rest[2], rest[3]));
     }
+  }
   sum = add[0] + add[1];
 }
 
-// S^T of 32 keys: K rows from LDS (row c of the 32 at `lds`), Q^T from registers.
+// S^T of 32 keys, added to c0: K rows from LDS (row c of the 32 at `lds`), Q^T from registers.
 template <int T, int D>
 __device__ __forceinline__ f32x16_t attn_qk(const uint4* lds, const s16x8_t (&qf)[D / 16], int c,
-                                            int h) {
+                                            int h, const f32x16_t& c0) {
   const int kf = D == 128 ? (c & 15) : ((c >> 1) & 7);  // k_piece's
-  f32x16_t sc;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+  f32x16_t sc = c0;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
     sc = attn_mfma<T>(__builtin_bit_cast(s16x8_t, lds[c * (D / 8) + ((2 * i + h) ^ kf)]), qf[i], sc);
@@ -364,6 +388,7 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
   s16x8_t qf[D / 16];
   attn_load_q<T, D>(a, s, t, head, h, qf);
   const AttnScore<kCap, kSlope> score(a, head);
+  const f32x16_t c0 = attn_start(score);
   const int p = t + s.nk - s.nq;
   // Keys below `near` are at or before every row's p, or hidden behind it.
   const int near = a.causal && !a.prefix_lens ? INT_MAX : min(mw, rows - 1) / group + s.nk - s.nq + 1;
@@ -387,7 +412,7 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     const uint4* k = st.k + wk * U * 32 * (D / 8);
     f32x16_t sc[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) sc[u] = attn_qk<T, D>(k + u * 32 * (D / 8), qf, c, h);
+    for (int u = 0; u < U; ++u) sc[u] = attn_qk<T, D>(k + u * 32 * (D / 8), qf, c, h, c0);
     issue(to, j1);
     // K of eight MFMAs is read ahead: one read an MFMA, as the compiler has
     // it, leaves most of an LDS read's 100 to 200 cycles exposed.
@@ -404,7 +429,7 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
       __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
     }
     s16x8_t pf[2 * U];
-    float shift;
+    float shift[U];
     attn_top<D>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
                                              j0 + 32 * U <= near, shift), o, top, sum);
     attn_weights<T, U, kCap, kSlope>(score, sc, shift, top, sum, pf);
