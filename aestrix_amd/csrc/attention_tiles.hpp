@@ -299,6 +299,37 @@ __device__ __forceinline__ void attn_load_q(const AttnArgs& a, const AttnSeq& s,
   }
 }
 
+// A row's 64-bit offset from the lane that holds it.
+__device__ __forceinline__ int64_t lane_offset(int64_t v, int from) {
+  const uint32_t lo = __shfl((uint32_t)v, from, 64), hi = __shfl((uint32_t)(v >> 32), from, 64);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// The wave's 32 rows between memory and a row a lane, through 32 rows of LDS of its
+// own: memory sees whole rows, D / 8 lanes of 16 bytes each, where a row a lane
+// touches 32 lines an instruction.  16 prompts of 512 rows, 32 / 8 heads, 69 us against
+// 82 (with neither loads of Q nor stores, 43), 8 x 250 rows on 64 keys 13.4 / 14.9; not with
+// 64 rows a workgroup, which are few and wait for LDS longer (4 x 120 on 64 keys
+// 8.0 / 7.5), nor for Q with 256, whose LDS would not hold it, and with heads of 64
+// elements, whose rows are a line each (level; the capped kernel would take 131
+// registers, 99 us for 97).  Pieces are swizzled as k_piece's, by the row.
+template <int D>
+struct AttnRows {
+  static constexpr int kLanes = D / 8, kRows = 64 / kLanes, kSteps = 32 / kRows;
+  uint4* lds;
+  int lane;
+  __device__ __forceinline__ int row(int k) const { return k * kRows + lane / kLanes; }
+  __device__ __forceinline__ int piece() const { return lane % kLanes; }
+  __device__ __forceinline__ uint4& at(int row, int piece) const {
+    return lds[row * kLanes + (piece ^ (row & (kLanes - 1)))];
+  }
+  // LDS of one wave is in order; this keeps the compiler to it.
+  __device__ __forceinline__ void fence() const {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
 template <int D>
 struct AttnStage {
   uint4 k[kAttnKeys * D / 8];
@@ -383,10 +414,29 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     attn_load<D, NW>(kbase + j0 * kb, kb, n, a.dim, k_off, st.k, wave);
     attn_load<D, NW>(vbase + j0 * vb, vb, n, a.dim, v_off, st.v, wave);
   };
-  if (begin < end) issue(st0, begin);
-
   s16x8_t qf[D / 16];
-  attn_load_q<T, D>(a, s, t, head, h, qf);
+  if constexpr (WM == 4 && D == 128) {
+    // st1 is free until the first tile is in use.
+    const AttnRows<D> part{st1.k + wave * (32 * D / 8), lane};
+    const S* q = static_cast<const S*>(a.q) + s.q_at;
+    const int64_t q_off = t * a.q_row + head * a.q_head;
+    uint4 v[AttnRows<D>::kSteps];
+#pragma unroll
+    for (int k = 0; k < AttnRows<D>::kSteps; ++k) {
+      const int64_t off = lane_offset(q_off, part.row(k));
+      v[k] = make_uint4(0, 0, 0, 0);
+      if (part.piece() * 8 < a.dim) v[k] = *reinterpret_cast<const uint4*>(q + off + part.piece() * 8);
+    }
+    if (begin < end) issue(st0, begin);
+#pragma unroll
+    for (int k = 0; k < AttnRows<D>::kSteps; ++k) part.at(part.row(k), part.piece()) = v[k];
+    part.fence();
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) qf[i] = __builtin_bit_cast(s16x8_t, part.at(c, 2 * i + h));
+  } else {
+    if (begin < end) issue(st0, begin);
+    attn_load_q<T, D>(a, s, t, head, h, qf);
+  }
   const AttnScore<kCap, kSlope> score(a, head);
   const f32x16_t c0 = attn_start(score);
   const int p = t + s.nk - s.nq;
@@ -506,7 +556,6 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     }
   } else {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
     bool finite = true;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -515,16 +564,36 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
         o[i][e] *= inv;
         finite = finite && __builtin_fabsf(o[i][e]) < INFINITY;
       }
-    if (mw + c < rows)
+    S* out = static_cast<S*>(a.out) + s.out_at;
+    const int64_t out_off = t * a.out_row + head * a.out_head;
+    auto packed = [&](int i, int e) {
+      return make_uint2(Elem<T>::pack2(o[i][e], o[i][e + 1]), Elem<T>::pack2(o[i][e + 2], o[i][e + 3]));
+    };
+    if constexpr (WK == 1) {
+      meet();  // through the LDS where the tiles were
+      const AttnRows<D> part{reinterpret_cast<uint4*>(wm < 4 ? &st0 : &st1) + wm % 4 * (32 * D / 8), lane};
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          reinterpret_cast<uint2*>(&part.at(c, i * 4 + e / 4))[h] = packed(i, e);
+      part.fence();
+#pragma unroll
+      for (int k = 0; k < AttnRows<D>::kSteps; ++k) {
+        const int64_t off = lane_offset(out_off, part.row(k));
+        const uint4 v = part.at(part.row(k), part.piece());
+        if (mw + part.row(k) < rows && part.piece() * 8 < a.dim)
+          *reinterpret_cast<uint4*>(out + off + part.piece() * 8) = v;
+      }
+    } else if (mw + c < rows) {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const int d = i * 32 + 2 * e + 4 * h;
-          if (d < a.dim)
-            *reinterpret_cast<uint2*>(out + d) = make_uint2(Elem<T>::pack2(o[i][e], o[i][e + 1]),
-                                                            Elem<T>::pack2(o[i][e + 2], o[i][e + 3]));
+          if (d < a.dim) *reinterpret_cast<uint2*>(out + out_off + d) = packed(i, e);
         }
+    }
     // A tile multiplies what it hides by zero, which a NaN or an infinity
     // outlives: such rows again, from the keys they see alone.
     uint64_t again = __builtin_amdgcn_ballot_w64(!finite && mw + c < rows);
