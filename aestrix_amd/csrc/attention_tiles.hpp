@@ -25,9 +25,9 @@
 // lane each), or one of eight has it, so that one wave of a SIMD multiplies while
 // the other weighs: a tile of 64 keys is 32 MFMAs
 // of 32 cycles a wave and some 130 VALU instructions, 32 of them exponentials
-// (8 cycles).  Measured, D = 128: 4608 x 4608 of 24 heads in f16 255-285 us
-// (870-970 TFLOP/s, the clock at 1.8 GHz; a large hipBLASLt product 1467), 16384 causal
-// rows of 32 / 8 heads in bf16 1.97 ms (1114), with slopes 2.08-2.11.  The matrix cores
+// (8 cycles).  Measured, D = 128: 4608 x 4608 of 24 heads in f16 252-285 us
+// (870-980 TFLOP/s, the clock at 1.8 GHz; a large hipBLASLt product 1467), 16384 causal
+// rows of 32 / 8 heads in bf16 1.97 ms (1114), with slopes 2.02-2.06.  The matrix cores
 // are busy for half of the cycles.  With parts left out, the last took 2.05 ms of four
 // waves a workgroup, 1.88 without the loads, 1.60 without the LDS reads, 1.65
 // without the weighing: LDS, written and read, is what the rest waits for.
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
   s16x8_t qf[D / 16];
   if constexpr (WM == 4 && D == 128) {
     // st1 is free until the first tile is in use.
-    const AttnRows<D> part{st1.k + wave * (32 * D / 8), lane};
+    const AttnRows<D> part{reinterpret_cast<uint4*>(&st1) + wave * (32 * D / 8), lane};
     const S* q = static_cast<const S*>(a.q) + s.q_at;
     const int64_t q_off = t * a.q_row + head * a.q_head;
     uint4 v[AttnRows<D>::kSteps];
