@@ -19,7 +19,7 @@
 // operand is read through the LDS transpose loads, 4 keys of 16 columns each.
 // 16-byte pieces of a row are swizzled (XOR with the row) at their source, so
 // the row-per-lane reads of K and the 4-row reads of V touch every bank evenly
-// (no conflicts counted).
+// (no conflicts counted; the outputs' way through LDS has some).
 //
 // Two workgroups of four waves share a CU (64 KB of LDS and up to 256 registers a
 // lane each), or one of eight has it, so that one wave of a SIMD multiplies while

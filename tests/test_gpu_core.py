@@ -301,6 +301,57 @@ def test_attention_wide_tiles(dim, dtype, softcap, slope):
         pytest.skip("this card's plan takes other tiles")
 
 
+def tile_rows(n, nq, nk, heads, kv, dim, dtype, causal):
+    p = imq.attention_plan(*(torch.empty((n, a, b, dim), dtype=dtype, device="cuda")
+                             for a, b in ((nq, heads), (nk, kv), (nk, kv))), causal=causal)
+    return p["tile_rows"], p["splits"]
+
+
+@pytest.mark.parametrize("softcap,slope", [(0.0, False), (30.0, False), (0.0, True), (5.0, True)])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (128, F16), (72, BF16), (64, F16)])
+def test_attention_128_row_tiles(dim, dtype, softcap, slope):
+    if tile_rows(7, 301, 333, 16, 4, dim, dtype, True) != (128, 1):  # as on 256 CUs
+        pytest.skip("this card's plan takes other tiles")
+    kw = dict(softcap=softcap, slope=slope)
+    qn, kn = [301, 0, 1, 300, 64, 129, 301], [333, 70, 9, 3, 64, 130, 0]
+    run_batch(301, 333, 16, 4, dim, dtype, causal=True, qn=qn, kn=kn, **kw)
+    run_batch(301, 333, 16, 4, dim, dtype, n=7, **kw)
+    run_batch(301, 333, 16, 4, dim, dtype, causal=True, kn=[333] * 7, prefix=[0, 1, 64, 100, 333, 31, 200], **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [128, 64])
+def test_attention_128_row_tiles_of_documents(dim, dtype):
+    lens = [301, 0, 70, 64, 200, 3, 0, 129, 301, 256, 130]
+    packed(lens, lens, 16, 4, dim, dtype, True, prefix=[0, 0, 30, 64, 100, 0, 0, 5, 301, 1, 2], softcap=20.0)
+    packed(lens, lens, 12, 4, dim, dtype, False)
+
+
+def test_attention_128_row_tiles_split():
+    if tile_rows(1, 1100, 12400, 16, 16, 128, BF16, False) != (128, 3):
+        pytest.skip("this card's plan takes other tiles")
+    run_batch(1100, 12400, 16, 16, 128, BF16)
+
+
+def test_attention_128_row_tiles_views_and_hidden_keys():
+    """Columns of a projection, an output between other columns, NaN and infinities behind the keys."""
+    g = gen(28)
+    qkv = randn(g, 7, 301, 24 * 128, dtype=F16)
+    q, k, v = (t.unflatten(2, (-1, 128)) for t in qkv.split([16 * 128, 4 * 128, 4 * 128], 2))
+    kn = [301, 290, 64, 65, 1, 0, 200]
+    for s, b in enumerate(kn):
+        k[s, b:], v[s, b:, 0], v[s, b:, 1] = float("nan"), float("inf"), float("nan")
+    wide = torch.full((7, 301, 18 * 128), 9.0, dtype=F16, device="cuda")
+    out = wide[..., 128:17 * 128].unflatten(2, (16, 128))
+    lens = torch.tensor(kn, dtype=torch.int32, device="cuda")
+    imq.attention(q, k, v, causal=True, q_lens=lens, k_lens=lens, out=out)
+    for s, b in enumerate(kn):
+        want, bound = attention_sequence(q[s, :b], k[s, :b], v[s, :b], scale=128 ** -0.5, causal=True)
+        check(out[s, :b], want, bound, f"sequence {s}")
+        assert bool((out[s, b:] == 9.0).all()), "rows behind the last query changed"
+    assert bool((wide[..., :128] == 9.0).all() and (wide[..., 17 * 128:] == 9.0).all())
+
+
 @pytest.mark.parametrize("n,nq,nk,heads,kv,causal", [(150, 1000, 40, 7, 7, False), (45, 4000, 33, 6, 6, False),
                                                      (301, 150, 150, 24, 8, True)])
 def test_attention_many_sequences(n, nq, nk, heads, kv, causal):
