@@ -23,11 +23,10 @@
 //
 // Two workgroups of four waves share a CU (64 KB of LDS and up to 256 registers a
 // lane each), or one of eight has it, so that one wave of a SIMD multiplies while
-// the other weighs: a tile of 64 keys is 32 MFMAs
-// of 32 cycles a wave and some 130 VALU instructions, 32 of them exponentials
-// (8 cycles).  Measured, D = 128: 4608 x 4608 of 24 heads in f16 252-285 us
+// the other weighs: a tile of 64 keys is 32 MFMAs of 32 cycles a wave and some 130
+// VALU instructions, 32 of them exponentials (8 cycles).  Measured, D = 128: 4608 x 4608 of 24 heads in f16 252-285 us
 // (870-980 TFLOP/s, the clock at 1.8 GHz; a large hipBLASLt product 1467), 16384 causal
-// rows of 32 / 8 heads in bf16 1.97 ms (1114), with slopes 2.02-2.06.  The matrix cores
+// rows of 32 / 8 heads in bf16 1.97 ms (1114), with slopes 2.02-2.09.  The matrix cores
 // are busy for half of the cycles.  With parts left out, the last took 2.05 ms of four
 // waves a workgroup, 1.88 without the loads, 1.60 without the LDS reads, 1.65
 // without the weighing: LDS, written and read, is what the rest waits for.
