@@ -13,6 +13,7 @@
 #include <mutex>
 #include <new>
 #include <string>
+#include <utility>
 
 #include "ctx.hpp"
 #include "imq.h"
@@ -23,9 +24,10 @@ imq_ctx::~imq_ctx() {
     if (staging_done[i]) (void)hipEventDestroy(staging_done[i]);
     if (staging[i]) (void)hipHostFree(staging[i]);
   }
-  for (auto& kv : split_ws)
-    if (kv.second.first) (void)hipFree(kv.second.first);
-  for (void* p : retired_ws) (void)hipFree(p);
+  for (auto& kv : split_ws) {
+    if (kv.second.p) (void)hipFree(kv.second.p);
+    for (void* p : kv.second.retired) (void)hipFree(p);
+  }
 }
 
 namespace imq {
@@ -118,29 +120,37 @@ int bind_device(imq_ctx* ctx) {
   return e == hipSuccess ? IMQ_OK : hip_fail(ctx, e, "hipSetDevice");
 }
 
-// The split-K workspace of stream st, at least `need` bytes; empty (run
-// unsplit) when it would have to grow during stream capture or the
-// allocation fails.  A workspace that is outgrown is retired, not freed: a
-// graph captured earlier on this stream still addresses it, and so may the
-// stream's queued work; retired buffers are freed with the context.
-SplitWs split_ws(imq_ctx* ctx, hipStream_t st, size_t need) {
+// Empty (run unsplit) when the workspace would have to grow during stream
+// capture or an allocation fails.  A workspace that is outgrown is retired, not
+// freed: a graph captured earlier on this stream still addresses it, and so may
+// the stream's queued work; retired buffers are freed with the context.
+SplitHold split_ws(imq_ctx* ctx, hipStream_t st, size_t need) {
   if (need == 0) return {};
-  std::lock_guard<std::mutex> lk(ctx->ws_mu);
-  auto& e = ctx->split_ws[st];
-  if (e.second >= need) return {static_cast<float*>(e.first), e.second};
-  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(st, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) {
-    (void)hipGetLastError();
+  try {
+    std::unique_lock<std::mutex> map_lock(ctx->ws_mu);
+    imq_ctx::StreamWs& w = ctx->split_ws[st];
+    map_lock.unlock();
+    std::unique_lock<std::mutex> lock(w.mu);
+    if (w.bytes < need) {
+      hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+      if (hipStreamIsCapturing(st, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) {
+        (void)hipGetLastError();
+        return {};
+      }
+      w.retired.reserve(w.retired.size() + 1);
+      void* p = nullptr;
+      if (hipMalloc(&p, need) != hipSuccess) {
+        (void)hipGetLastError();
+        return {};
+      }
+      if (w.p) w.retired.push_back(w.p);
+      w.p = p;
+      w.bytes = need;
+    }
+    return {SplitWs{static_cast<float*>(w.p), w.bytes}, std::move(lock)};
+  } catch (...) {  // host memory
     return {};
   }
-  void* p = nullptr;
-  if (hipMalloc(&p, need) != hipSuccess) {
-    (void)hipGetLastError();
-    return {};
-  }
-  if (e.first) ctx->retired_ws.push_back(e.first);
-  e = {p, need};
-  return {static_cast<float*>(p), need};
 }
 
 }  // namespace detail
@@ -242,12 +252,14 @@ int run_qmm(imq_ctx* ctx, const char* fn, Regime regime, const uint32_t* w, cons
   // The few-row kernel may split K over a workspace (long K, few row tiles);
   // past kDispatchSkinnyMaxM rows it runs only that way, and only with the
   // workspace in hand (otherwise the tile kernel takes the call).
+  SplitHold hold;  // to the end: the launches below
   imq::SplitWs sws{};
   bool skinny = false;
   if (few) {
     const size_t need = imq::qskinny_split_bytes(k, n, m);
     if (regime == Regime::kAuto) {
-      sws = split_ws(ctx, st, need);
+      hold = split_ws(ctx, st, need);
+      sws = hold.ws;
     } else if (regime == Regime::kAutoNoAlloc && need > 0) {
       // imq_qmm_t would split here; running unsplit (or on the tile kernel)
       // would change the bits, so a plan the static scratch cannot hold is
@@ -271,7 +283,9 @@ int run_qmm(imq_ctx* ctx, const char* fn, Regime regime, const uint32_t* w, cons
     // tile kernel (the fused output stages equal it bit for bit).
     imq::SplitWs ws{};
     if (regime == Regime::kAuto) {
-      ws = split_ws(ctx, st, imq::qgemm_split_bytes(k, n, m));
+      hold = {};  // (of few rows that do not run split: another size)
+      hold = split_ws(ctx, st, imq::qgemm_split_bytes(k, n, m));
+      ws = hold.ws;
     } else if (regime == Regime::kAutoNoAlloc) {
       const size_t need = imq::qgemm_split_bytes(k, n, m);
       if (need > imq::kStaticScratchBytes)

@@ -220,15 +220,15 @@ int imq_attention(imq_ctx* ctx, const imq_attention_args* args, imq_stream strea
   if ((rc = bind_device(ctx)) != IMQ_OK) return rc;
   const auto st = static_cast<hipStream_t>(stream);
   imq::AttnPlan plan = imq::attention_plan(a, ctx->cus);
-  float* ws = nullptr;
+  SplitHold hold;  // until the join is enqueued
   if (plan.bytes > 0) {
-    ws = split_ws(ctx, st, plan.bytes).p;
-    if (!ws) {  // it would have to grow under capture, or memory is short
+    hold = split_ws(ctx, st, plan.bytes);
+    if (!hold.ws.p) {  // it would have to grow under capture, or memory is short
       plan.splits = 1;
       plan.bytes = 0;
     }
   }
-  const hipError_t e = imq::launch_attention(a, plan, ws, args->dtype, st);
+  const hipError_t e = imq::launch_attention(a, plan, hold.ws.p, args->dtype, st);
   return e == hipSuccess ? IMQ_OK : hip_fail(ctx, e, fn);
 }
 

@@ -57,13 +57,20 @@ struct imq_ctx {
   hipEvent_t staging_done[kStagingBuffers] = {};
   int staging_next = 0;
   std::unique_ptr<imq::CopyPool> copy_pool;  // created with the staging buffers
-  // Split-K workspaces of the qGEMM, one per stream: calls on one stream run
-  // in order, so they never overlap on a workspace.  Grown (never shrunk) on
-  // demand outside stream capture; an outgrown one is kept until the context
-  // is destroyed (graphs captured earlier may still address it).
-  std::mutex ws_mu;
-  std::unordered_map<hipStream_t, std::pair<void*, size_t>> split_ws;
-  std::vector<void*> retired_ws;  // outgrown workspaces, freed with the context
+  // Split workspaces of imq_qmm_t and imq_attention, one per stream: kernels of
+  // one stream run in order, so a call's never overlap another's on a workspace
+  // as long as the call enqueues them one after the other, with `mu` held.
+  // Grown (never shrunk) on demand outside stream capture; an outgrown one is
+  // kept until the context is destroyed (graphs captured earlier may still
+  // address it).
+  struct StreamWs {
+    std::mutex mu;
+    void* p = nullptr;
+    size_t bytes = 0;
+    std::vector<void*> retired;
+  };
+  std::mutex ws_mu;  // of the map; entries stay where they are
+  std::unordered_map<hipStream_t, StreamWs> split_ws;
   // Device address of the library's static split-K scratch on this device
   // (imq_qmm_t_noalloc), looked up at imq_create.
   void* static_scratch = nullptr;
@@ -81,8 +88,16 @@ int hip_fail(imq_ctx* ctx, hipError_t e, const char* what);
 bool aligned(const void* p, size_t a);
 size_t elem_size(imq_dtype dtype);
 int bind_device(imq_ctx* ctx);
-// The split workspace of stream st, at least `need` bytes, or empty.
-SplitWs split_ws(imq_ctx* ctx, hipStream_t st, size_t need);
+// A stream's split workspace in use: no other call enqueues kernels on it while
+// this lives.  ws.p NULL: not to be had, and nothing held.
+struct SplitHold {
+  SplitWs ws;
+  std::unique_lock<std::mutex> lock;
+};
+// The split workspace of stream st, at least `need` bytes, or none.  Held until
+// the last kernel that uses it is enqueued: of two threads' calls on one stream,
+// the second's first kernel must not come before the first's join.
+SplitHold split_ws(imq_ctx* ctx, hipStream_t st, size_t need);
 
 }  // namespace detail
 }  // namespace imq
