@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
   constexpr int kPieces = kFewKeys * D / 8, kLoads = kPieces / 64;
   // bf16 weights carry 8 bits; what a rounding to them loses, up to 2^-9 of a
   // weight, is multiplied with V as well: the matrix cores have the time.  (f16
-  // weights lose 2^-12.)
+  // weights lose 2^-12, or 2^-36 of the row's largest where that is more.)
   constexpr bool kRest = T == kBf16;
   __shared__ uint4 kbuf[kFewWaves][kPieces];
   __shared__ uint4 vbuf[kFewWaves][kPieces];
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
     __builtin_amdgcn_sched_barrier(0);
     s16x8_t pf[kRest ? 4 : 2];
     float shift[1];
-    attn_top<D>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
+    attn_top<T, D>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
                                              j0 + kFewKeys <= near, shift), o, top, sum);
     attn_weights<T, 1, kCap, kSlope, kRest>(score, sc, shift, top, sum, pf);
     __builtin_amdgcn_sched_barrier(0);

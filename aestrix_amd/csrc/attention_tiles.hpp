@@ -172,12 +172,23 @@ __device__ __forceinline__ float attn_scores(const AttnScore<kCap, kSlope>& scor
   return pair_max(mx);
 }
 
+// How a weight is held until the sums are divided by the weights' own: exp2(score -
+// top) times 2^kAttnLift, while top is behind the row's largest score by up to
+// kAttnLag, so that the largest weight is between 2^kAttnLift and 2^(kAttnLift +
+// kAttnLag).  f16 keeps 11 bits down to 2^-14 only and nothing under 2^-25: weights
+// are lifted as far as it goes up (2^16), so that those down to 2^-25 of the row's
+// largest keep their bits and none above 2^-36 is lost; at 2^0 to 2^8, 6000 keys 2^-25
+// of the largest came to nothing.  bf16 has fp32's range.
+template <int T>
+constexpr float kAttnLag = T == kF16 ? 4.f : 8.f;
+template <int T>
+constexpr float kAttnLift = T == kF16 ? 11.f : 0.f;
+
 // Moves the running maximum on, and the sums with it: only where a row's has
-// grown by 2^8, until then weights are up to 2^8, which costs no precision in
-// either type.
-template <int D>
+// grown by kAttnLag.
+template <int T, int D>
 __device__ __forceinline__ void attn_top(float mx, f32x16_t (&o)[D / 32], float& top, float& sum) {
-  if (__builtin_amdgcn_ballot_w64(mx > top + 8.f)) {
+  if (__builtin_amdgcn_ballot_w64(mx > top + kAttnLag<T>)) {
     const float next = fmaxf(top, mx);
     const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
     top = next;
@@ -208,7 +219,7 @@ __device__ __forceinline__ float attn_add2(uint32_t w, float x) {
   else return dot2_bf16(w, 0x3F803F80u, x);
 }
 
-// Scores to weights, exp2(score - top): P^T fragments, and their sum.  The sum
+// Scores to weights, exp2(score - top + kAttnLift): P^T fragments, and their sum.  The sum
 // is that of the weights as rounded to T, which are what V is multiplied by;
 // two a dot2 instruction.  kRest: the weights' remainders after that rounding
 // as fragments of their own, for a second product with V.
@@ -221,7 +232,8 @@ __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& scor
   float add[2] = {sum, 0.f};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const float base = (top == -INFINITY ? 0.f : top) - (kSlope ? shift[u] : kCap ? score.top : 0.f);
+    const float base = (top == -INFINITY ? 0.f : top - kAttnLift<T>) -
+                       (kSlope ? shift[u] : kCap ? score.top : 0.f);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       uint32_t w[4], rest[4];
@@ -479,7 +491,7 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     }
     s16x8_t pf[2 * U];
     float shift[U];
-    attn_top<D>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
+    attn_top<T, D>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
                                              j0 + 32 * U <= near, shift), o, top, sum);
     attn_weights<T, U, kCap, kSlope>(score, sc, shift, top, sum, pf);
     attn_pv<T, D, 2 * U>(st.v + wk * U * 32 * (D / 8), pf, o, lane);
