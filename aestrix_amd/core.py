@@ -291,7 +291,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
 
     Scores are scale * q . k (scale: 1 / sqrt(dim) by default), then capped to
     softcap * tanh(score / softcap) where softcap > 0 (up to 4096), then lowered by slopes[head] times
-    the distance.  The last query stands at the last key; ``causal`` hides later keys but
+    the distance (float32 [heads], up to 2^20 in size; scale then from 2^-64 on).  The last query stands at the last key; ``causal`` hides later keys but
     for the first prefix_lens[s] of a sequence.  A query that sees nothing gives zeros.
 
     * one sequence: q [rows, heads, dim], k and v [keys, kv_heads, dim];

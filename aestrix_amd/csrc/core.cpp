@@ -55,6 +55,10 @@ int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, i
   if (!std::isfinite((p->softcap > 0.f ? 2.f * p->scale / p->softcap : p->scale) * 1.5f))
     return fail(ctx, IMQ_EINVAL, "%s: scale %g over softcap %g leaves fp32", fn, (double)p->scale,
                 (double)p->softcap);
+  // Within a tile, what a slope takes is divided by the scale (attn_start, attn_scores):
+  // 2^20 a key over 2^30 keys, over 2^-64, stays in fp32.
+  if (p->slopes && p->softcap == 0.f && p->scale < 0x1p-64f)
+    return fail(ctx, IMQ_EUNSUPPORTED, "%s: scale %g with slopes (2^-64 and above)", fn, (double)p->scale);
   if (p->causal != 0 && p->causal != 1)
     return fail(ctx, IMQ_EINVAL, "%s: causal %d (0 or 1)", fn, p->causal);
   if (p->prefix_lens && !p->causal)

@@ -131,8 +131,8 @@ typedef struct imq_attention_args {
     const int32_t* q_lens;
     const int32_t* k_lens;
     const int32_t* prefix_lens;   /* [n_seq], or NULL; only with causal */
-    const float* slopes;          /* [heads], or NULL */
-    float scale;                  /* finite, > 0 */
+    const float* slopes;          /* [heads], or NULL; finite, up to 2^20 in size */
+    float scale;                  /* finite, > 0; with slopes and no cap from 2^-64 on */
     float softcap;                /* 0: none; else up to 4096: a capped score is right to some
                                      2^-21 of it */
     int causal;
