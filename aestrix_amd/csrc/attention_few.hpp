@@ -27,8 +27,8 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
                                                                     int splits, int chunk, float* ws) {
   using S = typename Elem<T>::S;
   constexpr int kPieces = kFewKeys * D / 8, kLoads = kPieces / 64;
-  // bf16 weights carry 8 bits; what a rounding to them loses, up to 2^-9 of a
-  // weight, is multiplied with V as well: the matrix cores have the time.  (f16
+  // bf16 weights carry 8 bits, and a second bf16 of each what that leaves, up to 2^-7
+  // of it, multiplied with V as well: the matrix cores have the time.  (f16
   // weights lose 2^-12, or 2^-36 of the row's largest where that is more.)
   constexpr bool kRest = T == kBf16;
   __shared__ uint4 kbuf[kFewWaves][kPieces];
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
     __builtin_amdgcn_sched_barrier(0);
     s16x8_t pf[kRest ? 4 : 2];
     float shift[1];
-    attn_top<T, D>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
+    attn_top<T>(attn_scores<1, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
                                              j0 + kFewKeys <= near, shift), o, top, sum);
     attn_weights<T, 1, kCap, kSlope, kRest>(score, sc, shift, top, sum, pf);
     __builtin_amdgcn_sched_barrier(0);
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
       const float big = fmaxf(fmaxf(__builtin_fabsf(acc.x), __builtin_fabsf(acc.y)),
                               fmaxf(__builtin_fabsf(acc.z), __builtin_fabsf(acc.w)));
       const bool nan = acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w;
-      if (nan || big == INFINITY) atomicOr(&bad, 1u << r);
+      if ((nan || big == INFINITY) && sums == sums) atomicOr(&bad, 1u << r);
       S* out = static_cast<S*>(a.out) + s.out_at + (r / group) * a.out_row +
                (kh * group + r % group) * a.out_head;
       if (d < a.dim)
@@ -187,14 +187,14 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
     }
   }
   if constexpr (!kSplit) {
-    // Rows that are not finite again, from the keys they see alone (attn_tiles_kernel).
     __syncthreads();
     float* qs = reinterpret_cast<float*>(kbuf[wave]);
+    const int odd = bad ? attn_spoilt<T>(a, s, kh, seen_lo, seen_hi + kFewKeys) : -1;
     for (unsigned again = bad; again; again &= again - 1) {
       const int r = __builtin_ctz(again);
-      if (r % kFewWaves != wave) continue;
-      const int tr = r / group;
-      attn_row<T, kCap, kSlope>(a, s, kh * group + r % group, tr, attn_seen(a, s, tr), qs);
+      const int tr = r / group, of = attn_seen(a, s, tr);
+      if (r % kFewWaves != wave || of > odd) continue;
+      attn_row<T, kCap, kSlope>(a, s, kh * group + r % group, tr, of, qs);
     }
   }
 }

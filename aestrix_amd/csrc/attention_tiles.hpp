@@ -35,8 +35,6 @@
 // a workgroup where a CU gets more than one, V and K lines read ahead into L2.
 #pragma once
 
-#include <climits>
-
 #include "attention.hpp"
 
 namespace imq {
@@ -186,15 +184,15 @@ constexpr float kAttnLift = T == kF16 ? 11.f : 0.f;
 
 // Moves the running maximum on, and the sums with it: only where a row's has
 // grown by kAttnLag.
-template <int T, int D>
-__device__ __forceinline__ void attn_top(float mx, f32x16_t (&o)[D / 32], float& top, float& sum) {
+template <int T, int N>
+__device__ __forceinline__ void attn_top(float mx, f32x16_t (&o)[N], float& top, float& sum) {
   if (__builtin_amdgcn_ballot_w64(mx > top + kAttnLag<T>)) {
     const float next = fmaxf(top, mx);
     const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
     top = next;
     sum *= keep;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[i][e] *= keep;
   }
@@ -221,8 +219,10 @@ __device__ __forceinline__ float attn_add2(uint32_t w, float x) {
 
 // Scores to weights, exp2(score - top + kAttnLift): P^T fragments, and their sum.  The sum
 // is that of the weights as rounded to T, which are what V is multiplied by;
-// two a dot2 instruction.  kRest: the weights' remainders after that rounding
-// as fragments of their own, for a second product with V.
+// two a dot2 instruction.  kRest: a weight as two bf16, the second as fragments of
+// its own, for a second product with V: its upper half, and what is left, with 2^-18 of
+// all of them (which the division by the sum takes away) so that neither is zero where
+// the weight is not: an infinite value stays what it is.
 template <int T, int U, bool kCap, bool kSlope, bool kRest = false>
 __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& score,
                                              const f32x16_t (&sc)[U], const float (&shift)[U],
@@ -242,13 +242,16 @@ __device__ __forceinline__ void attn_weights(const AttnScore<kCap, kSlope>& scor
         const float x0 = sc[u][half * 8 + e], x1 = sc[u][half * 8 + e + 1];
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x0, by, -base));
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x1, by, -base));
-        w[e / 2] = attn_pack2<T>(p0, p1);
-        add[(e / 2) & 1] = attn_add2<T>(w[e / 2], add[(e / 2) & 1]);
         if constexpr (kRest) {
-          rest[e / 2] = attn_pack2<T>(p0 - Elem<T>::param((uint16_t)(w[e / 2] & 0xFFFFu)),
-                                      p1 - Elem<T>::param((uint16_t)(w[e / 2] >> 16)));
+          const uint32_t b0 = __float_as_uint(p0) & 0xFFFF0000u, b1 = __float_as_uint(p1) & 0xFFFF0000u;
+          w[e / 2] = b0 >> 16 | b1;
+          rest[e / 2] = attn_pack2<T>(__builtin_fmaf(p0, 1.f + 0x1p-18f, -__uint_as_float(b0)),
+                                      __builtin_fmaf(p1, 1.f + 0x1p-18f, -__uint_as_float(b1)));
           add[(e / 2) & 1] = attn_add2<T>(rest[e / 2], add[(e / 2) & 1]);
+        } else {
+          w[e / 2] = attn_pack2<T>(p0, p1);
         }
+        add[(e / 2) & 1] = attn_add2<T>(w[e / 2], add[(e / 2) & 1]);
       }
       pf[u * 2 + half] = __builtin_bit_cast(s16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
       if constexpr (kRest)
@@ -491,7 +494,7 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     }
     s16x8_t pf[2 * U];
     float shift[U];
-    attn_top<T, D>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
+    attn_top<T>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
                                              j0 + 32 * U <= near, shift), o, top, sum);
     attn_weights<T, U, kCap, kSlope>(score, sc, shift, top, sum, pf);
     attn_pv<T, D, 2 * U>(st.v + wk * U * 32 * (D / 8), pf, o, lane);
@@ -605,9 +608,11 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
           if (d < a.dim) *reinterpret_cast<uint2*>(out + out_off + d) = packed(i, e);
         }
     }
-    // A tile multiplies what it hides by zero, which a NaN or an infinity
-    // outlives: such rows again, from the keys they see alone.
-    uint64_t again = __builtin_amdgcn_ballot_w64(!finite && mw + c < rows);
+    uint64_t again = __builtin_amdgcn_ballot_w64(!finite && sum == sum && mw + c < rows);
+    if (again) {
+      const int odd = attn_spoilt<T>(a, s, kh, seen_lo, seen_hi + kAttnKeys);
+      again = __builtin_amdgcn_ballot_w64(!finite && sum == sum && mw + c < rows && seen <= odd);
+    }
     again = (again | again >> 32) & 0xFFFFFFFFu;
     while (again) {
       const int r = __builtin_ctzll(again);
@@ -630,6 +635,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
   using S = typename Elem<T>::S;
   __shared__ float qs[4][D];
   __shared__ float sums[kParts > 1 ? 16 : 1][D + 2];
+  // Read with the first arguments, not each where it is used.
+  asm volatile("" ::"s"(ws), "s"(splits), "s"(chunk), "s"(tile_rows), "s"(a.out), "s"(a.causal),
+               "s"(a.max_q), "s"(a.max_k), "s"(a.out_row), "s"(a.out_head), "s"(a.prefix_lens));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slot = threadIdx.x / 16;
   const int64_t all = (int64_t)a.n_seq * a.kv_heads * tiles * tile_rows;
   const int64_t row = (int64_t)blockIdx.x * (16 / kParts) + slot / kParts;
@@ -711,31 +719,34 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
       }
     }
   }
-  bool finite = true;
+  bool again_row = false;
   if (live) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) {
       acc[e] *= inv;
-      finite = finite && __builtin_fabsf(acc[e]) < INFINITY;
+      again_row = again_row || !(__builtin_fabsf(acc[e]) < INFINITY);
     }
+    again_row = again_row && sum == sum;
 #pragma unroll
     for (int e = 0; e < D / 16; e += 4)
       if (d0 + e < a.dim)
         *reinterpret_cast<uint2*>(out + d0 + e) =
             make_uint2(Elem<T>::pack2(acc[e], acc[e + 1]), Elem<T>::pack2(acc[e + 2], acc[e + 3]));
   }
-  // Rows that are not finite again, from the keys they see alone (attn_tiles_kernel).
-  uint64_t again = __builtin_amdgcn_ballot_w64(!finite);
+  uint64_t again = __builtin_amdgcn_ballot_w64(again_row);
+  if (again == 0) return;
+  const AttnArgs a1 = attn_args_again();
   while (again) {
     const int l = __builtin_ctzll(again) & ~15;
     again &= ~(0xFFFFull << l);
     const int mr = __builtin_amdgcn_readlane(m, l), hr = __builtin_amdgcn_readlane(hs, l);
-    const AttnSeq sr = attn_seq(a, hr / a.kv_heads);
-    const int tr = mr / group;
-    attn_row<T, kCap, kSlope>(a, sr, (hr % a.kv_heads) * group + mr % group, tr,
-                              attn_seen(a, sr, tr), qs[wave]);
+    const AttnSeq sr = attn_seq(a1, hr / a1.kv_heads);
+    const int tr = mr / group, seen = attn_seen(a1, sr, tr), khr = hr % a1.kv_heads;
+    const int last = min(mr / tile_rows * tile_rows + tile_rows, sr.nq * group) - 1;
+    if (seen <= attn_spoilt<T>(a1, sr, khr, seen, attn_seen(a1, sr, last / group) + kAttnKeys))
+      attn_row<T, kCap, kSlope>(a1, sr, khr * group + mr % group, tr, seen, qs[wave]);
   }
 }
 

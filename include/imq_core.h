@@ -89,11 +89,12 @@ int imq_rope(imq_ctx* ctx, const imq_rope_heads* groups, int n_groups, int rows,
  *   o[t][h][d] = T( sum_j softmax_j(e)_j v[j][h'][d] ) over the keys seen; 0 where none is.
  * The last query stands at the last key (p), so a few queries over a cache
  * and a whole prompt are the same call.  Keys that a query does not see do
- * not touch its output, whatever they hold (NaN and infinities included); an
- * output that comes out not finite is made a second time, by the slower kernel.
+ * not touch its output, whatever they hold (NaN and infinities included): an
+ * output that comes out not finite, with such a value in a key near those that
+ * its query sees, is made a second time, by the slower kernel.
  * T: bf16 or f16; scores, softmax and sums in fp32, the softmax's weights
- * rounded to T before the product with v (up to 32 rows in bf16 with the
- * remainders of that rounding multiplied too; by rows, not rounded).
+ * rounded to T before the product with v (up to 32 rows in bf16 as two bf16
+ * each; by rows, not rounded).
  *
  * A sequence's rows:
  *   q_offsets NULL: its queries are rows 0.. of q + s * q_seq (max_q rows are
