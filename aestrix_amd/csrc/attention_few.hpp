@@ -173,7 +173,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a,
       if (d == 0)
         *reinterpret_cast<float2*>(ws + (int64_t)splits * all * D + at * 2) = make_float2(tops, sums);
     } else {
-      const float inv = sums == 0.f ? 0.f : 1.f / sums;
+      const float inv = attn_seen(a, s, r / group) > 0 ? 1.f / sums : 0.f;
       acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
       const float big = fmaxf(fmaxf(__builtin_fabsf(acc.x), __builtin_fabsf(acc.y)),
                               fmaxf(__builtin_fabsf(acc.z), __builtin_fabsf(acc.w)));

@@ -569,7 +569,8 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
                                    ((int64_t)split * all + row) * 2) = make_float2(top, sum);
     }
   } else {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    // (Of keys whose scores are all -infinity the sum is zero too, and the output NaN.)
+    const float inv = seen > 0 ? 1.f / sum : 0.f;
     bool finite = true;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -721,7 +722,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
   }
   bool again_row = false;
   if (live) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = attn_seen(a, s, t) > 0 ? 1.f / sum : 0.f;
     S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) {

@@ -86,7 +86,8 @@ int imq_rope(imq_ctx* ctx, const imq_rope_heads* groups, int n_groups, int rows,
  *   e_j = softcap * tanh(e_j / softcap)                  (softcap > 0)
  *   e_j = e_j - slopes[h] * |p - j|,  p = t + n_k - n_q   (slopes not NULL)
  *   key j is seen where causal is 0, or j <= p, or j < prefix_lens[s]
- *   o[t][h][d] = T( sum_j softmax_j(e)_j v[j][h'][d] ) over the keys seen; 0 where none is.
+ *   o[t][h][d] = T( sum_j softmax_j(e)_j v[j][h'][d] ) over the keys seen; 0 where none is
+ *     (NaN where the seen ones' scores are all -infinity).
  * The last query stands at the last key (p), so a few queries over a cache
  * and a whole prompt are the same call.  Keys that a query does not see do
  * not touch its output, whatever they hold (NaN and infinities included): an

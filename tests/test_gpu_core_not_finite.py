@@ -107,6 +107,25 @@ def test_hidden_ones_beside_visible_ones(nq, nk, heads, kv, dim, causal, plan):
                         expected(q[nq - n:], k[:n], v[:n], head, True)]), head)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("nq,nk,heads,kv,dim,causal,plan", PLANS)
+def test_scores_of_minus_infinity(nq, nk, heads, kv, dim, causal, plan, dtype):
+    """A query whose scores are all -infinity has no softmax, whichever kernel it takes; one that sees
+    no key gives zeros, and keys of such a score beside others have no weight."""
+    q, k, v = inputs(nq, nk, heads, kv, dim, dtype)
+    plan_is(q, k, v, plan, causal=causal)
+    k[..., 0] = 1.0
+    q[nq // 2, 0, 0] = -INF
+    q[nq // 3, -1, 0] = 1.0
+    k[nk // 2, -1, 0] = -INF
+    got = imq.attention(q, k, v, causal=causal)
+    for head in (0, heads - 1):
+        same(got[:, head], expected(q, k, v, head, causal), head)
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = imq.attention(q[None], k[None], v[None], causal=causal, k_lens=none)
+    assert not got.any()
+
+
 def test_overlapping_rows_of_values():
     """Rows of values that begin inside the one before (a window over a sequence): what a tile
     reads behind the last is part of those in front."""
