@@ -138,14 +138,22 @@ SplitHold split_ws(imq_ctx* ctx, hipStream_t st, size_t need) {
         return {};
       }
       w.retired.reserve(w.retired.size() + 1);
+      // Powers of two: calls that need a little more each time (keys of a cache that
+      // fills) allocate a few times, and what is retired stays below what is in use.
+      size_t bytes = (size_t)1 << 20;
+      while (bytes < need) bytes *= 2;
       void* p = nullptr;
-      if (hipMalloc(&p, need) != hipSuccess) {
+      if (hipMalloc(&p, bytes) != hipSuccess) {
         (void)hipGetLastError();
-        return {};
+        bytes = need;
+        if (hipMalloc(&p, bytes) != hipSuccess) {
+          (void)hipGetLastError();
+          return {};
+        }
       }
       if (w.p) w.retired.push_back(w.p);
       w.p = p;
-      w.bytes = need;
+      w.bytes = bytes;
     }
     return {SplitWs{static_cast<float*>(w.p), w.bytes}, std::move(lock)};
   } catch (...) {  // host memory
