@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -120,6 +121,16 @@ int bind_device(imq_ctx* ctx) {
   return e == hipSuccess ? IMQ_OK : hip_fail(ctx, e, "hipSetDevice");
 }
 
+// What tells streams apart.  hipStreamPerThread is one handle for every thread's own
+// stream: a number of the thread's instead, which no later thread gets (its stream may
+// begin while an ended thread's still runs) and no stream's address is.
+hipStream_t stream_key(hipStream_t st) {
+  if (st != hipStreamPerThread) return st;
+  static std::atomic<uintptr_t> threads{0};
+  static thread_local const uintptr_t mine = ++threads;
+  return reinterpret_cast<hipStream_t>(mine << 3 | 5);
+}
+
 // Empty (run unsplit) when the workspace would have to grow during stream
 // capture or an allocation fails.  A workspace that is outgrown is retired, not
 // freed: a graph captured earlier on this stream still addresses it, and so may
@@ -128,7 +139,7 @@ SplitHold split_ws(imq_ctx* ctx, hipStream_t st, size_t need) {
   if (need == 0) return {};
   try {
     std::unique_lock<std::mutex> map_lock(ctx->ws_mu);
-    imq_ctx::StreamWs& w = ctx->split_ws[st];
+    imq_ctx::StreamWs& w = ctx->split_ws[stream_key(st)];
     map_lock.unlock();
     std::unique_lock<std::mutex> lock(w.mu);
     if (w.bytes < need) {

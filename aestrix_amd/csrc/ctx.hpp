@@ -70,7 +70,7 @@ struct imq_ctx {
     std::vector<void*> retired;
   };
   std::mutex ws_mu;  // of the map; entries stay where they are
-  std::unordered_map<hipStream_t, StreamWs> split_ws;
+  std::unordered_map<hipStream_t, StreamWs> split_ws;  // by stream_key
   // Device address of the library's static split-K scratch on this device
   // (imq_qmm_t_noalloc), looked up at imq_create.
   void* static_scratch = nullptr;

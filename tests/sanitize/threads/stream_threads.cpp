@@ -55,6 +55,8 @@ hipError_t two_kernels(hipStream_t st, const void* ws) {
   return hipSuccess;
 }
 
+std::map<const void*, std::thread::id> per_thread;  // of the workspaces of threads' own streams
+
 // Both streams' calls are between their kernels at once, or the wait gives up.
 std::atomic<int> meeting{0};
 std::atomic<bool> met{false};
@@ -100,6 +102,12 @@ hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, float* ws, 
     for (int i = 0; i < 20000 && meeting < 2; ++i)
       std::this_thread::sleep_for(std::chrono::microseconds(100));
     if (meeting >= 2) met = true;
+  }
+  if (st == hipStreamPerThread) {
+    std::lock_guard<std::mutex> lk(log_mu);
+    const auto at = per_thread.emplace(ws, std::this_thread::get_id()).first;
+    if (at->second != std::this_thread::get_id()) die("two threads' own streams use one workspace");
+    return hipSuccess;
   }
   return two_kernels(st, ws);
 }
@@ -175,6 +183,19 @@ void streams() {
   if (!met) die("streams wait for each other");
 }
 
+// hipStreamPerThread is one handle for as many streams as there are threads.
+void own_streams() {
+  imq_ctx ctx;
+  ctx.cus = 256;
+  for (int round = 0; round < 2; ++round) {  // a thread's memory may be another one's afterwards
+    std::thread a([&] { attention(&ctx, hipStreamPerThread, 100); attention(&ctx, hipStreamPerThread, 200); });
+    std::thread b([&] { attention(&ctx, hipStreamPerThread, 100); attention(&ctx, hipStreamPerThread, 200); });
+    a.join(), b.join();
+    attention(&ctx, hipStreamPerThread, 100);
+  }
+  if (per_thread.size() != 5) die("threads' own streams have other than a workspace each");
+}
+
 // Where nothing may be allocated, calls run unsplit and leave no lock behind:
 // few rows past 16 fall through to the tiles, which ask again.
 void captured() {
@@ -197,6 +218,7 @@ int main() {
   streams();
   owner.clear();
   captured();
+  own_streams();
   printf("stream_threads: %d calls, %d allocations\n", calls.load(), allocations.load());
   return 0;
 }
