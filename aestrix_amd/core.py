@@ -111,8 +111,10 @@ def rope_frequencies(rot_dim: int, base: float = 1e6, *, scaling: str | None = N
     * ``"ntk"``: base * factor^(rot_dim / (rot_dim - 2)), which divides the slowest
       frequency by factor and keeps the fastest;
     * ``"yarn"``: pairs that turn more than beta_fast times over original_len are kept,
-      those under beta_slow divided by factor, a linear ramp over the pair's index
-      between; amplitude 0.1 ln(factor) + 1 (Peng et al., YaRN, 2023)."""
+      those under beta_slow divided by factor, between them a line over the pair's index,
+      from the last pair that is kept (at least the first) to the first that is divided,
+      which may lie past the last of rot_dim; amplitude 0.1 ln(factor) + 1 (after Peng et
+      al., YaRN, 2023, whose formula has the line over the turns)."""
     _require(rot_dim >= 2 and rot_dim % 2 == 0, "rot_dim must be even and positive")
     _require(base > 1.0 and factor >= 1.0, "base must be above 1 and factor at least 1")
     amplitude = 1.0
@@ -130,9 +132,8 @@ def rope_frequencies(rot_dim: int, base: float = 1e6, *, scaling: str | None = N
         def pair_of(turns: float) -> float:
             return rot_dim * math.log(original_len / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
-        lo = max(math.floor(pair_of(beta_fast)), 0)
-        hi = min(math.ceil(pair_of(beta_slow)), rot_dim // 2 - 1)
-        slow = ((j - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+        lo, hi = max(math.floor(pair_of(beta_fast)), 0), math.ceil(pair_of(beta_slow))
+        slow = ((j - lo) / (hi - lo)).clamp(0.0, 1.0) if hi > lo else (j >= hi).double()
         f = f * (1.0 - slow) + f / factor * slow
         amplitude = 0.1 * math.log(factor) + 1.0
     elif scaling not in (None, "ntk"):
