@@ -29,6 +29,42 @@ int64_t reach(std::initializer_list<std::pair<int64_t, int64_t>> extents) {
   return at < ((__int128)1 << 60) ? (int64_t)at : -1;
 }
 
+// Whether two of the places that these extents and strides give, `dim` elements each,
+// lie on each other.  Strides that fit into each other do not, in any order; of others
+// every difference of two places is looked at, as far as 2^20 steps go (then: yes).
+bool on_each_other(int64_t dim, std::initializer_list<std::pair<int64_t, int64_t>> extents) {
+  std::pair<int64_t, int64_t> e[3];  // (extent, stride) of those that step, strides rising
+  int n = 0;
+  for (const auto& x : extents)
+    if (x.first > 1) e[n++] = x;
+  std::sort(e, e + n, [](const auto& a, const auto& b) { return a.second < b.second; });
+  __int128 span = dim;
+  bool nested = true;
+  for (int i = 0; i < n; ++i) {
+    nested = nested && e[i].second >= span;
+    span += (__int128)(e[i].first - 1) * e[i].second;
+  }
+  if (nested) return false;
+  // The longest is solved for, the others are stepped through (both signs of one do).
+  std::sort(e, e + n, [](const auto& a, const auto& b) { return a.first > b.first; });
+  const int64_t n1 = n > 1 ? e[1].first : 1, n2 = n > 2 ? e[2].first : 1, s0 = e[0].second;
+  if (s0 < dim || (__int128)(2 * n1 - 1) * n2 > (1 << 20)) return true;
+  for (int64_t c = 0; c < n2; ++c)
+    for (int64_t b = c == 0 ? 0 : 1 - n1; b < n1; ++b) {
+      __int128 at = 0;
+      if (n > 1) at += (__int128)b * e[1].second;
+      if (n > 2) at += (__int128)c * e[2].second;
+      // The two multiples of s0 next to `at`.
+      const __int128 low = at >= 0 ? at / s0 : -((-at + s0 - 1) / s0);
+      for (__int128 a = low; a <= low + 1; ++a) {
+        if (a >= e[0].first || a <= -e[0].first || (a == 0 && b == 0 && c == 0)) continue;
+        const __int128 away = at - a * s0;
+        if (away < dim && -away < dim) return true;
+      }
+    }
+  return false;
+}
+
 int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, imq::AttnArgs* a) {
   if (!ctx) return fail(nullptr, IMQ_EINVAL, "%s: null context", fn);
   if (!p) return fail(ctx, IMQ_EINVAL, "%s: null arguments", fn);
@@ -76,8 +112,11 @@ int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, i
       reach({{p->n_seq, os}, {qr, p->out_row}, {p->heads, p->out_head}}) < 0)
     return fail(ctx, IMQ_EINVAL, "%s: a negative stride, or a tensor past 2^60 elements", fn);
   // Outputs that lie on each other: two rows, heads or sequences at one place.
+  // (Lengths may keep sequences apart that reach into each other's windows.)
+  const int64_t apart = p->q_offsets || p->q_lens ? 1 : p->n_seq;
   if ((p->heads > 1 && p->out_head < p->dim) || (qr > 1 && p->out_row < p->dim) ||
-      (!p->q_offsets && p->n_seq > 1 && p->out_seq < p->dim))
+      (!p->q_offsets && p->n_seq > 1 && p->out_seq < p->dim) ||
+      on_each_other(p->dim, {{p->heads, p->out_head}, {qr, p->out_row}, {apart, os}}))
     return fail(ctx, IMQ_EINVAL, "%s: out's strides (%lld, %lld, %lld) lay outputs on each other", fn,
                 (long long)p->out_seq, (long long)p->out_row, (long long)p->out_head);
   if (p->n_seq > 0 && p->max_q > 0) {
@@ -192,7 +231,8 @@ int imq_rope(imq_ctx* ctx, const imq_rope_heads* groups, int n_groups, int rows,
         reach({{rows, g.y_row}, {g.heads, g.y_head}}) < 0)
       return fail(ctx, IMQ_EINVAL, "%s: group %d: a negative stride, or a tensor past 2^60 elements",
                   fn, i);
-    if ((g.heads > 1 && g.y_head < dim) || (rows > 1 && g.y_row < dim))
+    if ((g.heads > 1 && g.y_head < dim) || (rows > 1 && g.y_row < dim) ||
+        on_each_other(dim, {{g.heads, g.y_head}, {rows, g.y_row}}))
       return fail(ctx, IMQ_EINVAL, "%s: group %d: y's strides (%lld, %lld) lay outputs on each other",
                   fn, i, (long long)g.y_row, (long long)g.y_head);
     if (rows > 0 && g.heads > 0) {
