@@ -67,7 +67,7 @@ def ln_mod(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
            out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """T(((x - mean) * rsqrt(var + eps) * (1 + scale) + shift) * post_scale) over x's last dim.
 
-    x: contiguous float32 or T [..., cols]; shift, scale: float32 [cols] or [n, cols];
+    x: contiguous float32 or T [..., cols], up to 2^20 columns; shift, scale: float32 [cols] or [n, cols];
     sets: int32, x's leading shape: the modulation each row takes (text and image rows of
     a joint residual in one launch), row 0's where it is not given.  T: ``out_dtype``,
     float16 or bfloat16 (default: x's own type, or float16 for float32)."""

@@ -164,6 +164,8 @@ int imq_ln_mod(imq_ctx* ctx, const void* x, imq_dtype x_dtype, const float* shif
     return fail(ctx, IMQ_EUNSUPPORTED, "%s: x dtype %d (f32, or y's dtype)", fn, (int)x_dtype);
   if (rows < 0 || cols <= 0 || n_sets <= 0)
     return fail(ctx, IMQ_EINVAL, "%s: rows %d, cols %d, n_sets %d", fn, rows, cols, n_sets);
+  // The sums are 256 threads' in fp32: 2^12 terms each are right to 2^-12.
+  if (cols > 1 << 20) return fail(ctx, IMQ_EUNSUPPORTED, "%s: %d columns (up to 2^20)", fn, cols);
   if (!sets && n_sets != 1)
     return fail(ctx, IMQ_EINVAL, "%s: %d modulations without sets", fn, n_sets);
   if (!std::isfinite(eps) || eps < 0.f)

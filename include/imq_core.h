@@ -37,7 +37,7 @@ extern "C" {
  * [n_sets, cols]; sets: int32 [rows] (clamped to [0, n_sets)): the text and
  * image rows of a joint residual take their own modulation in one launch.
  * post: the 1/16 of the f16 sandwich (dd_ln_mod_prescale), or 1.
- * x and y contiguous [rows, cols]; rows 0 is a no-op; y may be x where both
+ * x and y contiguous [rows, cols], cols up to 2^20; rows 0 is a no-op; y may be x where both
  * have the same type. */
 int imq_ln_mod(imq_ctx* ctx, const void* x, imq_dtype x_dtype, const float* shift,
                const float* scale, const int32_t* sets, int n_sets, void* y, imq_dtype y_dtype,

@@ -145,6 +145,19 @@ void outputs_on_each_other() {
   });
 }
 
+// A thread of 256 adds up a 256th of a row, one after another.
+void long_rows() {
+  auto* f = reinterpret_cast<float*>(mem);
+  auto call = [&](int want, int cols, int rows) {
+    expect(imq_ln_mod(&ctx, mem, IMQ_F32, f, f, nullptr, 1, mem + 2048, IMQ_F16, rows, cols, 0.f, 1.f, nullptr), want,
+           "a long row");
+  };
+  for (int rows : {1, 3}) {
+    call(IMQ_EHIP, 1 << 20, rows);
+    for (int cols : {(1 << 20) + 1, 1 << 24, INT32_MAX - 255, INT32_MAX}) call(IMQ_EUNSUPPORTED, cols, rows);
+  }
+}
+
 }  // namespace
 
 int main() {
@@ -152,6 +165,7 @@ int main() {
   ctx.cus = 256;
   scales_with_slopes();
   outputs_on_each_other();
+  long_rows();
   printf("core_arguments: %d checks\n", checks);
   return 0;
 }
