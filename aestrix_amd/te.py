@@ -205,6 +205,12 @@ class TextEncoderLayers:
             out = new_out(qkv, (rows, self.nq)) if lens is None else \
                 torch.zeros((rows, self.nq), dtype=self.dtype, device=self.device)
         _require(self._rows(out, self.nq, "out") == rows, "out rows must match qkv")
+        # What attention would refuse, before q and k are turned in place.
+        _require(lens is None or (lens.dtype == torch.int32 and lens.shape == (prompts,) and
+                                  lens.is_contiguous() and lens.device == qkv.device),
+                 f"lens must be a contiguous int32 [{prompts}] tensor on {qkv.device}")
+        a, b = qkv.data_ptr(), out.data_ptr()
+        _require(b >= a + qkv.nbytes or a >= b + out.nbytes, "out lies in qkv")
         d, l = self.head_dim, self.layers[layer]
         q, k, v = (t.unflatten(-1, (-1, d)) for t in qkv.split([self.nq, self.nkv, self.nkv], -1))
         rope(q, k, positions=positions, inv_freq=self.freq, amplitude=self.amplitude,
