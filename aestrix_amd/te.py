@@ -106,6 +106,7 @@ class TextEncoderLayers:
         self.device = torch.device("cuda", device_index(device))
         self.dtype = layers[0].qkv.s.dtype
         self.max_rows = max_rows
+        self.eps = float(eps)
         self._L = _lib.load()
         self._ctx = context(self.device)
         arr = (TeLayerWeights * len(layers))()
@@ -118,7 +119,7 @@ class TextEncoderLayers:
             arr[i].norm_post = l.norm_post.data_ptr()
         out = ctypes.c_void_p()
         with torch.cuda.device(self.device):
-            _lib.check(self._L.imq_te_create(self._ctx, arr, len(layers), max_rows, float(eps),
+            _lib.check(self._L.imq_te_create(self._ctx, arr, len(layers), max_rows, self.eps,
                                              ctypes.byref(out)), self._ctx)
         self._h = out
         dims = [ctypes.c_int() for _ in range(4)]
@@ -186,7 +187,7 @@ class TextEncoderLayers:
                   lens: torch.Tensor | None = None, positions: torch.Tensor | None = None,
                   out: torch.Tensor | None = None) -> torch.Tensor:
         """``encodeLayer`` between the q/k/v and the o projection (DirectTEEncoder.swift:382-389):
-        per-head RMSNorm (where the layer has ``norm_q`` / ``norm_k``) and RoPE of q and k,
+        per-head RMSNorm (where the layer has ``norm_q`` / ``norm_k``; the encoder's eps) and RoPE of q and k,
         in place in ``qkv``, then causal attention; attn_o [rows, nq].
 
         rows = prompts * window, prompt after prompt; lens (int32 [prompts]): the prompts'
@@ -214,7 +215,7 @@ class TextEncoderLayers:
         d, l = self.head_dim, self.layers[layer]
         q, k, v = (t.unflatten(-1, (-1, d)) for t in qkv.split([self.nq, self.nkv, self.nkv], -1))
         rope(q, k, positions=positions, inv_freq=self.freq, amplitude=self.amplitude,
-             q_weight=l.norm_q, k_weight=l.norm_k, eps=EPS, q_out=q, k_out=k)
+             q_weight=l.norm_q, k_weight=l.norm_k, eps=self.eps, q_out=q, k_out=k)
         window = (prompts, rows // prompts)
         attention(q.unflatten(0, window), k.unflatten(0, window), v.unflatten(0, window),
                   causal=True, q_lens=lens, k_lens=lens,

@@ -1,11 +1,13 @@
-"""``TextEncoderLayers.attn_core``: what it refuses."""
+"""``TextEncoderLayers.attn_core``: what it refuses, and the epsilon it takes."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
+import aestrix_amd as imq
 from aestrix_amd.te import TextEncoderLayers, random_te_layers
+from core_reference import check, rope
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +45,16 @@ def test_a_refused_call_leaves_qkv_alone():
             plan.attn_core(0, qkv, 2, **kw)
         torch.cuda.synchronize()
         assert torch.equal(qkv, keep), kw.keys()
+
+
+@pytest.mark.parametrize("eps", [1e-6, 0.5])
+def test_the_head_norms_take_the_encoders_epsilon(eps):
+    plan = encoder(eps=eps)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    qkv = torch.randn(20, plan.nq + 2 * plan.nkv, generator=g, device="cuda").to(BF16)
+    keep = qkv.clone()
+    plan.attn_core(0, qkv)
+    f, _ = imq.rope_frequencies(128, 1e6, device="cuda")
+    pos = torch.arange(20, dtype=torch.int32, device="cuda")
+    want, bound = rope(keep[:, :plan.nq].unflatten(1, (-1, 128)), pos, f, None, False, 1.0, plan.layers[0].norm_q, eps)
+    check(qkv[:, :plan.nq].unflatten(1, (-1, 128)), want, bound, f"q, epsilon {eps}")
