@@ -112,6 +112,11 @@ class DitModel:
         s, d, x = self.step, self.step.dims, self.x
         _require(e.dtype == torch.float32 and tuple(e.shape) == (d.l_txt, d.dim) and
                  e.device == x.device, f"e must be float32 [{d.l_txt}, {d.dim}] on {x.device}")
+        for name, t in vars(mod).items():  # another number of rows would go to the wrong ones
+            both = name.startswith(("attn", "mlp"))
+            _require(t.dtype == torch.float32 and t.device == x.device and
+                     (t.shape == (2, d.dim) if both else t.shape in ((d.dim,), (1, d.dim))),
+                     f"{name} must be float32 {'[2, ' if both else '['}{d.dim}] on {x.device}")
         if out is None:
             out = torch.empty_like(lat)
         x[:d.l_txt].copy_(e)
