@@ -19,9 +19,6 @@
 
 namespace imq {
 
-constexpr int kFewWaves = 4;
-constexpr int kFewKeys = 32;  // keys of a wave's tile
-
 template <int T, int D, bool kCap, bool kSlope, bool kSplit>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_few_kernel(AttnArgs a, int tile_rows,
                                                                     int splits, int chunk, float* ws) {

@@ -43,8 +43,6 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 
-constexpr int kAttnKeys = 64;  // keys of a tile
-
 template <int T>
 __device__ __forceinline__ f32x16_t attn_mfma(s16x8_t a, s16x8_t b, f32x16_t c) {
   if constexpr (T == kBf16)

@@ -44,6 +44,10 @@ struct AttnArgs {
   float scale, softcap;
 };
 
+constexpr int kAttnKeys = 64;  // keys of a tile (attn_tiles_kernel)
+constexpr int kFewWaves = 4;   // waves of a workgroup (attn_few_kernel) ...
+constexpr int kFewKeys = 32;   // ... and keys of a wave's tile
+
 struct AttnPlan {
   int kernel;     // an imq_attention_kernel
   int tile_rows;  // query rows (queries x heads a key head) of a workgroup
