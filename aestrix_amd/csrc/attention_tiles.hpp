@@ -174,11 +174,12 @@ __device__ __forceinline__ float attn_scores(const AttnScore<kCap, kSlope>& scor
 // kAttnLag).  f16 keeps 11 bits down to 2^-14 only and nothing under 2^-25: weights
 // are lifted as far as it goes up (2^16), so that those down to 2^-25 of the row's
 // largest keep their bits and none above 2^-36 is lost; at 2^0 to 2^8, 6000 keys 2^-25
-// of the largest came to nothing.  bf16 has fp32's range.
+// of the largest came to nothing.  bf16 has fp32's range: weights of 1 and less keep
+// the products with its largest values in fp32, as far as the sums go.
 template <int T>
 constexpr float kAttnLag = T == kF16 ? 4.f : 8.f;
 template <int T>
-constexpr float kAttnLift = T == kF16 ? 11.f : 0.f;
+constexpr float kAttnLift = T == kF16 ? 11.f : -8.f;
 
 // Moves the running maximum on, and the sums with it: only where a row's has
 // grown by kAttnLag.

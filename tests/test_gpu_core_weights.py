@@ -95,3 +95,26 @@ def test_one_key_outweighs_the_others(nq, nk, heads, kv, dim, causal, plan, at, 
     kv_of = [i * kv // heads for i in some]
     want, bound = exact(q[:, some], k[:, kv_of], v[:, kv_of], dim ** -0.5, causal, softcap, slopes)
     check(got[:, some], want, bound, f"{nq} x {nk}")
+
+
+@pytest.mark.parametrize("softcap", [0.0, 60.0])
+@pytest.mark.parametrize("nq,heads,kv,dim,causal,at,plan", [
+    (3, 600, 300, 64, False, 200, ("few", 6, False)), (1, 300, 300, 128, True, 200, ("few", 1, False)),
+    (40, 2, 2, 128, False, 100, ("tiles", 64, False)), (100, 200, 200, 128, False, 100, ("tiles", 128, False)),
+    (1100, 32, 32, 64, False, 100, ("tiles", 256, False)), (20, 3, 1, 33, False, 100, ("rows", 1, False))])
+def test_large_values(nq, heads, kv, dim, causal, at, plan, softcap):
+    """bf16 values of 2^121, of 250 keys of which one, behind a first tile of 32 or 64, weighs 2^7 times
+    the others: their sums with weights of 1 and less stay under 2^128, with weights of 2^7 they do not."""
+    q, k = torch.zeros(nq, heads, dim, device="cuda"), torch.zeros(250, kv, dim, device="cuda")
+    q[..., 0] = 16.0
+    k[at, :, 0] = 4.9 * dim ** 0.5 / 16.0
+    v = torch.full((250, kv, dim), 2.0 ** 121, device="cuda")
+    q, k, v = q.to(BF16), k.to(BF16), v.to(BF16)
+    kw = dict(causal=causal, softcap=softcap)
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:
+        p = imq.attention_plan(q, k, v, **kw)
+        assert (p["kernel"], p["tile_rows"], p["splits"] > 1) == plan, p
+    got = imq.attention(q, k, v, **kw)
+    want, bound = exact(q[:, :1], k[:, :1], v[:, :1], dim ** -0.5, causal, softcap, None)
+    for head in (0, heads - 1):
+        check(got[:, head:head + 1], want, bound, f"head {head}")
