@@ -67,10 +67,10 @@ def ln_mod(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
            out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """T(((x - mean) * rsqrt(var + eps) * (1 + scale) + shift) * post_scale) over x's last dim.
 
-    x: contiguous float32 or T [..., cols], up to 2^20 columns; shift, scale: float32 [cols] or [n, cols];
-    sets: int32, x's leading shape: the modulation each row takes (text and image rows of
-    a joint residual in one launch), row 0's where it is not given.  T: ``out_dtype``,
-    float16 or bfloat16 (default: x's own type, or float16 for float32)."""
+    x: contiguous float32 or T [..., cols], up to 2^20 columns; shift, scale: float32 [cols], or
+    [n, cols] with sets: int32, x's leading shape: the modulation each row takes (text and
+    image rows of a joint residual in one launch).  T: ``out_dtype``, float16 or bfloat16
+    (default: x's own type, or float16 for float32)."""
     idx = _device_of(x, "x")
     shape = x.shape
     if not (len(shape) >= 1 and x.is_contiguous()):
@@ -303,7 +303,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
 
     Views with a contiguous last dim are taken as they are; ``out`` overlaps none of
     q, k and v.  Rows of ``out`` that are no
-    query's are left as they were (in a new tensor: undefined)."""
+    query's are left as they were (in a new tensor: undefined).
+
+    Few queries over many keys split the keys over a workspace of the stream, which grows on
+    its first such call.  A call captured into a graph on a stream without one runs unsplit
+    (much slower for a token over a long cache: run it once on the stream that the graph is
+    then captured on); graphs captured on one stream share its workspace, so that replays of
+    two of them do not run at once, nor one beside calls on that stream."""
     idx, out, args = _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens,
                                      prefix_lens, q_offsets, k_offsets, max_q, max_k, out)
     ctx = context(idx)

@@ -7,8 +7,8 @@
 // waves walks key tiles of its own, 32 keys (tiles 4 n + wave of the range),
 // with its own LDS and no barrier.  K and V have one buffer each and take turns:
 // K of the next tile is loaded while the softmax and the product with V run, V
-// while the next scores are made, so 8 to 16 KB a wave are in flight, 8 waves
-// a CU.  The four waves' sums are joined through LDS at the end.
+// while the next scores are made, so 8 to 16 KB a wave are in flight, four
+// waves a CU (one workgroup, where keys are split).  The four waves' sums are joined through LDS at the end.
 // 131072 keys of 8 key heads: 93 us, 5.8 TB/s (and 5.2 for the join; the tiles'
 // kernel 149 in all); 8 sequences of up to 2048 keys: 9.1 us, from the MALL, and 4.0.
 #pragma once

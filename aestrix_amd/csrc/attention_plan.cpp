@@ -73,8 +73,9 @@ AttnPlan attention_plan(const AttnArgs& a, int cus) {
     p.near_hs = (int)(even && blocks >= 16 * places ? std::min<int64_t>(hs, 32) : hs);
     unit = 4 * kAttnKeys;
     ranges = cus / blocks;
-    // Two a CU from 4096 keys a range: 65 rows on 100000 keys 222 us against
-    // 288, 512 on 8192 98 against 105; but 256 on 2048 36 against 21.
+    // Two a CU from 4096 keys a range: 65 queries of 32 / 8 heads on 100000 keys 196 us
+    // against 280, 512 on 8192 90 / 94; but 256 on 2048 27 / 24, and 65 of 8 / 2
+    // heads on 100000, with 51 ranges for 25, 76 / 67.
     const int64_t two = 2 * cus / blocks;
     if (p.tile_rows == 256)
       ranges = 1;  // more than cus / 2 workgroups already, and one a CU

@@ -144,9 +144,9 @@ int imq_dequantize_rows_host(imq_ctx* ctx, const uint32_t* w, const void* scales
  * a larger one runs unsplit; an outgrown workspace stays allocated until
  * imq_destroy, so graphs captured earlier stay valid) and a second kernel
  * adds them in order, so the result is deterministic but its fp32 summation
- * order differs from imq_qgemm's.  A graph replay of a captured call and
- * other calls on the stream it was captured on share that stream's
- * workspace: do not run them concurrently. */
+ * order differs from imq_qgemm's.  Graph replays of captured calls and
+ * other calls on the stream they were captured on share that stream's
+ * workspace: do not run two of them concurrently. */
 int imq_qmm_t(imq_ctx* ctx, const uint32_t* w, const void* scales, const void* biases,
               const void* x, void* y, int k, int n, int m, int group_size, int bits,
               imq_dtype dtype, imq_stream stream);
