@@ -9,7 +9,7 @@ every row to every row (``DirectDiTStep.swift:360-373,408-503``).
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, fields
 from typing import Sequence
 
 import torch
@@ -47,6 +47,9 @@ class DitModulation:
     single_scale: torch.Tensor
     out_shift: torch.Tensor
     out_scale: torch.Tensor
+
+
+_MODULATIONS = tuple(f.name for f in fields(DitModulation))
 
 
 class DitModel:
@@ -112,7 +115,8 @@ class DitModel:
         s, d, x = self.step, self.step.dims, self.x
         _require(e.dtype == torch.float32 and tuple(e.shape) == (d.l_txt, d.dim) and
                  e.device == x.device, f"e must be float32 [{d.l_txt}, {d.dim}] on {x.device}")
-        for name, t in vars(mod).items():  # another number of rows would go to the wrong ones
+        for name in _MODULATIONS:  # another number of rows would go to the wrong ones
+            t = getattr(mod, name)
             both = name.startswith(("attn", "mlp"))
             _require(t.dtype == torch.float32 and t.device == x.device and
                      (t.shape == (2, d.dim) if both else t.shape in ((d.dim,), (1, d.dim))),
