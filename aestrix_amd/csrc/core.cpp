@@ -32,19 +32,26 @@ int64_t reach(std::initializer_list<std::pair<int64_t, int64_t>> extents) {
 // Whether two of the places that these extents and strides give, `dim` elements each,
 // lie on each other.  Strides that fit into each other do not, in any order; of others
 // every difference of two places is looked at, as far as 2^20 steps go (then: yes).
-bool on_each_other(int64_t dim, std::initializer_list<std::pair<int64_t, int64_t>> extents) {
-  std::pair<int64_t, int64_t> e[3];  // (extent, stride) of those that step, strides rising
+// (Their reach has been checked: sums stay under 2^61.)
+using Extent = std::pair<int64_t, int64_t>;
+inline bool nested(int64_t dim, const Extent* e, int n) {
+  int64_t span = dim;
+  bool fit = true;
+  for (int i = 0; i < n; ++i)
+    if (e[i].first > 1) {
+      fit = fit && e[i].second >= span;
+      span += (e[i].first - 1) * e[i].second;
+    }
+  return fit;
+}
+
+bool on_each_other_slow(int64_t dim, const Extent* extents, int count) {
+  Extent e[3];  // (extent, stride) of those that step, strides rising
   int n = 0;
-  for (const auto& x : extents)
-    if (x.first > 1) e[n++] = x;
+  for (int i = 0; i < count; ++i)
+    if (extents[i].first > 1) e[n++] = extents[i];
   std::sort(e, e + n, [](const auto& a, const auto& b) { return a.second < b.second; });
-  __int128 span = dim;
-  bool nested = true;
-  for (int i = 0; i < n; ++i) {
-    nested = nested && e[i].second >= span;
-    span += (__int128)(e[i].first - 1) * e[i].second;
-  }
-  if (nested) return false;
+  if (nested(dim, e, n)) return false;
   // The longest is solved for, the others are stepped through (both signs of one do).
   std::sort(e, e + n, [](const auto& a, const auto& b) { return a.first > b.first; });
   const int64_t n1 = n > 1 ? e[1].first : 1, n2 = n > 2 ? e[2].first : 1, s0 = e[0].second;
@@ -63,6 +70,12 @@ bool on_each_other(int64_t dim, std::initializer_list<std::pair<int64_t, int64_t
       }
     }
   return false;
+}
+
+// Mostly they rise as they are given: nothing is sorted then.
+template <int N>
+bool on_each_other(int64_t dim, const Extent (&e)[N]) {
+  return !nested(dim, e, N) && on_each_other_slow(dim, e, N);
 }
 
 int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, imq::AttnArgs* a) {
