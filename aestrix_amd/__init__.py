@@ -21,6 +21,7 @@ from ._lib import ImqError, ImqInvalid, ImqLibraryMissing, ImqUnsupported  # noq
 from .core import (  # noqa: F401
     attention,
     attention_plan,
+    attention_shared,
     ln_mod,
     rope,
     rope_frequencies,

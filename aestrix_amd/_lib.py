@@ -151,6 +151,7 @@ SIGNATURES = {
                   _p], _i),
     "imq_attention": ([_p, _p, _p], _i),
     "imq_attention_plan": ([_p, _p, _p], _i),
+    "imq_attention_shared": ([_p, _p, _p, _p], _i),
 }
 
 

@@ -6,7 +6,9 @@
   (``DirectDiTKernels.swift:61-122``, ``DirectGlueKernels.swift:14-75``), and
   ``rope_frequencies`` for the frequencies, scaled for long contexts or not;
 * ``attention`` -- softmax attention over padded batches, packed documents and
-  caches (``DirectDiTStep.swift:457-488``, ``DirectTEEncoder.swift:159-202``).
+  caches (``DirectDiTStep.swift:457-488``, ``DirectTEEncoder.swift:159-202``);
+* ``attention_shared`` -- the same where all sequences of a batch begin with the
+  same keys.
 
 Calls run on torch's current HIP stream; tensors may be strided views (columns
 of a projection's output, rows of a cache) whose last dimension is contiguous.
@@ -314,6 +316,51 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
                                      prefix_lens, q_offsets, k_offsets, max_q, max_k, out)
     ctx = context(idx)
     rc = run_on(idx, _lib.load().imq_attention, ctx, args, raw_stream(idx))
+    if rc:
+        _lib.check(rc, ctx)
+    return out
+
+
+# imq_shared_keys: k, v, strides, rows.
+_SHARED_KEYS = struct.Struct("@2P4qi4x")
+
+
+def _shared_keys(q, k, out, shared_k, shared_v, idx) -> bytes:
+    """shared_k and shared_v as imq_shared_keys, for checked q, k and out."""
+    shape = shared_k.shape
+    if not (len(shape) == 3 and shape == shared_v.shape and shape[1:] == k.shape[-2:] and
+            shared_k.dtype == q.dtype and shared_v.dtype == q.dtype and shared_k.is_cuda and
+            shared_v.is_cuda and shared_k.get_device() == idx and shared_v.get_device() == idx):
+        raise ValueError(f"shared_k and shared_v must be {q.dtype} [rows, {', '.join(map(str, k.shape[-2:]))}] "
+                         "tensors on q's device")
+    (kr, kh, kd), (vr, vh, vd) = shared_k.stride(), shared_v.stride()
+    if not (kd == 1 and vd == 1) and shared_k.numel():
+        raise ValueError("shared_k and shared_v must be contiguous in the head dim")
+    return _packed(_SHARED_KEYS, shared_k.data_ptr(), shared_v.data_ptr(), kr, kh, vr, vh, shape[0])
+
+
+def attention_shared(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, shared_k: torch.Tensor,
+                     shared_v: torch.Tensor, *, scale: float | None = None, causal: bool = False,
+                     softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                     q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None,
+                     prefix_lens: torch.Tensor | None = None, q_offsets: torch.Tensor | None = None,
+                     k_offsets: torch.Tensor | None = None, max_q: int | None = None,
+                     max_k: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``attention`` of sequences that all begin with the same keys: a system prompt, a
+    template, a document that many requests ask about.
+
+    shared_k, shared_v [rows, kv_heads, dim]: keys that come before every sequence's own (k
+    and v, with their lengths or offsets) and that every query sees, ``causal`` or not; own
+    keys are seen as ``attention`` would have it (prefix_lens count own keys).  The result is
+    that of ``attention`` over both as one sequence of keys (where no sequence has more
+    queries than own keys, or causal is False); the shared ones are read once for the batch.
+    Own keys may be none at all (k of no rows).  Everything else, and what is said of
+    workspaces and graphs, is ``attention``'s."""
+    idx, out, args = _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens,
+                                     prefix_lens, q_offsets, k_offsets, max_q, max_k, out)
+    shared = _shared_keys(q, k, out, shared_k, shared_v, idx)
+    ctx = context(idx)
+    rc = run_on(idx, _lib.load().imq_attention_shared, ctx, args, shared, raw_stream(idx))
     if rc:
         _lib.check(rc, ctx)
     return out

@@ -7,6 +7,7 @@
 #include <initializer_list>
 #include <utility>
 
+#include "core_checks.hpp"
 #include "core_kernels.hpp"
 #include "ctx.hpp"
 #include "imq.h"
@@ -17,17 +18,6 @@ using namespace imq::detail;
 namespace {
 
 bool known(imq_dtype t) { return t == IMQ_BF16 || t == IMQ_F16 || t == IMQ_F32; }
-
-// The largest element offset of a tensor walked by these extents and strides,
-// or -1 where a stride is negative or the bytes pass 2^62.
-int64_t reach(std::initializer_list<std::pair<int64_t, int64_t>> extents) {
-  __int128 at = 0;
-  for (const auto& e : extents) {
-    if (e.second < 0) return -1;
-    at += (__int128)(e.first > 0 ? e.first - 1 : 0) * e.second;
-  }
-  return at < ((__int128)1 << 60) ? (int64_t)at : -1;
-}
 
 // Whether two of the places that these extents and strides give, `dim` elements each,
 // lie on each other.  Strides that fit into each other do not, in any order; of others
@@ -78,7 +68,10 @@ bool on_each_other(int64_t dim, const Extent (&e)[N]) {
   return !nested(dim, e, N) && on_each_other_slow(dim, e, N);
 }
 
-int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, imq::AttnArgs* a) {
+}  // namespace
+
+int imq::detail::check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p,
+                                 imq::AttnArgs* a) {
   if (!ctx) return fail(nullptr, IMQ_EINVAL, "%s: null context", fn);
   if (!p) return fail(ctx, IMQ_EINVAL, "%s: null arguments", fn);
   if (p->dtype != IMQ_BF16 && p->dtype != IMQ_F16)
@@ -161,8 +154,6 @@ int check_attention(imq_ctx* ctx, const char* fn, const imq_attention_args* p, i
   a->causal = p->causal, a->scale = p->scale, a->softcap = p->softcap;
   return IMQ_OK;
 }
-
-}  // namespace
 
 extern "C" {
 

@@ -44,6 +44,13 @@ struct AttnArgs {
   float scale, softcap;
 };
 
+// imq_shared_keys with the strides in elements: keys in front of every sequence's own.
+struct AttnShared {
+  const void *k, *v;
+  int64_t k_row, k_head, v_row, v_head;
+  int rows;
+};
+
 constexpr int kAttnKeys = 64;  // keys of a tile (attn_tiles_kernel)
 constexpr int kFewWaves = 4;   // waves of a workgroup (attn_few_kernel) ...
 constexpr int kFewKeys = 32;   // ... and keys of a wave's tile
@@ -63,5 +70,8 @@ AttnPlan attention_plan(const AttnArgs& a, int cus);
 // ws: plan.bytes of device memory, NULL where the plan does not split.
 hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, float* ws, int dtype,
                             hipStream_t stream);
+
+hipError_t launch_attention_shared(const AttnArgs& a, const AttnShared& sh, int dtype,
+                                   hipStream_t stream);
 
 }  // namespace imq

@@ -8,9 +8,10 @@
  * dq_rmsnorm, DirectGlueKernels.swift:14-49), RoPE (dd_rope_interleaved,
  * DirectDiTKernels.swift:103-122; dq_rope, DirectGlueKernels.swift:54-75) and
  * softmax attention (steel_attention, DirectDiTStep.swift:457-488,
- * DirectTEEncoder.swift:159-202).  The three entry points here are that work:
+ * DirectTEEncoder.swift:159-202).  The first three entry points here are that work:
  * with them a caller of the block halves (imq_step.h) and of the layer halves
- * (imq_te.h) runs whole blocks and layers.
+ * (imq_te.h) runs whole blocks and layers.  imq_attention_shared is the attention
+ * of a batch whose sequences begin with the same keys.
  *
  * Conventions as in imq.h: an imq_status is returned, nothing throws, calls
  * are asynchronous on the given stream and may be captured into a graph,
@@ -165,6 +166,31 @@ typedef struct imq_attention_plan_info {
 /* The plan of an imq_attention call with its workspace in hand, after the same
  * checks of the arguments, without launching anything. */
 int imq_attention_plan(imq_ctx* ctx, const imq_attention_args* args, imq_attention_plan_info* out);
+
+/* ---- attention behind shared keys --------------------------------------------
+ * imq_attention for sequences that all begin with the same keys (a system
+ * prompt, a template, a document that many ask about), which are read once for
+ * the batch where a sequence's own queries are too few to make up for reading
+ * them: every query sees all `rows` of the shared keys, and of its sequence's
+ * own keys (args: k, v, lengths, offsets, causal, prefix_lens) what
+ * imq_attention would let it see.  The own keys stand behind the shared ones: where
+ * n_q <= n_k or causal is 0 the output is that of imq_attention over both as one
+ * sequence, to the rounding of its sums.  Distances (slopes) count from own key
+ * to own key, and to the shared key j as to an own key at j - rows.
+ * No own keys (max_k 0 or n_k 0) and no shared ones (rows 0) are allowed; a query
+ * that sees neither gives zeros.  rows + max_k stays under 2^31.
+ * Types, sizes, alignment, workspace and what spoilt keys do are imq_attention's.
+ * shared: k and v of T, element (j, h, d) at j * row + h * head + d, kv_heads heads of
+ * dim; out is none of them. */
+typedef struct imq_shared_keys {
+  const void* k;
+  const void* v;
+  int64_t k_row, k_head, v_row, v_head; /* element strides */
+  int rows;
+} imq_shared_keys;
+
+int imq_attention_shared(imq_ctx* ctx, const imq_attention_args* args,
+                         const imq_shared_keys* shared, imq_stream stream);
 
 #ifdef __cplusplus
 }
