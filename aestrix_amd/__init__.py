@@ -14,7 +14,9 @@ the C ABI of ``include/imq.h`` (``aestrix_amd/libimq.so``):
 post-qmm glue kernels into the MFMA kernel's epilogue; ``cast_prescale`` and
 ``apply_linear`` are the f16 sandwich around them (x / 16 to f16, qmm, x 16).
 ``ln_mod``, ``rope`` and ``attention`` (``include/imq_core.h``) are the work of
-a block between its projections.
+a block between its projections.  For many requests in one batch,
+``quantized_matmul_lora`` adds each row's own adapter to a projection and
+``attention_shared`` attends to keys that all sequences begin with.
 """
 
 from ._lib import ImqError, ImqInvalid, ImqLibraryMissing, ImqUnsupported  # noqa: F401
@@ -26,6 +28,7 @@ from .core import (  # noqa: F401
     rope,
     rope_frequencies,
 )
+from .lora import LoraAdapters, quantized_matmul_lora  # noqa: F401
 from .ops import (  # noqa: F401
     BITS,
     GROUP_SIZE,

@@ -50,6 +50,13 @@ class Plan(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t), ("tile_cols", ctypes.c_int)]
 
 
+class Lora(ctypes.Structure):
+    """imq_lora."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("first", ctypes.c_void_p),
+                ("scale", ctypes.c_void_p), ("count", ctypes.c_int), ("rows", ctypes.c_int),
+                ("max_rank", ctypes.c_int)]
+
+
 IMQ_ENTRY_QMM_T, IMQ_ENTRY_QGEMM, IMQ_ENTRY_QGEMV, IMQ_ENTRY_FUSED, IMQ_ENTRY_SWIGLU = 0, 1, 2, 3, 4
 DIT_GROUPS = {"qkv": 0, "attn_out": 1, "mlp_in": 2, "mlp_out": 3}
 KERNEL_NAMES = {0: "qgemv", 1: "few_row", 2: "tile", 3: "tile_reg"}
@@ -152,6 +159,8 @@ SIGNATURES = {
     "imq_attention": ([_p, _p, _p], _i),
     "imq_attention_plan": ([_p, _p, _p], _i),
     "imq_attention_shared": ([_p, _p, _p, _p], _i),
+    "imq_qmm_lora_workspace": ([_p, _p, _i, _i, _i, _i, _p], _i),
+    "imq_qmm_lora": ([_p] * 8 + [_i, _i, _i, _i, _i, _i, _p, ctypes.c_size_t, _p], _i),
 }
 
 

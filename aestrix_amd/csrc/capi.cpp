@@ -172,13 +172,6 @@ SplitHold split_ws(imq_ctx* ctx, hipStream_t st, size_t need) {
   }
 }
 
-}  // namespace detail
-}  // namespace imq
-
-using namespace imq::detail;
-
-namespace {
-
 // Shared validation of the quantized-matmul entry points.
 int check_qmm(imq_ctx* ctx, const char* fn, const uint32_t* w, const void* s, const void* b,
               const void* x, void* y, int k, int n, int m, int group_size, int bits,
@@ -204,6 +197,13 @@ int check_qmm(imq_ctx* ctx, const char* fn, const uint32_t* w, const void* s, co
     return fail(ctx, IMQ_EINVAL, "%s: scales, biases and y must be %zu-byte aligned", fn, es);
   return IMQ_OK;
 }
+
+}  // namespace detail
+}  // namespace imq
+
+using namespace imq::detail;
+
+namespace {
 
 // kAuto: the regime dispatcher (imq_qmm_t); kAutoNoAlloc: the same plan with
 // the split-K partial sums in the library's static scratch

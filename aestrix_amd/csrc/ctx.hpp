@@ -88,6 +88,9 @@ int hip_fail(imq_ctx* ctx, hipError_t e, const char* what);
 bool aligned(const void* p, size_t a);
 size_t elem_size(imq_dtype dtype);
 int bind_device(imq_ctx* ctx);
+// Shared validation of the quantized-matmul entry points.
+int check_qmm(imq_ctx* ctx, const char* fn, const uint32_t* w, const void* s, const void* b,
+              const void* x, void* y, int k, int n, int m, int group_size, int bits, imq_dtype dtype);
 // A stream's split workspace in use: no other call enqueues kernels on it while
 // this lives.  ws.p NULL: not to be had, and nothing held.
 struct SplitHold {

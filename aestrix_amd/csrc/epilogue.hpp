@@ -223,6 +223,11 @@ struct EpSwiGLU {
   }
 };
 
+// Stages with sums of their own behind the K loop: add_sums(acc, m0, n0, M, N) adds them
+// to a wave's 32 x 32 accumulators of the rows from m0 and the columns from n0 on.
+template <class EP>
+constexpr bool adds_sums = false;
+
 // Split-K partial sums: the fp32 accumulators themselves, unrounded, into
 // ws[split][row][...] (row pitch ldp); a second kernel adds the splits and
 // applies the real output stage.  Plain: column col at col (ldp = N).  PAIR

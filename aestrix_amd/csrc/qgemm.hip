@@ -6,6 +6,7 @@
 #include "epilogue.hpp"
 #include "imq_device.hpp"
 #include "imq_kernels.hpp"
+#include "lora_device.hpp"
 #include "qgemm_plan.hpp"
 
 namespace imq {
@@ -256,6 +257,36 @@ hipError_t launch_qgemm(const uint32_t* w, const void* scales, const void* biase
   switch (dtype) {
     case kBf16: return launch_t<kBf16>(w, s, b, xx, yy, k, n, m, stream, ws);
     case kF16: return launch_t<kF16>(w, s, b, xx, yy, k, n, m, stream, ws);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+namespace {
+
+template <int T>
+hipError_t launch_lora_t(const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
+                         const uint16_t* x, const LoraArgs& l, uint16_t* y, int k, int n, int m,
+                         hipStream_t stream) {
+  const EpLora<T> ep{{y, n, al16(y) && n % 8 == 0}, l};
+  if (!qgemm_big_supported(k, n, m))
+    return tile::launch_reg<T, EpLora<T>>(w, scales, biases, x, ep, k, n, m, stream);
+  const BigPlan p = pick_big_plan(m, n, k, device_cus(), false);
+  return k % 256 ? tile::launch_plan<T, EpLora<T>, true>(p, w, scales, biases, x, ep, k, n, m, stream)
+                 : tile::launch_plan<T, EpLora<T>, false>(p, w, scales, biases, x, ep, k, n, m, stream);
+}
+
+}  // namespace
+
+hipError_t launch_qgemm_lora(const uint32_t* w, const void* scales, const void* biases, const void* x,
+                             const LoraArgs& l, void* y, int k, int n, int m, int dtype,
+                             hipStream_t stream) {
+  const auto* s = static_cast<const uint16_t*>(scales);
+  const auto* b = static_cast<const uint16_t*>(biases);
+  const auto* xx = static_cast<const uint16_t*>(x);
+  auto* yy = static_cast<uint16_t*>(y);
+  switch (dtype) {
+    case kBf16: return launch_lora_t<kBf16>(w, s, b, xx, l, yy, k, n, m, stream);
+    case kF16: return launch_lora_t<kF16>(w, s, b, xx, l, yy, k, n, m, stream);
     default: return hipErrorInvalidValue;
   }
 }

@@ -251,6 +251,8 @@ __global__ __launch_bounds__(kThreads, (MT * NT * 16 > 128) ? 1 : 2) void qgemm_
     __syncthreads();
   }
 
+  if constexpr (adds_sums<EP>) ep.template add_sums<MT, NT>(acc, m0, nw0, M, N);
+
   // Epilogue: accumulator r of a 32x32 tile holds row 8*(r/4) + 4*h + r%4,
   // column r32.  Each output is rounded to T (Elem::out, the same RNE as the
   // staged stores of the large-M kernel) and handed to the output stage.
@@ -947,6 +949,7 @@ __device__ __forceinline__ void big_tile(const uint32_t* __restrict__ w,
         }
     }
   } else {
+  if constexpr (adds_sums<EP>) ep.template add_sums<MT, NT>(acc, m0, ncol0, M, N);
   // Output: the tile's T values are staged in the LDS ring, then written out
   // row by row, 16 bytes per lane.  Written straight from the MFMA layout, a
   // lane holds one column of 16 rows per 32x32 tile: 2-byte stores, 14 of

@@ -1,0 +1,113 @@
+"""Low-rank adapters of many requests beside a shared 4-bit projection (include/imq_lora.h).
+
+The reference has no adapters.  A server runs the rows of all its requests through one
+quantized projection; every row has its request's adapter, or none.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Sequence
+
+import torch
+
+from . import _lib
+from .ops import _DTYPES, BITS, GROUP_SIZE, _epi_args, _require, context, new_out, raw_stream, run_on
+
+_MAX_RANK = 256
+_FILL = 16  # ranks are filled up to multiples of this
+
+
+class LoraAdapters:
+    """A set of adapters for one projection, laid out once.
+
+    ``pairs``: (A [rank, K], B [N, rank]) of every adapter, bfloat16 or float16 on one device,
+    ranks from 1 to 256, not all alike if they are not; ``scales``: a factor each (alpha / rank),
+    one for all, or none.  Adapter i adds ``scales[i] * (x . A^T) . B^T``.
+
+    The tensors are copied: in bytes about what the adapters have, ranks filled up to multiples
+    of 16.  In float16 B is held with its largest element between 1 and 2 (a power of two, which
+    ``scales`` takes back), so that the products between A and B keep that type's range."""
+
+    def __init__(self, pairs: Sequence[tuple[torch.Tensor, torch.Tensor]],
+                 scales: float | Sequence[float] | None = None):
+        pairs = [tuple(p) for p in pairs]
+        _require(len(pairs) > 0 and all(len(p) == 2 for p in pairs), "pairs must be (A, B), one at least")
+        if scales is None or isinstance(scales, (int, float)):
+            scales = [1.0 if scales is None else scales] * len(pairs)
+        scales = [float(s) for s in scales]
+        _require(len(scales) == len(pairs), f"{len(scales)} scales for {len(pairs)} adapters")
+        _require(all(math.isfinite(s) and abs(s) < 3e38 for s in scales), "scales must be finite float32")
+        a0, b0 = pairs[0]
+        _require(a0.dim() == 2 and b0.dim() == 2, "A must be [rank, K] and B [N, rank]")
+        self.k, self.n, self.dtype, self.device = a0.shape[1], b0.shape[0], a0.dtype, a0.device
+        _require(a0.is_cuda, "tensors must be on a HIP device")
+        if self.dtype not in (torch.bfloat16, torch.float16):
+            raise _lib.ImqUnsupported(_lib.IMQ_EUNSUPPORTED, f"{self.dtype}: bfloat16 and float16 are provided")
+        _require(self.k > 0 and self.k % GROUP_SIZE == 0 and self.n > 0, f"K = {self.k} must be a multiple of 64, N > 0")
+        first = [0]
+        for a, b in pairs:
+            _require(a.dim() == 2 and b.dim() == 2 and a.shape[1] == self.k and b.shape[0] == self.n and
+                     a.shape[0] == b.shape[1], f"A must be [rank, {self.k}] and B [{self.n}, rank], "
+                     f"got {tuple(a.shape)} and {tuple(b.shape)}")
+            _require(1 <= a.shape[0] <= _MAX_RANK, f"rank {a.shape[0]}: 1 to {_MAX_RANK} are taken")
+            _require(a.dtype == b.dtype == self.dtype and a.device == b.device == self.device,
+                     "all A and B must share a dtype and a device")
+            first.append(first[-1] + -(-a.shape[0] // _FILL) * _FILL)
+        self.count, self.rows = len(pairs), first[-1]
+        self.max_rank = max(q - p for p, q in zip(first, first[1:]))
+        self.a = torch.zeros((self.rows, self.k), dtype=self.dtype, device=self.device)
+        self.b = torch.zeros(self.rows * self.n, dtype=self.dtype, device=self.device)
+        self.scale = torch.tensor(scales, dtype=torch.float32, device=self.device)
+        self.first = torch.tensor(first, dtype=torch.int32, device=self.device)
+        for i, (a, b) in enumerate(pairs):
+            rank = a.shape[0]
+            self.a[first[i]:first[i] + rank] = a
+            at = self.b[first[i] * self.n:first[i + 1] * self.n].view(self.n, -1)[:, :rank]
+            if self.dtype == torch.float16:
+                # 2^up brings the largest element to [1, 2) (none, or not finite: as it is).
+                top = b.abs().max().float()
+                up = torch.where((top > 0) & torch.isfinite(top), 1 - torch.frexp(top).exponent, 0)
+                at.copy_(torch.ldexp(b.float(), up))
+                self.scale[i] = torch.ldexp(self.scale[i], -up)
+            else:
+                at.copy_(b)
+        self._c = _lib.Lora(self.a.data_ptr(), self.b.data_ptr(), self.first.data_ptr(), self.scale.data_ptr(),
+                            self.count, self.rows, self.max_rank)
+        self._p = ctypes.addressof(self._c)
+
+
+def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
+                          adapters: LoraAdapters, which: torch.Tensor, group_size: int = GROUP_SIZE,
+                          bits: int = BITS, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y[..., N] = T(x . deq(W)^T + scale_i * (x . A_i^T) . B_i^T), i = which[...] the adapter of
+    each row of x, rounded once.
+
+    which: int32, x's leading shape; a row whose value is not one of 0 to count - 1 (-1) has no
+    adapter.  x, scales and biases as in ``quantized_matmul``, bfloat16 or float16, of the
+    adapters' type; ``out`` is not x.  The workspace is torch's, so that calls may be captured
+    into graphs and graphs replayed beside each other; a call's result does not depend on any of that."""
+    n, k, m, lead, x = _epi_args(x, w, scales, biases, group_size, bits)
+    idx = w.get_device()
+    if not (adapters.k == k and adapters.n == n and adapters.dtype == x.dtype and adapters.device == x.device):
+        raise ValueError(f"adapters of a {adapters.dtype} [{adapters.n}, {adapters.k}] projection on {adapters.device}, "
+                         f"this is {x.dtype} [{n}, {k}] on {x.device}")
+    if not (which.dtype == torch.int32 and which.shape == lead and which.is_contiguous() and which.device == x.device):
+        raise ValueError(f"which must be a contiguous int32 tensor of shape {lead} on x's device")
+    shape = lead + (n,)
+    if out is None:
+        out = new_out(x, shape)
+    _require(out.is_contiguous() and out.shape == shape and out.dtype == x.dtype and out.device == x.device,
+             "out must be a contiguous [..., N] tensor of x's dtype and device")
+    if m == 0:
+        return out
+    ctx = context(idx)
+    lib, dtype = _lib.load(), _DTYPES.get(x.dtype, -1)
+    need = ctypes.c_size_t()
+    _lib.check(lib.imq_qmm_lora_workspace(ctx, adapters._p, k, n, m, dtype, ctypes.byref(need)), ctx)
+    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+    _lib.check(run_on(idx, lib.imq_qmm_lora, ctx, w.data_ptr(), scales.data_ptr(), biases.data_ptr(), x.data_ptr(),
+                      adapters._p, which.data_ptr(), out.data_ptr(), k, n, m, group_size, bits, dtype,
+                      ws.data_ptr(), need.value, raw_stream(idx)), ctx)
+    return out
