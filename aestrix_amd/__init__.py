@@ -24,6 +24,7 @@ from .core import (  # noqa: F401
     attention,
     attention_plan,
     attention_shared,
+    attention_shared_plan,
     ln_mod,
     rope,
     rope_frequencies,

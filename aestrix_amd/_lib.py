@@ -159,6 +159,7 @@ SIGNATURES = {
     "imq_attention": ([_p, _p, _p], _i),
     "imq_attention_plan": ([_p, _p, _p], _i),
     "imq_attention_shared": ([_p, _p, _p, _p], _i),
+    "imq_attention_shared_plan": ([_p, _p, _p, _p], _i),
     "imq_qmm_lora_workspace": ([_p, _p, _i, _i, _i, _i, _p], _i),
     "imq_qmm_lora": ([_p] * 8 + [_i, _i, _i, _i, _i, _i, _p, ctypes.c_size_t, _p], _i),
 }

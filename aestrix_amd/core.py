@@ -366,6 +366,30 @@ def attention_shared(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, shared_k
     return out
 
 
+class SharedPlanInfo(ctypes.Structure):
+    """imq_shared_plan_info."""
+    _fields_ = [("kernel", ctypes.c_int), ("tile_rows", ctypes.c_int), ("splits", ctypes.c_int),
+                ("own_splits", ctypes.c_int), ("workspace_bytes", ctypes.c_size_t)]
+
+
+SHARED_KERNELS = {0: "rows", 1: "tiles", 2: "stream"}
+
+
+def attention_shared_plan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, shared_k: torch.Tensor,
+                          shared_v: torch.Tensor, *, scale=None, causal=False, softcap=0.0, slopes=None,
+                          q_lens=None, k_lens=None, prefix_lens=None, q_offsets=None, k_offsets=None,
+                          max_q=None, max_k=None, out=None) -> dict:
+    """The kernel, tile height, key ranges and workspace ``attention_shared`` would use."""
+    idx, out, args = _attention_args(q, k, v, scale, causal, softcap, slopes, q_lens, k_lens,
+                                     prefix_lens, q_offsets, k_offsets, max_q, max_k, out)
+    shared = _shared_keys(q, k, out, shared_k, shared_v, idx)
+    ctx = context(idx)
+    info = SharedPlanInfo()
+    _lib.check(_lib.load().imq_attention_shared_plan(ctx, args, shared, ctypes.addressof(info)), ctx)
+    return {"kernel": SHARED_KERNELS[info.kernel], "tile_rows": info.tile_rows, "splits": info.splits,
+            "own_splits": info.own_splits, "workspace_bytes": info.workspace_bytes}
+
+
 def attention_plan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale=None, causal=False,
                    softcap=0.0, slopes=None, q_lens=None, k_lens=None, prefix_lens=None,
                    q_offsets=None, k_offsets=None, max_q=None, max_k=None, out=None) -> dict:

@@ -62,6 +62,7 @@ struct AttnScore {
   float top;   // cap * log2(e)
   float fall;  // slope * log2(e)
 
+  AttnScore() = default;
   __device__ __forceinline__ AttnScore(const AttnArgs& a, int head) {
     mul = kCap ? 2.f * a.scale / a.softcap * kLog2e : a.scale * kLog2e;
     top = kCap ? a.softcap * kLog2e : 0.f;

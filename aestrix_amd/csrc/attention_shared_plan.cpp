@@ -1,0 +1,77 @@
+// attention_shared_plan.cpp -- which kernel an imq_attention_shared call takes and how its
+// keys are split (host code alone).
+#include <algorithm>
+
+#include "core_kernels.hpp"
+#include "imq_core.h"
+
+namespace imq {
+namespace {
+
+constexpr int kStreamStep = kFewWaves * kFewKeys;  // a tile for each wave
+
+// Ranges of at most `chunk` keys (whole steps) over `keys`.
+int ranges(int keys, int chunk) { return keys > 0 ? (keys + chunk - 1) / chunk : 0; }
+
+}  // namespace
+
+SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cus, bool workspace) {
+  SharedPlan p{};
+  p.kernel = IMQ_SHARED_ROWS;
+  const int64_t far = (int64_t)1 << 24;  // elements of a row, as for the own keys
+  const int64_t strides = sh.k_row | sh.k_head | sh.v_row | sh.v_head;
+  const int64_t own0 = ((int64_t)sh.rows + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
+  // (Rows of values that begin inside the row before: a tile's last would read on past
+  // the end of the shared ones.)
+  if (strides % 8 != 0 || ((uintptr_t)sh.k | (uintptr_t)sh.v) % 16 != 0 || sh.k_row > far - 128 ||
+      sh.v_row > far - 128 || sh.v_row < a.dim || own0 + a.max_k > (1 << 30))
+    return p;
+  // The walk over both.
+  AttnArgs walk = a;
+  walk.max_k = (int)own0 + a.max_k;
+  if (a.max_k == 0) walk.k = walk.v = nullptr;
+  p.tiles = attention_plan(walk, cus);
+  if (p.tiles.kernel == IMQ_ATTENTION_ROWS) return p;
+  const int rows = a.max_q * (a.heads / a.kv_heads);
+  const int64_t hs = (int64_t)a.n_seq * a.kv_heads;
+  p.kernel = IMQ_SHARED_TILES;
+  if (p.tiles.kernel == IMQ_ATTENTION_TILES) {
+    p.bytes = p.tiles.bytes;
+    if (p.tiles.splits == 1 || workspace) return p;
+  }
+  if (p.tiles.kernel == IMQ_ATTENTION_TILES || !workspace) {
+    // Unsplit, whatever the rows.
+    const int tile_rows = rows > 64 ? 128 : 64;
+    const int tiles = (rows + tile_rows - 1) / tile_rows;
+    p.tiles = AttnPlan{IMQ_ATTENTION_TILES, tile_rows, 1, tiles, (int)hs, 0, 0};
+    p.bytes = 0;
+    if (hs * tiles * 512 >= ((int64_t)1 << 32)) p.kernel = IMQ_SHARED_ROWS;
+    return p;
+  }
+  p.kernel = IMQ_SHARED_STREAM;
+  const int64_t batch = (int64_t)a.n_seq * rows;
+  p.s_rows = batch > 32 ? 64 : 32;
+  p.s_tiles = (int)((batch + p.s_rows - 1) / p.s_rows);
+  // A workgroup a CU: the keys of a range such that all ranges together are as many.  64
+  // rows take half as long again as 32.
+  const int64_t per = p.s_rows == 64 ? 3 : 2;
+  const int64_t work = (int64_t)a.kv_heads * p.s_tiles * sh.rows * per / 2 + hs * a.max_k;
+  int64_t chunk = (work + cus - 1) / cus;
+  chunk = std::max<int64_t>((chunk + kStreamStep - 1) / kStreamStep * kStreamStep, kStreamStep);
+  const int64_t s_chunk = std::max<int64_t>(chunk * 2 / per / kStreamStep * kStreamStep, kStreamStep);
+  p.s_splits = ranges(sh.rows, (int)std::min<int64_t>(s_chunk, 1 << 30));
+  // Ranges of one length.
+  p.s_chunk = (ranges(sh.rows, p.s_splits) + kStreamStep - 1) / kStreamStep * kStreamStep;
+  p.s_splits = ranges(sh.rows, p.s_chunk);
+  p.o_chunk = (int)std::min<int64_t>(chunk, 1 << 30);
+  p.o_splits = ranges(a.max_k, p.o_chunk);
+  const int64_t blocks = (int64_t)a.kv_heads * p.s_tiles * p.s_splits + hs * p.o_splits;
+  if (std::max(blocks, hs * rows) * 256 >= ((int64_t)1 << 32)) {
+    p.kernel = IMQ_SHARED_ROWS;
+    return p;
+  }
+  p.bytes = (size_t)(p.s_splits + p.o_splits) * hs * rows * ((a.dim > 64 ? 128 : 64) + 2) * sizeof(float);
+  return p;
+}
+
+}  // namespace imq

@@ -367,9 +367,11 @@ __device__ __forceinline__ void attn_load(const char* base, int64_t row_bytes, i
 // Waves of a workgroup with WM of them on rows of their own.
 constexpr int attn_waves(int wm) { return wm < 4 ? 4 : wm; }
 
-template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
-__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
-    AttnArgs a, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
+// kShared: `sh` stands before every sequence's keys.  The walk is over both: the shared keys
+// in whole tiles, the last one filled up, and the own ones from `own0` on.
+template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit, bool kShared>
+__device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& sh, int tiles, int first,
+                                           int near_hs, int splits, int chunk, float* ws) {
   using S = typename Elem<T>::S;
   // WM waves on rows of their own, WK on a part of every tile's keys each.
   constexpr int NW = attn_waves(WM), WK = NW / WM, U = 2 / WK, kRows = WM * 32;
@@ -408,27 +410,41 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
   const int seen_hi = mw >= rows ? 0 : __builtin_amdgcn_readfirstlane(
       attn_seen(a, s, min(mw + 31, rows - 1) / group));
   const int seen_lo = __builtin_amdgcn_readfirstlane(attn_seen(a, s, min(mw, rows - 1) / group));
+  const int own0 = kShared ? (sh.rows + kAttnKeys - 1) / kAttnKeys * kAttnKeys : 0;
   const int begin = kSplit ? split * chunk : 0;
-  const int end = kSplit ? min(seen_wg, begin + chunk) : seen_wg;
+  const int end = kSplit ? min(own0 + seen_wg, begin + chunk) : own0 + seen_wg;
   if (kSplit && begin >= end) return;  // the join reads the ranges up to seen_wg only
 
   // Sources of this thread's pieces in a tile.
   const int64_t kb = a.k_row * 2, vb = a.v_row * 2;
   uint32_t k_off[kLoads], v_off[kLoads];
+  auto sources = [&](int64_t kb, int64_t vb) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int at = (i * NW + wave) * 64 + lane, row = at / (D / 8), piece = at % (D / 8);
-    const int kp = k_piece<D>(row, piece), vp = v_piece<D>(row, piece);
-    k_off[i] = kp * 8 < a.dim ? (uint32_t)(row * kb + kp * 16) : 0x80000000u;
-    v_off[i] = vp * 8 < a.dim ? (uint32_t)(row * vb + vp * 16) : 0x80000000u;
-  }
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = (i * NW + wave) * 64 + lane, row = at / (D / 8), piece = at % (D / 8);
+      const int kp = k_piece<D>(row, piece), vp = v_piece<D>(row, piece);
+      k_off[i] = kp * 8 < a.dim ? (uint32_t)(row * kb + kp * 16) : 0x80000000u;
+      v_off[i] = vp * 8 < a.dim ? (uint32_t)(row * vb + vp * 16) : 0x80000000u;
+    }
+  };
+  if (kShared && begin < own0) sources(sh.k_row * 2, sh.v_row * 2);
+  else sources(kb, vb);
   const char* kbase = reinterpret_cast<const char*>(static_cast<const S*>(a.k) + s.k_at + kh * a.k_head);
   const char* vbase = reinterpret_cast<const char*>(static_cast<const S*>(a.v) + s.v_at + kh * a.v_head);
   auto issue = [&](AttnStage<D>& st, int j0) {
+    if (kShared && j0 < own0) {
+      const int64_t skb = sh.k_row * 2, svb = sh.v_row * 2;
+      const int n = j0 < end ? min(kAttnKeys, sh.rows - j0) : 0;
+      attn_load<D, NW>(static_cast<const char*>(sh.k) + kh * sh.k_head * 2 + j0 * skb, skb, n, a.dim,
+                       k_off, st.k, wave);
+      attn_load<D, NW>(static_cast<const char*>(sh.v) + kh * sh.v_head * 2 + j0 * svb, svb, n, a.dim,
+                       v_off, st.v, wave);
+      return;
+    }
     // Nothing past the last tile: rows below 1.
-    const int n = j0 < end ? min(kAttnKeys, s.nk - j0) : 0;
-    attn_load<D, NW>(kbase + j0 * kb, kb, n, a.dim, k_off, st.k, wave);
-    attn_load<D, NW>(vbase + j0 * vb, vb, n, a.dim, v_off, st.v, wave);
+    const int n = j0 < end ? min(kAttnKeys, s.nk - (j0 - own0)) : 0;
+    attn_load<D, NW>(kbase + (j0 - own0) * kb, kb, n, a.dim, k_off, st.k, wave);
+    attn_load<D, NW>(vbase + (j0 - own0) * vb, vb, n, a.dim, v_off, st.v, wave);
   };
   s16x8_t qf[D / 16];
   if constexpr (WM == 4 && D == 128) {
@@ -470,8 +486,17 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
   // would hold up the wave that has everyone wait.
   auto step = [&](const AttnStage<D>& st, AttnStage<D>& to, int j0) __attribute__((always_inline)) {
     const int j1 = j0 + kAttnKeys;
+    // What the rows see of the walk, where they stand in it, and `near`, among the shared
+    // keys and among the own ones.
+    const bool front = kShared && j0 < own0;
+    if (kShared && j1 == own0) sources(kb, vb);
+    const int walk_seen = front ? sh.rows : own0 + seen, walk_lo = front ? sh.rows : own0 + seen_lo;
+    const int walk_hi = front ? (mw >= rows ? 0 : sh.rows) : own0 + seen_hi;
+    const int walk_p = p + (front ? sh.rows : own0);
+    const int walk_near = front ? min(mw, rows - 1) / group + s.nk - s.nq + 1 + sh.rows
+                          : near == INT_MAX ? near : own0 + near;
     j0 += wk * (32 * U);
-    if (j0 >= seen_hi) {
+    if (j0 >= walk_hi) {
       issue(to, j1);
       return;
     }
@@ -496,8 +521,8 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     }
     s16x8_t pf[2 * U];
     float shift[U];
-    attn_top<T>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
-                                             j0 + 32 * U <= near, shift), o, top, sum);
+    attn_top<T>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, walk_seen, walk_lo, walk_p - j0,
+                                             j0 + 32 * U <= walk_near, shift), o, top, sum);
     attn_weights<T, U, kCap, kSlope>(score, sc, shift, top, sum, pf);
     attn_pv<T, D, 2 * U>(st.v + wk * U * 32 * (D / 8), pf, o, lane);
   };
@@ -572,7 +597,7 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     }
   } else {
     // (Of keys whose scores are all -infinity the sum is zero too, and the output NaN.)
-    const float inv = seen > 0 ? 1.f / sum : 0.f;
+    const float inv = kShared || seen > 0 ? 1.f / sum : 0.f;
     bool finite = true;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -621,9 +646,16 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
       const int r = __builtin_ctzll(again);
       again &= again - 1;
       const int tr = (mw + r) / group;
-      attn_row<T, kCap, kSlope>(a, s, kh * group + (mw + r) % group, tr, attn_seen(a, s, tr), qs[wave]);
+      attn_row<T, kCap, kSlope, kShared>(a, s, kh * group + (mw + r) % group, tr, attn_seen(a, s, tr),
+                                         qs[wave], sh);
     }
   }
+}
+
+template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
+__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
+    AttnArgs a, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
+  attn_tiles<T, D, WM, kCap, kSlope, kSplit, false>(a, AttnShared{}, tiles, first, near_hs, splits, chunk, ws);
 }
 
 // Joins the key ranges of a split plan: 16 lanes a row, D / 16 columns each,
@@ -632,9 +664,11 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
 // tile's ranges up to the last key that its last row sees are written, the
 // others not.  Bound by the latency of its loads: four ranges a group are in
 // flight together.
-template <int T, int D, int kParts, bool kCap, bool kSlope>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_rows, int tiles,
-                                                        int splits, int chunk, const float* ws) {
+// kShared: a tile's first `front` ranges are the shared keys', and the others are counted
+// from `own0` keys before its own.
+template <int T, int D, int kParts, bool kCap, bool kSlope, bool kShared>
+__device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& sh, int tile_rows, int tiles,
+                                          int splits, int chunk, int front, int own0, const float* ws) {
   using S = typename Elem<T>::S;
   __shared__ float qs[4][D];
   __shared__ float sums[kParts > 1 ? 16 : 1][D + 2];
@@ -659,7 +693,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
   float acc[D / 16] = {}, top = -INFINITY, sum = 0.f;
   if (live) {
     const int last = min(m / tile_rows * tile_rows + tile_rows, rows) - 1;
-    const int used = (int)(((int64_t)attn_seen(a, s, last / group) + chunk - 1) / chunk);
+    const int used = front + (int)(((int64_t)attn_seen(a, s, last / group) + own0 + chunk - 1) / chunk);
     const float2* ml = reinterpret_cast<const float2*>(ws + (int64_t)splits * all * D) + row;
     const float* po = ws + row * D + d0;
     for (int i = part; i < used; i += 4 * kParts) {
@@ -724,7 +758,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
   }
   bool again_row = false;
   if (live) {
-    const float inv = attn_seen(a, s, t) > 0 ? 1.f / sum : 0.f;
+    const float inv = kShared || attn_seen(a, s, t) > 0 ? 1.f / sum : 0.f;
     S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) {
@@ -749,8 +783,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_row
     const int tr = mr / group, seen = attn_seen(a1, sr, tr), khr = hr % a1.kv_heads;
     const int last = min(mr / tile_rows * tile_rows + tile_rows, sr.nq * group) - 1;
     if (seen <= attn_spoilt<T>(a1, sr, khr, seen, attn_seen(a1, sr, last / group) + kAttnKeys))
-      attn_row<T, kCap, kSlope>(a1, sr, khr * group + mr % group, tr, seen, qs[wave]);
+      attn_row<T, kCap, kSlope, kShared>(a1, sr, khr * group + mr % group, tr, seen, qs[wave], sh);
   }
+}
+
+template <int T, int D, int kParts, bool kCap, bool kSlope>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_rows, int tiles,
+                                                        int splits, int chunk, const float* ws) {
+  attn_join<T, D, kParts, kCap, kSlope, false>(a, AttnShared{}, tile_rows, tiles, splits, chunk, 0, 0, ws);
 }
 
 }  // namespace imq

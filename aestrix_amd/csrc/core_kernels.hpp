@@ -71,7 +71,21 @@ AttnPlan attention_plan(const AttnArgs& a, int cus);
 hipError_t launch_attention(const AttnArgs& a, const AttnPlan& plan, float* ws, int dtype,
                             hipStream_t stream);
 
-hipError_t launch_attention_shared(const AttnArgs& a, const AttnShared& sh, int dtype,
-                                   hipStream_t stream);
+// How a call behind shared keys runs.
+struct SharedPlan {
+  int kernel;      // an imq_shared_kernel
+  AttnPlan tiles;  // IMQ_SHARED_TILES: of the walk over the shared and the own keys
+  // IMQ_SHARED_STREAM: rows of the batch against the shared keys, in tiles of s_rows, and the
+  // ranges of the shared and of each sequence's own keys.
+  int s_rows, s_tiles, s_splits, s_chunk, o_splits, o_chunk;
+  size_t bytes;    // workspace of the partial sums
+};
+// workspace: there is one.
+SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cus, bool workspace);
+// ws: plan.bytes of device memory.
+hipError_t launch_attention_shared_bf16(const AttnArgs& a, const AttnShared& sh, const SharedPlan& p, float* ws,
+                                        hipStream_t stream);
+hipError_t launch_attention_shared_f16(const AttnArgs& a, const AttnShared& sh, const SharedPlan& p, float* ws,
+                                       hipStream_t stream);
 
 }  // namespace imq

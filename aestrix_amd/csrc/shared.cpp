@@ -45,9 +45,35 @@ int imq_attention_shared(imq_ctx* ctx, const imq_attention_args* args,
   if (sh.rows == 0) return imq_attention(ctx, args, stream);
   if (a.n_seq == 0 || a.max_q == 0) return IMQ_OK;
   if ((rc = bind_device(ctx)) != IMQ_OK) return rc;
-  const hipError_t e =
-      imq::launch_attention_shared(a, sh, args->dtype, static_cast<hipStream_t>(stream));
+  const auto st = static_cast<hipStream_t>(stream);
+  imq::SharedPlan plan = imq::attention_shared_plan(a, sh, ctx->cus, true);
+  SplitHold hold;  // until the join is enqueued
+  if (plan.bytes > 0) {
+    hold = split_ws(ctx, st, plan.bytes);
+    // It would have to grow under capture, or memory is short.
+    if (!hold.ws.p) plan = imq::attention_shared_plan(a, sh, ctx->cus, false);
+  }
+  const hipError_t e = args->dtype == IMQ_BF16
+                           ? imq::launch_attention_shared_bf16(a, sh, plan, hold.ws.p, st)
+                           : imq::launch_attention_shared_f16(a, sh, plan, hold.ws.p, st);
   return e == hipSuccess ? IMQ_OK : hip_fail(ctx, e, fn);
+}
+
+int imq_attention_shared_plan(imq_ctx* ctx, const imq_attention_args* args, const imq_shared_keys* shared,
+                              imq_shared_plan_info* out) {
+  const char* fn = "imq_attention_shared_plan";
+  imq::AttnArgs a{};
+  imq::AttnShared sh{};
+  int rc = check_attention(ctx, fn, args, &a);
+  if (rc != IMQ_OK || (rc = check_shared(ctx, fn, args, shared, &sh)) != IMQ_OK) return rc;
+  if (!out) return fail(ctx, IMQ_EINVAL, "%s: null output", fn);
+  const imq::SharedPlan p = imq::attention_shared_plan(a, sh, ctx->cus, true);
+  out->kernel = p.kernel;
+  out->tile_rows = p.kernel == IMQ_SHARED_STREAM ? p.s_rows : p.kernel == IMQ_SHARED_TILES ? p.tiles.tile_rows : 1;
+  out->splits = p.kernel == IMQ_SHARED_STREAM ? p.s_splits : p.kernel == IMQ_SHARED_TILES ? p.tiles.splits : 1;
+  out->own_splits = p.kernel == IMQ_SHARED_STREAM ? p.o_splits : 0;
+  out->workspace_bytes = p.bytes;
+  return IMQ_OK;
 }
 
 }  // extern "C"

@@ -192,6 +192,25 @@ typedef struct imq_shared_keys {
 int imq_attention_shared(imq_ctx* ctx, const imq_attention_args* args,
                          const imq_shared_keys* shared, imq_stream stream);
 
+typedef enum imq_shared_kernel {
+  IMQ_SHARED_ROWS = 0,  /* a wave a row (dims past 128 or not a multiple of 8, unaligned tensors) */
+  IMQ_SHARED_TILES = 1, /* a sequence's tiles walk the shared and then the own keys */
+  IMQ_SHARED_STREAM = 2 /* up to 32 rows a sequence: all sequences' rows together against the shared
+                           keys, each one's against its own, and a join */
+} imq_shared_kernel;
+
+typedef struct imq_shared_plan_info {
+  int kernel;     /* an imq_shared_kernel */
+  int tile_rows;  /* rows (queries times heads a key head) of a workgroup, shared keys */
+  int splits;     /* ranges of the shared keys (of the walk over both: IMQ_SHARED_TILES) */
+  int own_splits; /* ranges of a sequence's own keys (IMQ_SHARED_STREAM) */
+  size_t workspace_bytes;
+} imq_shared_plan_info;
+
+/* What imq_attention_shared would run, as imq_attention_plan. */
+int imq_attention_shared_plan(imq_ctx* ctx, const imq_attention_args* args,
+                              const imq_shared_keys* shared, imq_shared_plan_info* out);
+
 #ifdef __cplusplus
 }
 #endif

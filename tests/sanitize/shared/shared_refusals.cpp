@@ -19,11 +19,15 @@ hipError_t launch_ln_mod(const void*, int, const float*, const float*, const int
   return hipErrorNoDevice;
 }
 hipError_t launch_rope(const RopeArgs&, bool, int, hipStream_t) { return hipErrorNoDevice; }
-AttnPlan attention_plan(const AttnArgs&, int) { return AttnPlan{IMQ_ATTENTION_ROWS, 1, 1, 0, 0, 0}; }
 hipError_t launch_attention(const AttnArgs&, const AttnPlan&, float*, int, hipStream_t) {
   return hipErrorNoDevice;
 }
-hipError_t launch_attention_shared(const AttnArgs&, const AttnShared&, int, hipStream_t) {
+hipError_t launch_attention_shared_bf16(const AttnArgs&, const AttnShared&, const SharedPlan&, float*,
+                                        hipStream_t) {
+  return hipErrorNoDevice;
+}
+hipError_t launch_attention_shared_f16(const AttnArgs&, const AttnShared&, const SharedPlan&, float*,
+                                       hipStream_t) {
   return hipErrorNoDevice;
 }
 }  // namespace imq
