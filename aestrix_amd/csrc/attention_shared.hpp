@@ -22,12 +22,19 @@ namespace imq {
 
 // ---- few rows a sequence
 
-template <int D>
+// With R = 2 the queries lie in LDS, as the fragments that a wave reads, and two workgroups
+// have all of a CU's: what the end needs takes their place.
+template <int D, int R>
 struct StreamLds {
   uint4 k[kFewWaves][kFewKeys * D / 8];
   uint4 v[kFewWaves][kFewKeys * D / 8];
-  float2 ml[kFewWaves][32];
-  int64_t dst[32];
+  union {
+    uint4 q[R > 1 ? R * D / 16 : 1][64];
+    struct {
+      float2 ml[kFewWaves][32];
+      int dst[32];
+    } end;
+  };
 };
 
 // Keys at k and v, `rows` of them that may be read.
@@ -44,12 +51,12 @@ struct StreamKeys {
 // buffer each and take turns: K of the next tile is loaded while the weights and the product
 // with V are made, V while the next scores are.  With R = 2 a fragment of K or V is read from
 // LDS once for two MFMAs.
-template <int T, int D, int R, bool kCap, bool kSlope>
-__device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D>& lds, const StreamKeys& keys,
+template <int T, int D, int R, int kLdsR, bool kCap, bool kSlope>
+__device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D, kLdsR>& lds, const StreamKeys& keys,
                                             int begin, int end, const s16x8_t (&qf)[R][D / 16],
                                             const AttnScore<kCap, kSlope> (&score)[R], const int (&seen)[R],
                                             int seen_lo, const int (&p)[R], int near,
-                                            const int64_t (&dst)[R], float* po, float2* pml) {
+                                            const int (&dst)[R], float* po, float2* pml) {
   constexpr int kPieces = kFewKeys * D / 8, kLoads = kPieces / 64;
   // bf16 weights as two bf16 each, as in attn_few_kernel: the matrix cores have the time.
   constexpr bool kRest = T == kBf16;
@@ -81,11 +88,10 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D>& lds
   load(keys.k, keys.kb, k_off, kl, min(first, end - 1));
   load(keys.v, keys.vb, v_off, vl, min(first, end - 1));
   __builtin_amdgcn_sched_barrier(0);
-  f32x16_t c0[R], o[R][D / 32];
+  f32x16_t o[R][D / 32];
   float top[R], sum[R];
 #pragma unroll
   for (int g = 0; g < R; ++g) {
-    c0[g] = attn_start(score[g]);
     top[g] = -INFINITY, sum[g] = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -95,6 +101,17 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D>& lds
   __builtin_amdgcn_sched_barrier(0);
   IMQ_WAIT_VMCNT(2 * kLoads);  // what the caller loaded is in registers
   __builtin_amdgcn_sched_barrier(0);
+  if constexpr (R > 1) {
+#pragma unroll
+    for (int g = 0; g < R; ++g)
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        if (i % kFewWaves == wave) lds.q[g * (D / 16) + i][lane] = __builtin_bit_cast(uint4, qf[g][i]);
+    __builtin_amdgcn_sched_barrier(0);
+    IMQ_WAIT_LGKM_0();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  }
   const int kf = D == 128 ? (c & 15) : ((c >> 1) & 7);           // k_piece's
   const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2);           // of 8 rows
   const int vf = D == 128 ? 4 * (vr & 3) : 4 * ((vr >> 1) & 1);  // v_piece's
@@ -107,12 +124,20 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D>& lds
     __builtin_amdgcn_sched_barrier(0);
     f32x16_t sc[R][1];
 #pragma unroll
-    for (int g = 0; g < R; ++g) sc[g][0] = c0[g];
+    for (int g = 0; g < R; ++g) {
+      // Made anew for every tile: kept, it takes 16 registers a row that there are not.
+      AttnScore<kCap, kSlope> from = score[g];
+      if constexpr (kSlope && !kCap) asm volatile("" : "+v"(from.fall));
+      sc[g][0] = attn_start(from);
+    }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       const s16x8_t kv = __builtin_bit_cast(s16x8_t, kl[c * (D / 8) + ((2 * i + h) ^ kf)]);
 #pragma unroll
-      for (int g = 0; g < R; ++g) sc[g][0] = attn_mfma<T>(kv, qf[g][i], sc[g][0]);
+      for (int g = 0; g < R; ++g) {
+        const s16x8_t qv = R > 1 ? __builtin_bit_cast(s16x8_t, lds.q[g * (D / 16) + i][lane]) : qf[g][i];
+        sc[g][0] = attn_mfma<T>(kv, qv, sc[g][0]);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
     IMQ_WAIT_LGKM_0();  // K has been read
@@ -162,7 +187,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D>& lds
   // into its V buffer.
 #pragma unroll
   for (int g = 0; g < R; ++g) {
-    if (g > 0) __syncthreads();  // the last 32 rows have been read
+    if (R > 1) __syncthreads();  // the queries, or the last 32 rows, have been read
     const float total = pair_sum(sum[g]);
     float* part = reinterpret_cast<float*>(c < 16 ? lds.k[wave] : lds.v[wave]) + (c & 15) * D;
 #pragma unroll
@@ -171,25 +196,25 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D>& lds
       for (int e = 0; e < 16; e += 4)
         *reinterpret_cast<float4*>(part + i * 32 + 2 * e + 4 * h) =
             make_float4(o[g][i][e], o[g][i][e + 1], o[g][i][e + 2], o[g][i][e + 3]);
-    if (h == 0) lds.ml[wave][c] = make_float2(top[g], total);
-    if (threadIdx.x < 32) lds.dst[c] = dst[g];
+    if (h == 0) lds.end.ml[wave][c] = make_float2(top[g], total);
+    if (threadIdx.x < 32) lds.end.dst[c] = dst[g];
     __syncthreads();
     constexpr int kPer = D / 4;  // threads of a row, four columns each
 #pragma unroll
     for (int r = threadIdx.x / kPer; r < 32; r += kFewWaves * 64 / kPer) {
-      const int64_t to = lds.dst[r];
+      const int64_t to = lds.end.dst[r];
       if (to < 0) continue;
       const int d = threadIdx.x % kPer * 4;
       float tops = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) tops = fmaxf(tops, lds.ml[w][r].x);
+      for (int w = 0; w < kFewWaves; ++w) tops = fmaxf(tops, lds.end.ml[w][r].x);
       const float base = tops == -INFINITY ? 0.f : tops;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       float sums = 0.f;
 #pragma unroll
       for (int w = 0; w < kFewWaves; ++w) {
-        const float keep = __builtin_amdgcn_exp2f(lds.ml[w][r].x - base);
-        sums = __builtin_fmaf(lds.ml[w][r].y, keep, sums);
+        const float keep = __builtin_amdgcn_exp2f(lds.end.ml[w][r].x - base);
+        sums = __builtin_fmaf(lds.end.ml[w][r].y, keep, sums);
         const float4 v = *reinterpret_cast<const float4*>(
             reinterpret_cast<const float*>(r < 16 ? lds.k[w] : lds.v[w]) + (r & 15) * D + d);
         acc.x = __builtin_fmaf(v.x, keep, acc.x);
@@ -208,11 +233,11 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D>& lds
 // the batch and s_chunk shared keys, then one for a sequence, key head and o_chunk own keys.
 // Ranges to ws as attn_join has them, the shared keys' s_splits first.
 template <int T, int D, int R, bool kCap, bool kSlope>
-__global__ __launch_bounds__(kFewWaves * 64, 1) void attn_stream_kernel(
+__global__ __launch_bounds__(kFewWaves * 64, 2) void attn_stream_kernel(
     AttnArgs a, AttnShared sh, int rows, int s_tiles, int s_splits, int s_chunk, int o_splits, int o_chunk,
     float* ws) {
   using S = typename Elem<T>::S;
-  __shared__ StreamLds<D> lds;
+  __shared__ StreamLds<D, R> lds;
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int group = a.heads / a.kv_heads, hs_n = a.n_seq * a.kv_heads;
   const int64_t all = (int64_t)hs_n * rows;
@@ -222,7 +247,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 1) void attn_stream_kernel(
     const int kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
     const int tile = rest % s_tiles, split = rest / s_tiles;
     s16x8_t qf[R][D / 16];
-    int64_t dst[R];
+    int dst[R];
     int seen[R], p[R], at[R];
 #pragma unroll
     for (int g = 0; g < R; ++g) {
@@ -232,7 +257,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 1) void attn_stream_kernel(
       int t = r / group;
       at[g] = kh * group + r % group;
       const bool live = m < a.n_seq * rows && t < s.nq;
-      dst[g] = live ? ((int64_t)seq * a.kv_heads + kh) * rows + r : -1;
+      dst[g] = live ? (seq * a.kv_heads + kh) * rows + r : -1;  // up to 2^25
       seen[g] = sh.rows;
       p[g] = t + s.nk - s.nq + sh.rows;
       if (!live) s.q_at = 0, t = 0;  // a row that is there
@@ -254,7 +279,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 1) void attn_stream_kernel(
     const StreamKeys keys{static_cast<const char*>(sh.k) + kh * sh.k_head * 2,
                           static_cast<const char*>(sh.v) + kh * sh.v_head * 2, sh.k_row * 2, sh.v_row * 2,
                           sh.rows};
-    attn_stream<T, D, R, kCap, kSlope>(a, lds, keys, begin, min(sh.rows, begin + s_chunk), qf, score, seen,
+    attn_stream<T, D, R, R, kCap, kSlope>(a, lds, keys, begin, min(sh.rows, begin + s_chunk), qf, score, seen,
                                        sh.rows, p, near, dst, ws + split * all * D, ml + split * all);
     return;
   }
@@ -272,7 +297,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 1) void attn_stream_kernel(
   s16x8_t qf[1][D / 16];
   attn_load_q<T, D>(a, s, t, head, h, qf[0]);
   const AttnScore<kCap, kSlope> score[1] = {AttnScore<kCap, kSlope>(a, head)};
-  const int64_t dst[1] = {c < live ? (int64_t)hs * rows + c : -1};
+  const int dst[1] = {c < live ? hs * rows + c : -1};
   // Keys below `near` are at or before every row's p, or hidden behind it.
   const int near = a.causal && !a.prefix_lens ? INT_MAX : s.nk - s.nq + 1;
   const StreamKeys keys{
@@ -280,7 +305,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 1) void attn_stream_kernel(
       reinterpret_cast<const char*>(static_cast<const S*>(a.v) + s.v_at + kh * a.v_head), a.k_row * 2,
       a.v_row * 2, s.nk};
   const int64_t range = s_splits + split;
-  attn_stream<T, D, 1, kCap, kSlope>(a, lds, keys, begin, end, qf, score, seen, seen_lo, p, near, dst,
+  attn_stream<T, D, 1, R, kCap, kSlope>(a, lds, keys, begin, end, qf, score, seen, seen_lo, p, near, dst,
                                      ws + range * all * D, ml + range * all);
 }
 
@@ -343,7 +368,7 @@ hipError_t launch_stream(const AttnArgs& a, const AttnShared& sh, const SharedPl
 }
 
 template <int T, int D, int WM, bool kCap, bool kSlope>
-hipError_t launch_shared_tiles(const AttnArgs& a, const AttnShared& sh, const AttnPlan& plan, float* ws,
+hipError_t launch_shared_tiles(const AttnArgs& a, const AttnShared& sh, const AttnPlan& plan, int own0, float* ws,
                                hipStream_t stream) {
   constexpr int kRows = WM * 32;
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
@@ -356,7 +381,7 @@ hipError_t launch_shared_tiles(const AttnArgs& a, const AttnShared& sh, const At
                          dim3((unsigned)(blocks * plan.splits)), block, 0, stream, a, sh, tiles, plan.first,
                          1, plan.splits, plan.chunk, ws);
       launch_shared_join<T, D, kCap, kSlope>(a, sh, kRows, tiles, blocks * kRows, plan.splits, plan.chunk, 0,
-                                             (sh.rows + kAttnKeys - 1) / kAttnKeys * kAttnKeys, ws, stream);
+                                             own0, ws, stream);
       return hipGetLastError();
     }
   }
@@ -385,12 +410,12 @@ hipError_t launch_shared_scored(const AttnArgs& a, const AttnShared& sh, const S
     default: break;
   }
   switch (wide ? p.tiles.tile_rows : -p.tiles.tile_rows) {
-    case 256: return launch_shared_tiles<T, 128, 8, kCap, kSlope>(a, sh, p.tiles, ws, stream);
-    case 128: return launch_shared_tiles<T, 128, 4, kCap, kSlope>(a, sh, p.tiles, ws, stream);
-    case 64: return launch_shared_tiles<T, 128, 2, kCap, kSlope>(a, sh, p.tiles, ws, stream);
-    case -256: return launch_shared_tiles<T, 64, 8, kCap, kSlope>(a, sh, p.tiles, ws, stream);
-    case -128: return launch_shared_tiles<T, 64, 4, kCap, kSlope>(a, sh, p.tiles, ws, stream);
-    case -64: return launch_shared_tiles<T, 64, 2, kCap, kSlope>(a, sh, p.tiles, ws, stream);
+    case 256: return launch_shared_tiles<T, 128, 8, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
+    case 128: return launch_shared_tiles<T, 128, 4, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
+    case 64: return launch_shared_tiles<T, 128, 2, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
+    case -256: return launch_shared_tiles<T, 64, 8, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
+    case -128: return launch_shared_tiles<T, 64, 4, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
+    case -64: return launch_shared_tiles<T, 64, 2, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
     default: return hipErrorInvalidValue;
   }
 }

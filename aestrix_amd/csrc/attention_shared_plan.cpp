@@ -20,7 +20,7 @@ SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cu
   p.kernel = IMQ_SHARED_ROWS;
   const int64_t far = (int64_t)1 << 24;  // elements of a row, as for the own keys
   const int64_t strides = sh.k_row | sh.k_head | sh.v_row | sh.v_head;
-  const int64_t own0 = ((int64_t)sh.rows + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
+  const int64_t own0 = ((int64_t)sh.rows + 2 * kAttnKeys - 1) / (2 * kAttnKeys) * (2 * kAttnKeys);
   // (Rows of values that begin inside the row before: a tile's last would read on past
   // the end of the shared ones.)
   if (strides % 8 != 0 || ((uintptr_t)sh.k | (uintptr_t)sh.v) % 16 != 0 || sh.k_row > far - 128 ||
@@ -29,8 +29,14 @@ SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cu
   // The walk over both.
   AttnArgs walk = a;
   walk.max_k = (int)own0 + a.max_k;
+  p.own0 = (int)own0;
   if (a.max_k == 0) walk.k = walk.v = nullptr;
   p.tiles = attention_plan(walk, cus);
+  if (p.tiles.chunk % (2 * kAttnKeys)) {  // ranges of whole pairs of tiles
+    const int chunk = p.tiles.chunk + kAttnKeys, splits = ranges(walk.max_k, chunk);
+    p.tiles.bytes = p.tiles.bytes / p.tiles.splits * splits;
+    p.tiles.chunk = chunk, p.tiles.splits = splits;
+  }
   if (p.tiles.kernel == IMQ_ATTENTION_ROWS) return p;
   const int rows = a.max_q * (a.heads / a.kv_heads);
   const int64_t hs = (int64_t)a.n_seq * a.kv_heads;
