@@ -1,56 +1,356 @@
-// lora.hip -- the first product of adapters beside a projection: u = scale * A x, a row's
-// adapter's (include/imq_lora.h).
+// lora.hip -- the products of adapters beside a projection that stand outside its kernels: u =
+// scale * A x, a row's adapter's, and the join of the projection's partial sums with B u
+// (include/imq_lora.h).
 #include "lora_device.hpp"
 
 namespace imq {
 namespace {
 
-constexpr int kThreads = 256;
+// ---- u
 
-// A wave per row and rank.
+// The rows of a tile by what adapters they name; a lane's row is r32 (in both halves).
+struct LoraRows {
+  int id;     // of this lane's row, -1: none
+  LoraAt at;  // its adapter's, looked up for all rows together
+
+  __device__ __forceinline__ LoraRows(const LoraArgs& l, int row, int m) {
+    id = row < m ? lora_of(l, row) : -1;
+    at = lora_at(l, max(id, 0));
+  }
+  // The j-th adapter (from 0) that they name, in the order of their first rows, and its rows; -1
+  // where there are fewer.
+  __device__ __forceinline__ int nth(int j, uint32_t& rows, LoraAt& to) const {
+    uint32_t left = (uint32_t)__builtin_amdgcn_ballot_w64(id >= 0);
+    while (left) {
+      const int lead = __builtin_ctz(left), i = __builtin_amdgcn_readlane(id, lead);
+      rows = (uint32_t)__builtin_amdgcn_ballot_w64(id == i);
+      if (j-- == 0) {
+        to = LoraAt{__builtin_amdgcn_readlane(at.row, lead), __builtin_amdgcn_readlane(at.rank, lead)};
+        return i;
+      }
+      left &= ~rows;
+    }
+    return -1;
+  }
+};
+
+// u of row `row` and rank `rank` to its place: the upper half, and what it leaves (nothing where
+// it is infinite).
 template <int T>
-__global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs l, const uint16_t* x, int k,
-                                                              int m) {
+__device__ __forceinline__ void lora_put(const LoraArgs& l, int row, int rank, float u) {
+  const uint16_t hi = Elem<T>::out(u);
+  const float v = staged_value<T>(hi);
+  const uint16_t lo = Elem<T>::out(__builtin_fabsf(v) < INFINITY ? u - v : 0.f);
+  uint16_t* to = l.u + (((size_t)(row / 32) * (l.max_rank / 16) + rank / 16) * 2 * 64 + row % 32 +
+                        32 * (rank >> 3 & 1)) * 8 + (rank & 7);
+  to[0] = hi;
+  to[64 * 8] = lo;
+}
+
+// Few rows: a wave per row and rank.  Bound by reading A, and by the latency of that: eight
+// pieces of 1 KB of each of the two rows are on their way together.
+constexpr int kDotWaves = 4, kDotMaxM = 64;
+template <int T>
+__global__ __launch_bounds__(kDotWaves * 64) void lora_dot_kernel(LoraArgs l, const uint16_t* x, int k, int m) {
   const int lane = threadIdx.x & 63;
-  const int64_t items = (int64_t)m * l.max_rank, step = (int64_t)gridDim.x * (kThreads / 64);
-  for (int64_t at = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); at < items; at += step) {
-    const int row = (int)(at / l.max_rank), r = (int)(at % l.max_rank);
-    const int i = lora_of(l, row);
-    if (i < 0) continue;
-    const LoraAt to = lora_at(l, i);
-    if (r >= to.rank) continue;
-    const uint16_t* a = l.a + (size_t)(to.row + r) * k;
-    const uint16_t* xr = x + (size_t)row * k;
-    float sum = 0.f;
-    for (int c = lane * 8; c < k; c += 512) {
-      const uint4 av = *reinterpret_cast<const uint4*>(a + c), xv = *reinterpret_cast<const uint4*>(xr + c);
-      const uint32_t aw[4] = {av.x, av.y, av.z, av.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
+  const int at = blockIdx.x * kDotWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = at / l.max_rank, r = at % l.max_rank;  // up to 64 rows
+  if (row >= m) return;
+  const int i = lora_of(l, row);
+  if (i < 0) return;
+  const LoraAt to = lora_at(l, i);
+  if (r >= to.rank) return;
+  const __amdgpu_buffer_rsrc_t ar = make_rsrc(l.a + (size_t)(to.row + r) * k, (uint32_t)k * 2);
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(x + (size_t)row * k, (uint32_t)k * 2);
+  float sum[2] = {0.f, 0.f};
+  constexpr int kAhead = 8;
+  for (int c = 0; c < k; c += kAhead * 512) {
+    u32x4_t av[kAhead], xv[kAhead];  // (past the end: zeros)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        sum = T == kBf16 ? dot2_bf16(aw[e], xw[e], sum) : dot2_f16(aw[e], xw[e], sum);
+    for (int p = 0; p < kAhead; ++p) {
+      av[p] = load_b128(ar, lane * 16, (uint32_t)c * 2 + p * 1024);
+      xv[p] = load_b128(xr, lane * 16, (uint32_t)c * 2 + p * 1024);
     }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    if (lane == 0) l.u[at] = sum * l.scale[i];
+    for (int p = 0; p < kAhead; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sum[e & 1] = T == kBf16 ? dot2_bf16(av[p][e], xv[p][e], sum[e & 1])
+                                : dot2_f16(av[p][e], xv[p][e], sum[e & 1]);
+  }
+  float u = sum[0] + sum[1];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) u += __shfl_xor(u, off, 64);
+  if (lane == 0) lora_put<T>(l, row, r, u * l.scale[i]);
+}
+
+// More rows.  A workgroup: 32 of them against 32 ranks (blockIdx.y) of the adapters that they
+// name, one after the other.  Its eight waves take K in turn, 64 at a time, from buffers of their
+// own: whole 128-byte lines of x's and A's rows straight to LDS (operands loaded straight to
+// registers touch 32 bytes of a line each, and 16 such waves took 35 us of 4608 rows of 2560), the
+// next piece on its way while one is multiplied.  16-byte pieces are swizzled by the row at their
+// source, so that the operand reads touch every bank evenly.  The waves' sums are added through LDS.
+constexpr int kShrinkWaves = 8;
+struct ShrinkBuf {
+  uint4 x[32 * 8], a[32 * 8];
+};
+template <int T>
+__global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs l, const uint16_t* x,
+                                                                       int k, int m) {
+  __shared__ union {
+    ShrinkBuf buf[kShrinkWaves][2];
+    float sums[kShrinkWaves][32 * 32];
+  } lds;
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x, r0 = blockIdx.y * 32;
+  const int pieces = k / 64;
+  const uint32_t kb = (uint32_t)k * 2;
+  // This lane's 16 bytes of the rows 8 s + lane / 8; grouped rows stand anywhere in x, which is
+  // under 2^31 bytes then.
+  const __amdgpu_buffer_rsrc_t xr =
+      l.order ? make_rsrc(x, (uint32_t)m * kb)
+              : make_rsrc(x + (size_t)tile * 32 * k, (uint32_t)min(32, m - tile * 32) * kb);
+  uint32_t x_off[4], a_off[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const uint32_t r = s * 8 + lane / 8, c = ((lane ^ r) & 7) * 16;
+    a_off[s] = r * kb + c;
+    x_off[s] = l.order ? (uint32_t)l.order[min(tile * 32 + (int)r, m - 1)] * kb + c : a_off[s];
+  }
+  auto load_x = [&](int p, int set) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      load_lds16(xr, x_off[s], (uint32_t)min(p, pieces - 1) * 128, lds.buf[wave][set].x + s * 64);
+  };
+  // The first adapter's x, before it is known which that is.
+  load_x(wave, 0);
+  const LoraRows of_tile(l, tile * 32 + r32, m);
+  uint32_t rows;
+  LoraAt at;
+  bool ahead = true;
+  for (int j = 0;; ++j) {
+    const int i = of_tile.nth(j, rows, at);
+    if (i < 0) break;
+    if (r0 >= at.rank) continue;
+    // (Ranks past the last are zeros.)
+    const __amdgpu_buffer_rsrc_t ar =
+        make_rsrc(l.a + (size_t)(at.row + r0) * k, (uint32_t)min(32, at.rank - r0) * kb);
+    f32x16_t c;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) c[e] = 0.f;
+    // (Past the last piece it is loaded again, so that the counts of loads in flight hold.)
+    auto load_a = [&](int p, int set) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        load_lds16(ar, a_off[s], (uint32_t)min(p, pieces - 1) * 128, lds.buf[wave][set].a + s * 64);
+    };
+    if (!ahead) load_x(wave, 0);
+    ahead = false;
+    load_a(wave, 0);
+    int set = 0;
+    for (int p = wave; p < pieces; p += kShrinkWaves, set ^= 1) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_x(p + kShrinkWaves, set ^ 1);
+      load_a(p + kShrinkWaves, set ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
+      IMQ_WAIT_VMCNT(8);  // this piece has landed
+      __builtin_amdgcn_sched_barrier(0);
+      const ShrinkBuf& from = lds.buf[wave][set];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int slot = r32 * 8 + ((2 * s + h) ^ (r32 & 7));
+        c = lora_mfma<T>(__builtin_bit_cast(u32x4_t, from.x[slot]), __builtin_bit_cast(u32x4_t, from.a[slot]), c);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      IMQ_WAIT_LGKM_0();  // and has been read
+    }
+    const float scale = l.scale[i];
+    __builtin_amdgcn_sched_barrier(0);
+    IMQ_WAIT_VMCNT(0);
+    __syncthreads();  // every wave's pieces have landed and been read
+#pragma unroll
+    for (int e = 0; e < 16; ++e) lds.sums[wave][(8 * (e >> 2) + 4 * h + (e & 3)) * 32 + r32] = c[e];
+    __syncthreads();
+#pragma unroll
+    for (int o = threadIdx.x; o < 32 * 32; o += kShrinkWaves * 64) {
+      const int of = o >> 5, rank = r0 + (o & 31);
+      float u = 0.f;
+#pragma unroll
+      for (int v = 0; v < kShrinkWaves; ++v) u += lds.sums[v][o];
+      if ((rows >> of & 1u) && rank < at.rank) lora_put<T>(l, tile * 32 + of, rank, u * scale);
+    }
+    __syncthreads();  // the sums have been read
+  }
+  IMQ_WAIT_VMCNT(0);  // x of no adapter, before the workgroup's LDS is another's
+}
+
+// ---- the order of the rows
+
+// One workgroup: each of its 16 waves counts the rows of a stretch by adapter, the counts are
+// added up over adapters and waves, and each wave gives its rows their places, 64 at a time, in
+// their order.  Up to kOrderKeep * 1024 rows are read once, all together.  More adapters than
+// kOrderBins - 1: the rows stay as they are.
+constexpr int kOrderWaves = 16, kOrderBins = 1024, kOrderKeep = 8;
+__global__ __launch_bounds__(kOrderWaves * 64) void lora_order_kernel(LoraArgs l, int32_t* order,
+                                                                     int32_t* which_at, int m) {
+  __shared__ int at[kOrderWaves][kOrderBins];
+  __shared__ int sums[kOrderBins];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bins = l.count + 1;  // the last one: no adapter
+  if (bins > kOrderBins) {
+    for (int r = threadIdx.x; r < m; r += kOrderWaves * 64) {
+      order[r] = r;
+      which_at[r] = lora_of(l, r);
+    }
+    return;
+  }
+  const int per = ((m + kOrderWaves - 1) / kOrderWaves + 63) / 64 * 64;
+  const int begin = min(wave * per, m), end = min(begin + per, m);
+  auto bin = [&](int r) {
+    const int i = r < end ? lora_of(l, r) : -2;
+    return i == -1 ? l.count : i;  // below 0: no row
+  };
+  int kept[kOrderKeep];
+#pragma unroll
+  for (int t = 0; t < kOrderKeep; ++t) kept[t] = bin(begin + t * 64 + lane);
+  for (int w = 0; w < kOrderWaves; ++w)
+    if ((int)threadIdx.x < bins) at[w][threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < kOrderKeep; ++t)
+    if (kept[t] >= 0) atomicAdd(&at[wave][kept[t]], 1);
+  for (int r = begin + kOrderKeep * 64 + lane; r < end; r += 64) atomicAdd(&at[wave][bin(r)], 1);
+  __syncthreads();
+  // Of every bin its rows, then over the bins (a scan by doubling steps).
+  int mine = 0;
+  if ((int)threadIdx.x < bins)
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) mine += at[w][threadIdx.x];
+  sums[threadIdx.x] = mine;
+  __syncthreads();
+  for (int step = 1; step < bins; step *= 2) {
+    const int v = (int)threadIdx.x >= step ? sums[threadIdx.x - step] : 0;
+    __syncthreads();
+    sums[threadIdx.x] += v;
+    __syncthreads();
+  }
+  if ((int)threadIdx.x < bins) {
+    int from = sums[threadIdx.x] - mine;
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) {
+      const int n = at[w][threadIdx.x];
+      at[w][threadIdx.x] = from;
+      from += n;
+    }
+  }
+  __syncthreads();
+  auto place = [&](int r, int b) {
+    uint64_t left = __builtin_amdgcn_ballot_w64(b >= 0);
+    while (left) {
+      const int i = __builtin_amdgcn_readlane(b, __builtin_ctzll(left));
+      const uint64_t rows = __builtin_amdgcn_ballot_w64(b == i);
+      left &= ~rows;
+      const int from = at[wave][i];
+      __builtin_amdgcn_wave_barrier();
+      if (b == i) {
+        const int to = from + __builtin_popcountll(rows & (((uint64_t)1 << lane) - 1));
+        order[to] = r;
+        which_at[to] = i < l.count ? i : -1;
+      }
+      if (lane == 0) at[wave][i] = from + __builtin_popcountll(rows);
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < kOrderKeep; ++t) place(begin + t * 64 + lane, kept[t]);
+  for (int r0 = begin + kOrderKeep * 64; r0 < end; r0 += 64) place(r0 + lane, bin(r0 + lane));
+}
+
+// ---- the join
+
+// A workgroup: 32 rows and 32 columns of y.  Its 16 waves take the adapters of the rows in
+// turn; each writes its rows' products to LDS (a row has one adapter), where the ranges' sums
+// are added to them in order.  Bound by the latency of what a wave loads for an adapter; the
+// ranges' sums are on the way meanwhile.
+constexpr int kJoinWaves = 16;
+template <int T>
+__global__ __launch_bounds__(kJoinWaves * 64) void lora_join_kernel(LoraArgs l, const float* part, int splits,
+                                                                   uint16_t* y, int n, int m) {
+  __shared__ float add[32 * 32];
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 32, tile = blockIdx.y;
+  const LoraRows of_tile(l, tile * 32 + r32, m);
+  constexpr int kOuts = 32 * 32 / (kJoinWaves * 64);  // outputs of a thread
+  const int col = n0 + (int)(threadIdx.x & 31), of = threadIdx.x >> 5;
+  float sum[kOuts];
+#pragma unroll
+  for (int o = 0; o < kOuts; ++o) {
+    sum[o] = 0.f;
+    add[o * kJoinWaves * 64 + threadIdx.x] = 0.f;
+  }
+  for (int sp = 0; sp < splits; ++sp)
+#pragma unroll
+    for (int o = 0; o < kOuts; ++o) {
+      const size_t r = min(tile * 32 + of + o * (kJoinWaves * 2), m - 1);
+      sum[o] += part[((size_t)sp * m + r) * n + min(col, n - 1)];
+    }
+  __syncthreads();
+  uint32_t rows;
+  LoraAt at;
+  for (int j = wave; of_tile.nth(j, rows, at) >= 0; j += kJoinWaves) {
+    f32x16_t c[1];
+    lora_product<T, 1>(l, at, tile, n0, n, c);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int r = 8 * (e >> 2) + 4 * h + (e & 3);
+      if (rows >> r & 1u) add[r * 32 + r32] = c[0][e];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int o = 0; o < kOuts; ++o) {
+    const int r = of + o * (kJoinWaves * 2);
+    if (tile * 32 + r < m && col < n)
+      y[(size_t)(tile * 32 + r) * n + col] = Elem<T>::out(sum[o] + add[r * 32 + (threadIdx.x & 31)]);
   }
 }
 
 }  // namespace
 
+hipError_t launch_lora_order(const LoraArgs& l, int32_t* order, int32_t* which_at, int m, hipStream_t stream) {
+  hipLaunchKernelGGL(lora_order_kernel, dim3(1), dim3(kOrderWaves * 64), 0, stream, l, order, which_at, m);
+  return hipGetLastError();
+}
+
 hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, int dtype,
                               hipStream_t stream) {
-  const int64_t blocks = ((int64_t)m * l.max_rank + kThreads / 64 - 1) / (kThreads / 64);
-  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)));
   const auto* xx = static_cast<const uint16_t*>(x);
-  switch (dtype) {
-    case kBf16:
-      hipLaunchKernelGGL((lora_shrink_kernel<kBf16>), grid, dim3(kThreads), 0, stream, l, xx, k, m);
-      break;
-    case kF16:
-      hipLaunchKernelGGL((lora_shrink_kernel<kF16>), grid, dim3(kThreads), 0, stream, l, xx, k, m);
-      break;
-    default: return hipErrorInvalidValue;
+  if (m <= kDotMaxM) {
+    const dim3 grid((unsigned)((m * l.max_rank + kDotWaves - 1) / kDotWaves)), block(kDotWaves * 64);
+    if (dtype == kBf16)
+      hipLaunchKernelGGL((lora_dot_kernel<kBf16>), grid, block, 0, stream, l, xx, k, m);
+    else
+      hipLaunchKernelGGL((lora_dot_kernel<kF16>), grid, block, 0, stream, l, xx, k, m);
+    return hipGetLastError();
   }
+  const dim3 grid((unsigned)((m + 31) / 32), (unsigned)((l.max_rank + 31) / 32)), block(kShrinkWaves * 64);
+  if (dtype == kBf16)
+    hipLaunchKernelGGL((lora_shrink_kernel<kBf16>), grid, block, 0, stream, l, xx, k, m);
+  else
+    hipLaunchKernelGGL((lora_shrink_kernel<kF16>), grid, block, 0, stream, l, xx, k, m);
+  return hipGetLastError();
+}
+
+hipError_t launch_lora_join(const LoraArgs& l, const float* part, int splits, void* y, int n, int m,
+                            int dtype, hipStream_t stream) {
+  const dim3 grid((unsigned)((n + 31) / 32), (unsigned)((m + 31) / 32)), block(kJoinWaves * 64);
+  auto* yy = static_cast<uint16_t*>(y);
+  if (dtype == kBf16)
+    hipLaunchKernelGGL((lora_join_kernel<kBf16>), grid, block, 0, stream, l, part, splits, yy, n, m);
+  else
+    hipLaunchKernelGGL((lora_join_kernel<kF16>), grid, block, 0, stream, l, part, splits, yy, n, m);
   return hipGetLastError();
 }
 

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 namespace imq {
@@ -16,16 +17,42 @@ struct LoraArgs {
   const int32_t* first;
   const float* scale;
   const int32_t* which;
-  float* u;  // [m][max_rank]: scale * A x of each row's adapter
+  // u = scale * A x of each row's adapter, as operand fragments of the second product:
+  // [32 rows][16 ranks][upper halves, what they leave][64 lanes][8], lane r + 32 h row r's
+  // ranks 8 h to 8 h + 8.  Ranks past a row's adapter's are not written.
+  uint16_t* u;
   int count, rows, max_rank;
+  // Rows grouped by their adapters (launch_lora_order), or NULL: as they are.  `which` is then
+  // the places' (in the workspace), and u stands by places too.
+  const int32_t* order;
 };
+inline size_t lora_u_bytes(int m, int max_rank) {
+  return (size_t)((m + 31) / 32) * (max_rank / 16) * 2 * 64 * 8 * sizeof(uint16_t);
+}
 
+// How the projection of a call runs.
+struct LoraPlan {
+  int few;        // the few-row kernel's partial sums (qskinny.hip), ...
+  int splits;     // ... or the tile kernels': ranges of K, joined by launch_lora_join; 0: the
+                  // tile kernels add B u themselves
+  int mt, nt, split_steps;  // their tiles (BigPlan)
+  bool order;     // grouped rows (launch_lora_order)
+  size_t bytes;   // of the partial sums
+};
+LoraPlan lora_plan(int k, int n, int m, int count, int dtype);
+
+// Groups the rows by their adapters, those without one last, each group in its rows' order:
+// order [m] the row at a place, which_at [m] its adapter (lora.hip).
+hipError_t launch_lora_order(const LoraArgs& l, int32_t* order, int32_t* which_at, int m, hipStream_t stream);
 // u of every row (lora.hip).
 hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, int dtype,
                               hipStream_t stream);
-// y = T(x . deq(W)^T + B u) (qgemm.hip).
-hipError_t launch_qgemm_lora(const uint32_t* w, const void* scales, const void* biases, const void* x,
-                             const LoraArgs& l, void* y, int k, int n, int m, int dtype,
-                             hipStream_t stream);
+// y = T(sum of the ranges + B u) (lora.hip); part: fp32 [splits][m][n].
+hipError_t launch_lora_join(const LoraArgs& l, const float* part, int splits, void* y, int n, int m,
+                            int dtype, hipStream_t stream);
+// The projection: partial sums to part where the plan has them, else y (qgemm.hip).
+hipError_t launch_qgemm_lora(const LoraPlan& p, const uint32_t* w, const void* scales, const void* biases,
+                             const void* x, const LoraArgs& l, float* part, void* y, int k, int n, int m,
+                             int dtype, hipStream_t stream);
 
 }  // namespace imq

@@ -2,6 +2,9 @@
 // (include/imq_lora.h) and the tile kernels' output stage with them.
 #pragma once
 
+#include <climits>
+#include <type_traits>
+
 #include "epilogue.hpp"
 #include "imq_device.hpp"
 #include "lora.hpp"
@@ -22,19 +25,11 @@ __device__ __forceinline__ int lora_of(const LoraArgs& l, int row) {
   return (unsigned)i < (unsigned)l.count ? i : -1;
 }
 
-// Eight values of u as two of T each: the upper halves, and what they leave.
-template <int T>
-__device__ __forceinline__ void lora_split(const float* u, u32x4_t& hi, u32x4_t& lo) {
-  const float4 a = reinterpret_cast<const float4*>(u)[0], b = reinterpret_cast<const float4*>(u)[1];
-  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    hi[e] = Elem<T>::pack2(v[2 * e], v[2 * e + 1]);
-    const float h0 = staged_value<T>(hi[e] & 0xFFFFu), h1 = staged_value<T>(hi[e] >> 16);
-    // (Infinite as T: nothing is left, rather than a NaN.)
-    lo[e] = Elem<T>::pack2(__builtin_fabsf(h0) < INFINITY ? v[2 * e] - h0 : 0.f,
-                           __builtin_fabsf(h1) < INFINITY ? v[2 * e + 1] - h1 : 0.f);
-  }
+// u's fragment of 32 rows (tile), 16 ranks (chunk) and upper halves or what they leave (part)
+// for this lane.
+__device__ __forceinline__ const u32x4_t* lora_u(const LoraArgs& l, int tile, int chunk, int part) {
+  return reinterpret_cast<const u32x4_t*>(l.u) +
+         (((size_t)tile * (l.max_rank / 16) + chunk) * 2 + part) * 64 + (threadIdx.x & 63);
 }
 
 template <int T>
@@ -47,50 +42,160 @@ __device__ __forceinline__ f32x16_t lora_mfma(u32x4_t a, u32x4_t b, f32x16_t c) 
                                                   __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// acc[mt][nt] += B u of the rows from m0 and the columns from n0 on (32 x 32 each, in
-// the accumulators' layout).  Of every 32 rows the adapters that they name one after the
-// other: the product of all 32 rows' u with B_i, B's rows straight from memory in operand
-// layout (a lane's column and eight ranks are 16 bytes), and then that of the rows that
-// name it added: a product of its own, so that an adapter's NaN stays with its rows.
-template <int T, int MT, int NT>
-__device__ __forceinline__ void lora_tail(const LoraArgs& l, f32x16_t (&acc)[MT][NT], int m0, int n0,
-                                          int M, int N) {
+// c[nt] = B_i u of 32 rows (tile) and 32 NT columns from n0 on, in the accumulators' layout.
+// B's rows come straight from memory in operand layout: a lane's column and eight ranks are 16
+// bytes.
+template <int T, int NT>
+__device__ __forceinline__ void lora_product(const LoraArgs& l, const LoraAt& at, int tile, int n0, int N,
+                                             f32x16_t (&c)[NT]) {
   const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  const u32x4_t* b[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    b[nt] = reinterpret_cast<const u32x4_t*>(l.b + (size_t)at.row * N +
+                                             (size_t)min(n0 + nt * 32 + r32, N - 1) * at.rank) + h;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) c[nt][e] = 0.f;
+  }
+  const u32x4_t* u = lora_u(l, tile, 0, 0);
+  for (int r = 0; r < at.rank / 16; ++r) {
+    const u32x4_t hi = u[r * 128], lo = u[r * 128 + 64];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const u32x4_t bv = b[nt][2 * r];
+      c[nt] = lora_mfma<T>(hi, bv, c[nt]);
+      c[nt] = lora_mfma<T>(lo, bv, c[nt]);
+    }
+  }
+}
+
+// The smallest of the wave's values.
+__device__ __forceinline__ int lora_least(int v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Two values of T, those that are not finite as zero; odd: raised where there are any.
+template <int T>
+__device__ __forceinline__ uint32_t lora_finite(uint32_t v, uint32_t& odd) {
+  constexpr uint32_t kExp = T == kBf16 ? 0x7F80u : 0x7C00u;
+  const uint32_t bad = ((v & kExp) == kExp ? 0xFFFFu : 0u) | ((v >> 16 & kExp) == kExp ? 0xFFFF0000u : 0u);
+  odd |= bad;
+  return v & ~bad;
+}
+
+// acc[mt][nt] += B u of the rows from m0 (a multiple of 32) and the columns from n0 on, 32 x 32
+// each, in the accumulators' layout.  lds: MT * 8 KB that the whole workgroup of four waves is
+// done with once it meets; every wave has the same rows.
+//
+// u of the workgroup's rows comes to LDS, 64 ranks at a time, straight from memory.  Then the
+// adapters that the rows name one after the other, the product of all rows with each: for every
+// 16 ranks B's fragments, straight from memory in operand layout (a lane's column and eight ranks
+// are 16 bytes) and one product ahead.  A row that names another adapter has u = 0 here, and of B
+// what is not finite is zero too, so that an adapter's NaN stays with its rows; they are NaN in
+// that column.  (A product apart from the accumulators, added row by row, had the compiler move
+// 192 of 256 accumulators about in every iteration of the K loop, 478 us for 418.)
+template <int T, int MT, int NT>
+__device__ __forceinline__ void lora_tail(const LoraArgs& l, f32x16_t (&acc)[MT][NT], uint4* lds, int m0,
+                                          int n0, int M, int N) {
+  constexpr int kWaves = 4, kBlock = 4;  // 16-rank chunks at a time
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id[MT], least = INT_MAX;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int row = m0 + mt * 32 + r32;
-    const int id = row < M ? lora_of(l, row) : -1;
-    const float* u = l.u + (size_t)min(row, M - 1) * l.max_rank + 8 * h;
-    uint32_t left = (uint32_t)__builtin_amdgcn_ballot_w64(id >= 0);
-    while (left) {
-      const int i = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
-      const uint32_t rows = (uint32_t)__builtin_amdgcn_ballot_w64(id == i);
-      left &= ~rows;
-      const LoraAt at = lora_at(l, i);
-      const uint16_t* b[NT];
-      f32x16_t c[NT];
+    id[mt] = row < M ? lora_of(l, row) : -1;
+    least = min(least, id[mt] < 0 ? INT_MAX : id[mt]);
+  }
+  const int i0 = lora_least(least);
+  if (i0 == INT_MAX) return;
+  auto after = [&](int i) {
+    int v = INT_MAX;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        b[nt] = l.b + (size_t)at.row * N + (size_t)min(n0 + nt * 32 + r32, N - 1) * at.rank + 8 * h;
+    for (int mt = 0; mt < MT; ++mt) v = min(v, id[mt] > i ? id[mt] : INT_MAX);
+    return lora_least(v);
+  };
+  // u from this tile on; past the end zeros.
+  const uint32_t per = (uint32_t)l.max_rank / 16 * 2048;  // bytes of 32 rows
+  const __amdgpu_buffer_rsrc_t ur =
+      make_rsrc(reinterpret_cast<const char*>(l.u) + (size_t)(m0 / 32) * per,
+                (uint32_t)min(MT, (M + 31) / 32 - m0 / 32) * per);
+  for (int r0 = 0; r0 < l.max_rank / 16; r0 += kBlock) {
+    // Every wave is done with this LDS, and nothing of its own is on its way there.
+    __builtin_amdgcn_sched_barrier(0);
+    IMQ_WAIT_VM_LGKM_0();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) c[nt][e] = 0.f;
-      }
-      for (int r = 0; r < at.rank; r += 16) {
-        u32x4_t hi, lo;
-        lora_split<T>(u + r, hi, lo);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const u32x4_t bv = *reinterpret_cast<const u32x4_t*>(b[nt] + r);
-          c[nt] = lora_mfma<T>(hi, bv, c[nt]);
-          c[nt] = lora_mfma<T>(lo, bv, c[nt]);
-        }
-      }
-      const uint32_t mine = rows >> (4 * h);
+    for (int p = 0; p < kBlock * MT * 2 / kWaves; ++p) {
+      const int at = p * kWaves + wave, c = at / (2 * MT), mt = at / 2 % MT, part = at % 2;
+      load_lds16(ur, lane * 16, mt * per + (r0 + c) * 2048 + part * 1024, lds + at * 64);
+    }
+    u32x4_t bf[NT];
+    auto load_b = [&](const LoraAt& at, int r) {
+      if (at.rank == 0) return;
+      r = min(r, at.rank / 16 - 1);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
+        bf[nt] = *reinterpret_cast<const u32x4_t*>(l.b + (size_t)at.row * N +
+                                                   (size_t)min(n0 + nt * 32 + r32, N - 1) * at.rank +
+                                                   16 * r + 8 * h);
+    };
+    LoraAt at = lora_at(l, i0);
+    load_b(at, r0);
+    __builtin_amdgcn_sched_barrier(0);
+    IMQ_WAIT_VMCNT(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    for (int i = i0;;) {
+      const int next = after(i);
+      const LoraAt then = next == INT_MAX ? at : lora_at(l, next);
+      const int chunks = min(at.rank / 16 - r0, kBlock);
+      if (chunks <= 0) load_b(then, r0);
+      uint32_t odd[NT];
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          acc[mt][nt][e] += (mine >> (8 * (e >> 2) + (e & 3))) & 1u ? c[nt][e] : 0.f;
+      for (int nt = 0; nt < NT; ++nt) odd[nt] = 0;
+      for (int c = 0; c < chunks; ++c) {
+        u32x4_t bn[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bn[nt][e] = lora_finite<T>(bf[nt][e], odd[nt]);
+        if (c + 1 < chunks) load_b(at, r0 + c + 1);
+        else load_b(then, r0);
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const u32x4_t u = __builtin_bit_cast(u32x4_t, lds[((c * MT + mt) * 2 + part) * 64 + lane]);
+            const u32x4_t a = id[mt] == i ? u : u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = lora_mfma<T>(a, bn[nt], acc[mt][nt]);
+          }
+      }
+      uint32_t any = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) any |= odd[nt];
+      if (__builtin_amdgcn_ballot_w64(any != 0)) {
+        // NaN where a row that names it meets such a column, by matrix instructions alone:
+        // bf16's largest value squared, which is infinite, less the same.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint64_t cols = __builtin_amdgcn_ballot_w64(odd[nt] != 0);  // a column's ranks are in two lanes
+          const uint32_t col = (uint32_t)(cols | cols >> 32) >> r32 & 1u ? 0x7F7F7F7Fu : 0u;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int sign = 0; sign < 2; ++sign) {
+              const uint32_t row = id[mt] == i ? (sign ? 0xFF7FFF7Fu : 0x7F7F7F7Fu) : 0u;
+              acc[mt][nt] = lora_mfma<kBf16>(u32x4_t{row, row, row, row}, u32x4_t{col, col, col, col}, acc[mt][nt]);
+            }
+        }
+      }
+      if (next == INT_MAX) break;
+      i = next, at = then;
     }
   }
 }
@@ -99,9 +204,17 @@ __device__ __forceinline__ void lora_tail(const LoraArgs& l, f32x16_t (&acc)[MT]
 template <int T>
 struct EpLora : EpStore<T> {
   LoraArgs lora;
+  __device__ __forceinline__ int row_at(int place) const { return lora.order ? lora.order[place] : place; }
+  __device__ __forceinline__ void emit1(int row, int col, uint16_t v) const {
+    EpStore<T>::emit1(row_at(row), col, v);
+  }
+  __device__ __forceinline__ void emit8(int row, int col, uint4 v) const {
+    EpStore<T>::emit8(row_at(row), col, v);
+  }
   template <int MT, int NT>
-  __device__ __forceinline__ void add_sums(f32x16_t (&acc)[MT][NT], int m0, int n0, int M, int N) const {
-    lora_tail<T, MT, NT>(lora, acc, m0, n0, M, N);
+  __device__ __forceinline__ void add_sums(f32x16_t (&acc)[MT][NT], uint4* lds, int m0, int n0, int M,
+                                           int N) const {
+    lora_tail<T, MT, NT>(lora, acc, lds, m0, n0, M, N);
   }
 };
 template <int T>

@@ -261,32 +261,63 @@ hipError_t launch_qgemm(const uint32_t* w, const void* scales, const void* biase
   }
 }
 
+// Rows up to which the adapters' second product is left to the join whether K is split or not:
+// more rows than that name an adapter of their own in stretches.
+constexpr int kLoraJoinMaxM = 128;
+
+LoraPlan lora_plan(int k, int n, int m, int count, int dtype) {
+  LoraPlan p{};
+  if (m <= kQskinnyMaxM && qskinny_supported(k, n, m, dtype)) {
+    p.bytes = qskinny_resid_split_bytes(k, n, m);
+    p.splits = (int)(p.bytes / ((size_t)m * n * sizeof(float)));
+    p.few = p.splits > 0;
+    if (p.few) return p;
+  }
+  if (!qgemm_big_supported(k, n, m)) return p;
+  const BigPlan b = pick_big_plan(m, n, k, device_cus(), true);
+  if (b.splits > 1 || m <= kLoraJoinMaxM) {
+    p.splits = b.splits;
+    p.bytes = (size_t)b.splits * m * n * sizeof(float);
+  }
+  p.mt = b.mt, p.nt = b.nt, p.split_steps = b.split_steps;
+  // A tile takes the adapters that its rows name one after the other.
+  p.order = p.splits == 0 && count > 1;
+  return p;
+}
+
 namespace {
 
 template <int T>
-hipError_t launch_lora_t(const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
-                         const uint16_t* x, const LoraArgs& l, uint16_t* y, int k, int n, int m,
-                         hipStream_t stream) {
+hipError_t launch_lora_t(const LoraPlan& p, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
+                         const uint16_t* x, const LoraArgs& l, float* part, uint16_t* y, int k, int n,
+                         int m, hipStream_t stream) {
+  const BigPlan b{p.mt, p.nt, p.splits > 0 ? p.splits : 1, p.split_steps};
+  const bool tail = k % 256 != 0;
+  if (p.splits > 0) {
+    using Part = EpPartial<false>;
+    const Part ep{part, n, n, 0, 0};
+    return tail ? tile::launch_plan<T, Part, true>(b, w, scales, biases, x, ep, k, n, m, stream)
+                : tile::launch_plan<T, Part, false>(b, w, scales, biases, x, ep, k, n, m, stream);
+  }
   const EpLora<T> ep{{y, n, al16(y) && n % 8 == 0}, l};
-  if (!qgemm_big_supported(k, n, m))
-    return tile::launch_reg<T, EpLora<T>>(w, scales, biases, x, ep, k, n, m, stream);
-  const BigPlan p = pick_big_plan(m, n, k, device_cus(), false);
-  return k % 256 ? tile::launch_plan<T, EpLora<T>, true>(p, w, scales, biases, x, ep, k, n, m, stream)
-                 : tile::launch_plan<T, EpLora<T>, false>(p, w, scales, biases, x, ep, k, n, m, stream);
+  if (p.mt == 0) return tile::launch_reg<T, EpLora<T>>(w, scales, biases, x, ep, k, n, m, stream);
+  return tail ? tile::launch_plan<T, EpLora<T>, true>(b, w, scales, biases, x, ep, k, n, m, stream)
+              : tile::launch_plan<T, EpLora<T>, false>(b, w, scales, biases, x, ep, k, n, m, stream);
 }
 
 }  // namespace
 
-hipError_t launch_qgemm_lora(const uint32_t* w, const void* scales, const void* biases, const void* x,
-                             const LoraArgs& l, void* y, int k, int n, int m, int dtype,
-                             hipStream_t stream) {
+hipError_t launch_qgemm_lora(const LoraPlan& p, const uint32_t* w, const void* scales, const void* biases,
+                             const void* x, const LoraArgs& l, float* part, void* y, int k, int n, int m,
+                             int dtype, hipStream_t stream) {
+  if (p.few) return launch_qskinny_partials(w, scales, biases, x, part, k, n, m, dtype, stream);
   const auto* s = static_cast<const uint16_t*>(scales);
   const auto* b = static_cast<const uint16_t*>(biases);
   const auto* xx = static_cast<const uint16_t*>(x);
   auto* yy = static_cast<uint16_t*>(y);
   switch (dtype) {
-    case kBf16: return launch_lora_t<kBf16>(w, s, b, xx, l, yy, k, n, m, stream);
-    case kF16: return launch_lora_t<kF16>(w, s, b, xx, l, yy, k, n, m, stream);
+    case kBf16: return launch_lora_t<kBf16>(p, w, s, b, xx, l, part, yy, k, n, m, stream);
+    case kF16: return launch_lora_t<kF16>(p, w, s, b, xx, l, part, yy, k, n, m, stream);
     default: return hipErrorInvalidValue;
   }
 }

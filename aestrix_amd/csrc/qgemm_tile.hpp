@@ -251,7 +251,7 @@ __global__ __launch_bounds__(kThreads, (MT * NT * 16 > 128) ? 1 : 2) void qgemm_
     __syncthreads();
   }
 
-  if constexpr (adds_sums<EP>) ep.template add_sums<MT, NT>(acc, m0, nw0, M, N);
+  if constexpr (adds_sums<EP>) ep.template add_sums<MT, NT>(acc, &a_lds[0][0], m0, nw0, M, N);
 
   // Epilogue: accumulator r of a 32x32 tile holds row 8*(r/4) + 4*h + r%4,
   // column r32.  Each output is rounded to T (Elem::out, the same RNE as the
@@ -834,7 +834,8 @@ __device__ __forceinline__ void big_tile(const uint32_t* __restrict__ w,
     const int slot = i * kThreads + tid;
     const int row = slot / (8 * kBigKG);
     const int c = a_chunk_kg<kBigKG>(row, slot % (8 * kBigKG));
-    const uint32_t gr = (uint32_t)min(m0 + row, M - 1);
+    uint32_t gr = (uint32_t)min(m0 + row, M - 1);
+    if constexpr (adds_sums<EP>) gr = ep.row_at(gr);
     src.a_off[i] = (gr * (uint32_t)K + (uint32_t)c * 8u) * 2u;
   }
   // In MFMA operand layout lane (r32, h) of column tile nt owns weight row
@@ -949,7 +950,7 @@ __device__ __forceinline__ void big_tile(const uint32_t* __restrict__ w,
         }
     }
   } else {
-  if constexpr (adds_sums<EP>) ep.template add_sums<MT, NT>(acc, m0, ncol0, M, N);
+  if constexpr (adds_sums<EP>) ep.template add_sums<MT, NT>(acc, ring.a[0], m0, ncol0, M, N);
   // Output: the tile's T values are staged in the LDS ring, then written out
   // row by row, 16 bytes per lane.  Written straight from the MFMA layout, a
   // lane holds one column of 16 rows per 32x32 tile: 2-byte stores, 14 of

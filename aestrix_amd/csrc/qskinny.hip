@@ -1360,6 +1360,17 @@ size_t qskinny_resid_split_bytes(int k, int n, int m) {
   return sp.ok ? (size_t)sp.splits * m * n * sizeof(float) : 0;
 }
 
+hipError_t launch_qskinny_partials(const uint32_t* w, const void* scales, const void* biases, const void* x,
+                                   float* ws, int k, int n, int m, int dtype, hipStream_t stream) {
+  const SplitPlan sp = plan_split(k, n, m, true);
+  if (!sp.ok || !qskinny_supported(k, n, m, dtype)) return hipErrorInvalidValue;
+  const auto* s = static_cast<const uint16_t*>(scales);
+  const auto* b = static_cast<const uint16_t*>(biases);
+  const auto* xx = static_cast<const uint16_t*>(x);
+  return dtype == kBf16 ? launch_split_partials<kBf16>(w, s, b, xx, ws, k, n, m, sp, stream)
+                        : launch_split_partials<kF16>(w, s, b, xx, ws, k, n, m, sp, stream);
+}
+
 int qskinny_splits(int k, int n, int m) {
   const SplitPlan sp = plan_split(k, n, m);
   return sp.ok ? sp.splits : 1;

@@ -17,8 +17,13 @@ namespace imq {
 hipError_t launch_lora_shrink(const LoraArgs&, const void*, int, int, int, hipStream_t) {
   return hipErrorNoDevice;
 }
-hipError_t launch_qgemm_lora(const uint32_t*, const void*, const void*, const void*, const LoraArgs&,
-                             void*, int, int, int, int, hipStream_t) {
+hipError_t launch_lora_join(const LoraArgs&, const float*, int, void*, int, int, int, hipStream_t) {
+  return hipErrorNoDevice;
+}
+hipError_t launch_lora_order(const LoraArgs&, int32_t*, int32_t*, int, hipStream_t) { return hipErrorNoDevice; }
+LoraPlan lora_plan(int, int n, int m, int, int) { return LoraPlan{0, 2, 1, 2, 2, false, (size_t)8 * m * n}; }
+hipError_t launch_qgemm_lora(const LoraPlan&, const uint32_t*, const void*, const void*, const void*,
+                             const LoraArgs&, float*, void*, int, int, int, int, hipStream_t) {
   return hipErrorNoDevice;
 }
 }  // namespace imq
@@ -76,6 +81,8 @@ int main() {
     lora(IMQ_EINVAL, "count", [&](Call& c) { c.l.count = bad; }, IMQ_EINVAL);
     lora(IMQ_EINVAL, "max_rank", [&](Call& c) { c.l.max_rank = bad; }, IMQ_EINVAL);
   }
+  lora(IMQ_EHIP, "k 2^25", [](Call& c) { c.k = 1 << 25; }, IMQ_OK);
+  lora(IMQ_EUNSUPPORTED, "k past 2^25", [](Call& c) { c.k = (1 << 25) + 64; }, IMQ_EUNSUPPORTED);
   lora(IMQ_EINVAL, "k 96", [](Call& c) { c.k = 96; }, IMQ_EINVAL);
   for (int bad : {-16, 8, 63}) lora(IMQ_EINVAL, "rows", [&](Call& c) { c.l.rows = bad; }, IMQ_EINVAL);
   for (int bad : {8, 33}) lora(IMQ_EINVAL, "max_rank", [&](Call& c) { c.l.max_rank = bad; }, IMQ_EINVAL);
