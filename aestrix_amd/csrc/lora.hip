@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kDotWaves * 64) void lora_dot_kernel(LoraArgs l, co
 }
 
 // More rows.  A workgroup: 32 of them against 32 ranks (blockIdx.y) of the adapters that they
-// name, one after the other.  Its eight waves take K in turn, 64 at a time, from buffers of their
+// name, every second one (blockIdx.z).  Its eight waves take K in turn, 64 at a time, from buffers of their
 // own: whole 128-byte lines of x's and A's rows straight to LDS (operands loaded straight to
 // registers touch 32 bytes of a line each, and 16 such waves took 35 us of 4608 rows of 2560), the
 // next piece on its way while one is multiplied.  16-byte pieces are swizzled by the row at their
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
   uint32_t rows;
   LoraAt at;
   bool ahead = true;
-  for (int j = 0;; ++j) {
+  for (int j = blockIdx.z;; j += gridDim.z) {
     const int i = of_tile.nth(j, rows, at);
     if (i < 0) break;
     if (r0 >= at.rank) continue;
@@ -189,82 +189,95 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
 
 // One workgroup: each of its 16 waves counts the rows of a stretch by adapter, the counts are
 // added up over adapters and waves, and each wave gives its rows their places, 64 at a time, in
-// their order.  Up to kOrderKeep * 1024 rows are read once, all together.  More adapters than
-// kOrderBins - 1: the rows stay as they are.
-constexpr int kOrderWaves = 16, kOrderBins = 1024, kOrderKeep = 8;
+// their order.  The adapters of kOrderKeep rows stay in LDS in between.  Loops are kept rolled: of
+// code that runs once, fetching it is what takes the time.  More adapters than kOrderBins - 1: the
+// rows stay as they are.
+constexpr int kOrderWaves = 16, kOrderBins = 1024, kOrderKeep = 16384;
 __global__ __launch_bounds__(kOrderWaves * 64) void lora_order_kernel(LoraArgs l, int32_t* order,
                                                                      int32_t* which_at, int m) {
   __shared__ int at[kOrderWaves][kOrderBins];
   __shared__ int sums[kOrderBins];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ uint16_t kept[kOrderKeep];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int bins = l.count + 1;  // the last one: no adapter
   if (bins > kOrderBins) {
-    for (int r = threadIdx.x; r < m; r += kOrderWaves * 64) {
+    for (int r = t; r < m; r += kOrderWaves * 64) {
       order[r] = r;
       which_at[r] = lora_of(l, r);
     }
     return;
   }
+  auto load = [&](int r) {
+    const int i = lora_of(l, r);
+    return i < 0 ? l.count : i;
+  };
+  const int few = min(m, kOrderKeep);
+  for (int r = t * 4; r < few; r += kOrderWaves * 256) {  // four at a time, whatever the alignment
+    int v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = load(min(r + e, few - 1));
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (r + e < few) kept[r + e] = (uint16_t)v[e];
+  }
+  if (t < bins)
+#pragma unroll 1
+    for (int w = 0; w < kOrderWaves; ++w) at[w][t] = 0;
+  __syncthreads();
   const int per = ((m + kOrderWaves - 1) / kOrderWaves + 63) / 64 * 64;
   const int begin = min(wave * per, m), end = min(begin + per, m);
-  auto bin = [&](int r) {
-    const int i = r < end ? lora_of(l, r) : -2;
-    return i == -1 ? l.count : i;  // below 0: no row
+  auto bin = [&](int r) { return r < kOrderKeep ? (int)kept[r] : load(r); };
+  // The rows of [begin, end) 64 at a time, by the bins that they have; a bin's count or place is its
+  // wave's alone.  (Atomics of 64 lanes on one bin took 4 us of 4000 rows' 9.)
+  auto each = [&](auto visit) {
+#pragma unroll 1
+    for (int r0 = begin; r0 < end; r0 += 64) {
+      const int r = r0 + lane, b = r < end ? bin(r) : -1;
+      uint64_t left = __builtin_amdgcn_ballot_w64(b >= 0);
+      while (left) {
+        const int i = __builtin_amdgcn_readlane(b, __builtin_ctzll(left));
+        const uint64_t rows = __builtin_amdgcn_ballot_w64(b == i);
+        left &= ~rows;
+        const int from = at[wave][i];
+        __builtin_amdgcn_wave_barrier();
+        visit(r, i, rows, from, b == i);
+        if (lane == 0) at[wave][i] = from + __builtin_popcountll(rows);
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
   };
-  int kept[kOrderKeep];
-#pragma unroll
-  for (int t = 0; t < kOrderKeep; ++t) kept[t] = bin(begin + t * 64 + lane);
-  for (int w = 0; w < kOrderWaves; ++w)
-    if ((int)threadIdx.x < bins) at[w][threadIdx.x] = 0;
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < kOrderKeep; ++t)
-    if (kept[t] >= 0) atomicAdd(&at[wave][kept[t]], 1);
-  for (int r = begin + kOrderKeep * 64 + lane; r < end; r += 64) atomicAdd(&at[wave][bin(r)], 1);
+  each([](int, int, uint64_t, int, bool) {});
   __syncthreads();
   // Of every bin its rows, then over the bins (a scan by doubling steps).
   int mine = 0;
-  if ((int)threadIdx.x < bins)
-#pragma unroll
-    for (int w = 0; w < kOrderWaves; ++w) mine += at[w][threadIdx.x];
-  sums[threadIdx.x] = mine;
+  if (t < bins)
+#pragma unroll 1
+    for (int w = 0; w < kOrderWaves; ++w) mine += at[w][t];
+  sums[t] = mine;
   __syncthreads();
+#pragma unroll 1
   for (int step = 1; step < bins; step *= 2) {
-    const int v = (int)threadIdx.x >= step ? sums[threadIdx.x - step] : 0;
+    const int v = t >= step ? sums[t - step] : 0;
     __syncthreads();
-    sums[threadIdx.x] += v;
+    sums[t] += v;
     __syncthreads();
   }
-  if ((int)threadIdx.x < bins) {
-    int from = sums[threadIdx.x] - mine;
-#pragma unroll
+  if (t < bins) {
+    int from = sums[t] - mine;
+#pragma unroll 1
     for (int w = 0; w < kOrderWaves; ++w) {
-      const int n = at[w][threadIdx.x];
-      at[w][threadIdx.x] = from;
+      const int n = at[w][t];
+      at[w][t] = from;
       from += n;
     }
   }
   __syncthreads();
-  auto place = [&](int r, int b) {
-    uint64_t left = __builtin_amdgcn_ballot_w64(b >= 0);
-    while (left) {
-      const int i = __builtin_amdgcn_readlane(b, __builtin_ctzll(left));
-      const uint64_t rows = __builtin_amdgcn_ballot_w64(b == i);
-      left &= ~rows;
-      const int from = at[wave][i];
-      __builtin_amdgcn_wave_barrier();
-      if (b == i) {
-        const int to = from + __builtin_popcountll(rows & (((uint64_t)1 << lane) - 1));
-        order[to] = r;
-        which_at[to] = i < l.count ? i : -1;
-      }
-      if (lane == 0) at[wave][i] = from + __builtin_popcountll(rows);
-      __builtin_amdgcn_wave_barrier();
-    }
-  };
-#pragma unroll
-  for (int t = 0; t < kOrderKeep; ++t) place(begin + t * 64 + lane, kept[t]);
-  for (int r0 = begin + kOrderKeep * 64; r0 < end; r0 += 64) place(r0 + lane, bin(r0 + lane));
+  each([&](int r, int i, uint64_t rows, int from, bool mine) {
+    if (!mine) return;
+    const int to = from + __builtin_popcountll(rows & (((uint64_t)1 << lane) - 1));
+    order[to] = r;
+    which_at[to] = i < l.count ? i : -1;
+  });
 }
 
 // ---- the join
@@ -290,11 +303,18 @@ __global__ __launch_bounds__(kJoinWaves * 64) void lora_join_kernel(LoraArgs l, 
     sum[o] = 0.f;
     add[o * kJoinWaves * 64 + threadIdx.x] = 0.f;
   }
-  for (int sp = 0; sp < splits; ++sp)
+  // Eight ranges at a time: their loads wait together.
+  constexpr int kAhead = 8;
+  for (int sp = 0; sp < splits; sp += kAhead)
 #pragma unroll
     for (int o = 0; o < kOuts; ++o) {
       const size_t r = min(tile * 32 + of + o * (kJoinWaves * 2), m - 1);
-      sum[o] += part[((size_t)sp * m + r) * n + min(col, n - 1)];
+      float v[kAhead];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e)
+        v[e] = part[((size_t)min(sp + e, splits - 1) * m + r) * n + min(col, n - 1)];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) sum[o] += sp + e < splits ? v[e] : 0.f;
     }
   __syncthreads();
   uint32_t rows;
@@ -335,7 +355,8 @@ hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, in
       hipLaunchKernelGGL((lora_dot_kernel<kF16>), grid, block, 0, stream, l, xx, k, m);
     return hipGetLastError();
   }
-  const dim3 grid((unsigned)((m + 31) / 32), (unsigned)((l.max_rank + 31) / 32)), block(kShrinkWaves * 64);
+  const dim3 grid((unsigned)((m + 31) / 32), (unsigned)((l.max_rank + 31) / 32), l.count > 1 ? 2 : 1),
+      block(kShrinkWaves * 64);
   if (dtype == kBf16)
     hipLaunchKernelGGL((lora_shrink_kernel<kBf16>), grid, block, 0, stream, l, xx, k, m);
   else
