@@ -375,15 +375,13 @@ hipError_t launch_shared_tiles(const AttnArgs& a, const AttnShared& sh, const At
   const int tiles = (int)((rows + kRows - 1) / kRows);
   const int64_t blocks = (int64_t)a.n_seq * a.kv_heads * tiles;
   const dim3 block(attn_waves(WM) * 64);
-  if constexpr (WM < 8) {  // the plan splits no keys of 256 rows
-    if (plan.splits > 1) {
-      hipLaunchKernelGGL((attn_shared_tiles_kernel<T, D, WM, kCap, kSlope, true>),
-                         dim3((unsigned)(blocks * plan.splits)), block, 0, stream, a, sh, tiles, plan.first,
-                         1, plan.splits, plan.chunk, ws);
-      launch_shared_join<T, D, kCap, kSlope>(a, sh, kRows, tiles, blocks * kRows, plan.splits, plan.chunk, 0,
-                                             own0, ws, stream);
-      return hipGetLastError();
-    }
+  if (plan.splits > 1) {
+    hipLaunchKernelGGL((attn_shared_tiles_kernel<T, D, WM, kCap, kSlope, true>),
+                       dim3((unsigned)(blocks * plan.splits)), block, 0, stream, a, sh, tiles, plan.first, 1,
+                       plan.splits, plan.chunk, ws);
+    launch_shared_join<T, D, kCap, kSlope>(a, sh, kRows, tiles, blocks * kRows, plan.splits, plan.chunk, 0,
+                                           own0, ws, stream);
+    return hipGetLastError();
   }
   hipLaunchKernelGGL((attn_shared_tiles_kernel<T, D, WM, kCap, kSlope, false>), dim3((unsigned)blocks), block,
                      0, stream, a, sh, tiles, plan.first, plan.near_hs, 1, 0, nullptr);
@@ -410,10 +408,8 @@ hipError_t launch_shared_scored(const AttnArgs& a, const AttnShared& sh, const S
     default: break;
   }
   switch (wide ? p.tiles.tile_rows : -p.tiles.tile_rows) {
-    case 256: return launch_shared_tiles<T, 128, 8, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
     case 128: return launch_shared_tiles<T, 128, 4, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
     case 64: return launch_shared_tiles<T, 128, 2, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
-    case -256: return launch_shared_tiles<T, 64, 8, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
     case -128: return launch_shared_tiles<T, 64, 4, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
     case -64: return launch_shared_tiles<T, 64, 2, kCap, kSlope>(a, sh, p.tiles, p.own0, ws, stream);
     default: return hipErrorInvalidValue;

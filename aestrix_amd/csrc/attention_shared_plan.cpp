@@ -42,6 +42,22 @@ SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cu
   const int64_t hs = (int64_t)a.n_seq * a.kv_heads;
   p.kernel = IMQ_SHARED_TILES;
   if (p.tiles.kernel == IMQ_ATTENTION_TILES) {
+    // Never 256 rows a workgroup, and one sequence after the other where not all workgroups are
+    // resident from the start: walks behind a long front are alike, and a sequence's fewer tiles
+    // leave no gaps then.  4 x 2048 rows of 32 / 8 heads behind 8192 keys, lengths 2048 / 1265 /
+    // 483 / 1749, 828 us against 1027 tile by tile and 1213 with 256 rows; 8 x 2048 of 16 / 4
+    // behind 4000 416 / 558 / 609, 32 x 800 behind 2000 553 / 635 / 657; of equal lengths 1175 /
+    // 1182 / 1219, 677 / 659 / 681 and 1084 / 1130 / 1137.
+    const int64_t hs = (int64_t)a.n_seq * a.kv_heads;
+    const int64_t all_rows = (int64_t)a.max_q * (a.heads / a.kv_heads);
+    if (p.tiles.tile_rows == 256) p.tiles.tile_rows = 128;
+    const int64_t tiles = (all_rows + p.tiles.tile_rows - 1) / p.tiles.tile_rows;
+    // (Of few tiles a sequence the empty ones come first, and a CU's share is more even: 61 documents
+    // of up to 154 rows behind 3001 keys 119 us against 165.)
+    if (p.tiles.splits == 1 && hs * tiles > 2 * cus && tiles >= 8) {
+      p.tiles.first = (int)tiles;
+      p.tiles.near_hs = a.kv_heads;
+    }
     p.bytes = p.tiles.bytes;
     if (p.tiles.splits == 1 || workspace) return p;
   }
