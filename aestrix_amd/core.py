@@ -372,7 +372,7 @@ class SharedPlanInfo(ctypes.Structure):
                 ("own_splits", ctypes.c_int), ("workspace_bytes", ctypes.c_size_t)]
 
 
-SHARED_KERNELS = {0: "rows", 1: "tiles", 2: "stream"}
+SHARED_KERNELS = {0: "rows", 1: "tiles", 2: "stream", 3: "packed"}
 
 
 def attention_shared_plan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, shared_k: torch.Tensor,

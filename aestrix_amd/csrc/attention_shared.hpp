@@ -231,7 +231,8 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, StreamLds<D, kLds
 // Every sequence's rows (rows: queries times heads a key head, up to 32) against the shared
 // keys, then against their own: first kv_heads * s_tiles * s_splits workgroups of 32 R rows of
 // the batch and s_chunk shared keys, then one for a sequence, key head and o_chunk own keys.
-// Ranges to ws as attn_join has them, the shared keys' s_splits first.
+// The ranges of the shared keys go to ws, those of the own ones behind them, each as a split
+// plan's.
 template <int T, int D, int R, bool kCap, bool kSlope>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_stream_kernel(
     AttnArgs a, AttnShared sh, int rows, int s_tiles, int s_splits, int s_chunk, int o_splits, int o_chunk,
@@ -241,9 +242,9 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_stream_kernel(
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int group = a.heads / a.kv_heads, hs_n = a.n_seq * a.kv_heads;
   const int64_t all = (int64_t)hs_n * rows;
-  float2* ml = reinterpret_cast<float2*>(ws + (int64_t)(s_splits + o_splits) * all * D);
   const int front = a.kv_heads * s_tiles * s_splits;
   if ((int)blockIdx.x < front) {
+    float2* ml = reinterpret_cast<float2*>(ws + s_splits * all * D);
     const int kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
     const int tile = rest % s_tiles, split = rest / s_tiles;
     s16x8_t qf[R][D / 16];
@@ -304,9 +305,10 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_stream_kernel(
       reinterpret_cast<const char*>(static_cast<const S*>(a.k) + s.k_at + kh * a.k_head),
       reinterpret_cast<const char*>(static_cast<const S*>(a.v) + s.v_at + kh * a.v_head), a.k_row * 2,
       a.v_row * 2, s.nk};
-  const int64_t range = s_splits + split;
+  ws += s_splits * all * (D + 2);
+  float2* ml = reinterpret_cast<float2*>(ws + o_splits * all * D);
   attn_stream<T, D, 1, R, kCap, kSlope>(a, lds, keys, begin, end, qf, score, seen, seen_lo, p, near, dst,
-                                     ws + range * all * D, ml + range * all);
+                                        ws + split * all * D, ml + split * all);
 }
 
 // ---- many rows a sequence
@@ -314,14 +316,30 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_stream_kernel(
 template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
 __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_shared_tiles_kernel(
     AttnArgs a, AttnShared sh, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
-  attn_tiles<T, D, WM, kCap, kSlope, kSplit, true>(a, sh, tiles, first, near_hs, splits, chunk, ws);
+  attn_tiles<T, D, WM, kCap, kSlope, kSplit, true>(a, sh, blockIdx.x, tiles, first, near_hs, splits, chunk, ws);
+}
+
+// Packed documents that fill few tiles: all rows as they stand in q against the shared keys
+// (front: one sequence of them, f_tiles * f_splits * kv_heads workgroups), and each document's
+// against its own, every workgroup's sums to ws.
+template <int T, int D, int WM, bool kCap>
+__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_shared_packed_kernel(
+    AttnArgs front, AttnArgs own, int f_tiles, int f_splits, int f_chunk, int o_tiles, int o_chunk, float* f_ws,
+    float* o_ws) {
+  const int blocks = f_tiles * f_splits * front.kv_heads;
+  if ((int)blockIdx.x < blocks)
+    attn_tiles<T, D, WM, kCap, false, true, false>(front, AttnShared{}, blockIdx.x, f_tiles, f_tiles, 1, f_splits,
+                                                   f_chunk, f_ws);
+  else
+    attn_tiles<T, D, WM, kCap, false, true, false>(own, AttnShared{}, blockIdx.x - blocks, o_tiles, o_tiles, 1, 1,
+                                                   o_chunk, o_ws);
 }
 
 template <int T, int D, int kParts, bool kCap, bool kSlope>
-__global__ __launch_bounds__(256) void attn_shared_join_kernel(AttnArgs a, AttnShared sh, int tile_rows,
-                                                               int tiles, int splits, int chunk, int front,
+__global__ __launch_bounds__(256) void attn_shared_join_kernel(AttnArgs a, AttnShared sh, AttnFront front,
+                                                               int tile_rows, int tiles, int splits, int chunk,
                                                                int own0, const float* ws) {
-  attn_join<T, D, kParts, kCap, kSlope, true>(a, sh, tile_rows, tiles, splits, chunk, front, own0, ws);
+  attn_join<T, D, kParts, kCap, kSlope, true>(a, sh, front, tile_rows, tiles, splits, chunk, own0, ws);
 }
 
 // ---- any alignment and head dim: a wave a row, from the definition
@@ -343,15 +361,17 @@ __global__ __launch_bounds__(256) void attn_shared_rows_kernel(AttnArgs a, AttnS
 
 // ---- launches
 
+// ranges: of a row, the front's among them.
 template <int T, int D, bool kCap, bool kSlope>
-void launch_shared_join(const AttnArgs& a, const AttnShared& sh, int tile_rows, int tiles, int64_t all,
-                        int splits, int chunk, int front, int own0, const float* ws, hipStream_t stream) {
-  if (splits > 4)
+void launch_shared_join(const AttnArgs& a, const AttnShared& sh, const AttnFront& front, int tile_rows,
+                        int tiles, int64_t all, int splits, int chunk, int own0, const float* ws,
+                        hipStream_t stream) {
+  if (front.ranges + splits > 4)
     hipLaunchKernelGGL((attn_shared_join_kernel<T, D, 16, kCap, kSlope>), dim3((unsigned)all), dim3(256), 0,
-                       stream, a, sh, tile_rows, tiles, splits, chunk, front, own0, ws);
+                       stream, a, sh, front, tile_rows, tiles, splits, chunk, own0, ws);
   else
     hipLaunchKernelGGL((attn_shared_join_kernel<T, D, 1, kCap, kSlope>), dim3((unsigned)((all + 15) / 16)),
-                       dim3(256), 0, stream, a, sh, tile_rows, tiles, splits, chunk, front, own0, ws);
+                       dim3(256), 0, stream, a, sh, front, tile_rows, tiles, splits, chunk, own0, ws);
 }
 
 template <int T, int D, int R, bool kCap, bool kSlope>
@@ -362,8 +382,32 @@ hipError_t launch_stream(const AttnArgs& a, const AttnShared& sh, const SharedPl
   const unsigned blocks = (unsigned)((int64_t)a.kv_heads * p.s_tiles * p.s_splits + hs * p.o_splits);
   hipLaunchKernelGGL((attn_stream_kernel<T, D, R, kCap, kSlope>), dim3(blocks), dim3(kFewWaves * 64), 0,
                      stream, a, sh, rows, p.s_tiles, p.s_splits, p.s_chunk, p.o_splits, p.o_chunk, ws);
-  launch_shared_join<T, D, kCap, kSlope>(a, sh, rows, 1, hs * rows, p.s_splits + p.o_splits, p.o_chunk,
-                                         p.s_splits, 0, ws, stream);
+  launch_shared_join<T, D, kCap, kSlope>(a, sh, AttnFront{ws, hs * rows, p.s_splits, 0}, rows, 1, hs * rows,
+                                         p.o_splits, p.o_chunk, 0, ws + p.s_splits * hs * rows * (D + 2), stream);
+  return hipGetLastError();
+}
+
+template <int T, int D, int WM, bool kCap>
+hipError_t launch_packed(const AttnArgs& a, const AttnShared& sh, const SharedPlan& p, float* ws,
+                         hipStream_t stream) {
+  constexpr int kRows = WM * 32;
+  AttnArgs f = a;  // one sequence of all rows
+  f.k = sh.k, f.k_row = sh.k_row, f.k_head = sh.k_head;
+  f.v = sh.v, f.v_row = sh.v_row, f.v_head = sh.v_head;
+  f.k_seq = f.v_seq = f.q_seq = f.out_seq = 0;
+  f.q_offsets = f.k_offsets = f.q_lens = f.k_lens = f.prefix_lens = nullptr;
+  f.n_seq = 1, f.max_q = a.q_rows, f.max_k = sh.rows, f.causal = 0;
+  const int group = a.heads / a.kv_heads;
+  const int o_tiles = (a.max_q * group + kRows - 1) / kRows;
+  const int64_t f_all = (int64_t)a.kv_heads * p.s_tiles * kRows;
+  const int64_t o_blocks = (int64_t)a.n_seq * a.kv_heads * o_tiles;
+  float* o_ws = ws + p.s_splits * f_all * (D + 2);
+  hipLaunchKernelGGL((attn_shared_packed_kernel<T, D, WM, kCap>),
+                     dim3((unsigned)((int64_t)a.kv_heads * p.s_tiles * p.s_splits + o_blocks)),
+                     dim3(attn_waves(WM) * 64), 0, stream, f, a, p.s_tiles, p.s_splits, p.s_chunk, o_tiles,
+                     p.o_chunk, ws, o_ws);
+  launch_shared_join<T, D, kCap, false>(a, sh, AttnFront{ws, f_all, p.s_splits, p.s_tiles * kRows}, kRows, o_tiles,
+                                        o_blocks * kRows, 1, p.o_chunk, 0, o_ws, stream);
   return hipGetLastError();
 }
 
@@ -379,8 +423,8 @@ hipError_t launch_shared_tiles(const AttnArgs& a, const AttnShared& sh, const At
     hipLaunchKernelGGL((attn_shared_tiles_kernel<T, D, WM, kCap, kSlope, true>),
                        dim3((unsigned)(blocks * plan.splits)), block, 0, stream, a, sh, tiles, plan.first, 1,
                        plan.splits, plan.chunk, ws);
-    launch_shared_join<T, D, kCap, kSlope>(a, sh, kRows, tiles, blocks * kRows, plan.splits, plan.chunk, 0,
-                                           own0, ws, stream);
+    launch_shared_join<T, D, kCap, kSlope>(a, sh, AttnFront{ws, 0, 0, 0}, kRows, tiles, blocks * kRows,
+                                           plan.splits, plan.chunk, own0, ws, stream);
     return hipGetLastError();
   }
   hipLaunchKernelGGL((attn_shared_tiles_kernel<T, D, WM, kCap, kSlope, false>), dim3((unsigned)blocks), block,
@@ -405,6 +449,11 @@ hipError_t launch_shared_scored(const AttnArgs& a, const AttnShared& sh, const S
                     : launch_stream<T, 64, 2, kCap, kSlope>(a, sh, p, ws, stream);
       return wide ? launch_stream<T, 128, 1, kCap, kSlope>(a, sh, p, ws, stream)
                   : launch_stream<T, 64, 1, kCap, kSlope>(a, sh, p, ws, stream);
+    case IMQ_SHARED_PACKED:
+      if constexpr (!kSlope)
+        return wide ? launch_packed<T, 128, 4, kCap>(a, sh, p, ws, stream)
+                    : launch_packed<T, 64, 4, kCap>(a, sh, p, ws, stream);
+      return hipErrorInvalidValue;
     default: break;
   }
   switch (wide ? p.tiles.tile_rows : -p.tiles.tile_rows) {

@@ -8,6 +8,7 @@
 namespace imq {
 namespace {
 
+constexpr int64_t kPackedBytes = (int64_t)256 << 20;  // of packed documents' sums, at most
 constexpr int kStreamStep = kFewWaves * kFewKeys;  // a tile for each wave
 
 // Ranges of at most `chunk` keys (whole steps) over `keys`.
@@ -59,6 +60,30 @@ SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cu
       p.tiles.near_hs = a.kv_heads;
     }
     p.bytes = p.tiles.bytes;
+    // Packed documents that leave much of their tiles empty: their rows in one stretch against the
+    // shared keys, if the sums' way through memory is worth it.  (Slopes would need every row's
+    // document there.)
+    const int group = a.heads / a.kv_heads;
+    const int64_t packed = ((int64_t)a.q_rows * group + 127) / 128;  // tiles of a key head
+    if (workspace && a.q_offsets && !a.slopes && p.tiles.splits == 1 && 2 * a.n_seq >= packed && sh.rows >= 512) {
+      const int64_t own = hs * ((all_rows + 127) / 128);
+      const int64_t blocks = a.kv_heads * packed;
+      const int splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * cus + blocks / 2) / blocks, sh.rows / 512));
+      const int chunk = (ranges(sh.rows, splits) + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
+      const int d = a.dim > 64 ? 128 : 64;
+      const int64_t bytes = (ranges(sh.rows, chunk) * blocks + own) * 128 * (d + 2) * (int64_t)sizeof(float);
+      if (bytes <= kPackedBytes && (blocks * splits + own) * 256 < ((int64_t)1 << 32)) {
+        p.kernel = IMQ_SHARED_PACKED;
+        p.s_rows = 128;
+        p.s_tiles = (int)packed;
+        p.s_chunk = chunk;
+        p.s_splits = ranges(sh.rows, chunk);
+        p.o_chunk = (std::max(a.max_k, 1) + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
+        p.o_splits = 1;
+        p.bytes = (size_t)bytes;
+        return p;
+      }
+    }
     if (p.tiles.splits == 1 || workspace) return p;
   }
   if (p.tiles.kernel == IMQ_ATTENTION_TILES || !workspace) {

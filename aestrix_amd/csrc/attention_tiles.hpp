@@ -376,8 +376,8 @@ __device__ __forceinline__ int attn_own0(const AttnShared& sh) {
 
 // kShared: `sh` stands before every sequence's keys; the walk is over both.
 template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit, bool kShared>
-__device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& sh, int tiles, int first,
-                                           int near_hs, int splits, int chunk, float* ws) {
+__device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& sh, int block, int tiles,
+                                           int first, int near_hs, int splits, int chunk, float* ws) {
   using S = typename Elem<T>::S;
   // WM waves on rows of their own, WK on a part of every tile's keys each.
   constexpr int NW = attn_waves(WM), WK = NW / WM, U = 2 / WK, kRows = WM * 32;
@@ -388,9 +388,9 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hs_n = a.n_seq * a.kv_heads;
   // near_hs sequences and key heads (all, where keys are split) at a time.
-  const int hs0 = kSplit ? 0 : blockIdx.x / (near_hs * tiles) * near_hs;
+  const int hs0 = kSplit ? 0 : block / (near_hs * tiles) * near_hs;
   const int hs_now = kSplit ? hs_n : min(near_hs, hs_n - hs0);
-  const int at = blockIdx.x - hs0 * tiles;
+  const int at = block - hs0 * tiles;
   const int hs = hs0 + at % hs_now, rest = at / hs_now;
   const int split = kSplit ? rest % splits : 0;
   // The last rows of a causal sequence have the most keys: they start first.
@@ -679,7 +679,8 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
 template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
 __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     AttnArgs a, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
-  attn_tiles<T, D, WM, kCap, kSlope, kSplit, false>(a, AttnShared{}, tiles, first, near_hs, splits, chunk, ws);
+  attn_tiles<T, D, WM, kCap, kSlope, kSplit, false>(a, AttnShared{}, blockIdx.x, tiles, first, near_hs, splits,
+                                                       chunk, ws);
 }
 
 // Joins the key ranges of a split plan: 16 lanes a row, D / 16 columns each,
@@ -688,11 +689,18 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
 // tile's ranges up to the last key that its last row sees are written, the
 // others not.  Bound by the latency of its loads: four ranges a group are in
 // flight together.
-// kShared: a tile's first `front` ranges are the shared keys', and the others are counted
-// from `own0` keys before its own.
+// kShared: a row's first front.ranges ranges are the shared keys', in front.ws, and the others
+// are counted from `own0` keys before its own.
+struct AttnFront {
+  const float* ws;  // as a split plan's, of `all` rows
+  int64_t all;
+  int ranges;
+  int packed;  // rows of a key head, which stand in q's order; 0: the same rows as the other ranges
+};
 template <int T, int D, int kParts, bool kCap, bool kSlope, bool kShared>
-__device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& sh, int tile_rows, int tiles,
-                                          int splits, int chunk, int front, int own0, const float* ws) {
+__device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& sh, const AttnFront& front,
+                                          int tile_rows, int tiles, int splits, int chunk, int own0,
+                                          const float* ws) {
   using S = typename Elem<T>::S;
   __shared__ float qs[4][D];
   __shared__ float sums[kParts > 1 ? 16 : 1][D + 2];
@@ -717,18 +725,39 @@ __device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& s
   float acc[D / 16] = {}, top = -INFINITY, sum = 0.f;
   if (live) {
     const int last = min(m / tile_rows * tile_rows + tile_rows, rows) - 1;
-    const int used = front + (int)(((int64_t)attn_seen(a, s, last / group) + own0 + chunk - 1) / chunk);
+    const int used = (kShared ? front.ranges : 0) +
+                     (int)(((int64_t)attn_seen(a, s, last / group) + own0 + chunk - 1) / chunk);
     const float2* ml = reinterpret_cast<const float2*>(ws + (int64_t)splits * all * D) + row;
     const float* po = ws + row * D + d0;
+    const float2* front_ml = nullptr;
+    const float* front_po = nullptr;
+    if constexpr (kShared) {
+      int64_t at = row;
+      if (front.packed)
+        at = (int64_t)kh * front.packed +
+             (int64_t)(min(max(a.q_offsets[hs / a.kv_heads], 0), a.q_rows) + t) * group + m % group;
+      front_ml = reinterpret_cast<const float2*>(front.ws + (int64_t)front.ranges * front.all * D) + at;
+      front_po = front.ws + at * D + d0;
+    }
     for (int i = part; i < used; i += 4 * kParts) {
       float2 v[4];
       float4 w[4][D / 64];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int64_t at = (int64_t)min(i + b * kParts, used - 1) * all;
-        v[b] = ml[at];
+        const int range = min(i + b * kParts, used - 1);
+        if constexpr (kShared) {
+          const bool in_front = range < front.ranges;
+          const int64_t at = in_front ? range * front.all : (range - front.ranges) * all;
+          v[b] = (in_front ? front_ml : ml)[at];
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) w[b][e] = reinterpret_cast<const float4*>(po + at * D)[e];
+          for (int e = 0; e < D / 64; ++e)
+            w[b][e] = reinterpret_cast<const float4*>((in_front ? front_po : po) + at * D)[e];
+        } else {
+          const int64_t at = (int64_t)range * all;
+          v[b] = ml[at];
+#pragma unroll
+          for (int e = 0; e < D / 64; ++e) w[b][e] = reinterpret_cast<const float4*>(po + at * D)[e];
+        }
       }
       float next = top;
 #pragma unroll
@@ -814,7 +843,7 @@ __device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& s
 template <int T, int D, int kParts, bool kCap, bool kSlope>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_rows, int tiles,
                                                         int splits, int chunk, const float* ws) {
-  attn_join<T, D, kParts, kCap, kSlope, false>(a, AttnShared{}, tile_rows, tiles, splits, chunk, 0, 0, ws);
+  attn_join<T, D, kParts, kCap, kSlope, false>(a, AttnShared{}, AttnFront{}, tile_rows, tiles, splits, chunk, 0, ws);
 }
 
 }  // namespace imq

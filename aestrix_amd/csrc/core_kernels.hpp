@@ -76,8 +76,8 @@ struct SharedPlan {
   int kernel;      // an imq_shared_kernel
   AttnPlan tiles;  // IMQ_SHARED_TILES: of the walk over the shared and the own keys,
   int own0;        // the own ones from its key own0 on
-  // IMQ_SHARED_STREAM: rows of the batch against the shared keys, in tiles of s_rows, and the
-  // ranges of the shared and of each sequence's own keys.
+  // IMQ_SHARED_STREAM, _PACKED: rows of the batch against the shared keys, in tiles of s_rows, and
+  // the ranges of the shared and of each sequence's own keys.
   int s_rows, s_tiles, s_splits, s_chunk, o_splits, o_chunk;
   size_t bytes;    // workspace of the partial sums
 };

@@ -69,9 +69,11 @@ int imq_attention_shared_plan(imq_ctx* ctx, const imq_attention_args* args, cons
   if (!out) return fail(ctx, IMQ_EINVAL, "%s: null output", fn);
   const imq::SharedPlan p = imq::attention_shared_plan(a, sh, ctx->cus, true);
   out->kernel = p.kernel;
-  out->tile_rows = p.kernel == IMQ_SHARED_STREAM ? p.s_rows : p.kernel == IMQ_SHARED_TILES ? p.tiles.tile_rows : 1;
-  out->splits = p.kernel == IMQ_SHARED_STREAM ? p.s_splits : p.kernel == IMQ_SHARED_TILES ? p.tiles.splits : 1;
-  out->own_splits = p.kernel == IMQ_SHARED_STREAM ? p.o_splits : 0;
+  const bool apart = p.kernel == IMQ_SHARED_STREAM || p.kernel == IMQ_SHARED_PACKED;
+  const bool tiles = p.kernel == IMQ_SHARED_TILES;
+  out->tile_rows = apart ? p.s_rows : tiles ? p.tiles.tile_rows : 1;
+  out->splits = apart ? p.s_splits : tiles ? p.tiles.splits : 1;
+  out->own_splits = apart ? p.o_splits : 0;
   out->workspace_bytes = p.bytes;
   return IMQ_OK;
 }

@@ -195,15 +195,16 @@ int imq_attention_shared(imq_ctx* ctx, const imq_attention_args* args,
 typedef enum imq_shared_kernel {
   IMQ_SHARED_ROWS = 0,  /* a wave a row (dims past 128 or not a multiple of 8, unaligned tensors) */
   IMQ_SHARED_TILES = 1, /* a sequence's tiles walk the shared and then the own keys */
-  IMQ_SHARED_STREAM = 2 /* up to 32 rows a sequence: all sequences' rows together against the shared
-                           keys, each one's against its own, and a join */
+  IMQ_SHARED_STREAM = 2, /* up to 32 rows a sequence: all sequences' rows together against the shared
+                            keys, each one's against its own, and a join */
+  IMQ_SHARED_PACKED = 3  /* packed documents of few tiles each: the same on the tiles */
 } imq_shared_kernel;
 
 typedef struct imq_shared_plan_info {
   int kernel;     /* an imq_shared_kernel */
   int tile_rows;  /* rows (queries times heads a key head) of a workgroup, shared keys */
   int splits;     /* ranges of the shared keys (of the walk over both: IMQ_SHARED_TILES) */
-  int own_splits; /* ranges of a sequence's own keys (IMQ_SHARED_STREAM) */
+  int own_splits; /* ranges of a sequence's own keys (IMQ_SHARED_STREAM, _PACKED) */
   size_t workspace_bytes;
 } imq_shared_plan_info;
 

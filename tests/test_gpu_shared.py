@@ -155,6 +155,43 @@ def test_documents_shorter_than_the_offsets_say():
     assert bool((out[30:40] == 9.0).all() and (out[70:] == 9.0).all())
 
 
+@pytest.mark.parametrize("dim,dtype,softcap", [(128, BF16, 0.0), (64, F16, 30.0), (72, BF16, 5.0)])
+def test_documents_of_few_tiles(dim, dtype, softcap):
+    """Many short documents in one stretch of rows: whole tiles of several against the shared keys."""
+    lens = [(7 * i) % 78 for i in range(40)]
+    q, k = torch.zeros(sum(lens) + 5, 6, dim, dtype=dtype, device="cuda"), torch.zeros(sum(lens) + 3, 2, dim, dtype=dtype, device="cuda")
+    sk = k.new_zeros((1000, 2, dim))
+    at = ints([sum(lens[:i]) for i in range(41)])
+    plan = imq.attention_shared_plan(q, k, k, sk, sk, q_offsets=at, k_offsets=at, max_q=77, max_k=77, softcap=softcap)
+    assert plan["kernel"] == "packed", plan
+    packed(1000, lens, lens, 6, 2, dim, dtype, True, softcap=softcap)
+    packed(777, lens, [max(0, 90 - n) for n in lens], 6, 2, dim, dtype, True, softcap=softcap)
+    packed(513, lens, lens, 12, 4, dim, dtype, False, softcap=softcap)
+    packed(600, lens, lens, 6, 3, dim, dtype, True, prefix=[n // 2 for n in lens], softcap=softcap)
+    packed(600, [1, 77, 0, 64], [0, 0, 0, 0], 6, 1, dim, dtype, True, softcap=softcap)
+
+
+def test_documents_of_few_tiles_hidden_keys():
+    """NaN and infinities behind the documents' keys and behind the diagonal; rows of no document."""
+    g = gen(31)
+    lens = [60, 5, 77, 0, 33, 64, 77, 40]
+    at = [sum(lens[:i]) + 3 for i in range(9)]  # three rows before the first document
+    n = at[-1] + 4
+    q, k, v = randn(g, n, 8, 128, dtype=BF16), *(randn(g, n, 2, 128, dtype=BF16) for _ in range(2))
+    sk, sv = (randn(g, 900, 2, 128, dtype=BF16) for _ in range(2))
+    q[:3], q[at[-1]:], k[:3], v[:3], k[at[-1]:], v[at[-1]:] = NAN, NAN, NAN, INF, NAN, INF
+    for i, m in zip(at, lens):
+        if m:
+            k[i + m - 1], v[i + m - 1] = NAN, INF
+    out = torch.full_like(q, 9.0)
+    imq.attention_shared(q, k, v, sk, sv, causal=True, q_offsets=ints(at), k_offsets=ints(at), max_q=77, max_k=77, out=out)
+    for i, m in zip(at, lens):
+        if m > 1:
+            want, bound = wanted(q[i:i + m - 1], k[i:i + m - 1], v[i:i + m - 1], sk, sv, scale=128 ** -0.5, causal=True)
+            check(out[i:i + m - 1], want, bound, f"document from {i}")
+    assert bool((out[:3] == 9.0).all() and (out[at[-1]:] == 9.0).all())
+
+
 def test_no_shared_keys_is_attention():
     g = gen(5)
     for nq, nk in ((1, 300), (100, 100)):
