@@ -316,23 +316,21 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_stream_kernel(
 template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
 __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_shared_tiles_kernel(
     AttnArgs a, AttnShared sh, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
-  attn_tiles<T, D, WM, kCap, kSlope, kSplit, true>(a, sh, blockIdx.x, tiles, first, near_hs, splits, chunk, ws);
+  attn_tiles<T, D, WM, kCap, kSlope, kSplit, kKeys>(a, sh, AttnFront{}, tiles, first, near_hs, splits, chunk, ws);
 }
 
-// Packed documents that fill few tiles: all rows as they stand in q against the shared keys
-// (front: one sequence of them, f_tiles * f_splits * kv_heads workgroups), and each document's
-// against its own, every workgroup's sums to ws.
+// Packed documents that fill few tiles: first all rows as they stand in q, one sequence, against
+// ranges of the shared keys, then each document's against its own, on from those sums.
 template <int T, int D, int WM, bool kCap>
-__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_shared_packed_kernel(
-    AttnArgs front, AttnArgs own, int f_tiles, int f_splits, int f_chunk, int o_tiles, int o_chunk, float* f_ws,
-    float* o_ws) {
-  const int blocks = f_tiles * f_splits * front.kv_heads;
-  if ((int)blockIdx.x < blocks)
-    attn_tiles<T, D, WM, kCap, false, true, false>(front, AttnShared{}, blockIdx.x, f_tiles, f_tiles, 1, f_splits,
-                                                   f_chunk, f_ws);
-  else
-    attn_tiles<T, D, WM, kCap, false, true, false>(own, AttnShared{}, blockIdx.x - blocks, o_tiles, o_tiles, 1, 1,
-                                                   o_chunk, o_ws);
+__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_packed_front_kernel(AttnArgs a, int tiles,
+                                                                                  int splits, int chunk,
+                                                                                  float* ws) {
+  attn_tiles<T, D, WM, kCap, false, true, kNone>(a, AttnShared{}, AttnFront{}, tiles, tiles, 1, splits, chunk, ws);
+}
+template <int T, int D, int WM, bool kCap>
+__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_packed_own_kernel(AttnArgs a, AttnShared sh,
+                                                                                AttnFront front, int tiles) {
+  attn_tiles<T, D, WM, kCap, false, false, kSums>(a, sh, front, tiles, tiles, a.n_seq * a.kv_heads, 1, 0, nullptr);
 }
 
 template <int T, int D, int kParts, bool kCap, bool kSlope>
@@ -400,14 +398,13 @@ hipError_t launch_packed(const AttnArgs& a, const AttnShared& sh, const SharedPl
   const int group = a.heads / a.kv_heads;
   const int o_tiles = (a.max_q * group + kRows - 1) / kRows;
   const int64_t f_all = (int64_t)a.kv_heads * p.s_tiles * kRows;
-  const int64_t o_blocks = (int64_t)a.n_seq * a.kv_heads * o_tiles;
-  float* o_ws = ws + p.s_splits * f_all * (D + 2);
-  hipLaunchKernelGGL((attn_shared_packed_kernel<T, D, WM, kCap>),
-                     dim3((unsigned)((int64_t)a.kv_heads * p.s_tiles * p.s_splits + o_blocks)),
-                     dim3(attn_waves(WM) * 64), 0, stream, f, a, p.s_tiles, p.s_splits, p.s_chunk, o_tiles,
-                     p.o_chunk, ws, o_ws);
-  launch_shared_join<T, D, kCap, false>(a, sh, AttnFront{ws, f_all, p.s_splits, p.s_tiles * kRows}, kRows, o_tiles,
-                                        o_blocks * kRows, 1, p.o_chunk, 0, o_ws, stream);
+  const dim3 block(attn_waves(WM) * 64);
+  hipLaunchKernelGGL((attn_packed_front_kernel<T, D, WM, kCap>),
+                     dim3((unsigned)((int64_t)a.kv_heads * p.s_tiles * p.s_splits)), block, 0, stream, f,
+                     p.s_tiles, p.s_splits, p.s_chunk, ws);
+  hipLaunchKernelGGL((attn_packed_own_kernel<T, D, WM, kCap>),
+                     dim3((unsigned)((int64_t)a.n_seq * a.kv_heads * o_tiles)), block, 0, stream, a, sh,
+                     AttnFront{ws, f_all, p.s_splits, p.s_tiles * kRows}, o_tiles);
   return hipGetLastError();
 }
 

@@ -71,14 +71,13 @@ SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cu
       const int splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * cus + blocks / 2) / blocks, sh.rows / 512));
       const int chunk = (ranges(sh.rows, splits) + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
       const int d = a.dim > 64 ? 128 : 64;
-      const int64_t bytes = (ranges(sh.rows, chunk) * blocks + own) * 128 * (d + 2) * (int64_t)sizeof(float);
-      if (bytes <= kPackedBytes && (blocks * splits + own) * 256 < ((int64_t)1 << 32)) {
+      const int64_t bytes = ranges(sh.rows, chunk) * blocks * 128 * (d + 2) * (int64_t)sizeof(float);
+      if (bytes <= kPackedBytes && std::max(blocks * splits, own) * 256 < ((int64_t)1 << 32)) {
         p.kernel = IMQ_SHARED_PACKED;
         p.s_rows = 128;
         p.s_tiles = (int)packed;
         p.s_chunk = chunk;
         p.s_splits = ranges(sh.rows, chunk);
-        p.o_chunk = (std::max(a.max_k, 1) + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
         p.o_splits = 1;
         p.bytes = (size_t)bytes;
         return p;

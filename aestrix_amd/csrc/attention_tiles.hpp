@@ -374,10 +374,26 @@ __device__ __forceinline__ int attn_own0(const AttnShared& sh) {
   return (sh.rows + 2 * kAttnKeys - 1) / (2 * kAttnKeys) * (2 * kAttnKeys);
 }
 
-// kShared: `sh` stands before every sequence's keys; the walk is over both.
-template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit, bool kShared>
-__device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& sh, int block, int tiles,
-                                           int first, int near_hs, int splits, int chunk, float* ws) {
+// Sums of ranges of shared keys.
+struct AttnFront {
+  const float* ws;  // as a split plan's, of `all` rows
+  int64_t all;
+  int ranges;
+  int packed;  // rows of a key head, which stand in q's order; 0: the same rows as other ranges
+};
+__device__ __forceinline__ int64_t attn_packed_row(const AttnArgs& a, const AttnFront& front, int seq, int kh,
+                                                   int t, int g) {
+  const int64_t q = min(max(a.q_offsets[seq], 0), a.q_rows) + t;
+  return (int64_t)kh * front.packed + q * (a.heads / a.kv_heads) + g;
+}
+
+// What stands before every sequence's keys: nothing, the keys `sh`, which the walk begins with,
+// or their sums, `front`'s, which it goes on from.
+enum AttnBefore { kNone, kKeys, kSums };
+template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit, AttnBefore kBefore>
+__device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& sh, const AttnFront& front,
+                                           int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
+  constexpr bool kShared = kBefore == kKeys;
   using S = typename Elem<T>::S;
   // WM waves on rows of their own, WK on a part of every tile's keys each.
   constexpr int NW = attn_waves(WM), WK = NW / WM, U = 2 / WK, kRows = WM * 32;
@@ -388,9 +404,9 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hs_n = a.n_seq * a.kv_heads;
   // near_hs sequences and key heads (all, where keys are split) at a time.
-  const int hs0 = kSplit ? 0 : block / (near_hs * tiles) * near_hs;
+  const int hs0 = kSplit ? 0 : blockIdx.x / (near_hs * tiles) * near_hs;
   const int hs_now = kSplit ? hs_n : min(near_hs, hs_n - hs0);
-  const int at = block - hs0 * tiles;
+  const int at = blockIdx.x - hs0 * tiles;
   const int hs = hs0 + at % hs_now, rest = at / hs_now;
   const int split = kSplit ? rest % splits : 0;
   // The last rows of a causal sequence have the most keys: they start first.
@@ -492,6 +508,29 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
   float top = -INFINITY, sum = 0.f;
+  if constexpr (kBefore == kSums) {
+    static_assert(WK == 1, "every wave has its rows alone");
+    const int64_t at = attn_packed_row(a, front, hs / a.kv_heads, kh, t, m % group);
+    const float2* ml = reinterpret_cast<const float2*>(front.ws + front.ranges * front.all * D) + at;
+    for (int r = 0; r < front.ranges; ++r) {
+      const float2 v = ml[r * front.all];
+      const float* po = front.ws + (r * front.all + at) * D;
+      const float next = fmaxf(top, v.x), base = next == -INFINITY ? 0.f : next;
+      const float keep0 = __builtin_amdgcn_exp2f(top - base), keep1 = __builtin_amdgcn_exp2f(v.x - base);
+      top = next;
+      sum = sum * keep0 + (h == 0 ? v.y * keep1 : 0.f);  // the lane 32 away's is added at the end
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(po + i * 32 + 2 * e + 4 * h);
+          o[i][e] = o[i][e] * keep0 + w.x * keep1;
+          o[i][e + 1] = o[i][e + 1] * keep0 + w.y * keep1;
+          o[i][e + 2] = o[i][e + 2] * keep0 + w.z * keep1;
+          o[i][e + 3] = o[i][e + 3] * keep0 + w.w * keep1;
+        }
+    }
+  }
 
   // The wave's keys of the tile that begins at j0.
   // The next tile's loads go out among the score's MFMAs: before them they
@@ -621,7 +660,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
     }
   } else {
     // (Of keys whose scores are all -infinity the sum is zero too, and the output NaN.)
-    const float inv = kShared || seen > 0 ? 1.f / sum : 0.f;
+    const float inv = kBefore != kNone || seen > 0 ? 1.f / sum : 0.f;
     bool finite = true;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -670,8 +709,8 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
       const int r = __builtin_ctzll(again);
       again &= again - 1;
       const int tr = (mw + r) / group;
-      attn_row<T, kCap, kSlope, kShared>(a, s, kh * group + (mw + r) % group, tr, attn_seen(a, s, tr),
-                                         qs[wave], sh);
+      attn_row<T, kCap, kSlope, kBefore != kNone>(a, s, kh * group + (mw + r) % group, tr,
+                                                  attn_seen(a, s, tr), qs[wave], sh);
     }
   }
 }
@@ -679,8 +718,8 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
 template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
 __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
     AttnArgs a, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
-  attn_tiles<T, D, WM, kCap, kSlope, kSplit, false>(a, AttnShared{}, blockIdx.x, tiles, first, near_hs, splits,
-                                                       chunk, ws);
+  attn_tiles<T, D, WM, kCap, kSlope, kSplit, kNone>(a, AttnShared{}, AttnFront{}, tiles, first, near_hs,
+                                                       splits, chunk, ws);
 }
 
 // Joins the key ranges of a split plan: 16 lanes a row, D / 16 columns each,
@@ -689,14 +728,8 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
 // tile's ranges up to the last key that its last row sees are written, the
 // others not.  Bound by the latency of its loads: four ranges a group are in
 // flight together.
-// kShared: a row's first front.ranges ranges are the shared keys', in front.ws, and the others
-// are counted from `own0` keys before its own.
-struct AttnFront {
-  const float* ws;  // as a split plan's, of `all` rows
-  int64_t all;
-  int ranges;
-  int packed;  // rows of a key head, which stand in q's order; 0: the same rows as the other ranges
-};
+// kShared: a row's first front.ranges ranges are the shared keys', and the others are counted
+// from `own0` keys before its own.
 template <int T, int D, int kParts, bool kCap, bool kSlope, bool kShared>
 __device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& sh, const AttnFront& front,
                                           int tile_rows, int tiles, int splits, int chunk, int own0,
@@ -732,12 +765,8 @@ __device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& s
     const float2* front_ml = nullptr;
     const float* front_po = nullptr;
     if constexpr (kShared) {
-      int64_t at = row;
-      if (front.packed)
-        at = (int64_t)kh * front.packed +
-             (int64_t)(min(max(a.q_offsets[hs / a.kv_heads], 0), a.q_rows) + t) * group + m % group;
-      front_ml = reinterpret_cast<const float2*>(front.ws + (int64_t)front.ranges * front.all * D) + at;
-      front_po = front.ws + at * D + d0;
+      front_ml = reinterpret_cast<const float2*>(front.ws + (int64_t)front.ranges * front.all * D) + row;
+      front_po = front.ws + row * D + d0;
     }
     for (int i = part; i < used; i += 4 * kParts) {
       float2 v[4];
