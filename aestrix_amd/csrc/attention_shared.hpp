@@ -359,12 +359,13 @@ __global__ __launch_bounds__(256) void attn_shared_rows_kernel(AttnArgs a, AttnS
 
 // ---- launches
 
-// ranges: of a row, the front's among them.
+// Up to kJoinFew ranges 16 lanes a row take them all, four at a time; more are shared by 256.
+constexpr int kJoinFew = 8;
 template <int T, int D, bool kCap, bool kSlope>
 void launch_shared_join(const AttnArgs& a, const AttnShared& sh, const AttnFront& front, int tile_rows,
                         int tiles, int64_t all, int splits, int chunk, int own0, const float* ws,
                         hipStream_t stream) {
-  if (front.ranges + splits > 4)
+  if (front.ranges + splits > kJoinFew)
     hipLaunchKernelGGL((attn_shared_join_kernel<T, D, 16, kCap, kSlope>), dim3((unsigned)all), dim3(256), 0,
                        stream, a, sh, front, tile_rows, tiles, splits, chunk, own0, ws);
   else

@@ -47,10 +47,10 @@ __device__ __forceinline__ void lora_put(const LoraArgs& l, int row, int rank, f
   to[64 * 8] = lo;
 }
 
-// Few rows: a wave per row and rank.  Bound by reading A, and by the latency of that: eight
+// Few rows: a wave per row and rank.  Bound by reading A, and by the latency of that: kAhead
 // pieces of 1 KB of each of the two rows are on their way together.
 constexpr int kDotWaves = 4, kDotMaxM = 64;
-template <int T>
+template <int T, int kAhead>
 __global__ __launch_bounds__(kDotWaves * 64) void lora_dot_kernel(LoraArgs l, const uint16_t* x, int k, int m) {
   const int lane = threadIdx.x & 63;
   const int at = blockIdx.x * kDotWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -63,7 +63,6 @@ __global__ __launch_bounds__(kDotWaves * 64) void lora_dot_kernel(LoraArgs l, co
   const __amdgpu_buffer_rsrc_t ar = make_rsrc(l.a + (size_t)(to.row + r) * k, (uint32_t)k * 2);
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(x + (size_t)row * k, (uint32_t)k * 2);
   float sum[2] = {0.f, 0.f};
-  constexpr int kAhead = 8;
   for (int c = 0; c < k; c += kAhead * 512) {
     u32x4_t av[kAhead], xv[kAhead];  // (past the end: zeros)
 #pragma unroll
@@ -71,6 +70,7 @@ __global__ __launch_bounds__(kDotWaves * 64) void lora_dot_kernel(LoraArgs l, co
       av[p] = load_b128(ar, lane * 16, (uint32_t)c * 2 + p * 1024);
       xv[p] = load_b128(xr, lane * 16, (uint32_t)c * 2 + p * 1024);
     }
+    __builtin_amdgcn_sched_barrier(0);  // all of them first, rather than few for more waves
 #pragma unroll
     for (int p = 0; p < kAhead; ++p)
 #pragma unroll
@@ -282,40 +282,69 @@ __global__ __launch_bounds__(kOrderWaves * 64) void lora_order_kernel(LoraArgs l
 
 // ---- the join
 
-// A workgroup: 32 rows and 32 columns of y.  Its 16 waves take the adapters of the rows in
+// Few rows: a thread an output, one row a workgroup, B's row against u in 32 bits.  Bound by the
+// latency of `which`, `first` and B, one after the other; the ranges' sums are on the way meanwhile.
+template <int T>
+__global__ __launch_bounds__(256) void lora_join_few_kernel(LoraArgs l, const float* part, int splits,
+                                                            uint16_t* y, int n, int m) {
+  __shared__ float us[kLoraMaxRank];
+  const int row = blockIdx.y, t = threadIdx.x, col = blockIdx.x * 256 + t;
+  const float* from = part + (size_t)row * n + min(col, n - 1);
+  const size_t range = (size_t)m * n;
+  constexpr int kAhead = 8;
+  float v[kAhead];
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e) v[e] = from[min(e, splits - 1) * range];
+  const int i = lora_of(l, row);
+  float dot = 0.f;
+  if (i >= 0) {
+    const LoraAt at = lora_at(l, i);
+    const u32x4_t* b = reinterpret_cast<const u32x4_t*>(l.b + (size_t)at.row * n + (size_t)min(col, n - 1) * at.rank);
+    if (t < at.rank) {
+      const uint16_t* u = l.u + (((size_t)(row / 32) * (l.max_rank / 16) + t / 16) * 2 * 64 + row % 32 +
+                                 32 * (t >> 3 & 1)) * 8 + (t & 7);
+      us[t] = staged_value<T>(u[0]) + staged_value<T>(u[64 * 8]);
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int r = 0; r < at.rank / 16; ++r) {
+      const u32x4_t w[2] = {b[2 * r], b[2 * r + 1]};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        dot = __builtin_fmaf(staged_value<T>(w[e / 4][e % 4] & 0xFFFFu), us[16 * r + 2 * e], dot);
+        dot = __builtin_fmaf(staged_value<T>(w[e / 4][e % 4] >> 16), us[16 * r + 2 * e + 1], dot);
+      }
+    }
+  }
+  float sum = v[0];
+#pragma unroll
+  for (int e = 1; e < kAhead; ++e) sum += e < splits ? v[e] : 0.f;
+  for (int sp = kAhead; sp < splits; ++sp) sum += from[sp * range];
+  if (col < n) y[(size_t)row * n + col] = Elem<T>::out(sum + dot);
+}
+
+// More.  A workgroup: 32 rows and 32 columns of y.  Its 16 waves take the adapters of the rows in
 // turn; each writes its rows' products to LDS (a row has one adapter), where the ranges' sums
 // are added to them in order.  Bound by the latency of what a wave loads for an adapter; the
 // ranges' sums are on the way meanwhile.
-constexpr int kJoinWaves = 16;
+constexpr int kJoinWaves = 16;  // a thread an output
 template <int T>
-__global__ __launch_bounds__(kJoinWaves * 64) void lora_join_kernel(LoraArgs l, const float* part, int splits,
+__global__ __launch_bounds__(kJoinWaves * 64, 8) void lora_join_kernel(LoraArgs l, const float* part, int splits,
                                                                    uint16_t* y, int n, int m) {
   __shared__ float add[32 * 32];
   const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * 32, tile = blockIdx.y;
+  const int col = n0 + (int)(threadIdx.x & 31), of = threadIdx.x >> 5;  // of this thread's output
+  const float* from = part + (size_t)min(tile * 32 + of, m - 1) * n + min(col, n - 1);
+  const size_t range = (size_t)m * n;
+  // The first ranges' sums are on their way while the adapters' products are made.
+  constexpr int kAhead = 4;
+  float v[kAhead];
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e) v[e] = from[min(e, splits - 1) * range];
   const LoraRows of_tile(l, tile * 32 + r32, m);
-  constexpr int kOuts = 32 * 32 / (kJoinWaves * 64);  // outputs of a thread
-  const int col = n0 + (int)(threadIdx.x & 31), of = threadIdx.x >> 5;
-  float sum[kOuts];
-#pragma unroll
-  for (int o = 0; o < kOuts; ++o) {
-    sum[o] = 0.f;
-    add[o * kJoinWaves * 64 + threadIdx.x] = 0.f;
-  }
-  // Eight ranges at a time: their loads wait together.
-  constexpr int kAhead = 8;
-  for (int sp = 0; sp < splits; sp += kAhead)
-#pragma unroll
-    for (int o = 0; o < kOuts; ++o) {
-      const size_t r = min(tile * 32 + of + o * (kJoinWaves * 2), m - 1);
-      float v[kAhead];
-#pragma unroll
-      for (int e = 0; e < kAhead; ++e)
-        v[e] = part[((size_t)min(sp + e, splits - 1) * m + r) * n + min(col, n - 1)];
-#pragma unroll
-      for (int e = 0; e < kAhead; ++e) sum[o] += sp + e < splits ? v[e] : 0.f;
-    }
+  add[threadIdx.x] = 0.f;
   __syncthreads();
   uint32_t rows;
   LoraAt at;
@@ -328,13 +357,13 @@ __global__ __launch_bounds__(kJoinWaves * 64) void lora_join_kernel(LoraArgs l, 
       if (rows >> r & 1u) add[r * 32 + r32] = c[0][e];
     }
   }
-  __syncthreads();
+  float sum = v[0];
 #pragma unroll
-  for (int o = 0; o < kOuts; ++o) {
-    const int r = of + o * (kJoinWaves * 2);
-    if (tile * 32 + r < m && col < n)
-      y[(size_t)(tile * 32 + r) * n + col] = Elem<T>::out(sum[o] + add[r * 32 + (threadIdx.x & 31)]);
-  }
+  for (int e = 1; e < kAhead; ++e) sum += e < splits ? v[e] : 0.f;
+  for (int sp = kAhead; sp < splits; ++sp) sum += from[sp * range];
+  __syncthreads();
+  if (tile * 32 + of < m && col < n)
+    y[(size_t)(tile * 32 + of) * n + col] = Elem<T>::out(sum + add[threadIdx.x]);
 }
 
 }  // namespace
@@ -349,10 +378,18 @@ hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, in
   const auto* xx = static_cast<const uint16_t*>(x);
   if (m <= kDotMaxM) {
     const dim3 grid((unsigned)((m * l.max_rank + kDotWaves - 1) / kDotWaves)), block(kDotWaves * 64);
-    if (dtype == kBf16)
-      hipLaunchKernelGGL((lora_dot_kernel<kBf16>), grid, block, 0, stream, l, xx, k, m);
-    else
-      hipLaunchKernelGGL((lora_dot_kernel<kF16>), grid, block, 0, stream, l, xx, k, m);
+    // Rows of more than 8 KB: 20 pieces at a time, of which shorter rows would have too few.
+    if (k > 4096) {
+      if (dtype == kBf16)
+        hipLaunchKernelGGL((lora_dot_kernel<kBf16, 20>), grid, block, 0, stream, l, xx, k, m);
+      else
+        hipLaunchKernelGGL((lora_dot_kernel<kF16, 20>), grid, block, 0, stream, l, xx, k, m);
+    } else {
+      if (dtype == kBf16)
+        hipLaunchKernelGGL((lora_dot_kernel<kBf16, 8>), grid, block, 0, stream, l, xx, k, m);
+      else
+        hipLaunchKernelGGL((lora_dot_kernel<kF16, 8>), grid, block, 0, stream, l, xx, k, m);
+    }
     return hipGetLastError();
   }
   const dim3 grid((unsigned)((m + 31) / 32), (unsigned)((l.max_rank + 31) / 32), l.count > 1 ? 2 : 1),
@@ -366,8 +403,16 @@ hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, in
 
 hipError_t launch_lora_join(const LoraArgs& l, const float* part, int splits, void* y, int n, int m,
                             int dtype, hipStream_t stream) {
-  const dim3 grid((unsigned)((n + 31) / 32), (unsigned)((m + 31) / 32)), block(kJoinWaves * 64);
   auto* yy = static_cast<uint16_t*>(y);
+  if (m <= kDotMaxM) {
+    const dim3 grid((unsigned)((n + 255) / 256), (unsigned)m);
+    if (dtype == kBf16)
+      hipLaunchKernelGGL((lora_join_few_kernel<kBf16>), grid, dim3(256), 0, stream, l, part, splits, yy, n, m);
+    else
+      hipLaunchKernelGGL((lora_join_few_kernel<kF16>), grid, dim3(256), 0, stream, l, part, splits, yy, n, m);
+    return hipGetLastError();
+  }
+  const dim3 grid((unsigned)((n + 31) / 32), (unsigned)((m + 31) / 32)), block(kJoinWaves * 64);
   if (dtype == kBf16)
     hipLaunchKernelGGL((lora_join_kernel<kBf16>), grid, block, 0, stream, l, part, splits, yy, n, m);
   else
