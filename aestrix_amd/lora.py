@@ -76,6 +76,7 @@ class LoraAdapters:
         self._c = _lib.Lora(self.a.data_ptr(), self.b.data_ptr(), self.first.data_ptr(), self.scale.data_ptr(),
                             self.count, self.rows, self.max_rank)
         self._p = ctypes.addressof(self._c)
+        self._bytes: dict[int, int] = {}  # of the workspace, by a call's rows
 
 
 def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
@@ -90,24 +91,31 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     into graphs and graphs replayed beside each other; a call's result does not depend on any of that."""
     n, k, m, lead, x = _epi_args(x, w, scales, biases, group_size, bits)
     idx = w.get_device()
-    if not (adapters.k == k and adapters.n == n and adapters.dtype == x.dtype and adapters.device == x.device):
+    device = x.device
+    if not (adapters.k == k and adapters.n == n and adapters.dtype == x.dtype and adapters.device == device):
         raise ValueError(f"adapters of a {adapters.dtype} [{adapters.n}, {adapters.k}] projection on {adapters.device}, "
-                         f"this is {x.dtype} [{n}, {k}] on {x.device}")
-    if not (which.dtype == torch.int32 and which.shape == lead and which.is_contiguous() and which.device == x.device):
+                         f"this is {x.dtype} [{n}, {k}] on {device}")
+    if not (which.dtype == torch.int32 and which.shape == lead and which.is_contiguous() and which.device == device):
         raise ValueError(f"which must be a contiguous int32 tensor of shape {lead} on x's device")
     shape = lead + (n,)
     if out is None:
         out = new_out(x, shape)
-    _require(out.is_contiguous() and out.shape == shape and out.dtype == x.dtype and out.device == x.device,
-             "out must be a contiguous [..., N] tensor of x's dtype and device")
+    elif not (out.is_contiguous() and out.shape == shape and out.dtype == x.dtype and out.device == device):
+        raise ValueError("out must be a contiguous [..., N] tensor of x's dtype and device")
     if m == 0:
         return out
     ctx = context(idx)
     lib, dtype = _lib.load(), _DTYPES.get(x.dtype, -1)
-    need = ctypes.c_size_t()
-    _lib.check(lib.imq_qmm_lora_workspace(ctx, adapters._p, k, n, m, dtype, ctypes.byref(need)), ctx)
-    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
-    _lib.check(run_on(idx, lib.imq_qmm_lora, ctx, w.data_ptr(), scales.data_ptr(), biases.data_ptr(), x.data_ptr(),
-                      adapters._p, which.data_ptr(), out.data_ptr(), k, n, m, group_size, bits, dtype,
-                      ws.data_ptr(), need.value, raw_stream(idx)), ctx)
+    need = adapters._bytes.get(m)
+    if need is None:
+        size = ctypes.c_size_t()
+        _lib.check(lib.imq_qmm_lora_workspace(ctx, adapters._p, k, n, m, dtype, ctypes.byref(size)), ctx)
+        need = adapters._bytes[m] = size.value
+    ws = x.new_empty((need + 1) // 2) if type(x) is torch.Tensor else \
+        torch.empty((need + 1) // 2, dtype=x.dtype, device=x.device)
+    rc = run_on(idx, lib.imq_qmm_lora, ctx, w.data_ptr(), scales.data_ptr(), biases.data_ptr(), x.data_ptr(),
+                adapters._p, which.data_ptr(), out.data_ptr(), k, n, m, group_size, bits, dtype, ws.data_ptr(),
+                need, raw_stream(idx))
+    if rc:
+        _lib.check(rc, ctx)
     return out
