@@ -268,9 +268,6 @@ hipError_t launch_qskinny(const uint32_t* w, const void* scales, const void* bia
 // row, also where a plain product would run unsplit (no unsplit kernel has
 // the residual add; the tile kernel's form is the alternative).
 size_t qskinny_resid_split_bytes(int k, int n, int m);
-// That K split's partial sums alone: ws [splits][m][n], qskinny_resid_split_bytes of them.
-hipError_t launch_qskinny_partials(const uint32_t* w, const void* scales, const void* biases, const void* x,
-                                   float* ws, int k, int n, int m, int dtype, hipStream_t stream);
 // y[m][j] = EpSwiGLU(gate sum j, up sum j) for j < width over a pair weight of
 // n = 2 width rows (gate rows [0, width), up rows [width, n)): the few-row
 // kernel's K split, its fp32 partial sums summed by the tile kernel's

@@ -81,7 +81,7 @@ int imq_qmm_lora(imq_ctx* ctx, const uint32_t* w, const void* scales, const void
     e = imq::launch_lora_order(l, order, order + m, m, st);
     l.order = order, l.which = order + m;
   }
-  if (e == hipSuccess) e = imq::launch_lora_shrink(l, x, k, m, (int)dtype, st);
+  if (e == hipSuccess && !plan.few) e = imq::launch_lora_shrink(l, x, k, m, (int)dtype, st);
   if (e == hipSuccess)
     e = imq::launch_qgemm_lora(plan, w, scales, biases, x, l, part, y, k, n, m, (int)dtype, st);
   if (e == hipSuccess && plan.splits > 0)

@@ -34,54 +34,10 @@ struct LoraRows {
   }
 };
 
-// u of row `row` and rank `rank` to its place: the upper half, and what it leaves (nothing where
-// it is infinite).
-template <int T>
-__device__ __forceinline__ void lora_put(const LoraArgs& l, int row, int rank, float u) {
-  const uint16_t hi = Elem<T>::out(u);
-  const float v = staged_value<T>(hi);
-  const uint16_t lo = Elem<T>::out(__builtin_fabsf(v) < INFINITY ? u - v : 0.f);
-  uint16_t* to = l.u + (((size_t)(row / 32) * (l.max_rank / 16) + rank / 16) * 2 * 64 + row % 32 +
-                        32 * (rank >> 3 & 1)) * 8 + (rank & 7);
-  to[0] = hi;
-  to[64 * 8] = lo;
-}
-
-// Few rows: a wave per row and rank.  Bound by reading A, and by the latency of that: kAhead
-// pieces of 1 KB of each of the two rows are on their way together.
 constexpr int kDotWaves = 4, kDotMaxM = 64;
 template <int T, int kAhead>
 __global__ __launch_bounds__(kDotWaves * 64) void lora_dot_kernel(LoraArgs l, const uint16_t* x, int k, int m) {
-  const int lane = threadIdx.x & 63;
-  const int at = blockIdx.x * kDotWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = at / l.max_rank, r = at % l.max_rank;  // up to 64 rows
-  if (row >= m) return;
-  const int i = lora_of(l, row);
-  if (i < 0) return;
-  const LoraAt to = lora_at(l, i);
-  if (r >= to.rank) return;
-  const __amdgpu_buffer_rsrc_t ar = make_rsrc(l.a + (size_t)(to.row + r) * k, (uint32_t)k * 2);
-  const __amdgpu_buffer_rsrc_t xr = make_rsrc(x + (size_t)row * k, (uint32_t)k * 2);
-  float sum[2] = {0.f, 0.f};
-  for (int c = 0; c < k; c += kAhead * 512) {
-    u32x4_t av[kAhead], xv[kAhead];  // (past the end: zeros)
-#pragma unroll
-    for (int p = 0; p < kAhead; ++p) {
-      av[p] = load_b128(ar, lane * 16, (uint32_t)c * 2 + p * 1024);
-      xv[p] = load_b128(xr, lane * 16, (uint32_t)c * 2 + p * 1024);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // all of them first, rather than few for more waves
-#pragma unroll
-    for (int p = 0; p < kAhead; ++p)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        sum[e & 1] = T == kBf16 ? dot2_bf16(av[p][e], xv[p][e], sum[e & 1])
-                                : dot2_f16(av[p][e], xv[p][e], sum[e & 1]);
-  }
-  float u = sum[0] + sum[1];
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) u += __shfl_xor(u, off, 64);
-  if (lane == 0) lora_put<T>(l, row, r, u * l.scale[i]);
+  lora_dot<T, kAhead>(l, x, k, m, blockIdx.x * kDotWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 }
 
 // More rows.  A workgroup: 32 of them against 32 ranks (blockIdx.y) of the adapters that they

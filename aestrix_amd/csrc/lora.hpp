@@ -32,7 +32,7 @@ inline size_t lora_u_bytes(int m, int max_rank) {
 
 // How the projection of a call runs.
 struct LoraPlan {
-  int few;        // the few-row kernel's partial sums (qskinny.hip), ...
+  int few;        // the few-row kernel's partial sums, with u beside them (qskinny.hip), ...
   int splits;     // ... or the tile kernels': ranges of K, joined by launch_lora_join; 0: the
                   // tile kernels add B u themselves
   int mt, nt, split_steps;  // their tiles (BigPlan)
@@ -50,6 +50,10 @@ hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, in
 // y = T(sum of the ranges + B u) (lora.hip); part: fp32 [splits][m][n].
 hipError_t launch_lora_join(const LoraArgs& l, const float* part, int splits, void* y, int n, int m,
                             int dtype, hipStream_t stream);
+// The few-row kernel's partial sums, ws fp32 [splits][m][n], and u beside them (qskinny.hip).
+hipError_t launch_qskinny_lora(const uint32_t* w, const void* scales, const void* biases, const void* x,
+                               float* ws, const LoraArgs& l, int k, int n, int m, int dtype,
+                               hipStream_t stream);
 // The projection: partial sums to part where the plan has them, else y (qgemm.hip).
 hipError_t launch_qgemm_lora(const LoraPlan& p, const uint32_t* w, const void* scales, const void* biases,
                              const void* x, const LoraArgs& l, float* part, void* y, int k, int n, int m,

@@ -310,7 +310,7 @@ hipError_t launch_lora_t(const LoraPlan& p, const uint32_t* w, const uint16_t* s
 hipError_t launch_qgemm_lora(const LoraPlan& p, const uint32_t* w, const void* scales, const void* biases,
                              const void* x, const LoraArgs& l, float* part, void* y, int k, int n, int m,
                              int dtype, hipStream_t stream) {
-  if (p.few) return launch_qskinny_partials(w, scales, biases, x, part, k, n, m, dtype, stream);
+  if (p.few) return launch_qskinny_lora(w, scales, biases, x, part, l, k, n, m, dtype, stream);
   const auto* s = static_cast<const uint16_t*>(scales);
   const auto* b = static_cast<const uint16_t*>(biases);
   const auto* xx = static_cast<const uint16_t*>(x);

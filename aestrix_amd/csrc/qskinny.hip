@@ -30,6 +30,7 @@
 #include "epilogue.hpp"
 #include "imq_device.hpp"
 #include "imq_kernels.hpp"
+#include "lora_device.hpp"
 
 namespace imq {
 namespace {
@@ -804,19 +805,18 @@ hipError_t launch_lds_t(const uint32_t* w, const uint16_t* s, const uint16_t* b,
 // chunk.  Fp32 partial sums go to ws[s][m][n]; qskinny_reduce_kernel (or a
 // fused-stage split sum) adds the splits in order (deterministic).
 template <int T, int R, int W, int TG, int CH>
-__global__ __launch_bounds__(64 * W) void qskinny_rows_kernel(const uint32_t* __restrict__ w,
-                                                              const uint16_t* __restrict__ scales,
-                                                              const uint16_t* __restrict__ biases,
-                                                              const uint16_t* __restrict__ x,
-                                                              float* __restrict__ ws, int M,
-                                                              int N, int K, int per, bool vec) {
+__device__ __forceinline__ void qskinny_rows(const uint32_t* __restrict__ w,
+                                             const uint16_t* __restrict__ scales,
+                                             const uint16_t* __restrict__ biases,
+                                             const uint16_t* __restrict__ x, float* __restrict__ ws, int M,
+                                             int N, int K, int per, bool vec, int block) {
   static_assert(CH % 4 == 0 && CH * R + CH / 2 * R <= 63, "the loads after x fit vmcnt");
   constexpr int kBlk = CH / 4;  // 16-byte scale (bias) blocks per row: 8 groups, 512 k each
   extern __shared__ uint4 xs[];  // x [M, 512 per], rows 1024 per + 16 bytes apart
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, h = lane >> 4;
-  const int n0 = ((int)blockIdx.x * W + wave) * (kRows * R);
+  const int n0 = (block * W + wave) * (kRows * R);
   const int gpr = K >> 6;
   const int p0 = (int)blockIdx.y * per;
   const int np = min(per, (K >> 9) - p0);  // pieces of 512 k in this range (>= 1)
@@ -933,6 +933,35 @@ __global__ __launch_bounds__(64 * W) void qskinny_rows_kernel(const uint32_t* __
       }
     }
   }
+}
+
+template <int T, int R, int W, int TG, int CH>
+__global__ __launch_bounds__(64 * W) void qskinny_rows_kernel(const uint32_t* __restrict__ w,
+                                                              const uint16_t* __restrict__ scales,
+                                                              const uint16_t* __restrict__ biases,
+                                                              const uint16_t* __restrict__ x,
+                                                              float* __restrict__ ws, int M,
+                                                              int N, int K, int per, bool vec) {
+  qskinny_rows<T, R, W, TG, CH>(w, scales, biases, x, ws, M, N, K, per, vec, (int)blockIdx.x);
+}
+
+// The same, and in the first `dots` workgroups of every split the adapters' u (lora_dot): it is
+// needed by the join alone, and the weights take longer.
+template <int T, int R, int W, int TG, int CH>
+__global__ __launch_bounds__(64 * W) void qskinny_lora_kernel(const uint32_t* __restrict__ w,
+                                                              const uint16_t* __restrict__ scales,
+                                                              const uint16_t* __restrict__ biases,
+                                                              const uint16_t* __restrict__ x,
+                                                              float* __restrict__ ws, int M,
+                                                              int N, int K, int per, bool vec, LoraArgs l,
+                                                              int dots) {
+  const int block = (int)blockIdx.x - dots;
+  if (block < 0)
+    lora_dot<T, 8>(l, x, K, M,
+                   (((int)blockIdx.y * dots + (int)blockIdx.x) * W) +
+                       __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6));
+  else
+    qskinny_rows<T, R, W, TG, CH>(w, scales, biases, x, ws, M, N, K, per, vec, block);
 }
 
 // Splits whose partial sums a thread of the split sum + RMSNorm loads before
@@ -1360,15 +1389,46 @@ size_t qskinny_resid_split_bytes(int k, int n, int m) {
   return sp.ok ? (size_t)sp.splits * m * n * sizeof(float) : 0;
 }
 
-hipError_t launch_qskinny_partials(const uint32_t* w, const void* scales, const void* biases, const void* x,
-                                   float* ws, int k, int n, int m, int dtype, hipStream_t stream) {
+namespace {
+
+template <int T, int R, int CH>
+hipError_t launch_lora_k(const uint32_t* w, const uint16_t* s, const uint16_t* b, const uint16_t* x, float* ws,
+                         const LoraArgs& l, int k, int n, int m, const SplitPlan& p, hipStream_t stream) {
+  constexpr int W = 4;  // rows_plan's
+  const bool vec = n % 4 == 0;
+  const int wg_rows = kRows * R * W, dots = (m * l.max_rank + W * p.splits - 1) / (W * p.splits);
+  const dim3 grid((unsigned)((n + wg_rows - 1) / wg_rows + dots), (unsigned)p.splits);
+  if (m > kRows)
+    hipLaunchKernelGGL((qskinny_lora_kernel<T, R, W, 2, CH>), grid, dim3(64 * W), split_x_bytes(p.per, m),
+                       stream, w, s, b, x, ws, m, n, k, p.per, vec, l, dots);
+  else
+    hipLaunchKernelGGL((qskinny_lora_kernel<T, R, W, 1, CH>), grid, dim3(64 * W), split_x_bytes(p.per, m),
+                       stream, w, s, b, x, ws, m, n, k, p.per, vec, l, dots);
+  return hipGetLastError();
+}
+
+template <int T>
+hipError_t launch_lora_t(const uint32_t* w, const uint16_t* s, const uint16_t* b, const uint16_t* x, float* ws,
+                         const LoraArgs& l, int k, int n, int m, const SplitPlan& p, hipStream_t stream) {
+  if (p.rr == 1)
+    return p.per == 1 ? launch_lora_k<T, 1, 4>(w, s, b, x, ws, l, k, n, m, p, stream)
+                      : launch_lora_k<T, 1, 8>(w, s, b, x, ws, l, k, n, m, p, stream);
+  return p.per == 1 ? launch_lora_k<T, 2, 4>(w, s, b, x, ws, l, k, n, m, p, stream)
+                    : launch_lora_k<T, 2, 8>(w, s, b, x, ws, l, k, n, m, p, stream);
+}
+
+}  // namespace
+
+hipError_t launch_qskinny_lora(const uint32_t* w, const void* scales, const void* biases, const void* x,
+                               float* ws, const LoraArgs& l, int k, int n, int m, int dtype,
+                               hipStream_t stream) {
   const SplitPlan sp = plan_split(k, n, m, true);
   if (!sp.ok || !qskinny_supported(k, n, m, dtype)) return hipErrorInvalidValue;
   const auto* s = static_cast<const uint16_t*>(scales);
   const auto* b = static_cast<const uint16_t*>(biases);
   const auto* xx = static_cast<const uint16_t*>(x);
-  return dtype == kBf16 ? launch_split_partials<kBf16>(w, s, b, xx, ws, k, n, m, sp, stream)
-                        : launch_split_partials<kF16>(w, s, b, xx, ws, k, n, m, sp, stream);
+  return dtype == kBf16 ? launch_lora_t<kBf16>(w, s, b, xx, ws, l, k, n, m, sp, stream)
+                        : launch_lora_t<kF16>(w, s, b, xx, ws, l, k, n, m, sp, stream);
 }
 
 int qskinny_splits(int k, int n, int m) {
