@@ -41,11 +41,13 @@ __global__ __launch_bounds__(kDotWaves * 64) void lora_dot_kernel(LoraArgs l, co
 }
 
 // More rows.  A workgroup: 32 of them against 32 ranks (blockIdx.y) of the adapters that they
-// name, every second one (blockIdx.z).  Its eight waves take K in turn, 64 at a time, from buffers of their
-// own: whole 128-byte lines of x's and A's rows straight to LDS (operands loaded straight to
-// registers touch 32 bytes of a line each, and 16 such waves took 35 us of 4608 rows of 2560), the
-// next piece on its way while one is multiplied.  16-byte pieces are swizzled by the row at their
-// source, so that the operand reads touch every bank evenly.  The waves' sums are added through LDS.
+// name, every second one (blockIdx.z).  Its eight waves take K in turn, 64 at a time, from buffers
+// of their own: whole 128-byte lines of x's and A's rows straight to LDS (operands loaded straight
+// to registers touch 32 bytes of a line each, and 16 such waves took 35 us of 4608 rows of 2560
+// against one adapter of rank 64, this 14), the next piece on its way while one is multiplied.
+// 16-byte pieces are swizzled by the row at their source, so that the operand reads touch every
+// bank evenly.  The waves' sums are added through LDS.  Bound by the latency of the loads, of
+// `which` and `first` before them: 4000 rows of 2560 in runs of 100 of rank 16 12 us.
 constexpr int kShrinkWaves = 8;
 struct ShrinkBuf {
   uint4 x[32 * 8], a[32 * 8];

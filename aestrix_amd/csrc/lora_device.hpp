@@ -16,7 +16,7 @@ struct LoraAt {
   int row, rank;
 };
 __device__ __forceinline__ LoraAt lora_at(const LoraArgs& l, int i) {
-  const int a = min(max(l.first[i], 0), l.rows), b = min(max(l.first[i + 1], a), l.rows);
+  const int a = min(max(l.first[i], 0), l.rows) & ~15, b = min(max(l.first[i + 1], a), l.rows);
   return LoraAt{a, min(b - a, l.max_rank) & ~15};
 }
 // The adapter of row `row` (< m), or -1.

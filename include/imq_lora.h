@@ -53,7 +53,8 @@ int imq_qmm_lora_workspace(imq_ctx* ctx, const imq_lora* lora, int k, int n, int
  * imq_qmm_lora_workspace's bytes of device memory, 16-byte aligned, this call's alone
  * until its kernels have run.  Other arguments and alignment as imq_qmm_t.  A row's
  * result does not depend on the rows beside it but for the order of fp32 sums, which
- * the sizes alone decide; what an adapter holds (infinities, NaN) reaches its rows only. */
+ * the sizes alone decide.  What an adapter holds reaches its rows only: where B_i is infinite or
+ * NaN, their outputs of that column are not finite. */
 int imq_qmm_lora(imq_ctx* ctx, const uint32_t* w, const void* scales, const void* biases,
                  const void* x, const imq_lora* lora, const int32_t* which, void* y, int k, int n,
                  int m, int group_size, int bits, imq_dtype dtype, void* ws, size_t ws_bytes,

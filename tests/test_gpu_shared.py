@@ -101,6 +101,9 @@ def test_more_queries_than_keys():
     """Queries before the first own key see the shared ones alone."""
     run_batch(90, 200, 50, 4, 2, 128, BF16, kn=[50, 0, 33])
     run_batch(90, 5, 3, 4, 2, 64, F16, kn=[3, 0, 1], slope=True)
+    for softcap in (0.0, 20.0):
+        run_batch(333, 200, 50, 4, 2, 128, BF16, kn=[50, 0, 33], slope=True, softcap=softcap)
+        run_batch(333, 200, 50, 4, 2, 64, F16, kn=[50, 0, 33], slope=True, softcap=softcap, causal=False)
 
 
 @pytest.mark.parametrize("nq,nk", [(90, 90), (1, 80), (8, 300), (257, 257)])
