@@ -83,14 +83,74 @@ struct AttnScore {
 // a key per lane for the scores, `dim` elements over the lanes for the product
 // with v, the running maximum and sum rescaled per 64 keys.  Only keys below
 // `seen` are read, so nothing that a mask hides can reach the output.
+// qs: dim floats of LDS of this wave's own.
+template <int T, bool kCap, bool kSlope>
+__device__ void attn_row(const AttnArgs& a, const AttnSeq& s, int head, int t, int seen,
+                         float* qs) {
+  using S = typename Elem<T>::S;
+  const int lane = threadIdx.x & 63;
+  const int kh = head / (a.heads / a.kv_heads);
+  const S* q = static_cast<const S*>(a.q) + s.q_at + t * a.q_row + head * a.q_head;
+  const S* k = static_cast<const S*>(a.k) + s.k_at + kh * a.k_head;
+  const S* v = static_cast<const S*>(a.v) + s.v_at + kh * a.v_head;
+  S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
+  const AttnScore<kCap, kSlope> score(a, head);
+  for (int d = lane; d < a.dim; d += 64) qs[d] = Elem<T>::param(q[d]);
+  __builtin_amdgcn_wave_barrier();
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
+  const int p = t + s.nk - s.nq;
+  for (int j0 = 0; j0 < seen; j0 += 64) {
+    const int j = j0 + lane;
+    float e = -INFINITY;
+    if (j < seen) {
+      const S* kr = k + (int64_t)j * a.k_row;
+      float dot = 0.f;
+      for (int d = 0; d < a.dim; ++d) dot = __builtin_fmaf(qs[d], Elem<T>::param(kr[d]), dot);
+      e = score(dot, (float)(p - j));
+    }
+    float m = e;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    // fmaxf drops a NaN; the weight below brings it back into the sum.
+    const float next = fmaxf(top, m);
+    const float base = next == -INFINITY ? 0.f : next;
+    const float keep = __builtin_amdgcn_exp2f(top - base);
+    const float w = __builtin_amdgcn_exp2f(e - base);
+    float ws = w;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) ws += __shfl_xor(ws, off, 64);
+    sum = sum * keep + ws;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= keep;
+    top = next;
+    const int n = min(64, seen - j0);
+    for (int i = 0; i < n; ++i) {
+      const float wi = __builtin_bit_cast(
+          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
+      const S* vr = v + (int64_t)(j0 + i) * a.v_row;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (lane + 64 * c < a.dim)
+          acc[c] = __builtin_fmaf(wi, Elem<T>::param(vr[lane + 64 * c]), acc[c]);
+    }
+  }
+  const float inv = seen > 0 ? 1.f / sum : 0.f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (lane + 64 * c < a.dim) {
+      const float o = acc[c] * inv;
+      out[lane + 64 * c] = (S)(Elem<T>::pack2(o, o) & 0xFFFFu);
+    }
+}
+
+// The same where the keys `sh` come before the sequence's own and are all seen.
 struct AttnRowSums {
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
 };
 
 // The first n keys at k and v (rows k_row and v_row apart), key j at p - j from the query.
-// kLow: weights are 2^-32 of what they are, so that the largest bf16 values of 2^32 keys add
-// up in fp32.
-template <int T, bool kLow, bool kCap, bool kSlope>
+// Weights are 2^-32 of what they are, so that the largest bf16 values of 2^32 keys add up in fp32.
+template <int T, bool kCap, bool kSlope>
 __device__ __forceinline__ void attn_row_keys(const AttnArgs& a, const typename Elem<T>::S* k,
                                               const typename Elem<T>::S* v, int64_t k_row,
                                               int64_t v_row, int n_keys, int p,
@@ -114,7 +174,7 @@ __device__ __forceinline__ void attn_row_keys(const AttnArgs& a, const typename 
     const float next = fmaxf(r.top, m);
     const float base = next == -INFINITY ? 0.f : next;
     const float keep = __builtin_amdgcn_exp2f(r.top - base);
-    const float w = __builtin_amdgcn_exp2f(e - base) * (kLow ? 0x1p-32f : 1.f);
+    const float w = __builtin_amdgcn_exp2f(e - base) * 0x1p-32f;
     float ws = w;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) ws += __shfl_xor(ws, off, 64);
@@ -135,11 +195,9 @@ __device__ __forceinline__ void attn_row_keys(const AttnArgs& a, const typename 
   }
 }
 
-// qs: dim floats of LDS of this wave's own.  sh (kShared): keys that come before the
-// sequence's own and are all seen.
-template <int T, bool kCap, bool kSlope, bool kShared = false>
-__device__ void attn_row(const AttnArgs& a, const AttnSeq& s, int head, int t, int seen, float* qs,
-                         const AttnShared& sh = AttnShared{}) {
+template <int T, bool kCap, bool kSlope>
+__device__ void attn_row_shared(const AttnArgs& a, const AttnShared& sh, const AttnSeq& s, int head, int t,
+                                int seen, float* qs) {
   using S = typename Elem<T>::S;
   const int lane = threadIdx.x & 63;
   const int kh = head / (a.heads / a.kv_heads);
@@ -152,12 +210,11 @@ __device__ void attn_row(const AttnArgs& a, const AttnSeq& s, int head, int t, i
   __builtin_amdgcn_wave_barrier();
   AttnRowSums r;
   const int p = t + s.nk - s.nq;
-  if constexpr (kShared)
-    attn_row_keys<T, true>(a, static_cast<const S*>(sh.k) + kh * sh.k_head,
-                     static_cast<const S*>(sh.v) + kh * sh.v_head, sh.k_row, sh.v_row, sh.rows,
-                     sh.rows + p, score, qs, r);
-  attn_row_keys<T, kShared>(a, k, v, a.k_row, a.v_row, seen, p, score, qs, r);
-  const float inv = seen > 0 || (kShared && sh.rows > 0) ? 1.f / r.sum : 0.f;
+  attn_row_keys<T>(a, static_cast<const S*>(sh.k) + kh * sh.k_head,
+                   static_cast<const S*>(sh.v) + kh * sh.v_head, sh.k_row, sh.v_row, sh.rows, sh.rows + p,
+                   score, qs, r);
+  attn_row_keys<T>(a, k, v, a.k_row, a.v_row, seen, p, score, qs, r);
+  const float inv = seen > 0 || sh.rows > 0 ? 1.f / r.sum : 0.f;
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     if (lane + 64 * c < a.dim) {

@@ -16,6 +16,7 @@
 
 #include "attention.hpp"
 #include "attention_tiles.hpp"
+#include "attention_walk.hpp"
 #include "imq_core.h"
 
 namespace imq {
@@ -311,35 +312,6 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void attn_stream_kernel(
                                         ws + split * all * D, ml + split * all);
 }
 
-// ---- many rows a sequence
-
-template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
-__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_shared_tiles_kernel(
-    AttnArgs a, AttnShared sh, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
-  attn_tiles<T, D, WM, kCap, kSlope, kSplit, kKeys>(a, sh, AttnFront{}, tiles, first, near_hs, splits, chunk, ws);
-}
-
-// Packed documents that fill few tiles: first all rows as they stand in q, one sequence, against
-// ranges of the shared keys, then each document's against its own, on from those sums.
-template <int T, int D, int WM, bool kCap>
-__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_packed_front_kernel(AttnArgs a, int tiles,
-                                                                                  int splits, int chunk,
-                                                                                  float* ws) {
-  attn_tiles<T, D, WM, kCap, false, true, kNone>(a, AttnShared{}, AttnFront{}, tiles, tiles, 1, splits, chunk, ws);
-}
-template <int T, int D, int WM, bool kCap>
-__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_packed_own_kernel(AttnArgs a, AttnShared sh,
-                                                                                AttnFront front, int tiles) {
-  attn_tiles<T, D, WM, kCap, false, false, kSums>(a, sh, front, tiles, tiles, a.n_seq * a.kv_heads, 1, 0, nullptr);
-}
-
-template <int T, int D, int kParts, bool kCap, bool kSlope>
-__global__ __launch_bounds__(256) void attn_shared_join_kernel(AttnArgs a, AttnShared sh, AttnFront front,
-                                                               int tile_rows, int tiles, int splits, int chunk,
-                                                               int own0, const float* ws) {
-  attn_join<T, D, kParts, kCap, kSlope, true>(a, sh, front, tile_rows, tiles, splits, chunk, own0, ws);
-}
-
 // ---- any alignment and head dim: a wave a row, from the definition
 
 template <int T, bool kCap, bool kSlope>
@@ -353,7 +325,7 @@ __global__ __launch_bounds__(256) void attn_shared_rows_kernel(AttnArgs a, AttnS
     const int t = (int)(row % a.max_q);
     const AttnSeq s = attn_seq(a, (int)(row / a.max_q));
     if (t >= s.nq) continue;
-    attn_row<T, kCap, kSlope, true>(a, s, head, t, attn_seen(a, s, t), qs[wave], sh);
+    attn_row_shared<T, kCap, kSlope>(a, sh, s, head, t, attn_seen(a, s, t), qs[wave]);
   }
 }
 
@@ -365,12 +337,14 @@ template <int T, int D, bool kCap, bool kSlope>
 void launch_shared_join(const AttnArgs& a, const AttnShared& sh, const AttnFront& front, int tile_rows,
                         int tiles, int64_t all, int splits, int chunk, int own0, const float* ws,
                         hipStream_t stream) {
+  const AttnJoinShared before{sh, front, own0};
   if (front.ranges + splits > kJoinFew)
-    hipLaunchKernelGGL((attn_shared_join_kernel<T, D, 16, kCap, kSlope>), dim3((unsigned)all), dim3(256), 0,
-                       stream, a, sh, front, tile_rows, tiles, splits, chunk, own0, ws);
+    hipLaunchKernelGGL((attn_shared_join_kernel<T, D, 16, kCap, kSlope>), dim3((unsigned)all), dim3(256),
+                       0, stream, a, tile_rows, tiles, splits, chunk, ws, before);
   else
-    hipLaunchKernelGGL((attn_shared_join_kernel<T, D, 1, kCap, kSlope>), dim3((unsigned)((all + 15) / 16)),
-                       dim3(256), 0, stream, a, sh, front, tile_rows, tiles, splits, chunk, own0, ws);
+    hipLaunchKernelGGL((attn_shared_join_kernel<T, D, 1, kCap, kSlope>),
+                       dim3((unsigned)((all + 15) / 16)), dim3(256), 0, stream, a, tile_rows, tiles, splits, chunk,
+                       ws, before);
 }
 
 template <int T, int D, int R, bool kCap, bool kSlope>
@@ -386,6 +360,8 @@ hipError_t launch_stream(const AttnArgs& a, const AttnShared& sh, const SharedPl
   return hipGetLastError();
 }
 
+// Packed documents that fill few tiles: first all rows as they stand in q, one sequence, against
+// ranges of the shared keys, then each document's against its own, on from those sums.
 template <int T, int D, int WM, bool kCap>
 hipError_t launch_packed(const AttnArgs& a, const AttnShared& sh, const SharedPlan& p, float* ws,
                          hipStream_t stream) {
@@ -400,12 +376,13 @@ hipError_t launch_packed(const AttnArgs& a, const AttnShared& sh, const SharedPl
   const int o_tiles = (a.max_q * group + kRows - 1) / kRows;
   const int64_t f_all = (int64_t)a.kv_heads * p.s_tiles * kRows;
   const dim3 block(attn_waves(WM) * 64);
-  hipLaunchKernelGGL((attn_packed_front_kernel<T, D, WM, kCap>),
+  hipLaunchKernelGGL((attn_tiles_kernel<T, D, WM, kCap, false, true>),
                      dim3((unsigned)((int64_t)a.kv_heads * p.s_tiles * p.s_splits)), block, 0, stream, f,
-                     p.s_tiles, p.s_splits, p.s_chunk, ws);
-  hipLaunchKernelGGL((attn_packed_own_kernel<T, D, WM, kCap>),
-                     dim3((unsigned)((int64_t)a.n_seq * a.kv_heads * o_tiles)), block, 0, stream, a, sh,
-                     AttnFront{ws, f_all, p.s_splits, p.s_tiles * kRows}, o_tiles);
+                     p.s_tiles, p.s_tiles, 1, p.s_splits, p.s_chunk, ws);
+  hipLaunchKernelGGL((attn_walk_kernel<T, D, WM, kCap, false, false, AttnSums>),
+                     dim3((unsigned)((int64_t)a.n_seq * a.kv_heads * o_tiles)), block, 0, stream, a, o_tiles,
+                     o_tiles, a.n_seq * a.kv_heads, 1, 0, nullptr,
+                     AttnSums{sh, AttnFront{ws, f_all, p.s_splits, p.s_tiles * kRows}});
   return hipGetLastError();
 }
 
@@ -418,15 +395,15 @@ hipError_t launch_shared_tiles(const AttnArgs& a, const AttnShared& sh, const At
   const int64_t blocks = (int64_t)a.n_seq * a.kv_heads * tiles;
   const dim3 block(attn_waves(WM) * 64);
   if (plan.splits > 1) {
-    hipLaunchKernelGGL((attn_shared_tiles_kernel<T, D, WM, kCap, kSlope, true>),
-                       dim3((unsigned)(blocks * plan.splits)), block, 0, stream, a, sh, tiles, plan.first, 1,
-                       plan.splits, plan.chunk, ws);
+    hipLaunchKernelGGL((attn_walk_kernel<T, D, WM, kCap, kSlope, true, AttnShared>),
+                       dim3((unsigned)(blocks * plan.splits)), block, 0, stream, a, tiles, plan.first, 1,
+                       plan.splits, plan.chunk, ws, sh);
     launch_shared_join<T, D, kCap, kSlope>(a, sh, AttnFront{ws, 0, 0, 0}, kRows, tiles, blocks * kRows,
                                            plan.splits, plan.chunk, own0, ws, stream);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((attn_shared_tiles_kernel<T, D, WM, kCap, kSlope, false>), dim3((unsigned)blocks), block,
-                     0, stream, a, sh, tiles, plan.first, plan.near_hs, 1, 0, nullptr);
+  hipLaunchKernelGGL((attn_walk_kernel<T, D, WM, kCap, kSlope, false, AttnShared>), dim3((unsigned)blocks), block,
+                     0, stream, a, tiles, plan.first, plan.near_hs, 1, 0, nullptr, sh);
   return hipGetLastError();
 }
 

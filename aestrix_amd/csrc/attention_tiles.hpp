@@ -35,8 +35,6 @@
 // a workgroup where a CU gets more than one, V and K lines read ahead into L2.
 #pragma once
 
-#include <type_traits>
-
 #include "attention.hpp"
 
 namespace imq {
@@ -369,31 +367,9 @@ __device__ __forceinline__ void attn_load(const char* base, int64_t row_bytes, i
 // Waves of a workgroup with WM of them on rows of their own.
 constexpr int attn_waves(int wm) { return wm < 4 ? 4 : wm; }
 
-// Where the own keys begin in a walk over shared and own ones: behind whole pairs of tiles.
-__device__ __forceinline__ int attn_own0(const AttnShared& sh) {
-  return (sh.rows + 2 * kAttnKeys - 1) / (2 * kAttnKeys) * (2 * kAttnKeys);
-}
-
-// Sums of ranges of shared keys.
-struct AttnFront {
-  const float* ws;  // as a split plan's, of `all` rows
-  int64_t all;
-  int ranges;
-  int packed;  // rows of a key head, which stand in q's order; 0: the same rows as other ranges
-};
-__device__ __forceinline__ int64_t attn_packed_row(const AttnArgs& a, const AttnFront& front, int seq, int kh,
-                                                   int t, int g) {
-  const int64_t q = min(max(a.q_offsets[seq], 0), a.q_rows) + t;
-  return (int64_t)kh * front.packed + q * (a.heads / a.kv_heads) + g;
-}
-
-// What stands before every sequence's keys: nothing, the keys `sh`, which the walk begins with,
-// or their sums, `front`'s, which it goes on from.
-enum AttnBefore { kNone, kKeys, kSums };
-template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit, AttnBefore kBefore>
-__device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& sh, const AttnFront& front,
-                                           int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
-  constexpr bool kShared = kBefore == kKeys;
+template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
+__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
+    AttnArgs a, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
   using S = typename Elem<T>::S;
   // WM waves on rows of their own, WK on a part of every tile's keys each.
   constexpr int NW = attn_waves(WM), WK = NW / WM, U = 2 / WK, kRows = WM * 32;
@@ -432,47 +408,27 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
   const int seen_hi = mw >= rows ? 0 : __builtin_amdgcn_readfirstlane(
       attn_seen(a, s, min(mw + 31, rows - 1) / group));
   const int seen_lo = __builtin_amdgcn_readfirstlane(attn_seen(a, s, min(mw, rows - 1) / group));
-  const int own0 = kShared ? attn_own0(sh) : 0;
   const int begin = kSplit ? split * chunk : 0;
-  const int end = kSplit ? min(own0 + seen_wg, begin + chunk) : own0 + seen_wg;
+  const int end = kSplit ? min(seen_wg, begin + chunk) : seen_wg;
   if (kSplit && begin >= end) return;  // the join reads the ranges up to seen_wg only
 
   // Sources of this thread's pieces in a tile.
   const int64_t kb = a.k_row * 2, vb = a.v_row * 2;
   uint32_t k_off[kLoads], v_off[kLoads];
-  auto sources = [&](int64_t kb, int64_t vb) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = (i * NW + wave) * 64 + lane, row = at / (D / 8), piece = at % (D / 8);
-      const int kp = k_piece<D>(row, piece), vp = v_piece<D>(row, piece);
-      k_off[i] = kp * 8 < a.dim ? (uint32_t)(row * kb + kp * 16) : 0x80000000u;
-      v_off[i] = vp * 8 < a.dim ? (uint32_t)(row * vb + vp * 16) : 0x80000000u;
-    }
-  };
-  sources(kb, vb);
+  for (int i = 0; i < kLoads; ++i) {
+    const int at = (i * NW + wave) * 64 + lane, row = at / (D / 8), piece = at % (D / 8);
+    const int kp = k_piece<D>(row, piece), vp = v_piece<D>(row, piece);
+    k_off[i] = kp * 8 < a.dim ? (uint32_t)(row * kb + kp * 16) : 0x80000000u;
+    v_off[i] = vp * 8 < a.dim ? (uint32_t)(row * vb + vp * 16) : 0x80000000u;
+  }
   const char* kbase = reinterpret_cast<const char*>(static_cast<const S*>(a.k) + s.k_at + kh * a.k_head);
   const char* vbase = reinterpret_cast<const char*>(static_cast<const S*>(a.v) + s.v_at + kh * a.v_head);
-  // Among the shared keys: their sources, until the own ones' turn.
-  const char *now_k = kbase - own0 * kb, *now_v = vbase - own0 * vb;  // of the walk's key 0
-  int64_t now_kb = kb, now_vb = vb;
-  int now_end = own0 + s.nk;
-  if (kShared && begin < own0) {
-    now_k = static_cast<const char*>(sh.k) + kh * sh.k_head * 2, now_kb = sh.k_row * 2;
-    now_v = static_cast<const char*>(sh.v) + kh * sh.v_head * 2, now_vb = sh.v_row * 2;
-    now_end = sh.rows;
-    sources(now_kb, now_vb);
-  }
   auto issue = [&](AttnStage<D>& st, int j0) {
     // Nothing past the last tile: rows below 1.
-    if constexpr (kShared) {
-      const int n = j0 < end ? min(kAttnKeys, now_end - j0) : 0;
-      attn_load<D, NW>(now_k + j0 * now_kb, now_kb, n, a.dim, k_off, st.k, wave);
-      attn_load<D, NW>(now_v + j0 * now_vb, now_vb, n, a.dim, v_off, st.v, wave);
-    } else {
-      const int n = j0 < end ? min(kAttnKeys, s.nk - j0) : 0;
-      attn_load<D, NW>(kbase + j0 * kb, kb, n, a.dim, k_off, st.k, wave);
-      attn_load<D, NW>(vbase + j0 * vb, vb, n, a.dim, v_off, st.v, wave);
-    }
+    const int n = j0 < end ? min(kAttnKeys, s.nk - j0) : 0;
+    attn_load<D, NW>(kbase + j0 * kb, kb, n, a.dim, k_off, st.k, wave);
+    attn_load<D, NW>(vbase + j0 * vb, vb, n, a.dim, v_off, st.v, wave);
   };
   s16x8_t qf[D / 16];
   if constexpr (WM == 4 && D == 128) {
@@ -508,52 +464,14 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
   float top = -INFINITY, sum = 0.f;
-  if constexpr (kBefore == kSums) {
-    static_assert(WK == 1, "every wave has its rows alone");
-    const int64_t at = attn_packed_row(a, front, hs / a.kv_heads, kh, t, m % group);
-    const float2* ml = reinterpret_cast<const float2*>(front.ws + front.ranges * front.all * D) + at;
-    for (int r = 0; r < front.ranges; ++r) {
-      const float2 v = ml[r * front.all];
-      const float* po = front.ws + (r * front.all + at) * D;
-      const float next = fmaxf(top, v.x), base = next == -INFINITY ? 0.f : next;
-      const float keep0 = __builtin_amdgcn_exp2f(top - base), keep1 = __builtin_amdgcn_exp2f(v.x - base);
-      top = next;
-      sum = sum * keep0 + (h == 0 ? v.y * keep1 : 0.f);  // the lane 32 away's is added at the end
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const float4 w = *reinterpret_cast<const float4*>(po + i * 32 + 2 * e + 4 * h);
-          o[i][e] = o[i][e] * keep0 + w.x * keep1;
-          o[i][e + 1] = o[i][e + 1] * keep0 + w.y * keep1;
-          o[i][e + 2] = o[i][e + 2] * keep0 + w.z * keep1;
-          o[i][e + 3] = o[i][e + 3] * keep0 + w.w * keep1;
-        }
-    }
-  }
 
   // The wave's keys of the tile that begins at j0.
   // The next tile's loads go out among the score's MFMAs: before them they
   // would hold up the wave that has everyone wait.
-  auto step = [&](auto in_front, const AttnStage<D>& st, AttnStage<D>& to,
-                  int j0) __attribute__((always_inline)) {
-    constexpr bool front = decltype(in_front)::value;
+  auto step = [&](const AttnStage<D>& st, AttnStage<D>& to, int j0) __attribute__((always_inline)) {
     const int j1 = j0 + kAttnKeys;
-    // What the rows see of the walk, where they stand in it, and `near`, among the shared
-    // keys and among the own ones.
-    if (front && j1 == own0) {
-      now_k = kbase - own0 * kb, now_kb = kb;
-      now_v = vbase - own0 * vb, now_vb = vb;
-      now_end = own0 + s.nk;
-      sources(kb, vb);
-    }
-    const int walk_seen = front ? sh.rows : own0 + seen, walk_lo = front ? sh.rows : own0 + seen_lo;
-    const int walk_hi = front ? (mw >= rows ? 0 : sh.rows) : own0 + seen_hi;
-    const int walk_p = p + (front ? sh.rows : own0);
-    const int walk_near = front ? min(mw, rows - 1) / group + s.nk - s.nq + 1 + sh.rows
-                          : near == INT_MAX ? near : own0 + near;
     j0 += wk * (32 * U);
-    if (j0 >= walk_hi) {
+    if (j0 >= seen_hi) {
       issue(to, j1);
       return;
     }
@@ -578,8 +496,8 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
     }
     s16x8_t pf[2 * U];
     float shift[U];
-    attn_top<T>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, walk_seen, walk_lo, walk_p - j0,
-                                             j0 + 32 * U <= walk_near, shift), o, top, sum);
+    attn_top<T>(attn_scores<U, kCap, kSlope>(score, sc, j0, h, seen, seen_lo, p - j0,
+                                             j0 + 32 * U <= near, shift), o, top, sum);
     attn_weights<T, U, kCap, kSlope>(score, sc, shift, top, sum, pf);
     attn_pv<T, D, 2 * U>(st.v + wk * U * 32 * (D / 8), pf, o, lane);
   };
@@ -592,19 +510,13 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto go = [&](auto in_front, int from, int to) __attribute__((always_inline)) {
-    for (int j0 = from; j0 < to; j0 += 2 * kAttnKeys) {
-      meet();
-      step(in_front, st0, st1, j0);
-      if (j0 + kAttnKeys >= to) break;
-      meet();
-      step(in_front, st1, st0, j0 + kAttnKeys);
-    }
-  };
-  // (Two loops: with one, whose steps tell the keys apart, 4 x 2048 rows of 32 / 8 heads behind
-  // 8192 shared keys took 1293 us, of all keys as own ones 1174.)
-  if constexpr (kShared) go(std::true_type{}, begin, min(own0, end));
-  go(std::false_type{}, max(begin, own0), end);
+  for (int j0 = begin; j0 < end; j0 += 2 * kAttnKeys) {
+    meet();
+    step(st0, st1, j0);
+    if (j0 + kAttnKeys >= end) break;
+    meet();
+    step(st1, st0, j0 + kAttnKeys);
+  }
   IMQ_WAIT_VMCNT(0);  // the loads past the last tile (of nothing), before their LDS is used again
   __builtin_amdgcn_sched_barrier(0);
 
@@ -660,7 +572,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
     }
   } else {
     // (Of keys whose scores are all -infinity the sum is zero too, and the output NaN.)
-    const float inv = kBefore != kNone || seen > 0 ? 1.f / sum : 0.f;
+    const float inv = seen > 0 ? 1.f / sum : 0.f;
     bool finite = true;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -709,17 +621,9 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnShared& 
       const int r = __builtin_ctzll(again);
       again &= again - 1;
       const int tr = (mw + r) / group;
-      attn_row<T, kCap, kSlope, kBefore != kNone>(a, s, kh * group + (mw + r) % group, tr,
-                                                  attn_seen(a, s, tr), qs[wave], sh);
+      attn_row<T, kCap, kSlope>(a, s, kh * group + (mw + r) % group, tr, attn_seen(a, s, tr), qs[wave]);
     }
   }
-}
-
-template <int T, int D, int WM, bool kCap, bool kSlope, bool kSplit>
-__global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
-    AttnArgs a, int tiles, int first, int near_hs, int splits, int chunk, float* ws) {
-  attn_tiles<T, D, WM, kCap, kSlope, kSplit, kNone>(a, AttnShared{}, AttnFront{}, tiles, first, near_hs,
-                                                       splits, chunk, ws);
 }
 
 // Joins the key ranges of a split plan: 16 lanes a row, D / 16 columns each,
@@ -728,12 +632,9 @@ __global__ __launch_bounds__(attn_waves(WM) * 64, 2) void attn_tiles_kernel(
 // tile's ranges up to the last key that its last row sees are written, the
 // others not.  Bound by the latency of its loads: four ranges a group are in
 // flight together.
-// kShared: a row's first front.ranges ranges are the shared keys', and the others are counted
-// from `own0` keys before its own.
-template <int T, int D, int kParts, bool kCap, bool kSlope, bool kShared>
-__device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& sh, const AttnFront& front,
-                                          int tile_rows, int tiles, int splits, int chunk, int own0,
-                                          const float* ws) {
+template <int T, int D, int kParts, bool kCap, bool kSlope>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_rows, int tiles,
+                                                        int splits, int chunk, const float* ws) {
   using S = typename Elem<T>::S;
   __shared__ float qs[4][D];
   __shared__ float sums[kParts > 1 ? 16 : 1][D + 2];
@@ -758,35 +659,18 @@ __device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& s
   float acc[D / 16] = {}, top = -INFINITY, sum = 0.f;
   if (live) {
     const int last = min(m / tile_rows * tile_rows + tile_rows, rows) - 1;
-    const int used = (kShared ? front.ranges : 0) +
-                     (int)(((int64_t)attn_seen(a, s, last / group) + own0 + chunk - 1) / chunk);
+    const int used = (int)(((int64_t)attn_seen(a, s, last / group) + chunk - 1) / chunk);
     const float2* ml = reinterpret_cast<const float2*>(ws + (int64_t)splits * all * D) + row;
     const float* po = ws + row * D + d0;
-    const float2* front_ml = nullptr;
-    const float* front_po = nullptr;
-    if constexpr (kShared) {
-      front_ml = reinterpret_cast<const float2*>(front.ws + (int64_t)front.ranges * front.all * D) + row;
-      front_po = front.ws + row * D + d0;
-    }
     for (int i = part; i < used; i += 4 * kParts) {
       float2 v[4];
       float4 w[4][D / 64];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int range = min(i + b * kParts, used - 1);
-        if constexpr (kShared) {
-          const bool in_front = range < front.ranges;
-          const int64_t at = in_front ? range * front.all : (range - front.ranges) * all;
-          v[b] = (in_front ? front_ml : ml)[at];
+        const int64_t at = (int64_t)min(i + b * kParts, used - 1) * all;
+        v[b] = ml[at];
 #pragma unroll
-          for (int e = 0; e < D / 64; ++e)
-            w[b][e] = reinterpret_cast<const float4*>((in_front ? front_po : po) + at * D)[e];
-        } else {
-          const int64_t at = (int64_t)range * all;
-          v[b] = ml[at];
-#pragma unroll
-          for (int e = 0; e < D / 64; ++e) w[b][e] = reinterpret_cast<const float4*>(po + at * D)[e];
-        }
+        for (int e = 0; e < D / 64; ++e) w[b][e] = reinterpret_cast<const float4*>(po + at * D)[e];
       }
       float next = top;
 #pragma unroll
@@ -840,7 +724,7 @@ __device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& s
   }
   bool again_row = false;
   if (live) {
-    const float inv = kShared || attn_seen(a, s, t) > 0 ? 1.f / sum : 0.f;
+    const float inv = attn_seen(a, s, t) > 0 ? 1.f / sum : 0.f;
     S* out = static_cast<S*>(a.out) + s.out_at + t * a.out_row + head * a.out_head;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) {
@@ -865,14 +749,8 @@ __device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnShared& s
     const int tr = mr / group, seen = attn_seen(a1, sr, tr), khr = hr % a1.kv_heads;
     const int last = min(mr / tile_rows * tile_rows + tile_rows, sr.nq * group) - 1;
     if (seen <= attn_spoilt<T>(a1, sr, khr, seen, attn_seen(a1, sr, last / group) + kAttnKeys))
-      attn_row<T, kCap, kSlope, kShared>(a1, sr, khr * group + mr % group, tr, seen, qs[wave], sh);
+      attn_row<T, kCap, kSlope>(a1, sr, khr * group + mr % group, tr, seen, qs[wave]);
   }
-}
-
-template <int T, int D, int kParts, bool kCap, bool kSlope>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int tile_rows, int tiles,
-                                                        int splits, int chunk, const float* ws) {
-  attn_join<T, D, kParts, kCap, kSlope, false>(a, AttnShared{}, AttnFront{}, tile_rows, tiles, splits, chunk, 0, ws);
 }
 
 }  // namespace imq
