@@ -5,3 +5,4 @@
 #include "../../../include/imq_cond.h"
 #include "../../../include/imq_te.h"
 #include "../../../include/imq_core.h"
+#include "../../../include/imq_lora.h"
