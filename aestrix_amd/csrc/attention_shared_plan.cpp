@@ -96,7 +96,14 @@ SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cu
   }
   p.kernel = IMQ_SHARED_STREAM;
   const int64_t batch = (int64_t)a.n_seq * rows;
-  p.s_rows = batch > 32 ? 64 : 32;
+  // 64 rows a workgroup, which halve the reads of the shared keys, where those are more than the
+  // L2s keep or the rows many; 32 give a range to more workgroups.  Tokens of 32 / 8 heads behind
+  // shared / own keys, 64 rows and 32: 64 behind 8192 / 600 55 and 58 us, behind 65536 / 600 164 and
+  // 189, behind 1024 / 256 27.6 and 23.9, 16 behind 4096 / 256 21.6 and 19.4; of 16 / 2 heads behind
+  // 8192 / 64 128 tokens 36.5 and 29.3, 512 79 and 82.
+  const int64_t tiles64 = (batch + 63) / 64;
+  const bool in_l2 = (int64_t)a.kv_heads * sh.rows * a.dim * 4 <= 1 << 24;
+  p.s_rows = batch > 32 && !(in_l2 && a.kv_heads * tiles64 * sh.rows < 1 << 19) ? 64 : 32;
   p.s_tiles = (int)((batch + p.s_rows - 1) / p.s_rows);
   // A workgroup a CU: the keys of a range such that all ranges together are as many.  64
   // rows take half as long again as 32.

@@ -79,6 +79,15 @@ def test_sizes(shared, n, nq, nk, heads, kv, dim, causal, dtype):
     run_batch(shared, nq, nk, heads, kv, dim, dtype, n=n, causal=causal)
 
 
+@pytest.mark.parametrize("softcap,slope", [(0.0, False), (0.0, True), (30.0, False), (5.0, True)])
+@pytest.mark.parametrize("shared,n,nq,nk,heads,kv,dim,dtype",
+                         [(4500, 9, 1, 90, 32, 8, 128, BF16), (8300, 33, 2, 40, 16, 16, 64, F16),
+                          (7400, 5, 4, 3, 32, 8, 72, F16), (9100, 70, 1, 130, 12, 4, 128, F16)])
+def test_long_shared_keys(shared, n, nq, nk, heads, kv, dim, dtype, softcap, slope):
+    """More than 32 rows of the batch behind keys that no cache keeps: 64 a workgroup."""
+    run_batch(shared, nq, nk, heads, kv, dim, dtype, n=n, causal=True, softcap=softcap, slope=slope)
+
+
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (F16, 72)])
 @pytest.mark.parametrize("softcap,slope", [(0.0, True), (30.0, False), (5.0, True)])
 @pytest.mark.parametrize("shared,n,nq,nk,causal", [(500, 6, 1, 60, True), (129, 3, 3, 9, False), (200, 2, 200, 200, True),
