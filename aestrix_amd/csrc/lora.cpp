@@ -48,7 +48,7 @@ int imq_qmm_lora_workspace(imq_ctx* ctx, const imq_lora* lora, int k, int n, int
   const int rc = check_lora(ctx, fn, lora, k, n, m, dtype);
   if (rc != IMQ_OK) return rc;
   if (!bytes) return fail(ctx, IMQ_EINVAL, "%s: null output", fn);
-  *bytes = workspace(lora, imq::lora_plan(k, n, m, lora->count, (int)dtype), m);
+  *bytes = workspace(lora, imq::lora_plan(k, n, m, lora->count, lora->max_rank, (int)dtype), m);
   return IMQ_OK;
 }
 
@@ -62,7 +62,7 @@ int imq_qmm_lora(imq_ctx* ctx, const uint32_t* w, const void* scales, const void
   if (!which || !aligned(which, 4))
     return fail(ctx, IMQ_EINVAL, "%s: which=%p must be a 4-byte aligned device pointer", fn,
                 (const void*)which);
-  const imq::LoraPlan plan = imq::lora_plan(k, n, m, lora->count, (int)dtype);
+  const imq::LoraPlan plan = imq::lora_plan(k, n, m, lora->count, lora->max_rank, (int)dtype);
   const size_t need = workspace(lora, plan, m);
   if (!ws || !aligned(ws, 16) || ws_bytes < need)
     return fail(ctx, IMQ_EINVAL, "%s: workspace %p of %zu bytes (16-byte aligned, %zu are needed)", fn, ws,

@@ -1,6 +1,8 @@
 // lora.hip -- the products of adapters beside a projection that stand outside its kernels: u =
 // scale * A x, a row's adapter's, and the join of the projection's partial sums with B u
 // (include/imq_lora.h).
+#include <algorithm>
+
 #include "lora_device.hpp"
 
 namespace imq {
@@ -34,7 +36,7 @@ struct LoraRows {
   }
 };
 
-constexpr int kDotWaves = 4, kDotMaxM = 64;
+constexpr int kDotWaves = 4;
 template <int T, int kAhead>
 __global__ __launch_bounds__(kDotWaves * 64) void lora_dot_kernel(LoraArgs l, const uint16_t* x, int k, int m) {
   lora_dot<T, kAhead>(l, x, k, m, blockIdx.x * kDotWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
@@ -240,8 +242,9 @@ __global__ __launch_bounds__(kOrderWaves * 64) void lora_order_kernel(LoraArgs l
 
 // ---- the join
 
-// Few rows: a thread an output, one row a workgroup, B's row against u in 32 bits.  Bound by the
-// latency of `which`, `first` and B, one after the other; the ranges' sums are on the way meanwhile.
+// A thread an output, one row a workgroup, B's row against u in 32 bits.  Bound by the latency of
+// `which`, `first` and B, one after the other, the ranges' sums on the way meanwhile ([16 x 6144] with
+// 16 adapters of rank 16 4.5 us), and of many rows or ranks by reading B's rows, each for its row alone.
 template <int T>
 __global__ __launch_bounds__(256) void lora_join_few_kernel(LoraArgs l, const float* part, int splits,
                                                             uint16_t* y, int n, int m) {
@@ -281,7 +284,7 @@ __global__ __launch_bounds__(256) void lora_join_few_kernel(LoraArgs l, const fl
   if (col < n) y[(size_t)row * n + col] = Elem<T>::out(sum + dot);
 }
 
-// More.  A workgroup: 32 rows and 32 columns of y.  Its 16 waves take the adapters of the rows in
+// Long rows of B for many rows of y.  A workgroup: 32 rows and 32 columns of y.  Its 16 waves take the adapters of the rows in
 // turn; each writes its rows' products to LDS (a row has one adapter), where the ranges' sums
 // are added to them in order.  Bound by the latency of what a wave loads for an adapter; the
 // ranges' sums are on the way meanwhile.
@@ -331,10 +334,33 @@ hipError_t launch_lora_order(const LoraArgs& l, int32_t* order, int32_t* which_a
   return hipGetLastError();
 }
 
+namespace {
+
+// Whether u is made a wave a row and rank: by the times of both in us.  That one reads A's and x's
+// rows out of the caches, some 30 TB/s, whatever adapters the rows name; a tile of 32 rows
+// takes its adapters two at a time, as many as it may have (all, or after grouping its share), 6 us
+// of K = 2560 and 12 of 9728 each turn.  160 rows of 24 adapters of rank 16 in turn against K = 9728
+// and N = 2560 30.8 us so, 168 by tiles; 64 rows of one adapter of rank 256 and K = 2560 44.7 and
+// 41.4; 512 rows of 32 adapters of rank 64, grouped, 74.8 and 64.4.
+bool lora_by_rows(const LoraArgs& l, int k, int m) {
+  const double rows_us = 2 + 4. * m * l.max_rank * k / 30e6;
+  const int most = std::min(std::min(l.count, m), l.order ? 1 + (int)((int64_t)l.count * 32 / m) : 32);
+  return rows_us <= (most + 1) / 2 * (3.5 + k * 0.0009) && (int64_t)m * l.max_rank < 1 << 24;
+}
+
+}  // namespace
+
+double lora_join_few_us(int n, int m, int max_rank) { return 2. * m * n * max_rank / 10e6; }
+double lora_join_tiles_us(int n, int m, int count, int max_rank) {
+  const int most = std::min(std::min(count, m), 32);
+  const double rows = (m + 31) / 32;
+  return 1.5 + (1.2 + 0.27 * most) * ((n + 31) / 32) * rows / 256 + 2. * rows * most * n * max_rank / 3e6;
+}
+
 hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, int dtype,
                               hipStream_t stream) {
   const auto* xx = static_cast<const uint16_t*>(x);
-  if (m <= kDotMaxM) {
+  if (lora_by_rows(l, k, m)) {
     const dim3 grid((unsigned)((m * l.max_rank + kDotWaves - 1) / kDotWaves)), block(kDotWaves * 64);
     // Rows of more than 8 KB: 20 pieces at a time, of which shorter rows would have too few.
     if (k > 4096) {
@@ -362,7 +388,7 @@ hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, in
 hipError_t launch_lora_join(const LoraArgs& l, const float* part, int splits, void* y, int n, int m,
                             int dtype, hipStream_t stream) {
   auto* yy = static_cast<uint16_t*>(y);
-  if (m <= kDotMaxM) {
+  if (m <= 65535 && lora_join_few_us(n, m, l.max_rank) <= lora_join_tiles_us(n, m, l.count, l.max_rank)) {
     const dim3 grid((unsigned)((n + 255) / 256), (unsigned)m);
     if (dtype == kBf16)
       hipLaunchKernelGGL((lora_join_few_kernel<kBf16>), grid, dim3(256), 0, stream, l, part, splits, yy, n, m);

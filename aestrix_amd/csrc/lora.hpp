@@ -39,7 +39,14 @@ struct LoraPlan {
   bool order;     // grouped rows (launch_lora_order)
   size_t bytes;   // of the partial sums
 };
-LoraPlan lora_plan(int k, int n, int m, int count, int dtype);
+LoraPlan lora_plan(int k, int n, int m, int count, int max_rank, int dtype);
+
+// About what the two joins take, us (lora.hip): a thread an output reads B's rows, 10 TB/s; tiles of
+// 32 x 32, 256 at a time, load every adapter that the rows may name, 3 TB/s.  160 rows of N = 2560 with
+// 24 adapters of rank 16 in turn 30.8 us a call with the first and 40.2 with the second, 64 rows of N = 6144
+// with one of rank 256 44.6 and 32.9.
+double lora_join_few_us(int n, int m, int max_rank);
+double lora_join_tiles_us(int n, int m, int count, int max_rank);
 
 // Groups the rows by their adapters, those without one last, each group in its rows' order:
 // order [m] the row at a place, which_at [m] its adapter (lora.hip).

@@ -50,7 +50,8 @@ __device__ __forceinline__ void lora_dot(const LoraArgs& l, const uint16_t* x, i
   const LoraAt to = lora_at(l, i);
   if (r >= to.rank) return;
   const __amdgpu_buffer_rsrc_t ar = make_rsrc(l.a + (size_t)(to.row + r) * k, (uint32_t)k * 2);
-  const __amdgpu_buffer_rsrc_t xr = make_rsrc(x + (size_t)row * k, (uint32_t)k * 2);
+  const int from = l.order ? l.order[row] : row;
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(x + (size_t)from * k, (uint32_t)k * 2);
   float sum[2] = {0.f, 0.f};
   for (int c = 0; c < k; c += kAhead * 512) {
     u32x4_t av[kAhead], xv[kAhead];  // (past the end: zeros)

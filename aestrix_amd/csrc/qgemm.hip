@@ -261,11 +261,19 @@ hipError_t launch_qgemm(const uint32_t* w, const void* scales, const void* biase
   }
 }
 
-// Rows up to which the adapters' second product is left to the join whether K is split or not:
-// more rows than that name an adapter of their own in stretches.
-constexpr int kLoraJoinMaxM = 128;
+// Whether the adapters' second product is left to a join where K is not split, by what either adds in
+// us: the sums' way through memory, a launch and the join, or the grouping of the rows and the tiles' turns,
+// one for each adapter that their rows name.  N = 19456, K = 2560, through a join and in the tiles: 160 rows
+// of 24 adapters of rank 16 in turn 50 and 66, of one of rank 64 60 and 37; 48 rows of 8 of rank 64 40 and
+// 45, of one 32 and 22; 256 rows of 32 of rank 16 70 and 98, 512 rows 118 and 95.
+bool lora_join_pays(const BigPlan& b, int n, int m, int count, int max_rank) {
+  const double join = 2 + 8. * m * n / 10e6 +
+                      std::min(lora_join_few_us(n, m, max_rank), lora_join_tiles_us(n, m, count, max_rank));
+  const int most = std::min(std::min(count, m), 1 + (int)((int64_t)count * 32 * b.mt / m));
+  return join < (count > 1 ? 6 : 0) + most * (0.3 + 0.55 * max_rank / 16);
+}
 
-LoraPlan lora_plan(int k, int n, int m, int count, int dtype) {
+LoraPlan lora_plan(int k, int n, int m, int count, int max_rank, int dtype) {
   LoraPlan p{};
   if (m <= kQskinnyMaxM && qskinny_supported(k, n, m, dtype)) {
     p.bytes = qskinny_resid_split_bytes(k, n, m);
@@ -275,7 +283,7 @@ LoraPlan lora_plan(int k, int n, int m, int count, int dtype) {
   }
   if (!qgemm_big_supported(k, n, m)) return p;
   const BigPlan b = pick_big_plan(m, n, k, device_cus(), true);
-  if (b.splits > 1 || m <= kLoraJoinMaxM) {
+  if (b.splits > 1 || lora_join_pays(b, n, m, count, max_rank)) {
     p.splits = b.splits;
     p.bytes = (size_t)b.splits * m * n * sizeof(float);
   }

@@ -21,7 +21,7 @@ hipError_t launch_lora_join(const LoraArgs&, const float*, int, void*, int, int,
   return hipErrorNoDevice;
 }
 hipError_t launch_lora_order(const LoraArgs&, int32_t*, int32_t*, int, hipStream_t) { return hipErrorNoDevice; }
-LoraPlan lora_plan(int, int n, int m, int, int) { return LoraPlan{0, 2, 1, 2, 2, false, (size_t)8 * m * n}; }
+LoraPlan lora_plan(int, int n, int m, int, int, int) { return LoraPlan{0, 2, 1, 2, 2, false, (size_t)8 * m * n}; }
 hipError_t launch_qgemm_lora(const LoraPlan&, const uint32_t*, const void*, const void*, const void*,
                              const LoraArgs&, float*, void*, int, int, int, int, hipStream_t) {
   return hipErrorNoDevice;

@@ -126,6 +126,16 @@ def test_ranks(rank, m):
     run(m, 512, 390, [rank, 1, rank], each(3), BF16)
 
 
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("m,k,n,rank,count", [(48, 2560, 6144, 64, 8), (64, 2560, 6144, 256, 1), (96, 9728, 2560, 64, 4),
+                                              (160, 2560, 6144, 16, 24), (160, 9728, 2560, 64, 1),
+                                              (256, 2560, 6144, 64, 2), (256, 2560, 6144, 64, 8),
+                                              (512, 2560, 6144, 16, 32), (512, 2560, 2560, 64, 32)])
+def test_rows_between_tokens_and_prompts(m, k, n, rank, count, t):
+    """u by rows or by tiles, grouped or not; B u by either join or in the projection's tiles."""
+    run(m, k, n, [rank] * count, each(count), t)
+
+
 @pytest.mark.parametrize("m", [1, 40, 300, 1200])
 def test_many_adapters(m):
     count = 200
