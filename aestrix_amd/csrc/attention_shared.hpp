@@ -3,13 +3,19 @@
 // element type in attention_shared_{bf16,f16}.hip.
 //
 // Sequences with many rows (queries times the heads of a key head) run the tiles of
-// attention_tiles.hpp, whose walk goes over the shared keys and then the own ones: the
-// matrix cores bind there, and the shared keys come out of the caches.
+// attention_walk.hpp, whose walk goes over the shared keys and then the own ones: the
+// matrix cores bind there, and the shared keys come out of the caches (4 x up to 2048 rows of
+// 32 / 8 heads of 128 behind 8192 keys, with slopes, 848 us, 966 TFLOP/s).  Packed documents that
+// fill few tiles: all rows in one stretch against the shared keys first (launch_packed; 61 of up to
+// 154 rows, capped, behind 3001 keys 76 us, 119 in tiles of their own).
 //
 // Up to 32 rows a sequence, single tokens mostly, are bound by reading keys.  So that the
 // shared ones are read once for the batch, the rows of all sequences stand together
-// against them, 64 a workgroup, and each sequence's own rows against its own keys, as
-// workgroups of one launch (attn_stream_kernel); a second one joins the ranges.
+// against them, 32 or 64 a workgroup, and each sequence's own rows against its own keys, as
+// workgroups of one launch (attn_stream_kernel); a second one joins the ranges.  Tokens of 32 / 8 heads
+// of 128, keys once each over the time: 16 behind 65536 keys 60 us and the join 6, 4.2 TB/s; 64 behind
+// 8192, with up to 1024 own ones, 54 and 5, 2.9 TB/s (the shared ones are read four times, three
+// out of the caches); 8 behind 512 7.5 and 4.5, the latency of a tile or two and of the join's loads.
 #pragma once
 
 #include <type_traits>

@@ -39,7 +39,8 @@ __device__ __forceinline__ void lora_put(const LoraArgs& l, int row, int rank, f
 }
 
 // u of row at / max_rank and rank at % max_rank (of few rows), by a wave.  Bound by reading A, and
-// by the latency of that: kAhead pieces of 1 KB of each of the two rows are on their way together.
+// by the latency of that: kAhead pieces of 1 KB of each of the two rows are on their way together (64
+// rows of K = 9728, rank 16, 24 adapters: 7.2 us).
 template <int T, int kAhead>
 __device__ __forceinline__ void lora_dot(const LoraArgs& l, const uint16_t* x, int k, int m, int at) {
   const int lane = threadIdx.x & 63;
