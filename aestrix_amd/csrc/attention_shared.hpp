@@ -5,9 +5,10 @@
 // Sequences with many rows (queries times the heads of a key head) run the tiles of
 // attention_walk.hpp, whose walk goes over the shared keys and then the own ones: the
 // matrix cores bind there, and the shared keys come out of the caches (4 x up to 2048 rows of
-// 32 / 8 heads of 128 behind 8192 keys, with slopes, 848 us, 966 TFLOP/s).  Packed documents that
-// fill few tiles: all rows in one stretch against the shared keys first (launch_packed; 61 of up to
-// 154 rows, capped, behind 3001 keys 76 us, 119 in tiles of their own).
+// 32 / 8 heads of 128 behind 8192 keys, with slopes, 848 us, 966 TFLOP/s).  Sequences that
+// fill little of their tiles: all rows in one stretch against the shared keys first (launch_packed; 61
+// documents of up to 154 rows, capped, behind 3001 keys 76 us, 119 in tiles of their own; 64 x 36 rows
+// behind 8192 124 and 213).
 //
 // Up to 32 rows a sequence, single tokens mostly, are bound by reading keys.  So that the
 // shared ones are read once for the batch, the rows of all sequences stand together
@@ -366,8 +367,8 @@ hipError_t launch_stream(const AttnArgs& a, const AttnShared& sh, const SharedPl
   return hipGetLastError();
 }
 
-// Packed documents that fill few tiles: first all rows as they stand in q, one sequence, against
-// ranges of the shared keys, then each document's against its own, on from those sums.
+// Sequences that fill little of their tiles: first all rows as they stand in q, one sequence, against
+// ranges of the shared keys, then each sequence's against its own, on from those sums.
 template <int T, int D, int WM, bool kCap>
 hipError_t launch_packed(const AttnArgs& a, const AttnShared& sh, const SharedPlan& p, float* ws,
                          hipStream_t stream) {
@@ -377,7 +378,7 @@ hipError_t launch_packed(const AttnArgs& a, const AttnShared& sh, const SharedPl
   f.v = sh.v, f.v_row = sh.v_row, f.v_head = sh.v_head;
   f.k_seq = f.v_seq = f.q_seq = f.out_seq = 0;
   f.q_offsets = f.k_offsets = f.q_lens = f.k_lens = f.prefix_lens = nullptr;
-  f.n_seq = 1, f.max_q = a.q_rows, f.max_k = sh.rows, f.causal = 0;
+  f.n_seq = 1, f.max_q = a.q_offsets ? a.q_rows : a.n_seq * a.max_q, f.max_k = sh.rows, f.causal = 0;
   const int group = a.heads / a.kv_heads;
   const int o_tiles = (a.max_q * group + kRows - 1) / kRows;
   const int64_t f_all = (int64_t)a.kv_heads * p.s_tiles * kRows;

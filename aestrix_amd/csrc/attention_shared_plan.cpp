@@ -60,12 +60,19 @@ SharedPlan attention_shared_plan(const AttnArgs& a, const AttnShared& sh, int cu
       p.tiles.near_hs = a.kv_heads;
     }
     p.bytes = p.tiles.bytes;
-    // Packed documents that leave much of their tiles empty: their rows in one stretch against the
-    // shared keys, if the sums' way through memory is worth it.  (Slopes would need every row's
-    // document there.)
+    // Packed documents, or batches whose queries lie one sequence behind the other, that leave much of
+    // their tiles empty: all rows in one stretch against the shared keys, if the sums' way through memory
+    // is worth it.  (Slopes would need every row's sequence there.)  64 sequences of 200 own keys behind 8192,
+    // 32 / 8 heads, in tiles and so: of 36 rows 213 and 126 us, 64 214 and 158, 80 235 and 212, but 96 235 and
+    // 256, 132 449 and 398, 160 448 and 404; 36 rows of 1000 own keys behind 2048 95 and 92; 32 x 80 behind 1000,
+    // where tiles of 64 rows fill the card, 18 and 29.
     const int group = a.heads / a.kv_heads;
-    const int64_t packed = ((int64_t)a.q_rows * group + 127) / 128;  // tiles of a key head
-    if (workspace && a.q_offsets && !a.slopes && p.tiles.splits == 1 && 2 * a.n_seq >= packed && sh.rows >= 512) {
+    const int64_t line = a.q_offsets ? a.q_rows : a.n_seq * (int64_t)a.max_q;
+    const int64_t packed = (line * group + 127) / 128;  // tiles of a key head
+    const bool empty = a.q_offsets ? 2 * a.n_seq >= packed
+                                   : a.q_seq == a.max_q * a.q_row && p.tiles.tile_rows == 128 &&
+                                         all_rows * 8 <= tiles * 128 * 5 && sh.rows >= 2 * (int64_t)a.max_k;
+    if (workspace && empty && !a.slopes && p.tiles.splits == 1 && sh.rows >= 512) {
       const int64_t own = hs * ((all_rows + 127) / 128);
       const int64_t blocks = a.kv_heads * packed;
       const int splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * cus + blocks / 2) / blocks, sh.rows / 512));

@@ -24,7 +24,7 @@ struct AttnFront {
 };
 __device__ __forceinline__ int64_t attn_packed_row(const AttnArgs& a, const AttnFront& front, int seq, int kh,
                                                    int t, int g) {
-  const int64_t q = min(max(a.q_offsets[seq], 0), a.q_rows) + t;
+  const int64_t q = (a.q_offsets ? (int64_t)min(max(a.q_offsets[seq], 0), a.q_rows) : (int64_t)seq * a.max_q) + t;
   return (int64_t)kh * front.packed + q * (a.heads / a.kv_heads) + g;
 }
 

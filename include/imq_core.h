@@ -197,7 +197,8 @@ typedef enum imq_shared_kernel {
   IMQ_SHARED_TILES = 1, /* a sequence's tiles walk the shared and then the own keys */
   IMQ_SHARED_STREAM = 2, /* up to 32 rows a sequence: all sequences' rows together against the shared
                             keys, each one's against its own, and a join */
-  IMQ_SHARED_PACKED = 3  /* packed documents of few tiles each: the same on the tiles */
+  IMQ_SHARED_PACKED = 3  /* packed documents, or a batch without gaps, that fill little of their tiles:
+                            the same on the tiles */
 } imq_shared_kernel;
 
 typedef struct imq_shared_plan_info {

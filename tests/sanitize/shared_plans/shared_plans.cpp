@@ -66,7 +66,8 @@ SharedPlan sound(const AttnArgs& a, int rows, bool workspace) {
     need(p.bytes == (size_t)((p.s_splits + p.o_splits) * hs * of_seq * columns * 4), "bytes", a, rows, p);
     need((a.kv_heads * (int64_t)p.s_tiles * p.s_splits + hs * p.o_splits) * 256 < (int64_t)1 << 32, "launch", a, rows, p);
   } else if (p.kernel == IMQ_SHARED_PACKED) {
-    need(a.q_offsets && p.s_rows == 128 && (int64_t)p.s_tiles * 128 >= a.q_rows * group, "rows", a, rows, p);
+    const int64_t line = a.q_offsets ? a.q_rows : (int64_t)a.n_seq * a.max_q;
+    need(p.s_rows == 128 && (int64_t)p.s_tiles * 128 >= line * group && line * group < (int64_t)1 << 31, "rows", a, rows, p);
     need(covers(p.s_splits, p.s_chunk, rows, 64), "ranges", a, rows, p);
     need(p.bytes == (size_t)(p.s_splits * a.kv_heads * (int64_t)p.s_tiles * 128 * columns * 4), "bytes", a, rows, p);
   } else if (p.kernel == IMQ_SHARED_TILES) {
@@ -106,6 +107,15 @@ int main() {
   expect("documents of few rows", args(61, 40, 40, 8, 2, 64, true), 3001, IMQ_SHARED_PACKED, 128);
   expect("behind 511 keys", args(61, 40, 40, 8, 2, 64, true), 511, IMQ_SHARED_TILES, 128);
   expect("behind 512", args(61, 40, 40, 8, 2, 64, true), 512, IMQ_SHARED_PACKED, 128);
+  expect("a batch of 36 rows", args(64, 9, 200, 32, 8, 128), 8192, IMQ_SHARED_PACKED, 128);
+  expect("of 80", args(64, 20, 200, 32, 8, 128), 8192, IMQ_SHARED_PACKED, 128);
+  expect("of 84", args(64, 21, 200, 32, 8, 128), 8192, IMQ_SHARED_TILES, 128);
+  expect("of 160", args(64, 40, 200, 32, 8, 128), 8192, IMQ_SHARED_PACKED, 128);
+  expect("half as many own keys", args(64, 9, 512, 32, 8, 128), 1024, IMQ_SHARED_PACKED, 128);
+  expect("one more", args(64, 9, 513, 32, 8, 128), 1024, IMQ_SHARED_TILES, 128);
+  AttnArgs apart = args(64, 9, 200, 32, 8, 128);
+  apart.q_seq += apart.q_row;
+  expect("rows between the sequences", apart, 8192, IMQ_SHARED_TILES, 128);
   expect("heads of 136", args(4, 1, 64, 8, 2, 136), 100, IMQ_SHARED_ROWS, 0);
   expect("heads of 68", args(4, 1, 64, 8, 2, 68), 100, IMQ_SHARED_ROWS, 0);
 

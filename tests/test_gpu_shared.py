@@ -88,6 +88,17 @@ def test_long_shared_keys(shared, n, nq, nk, heads, kv, dim, dtype, softcap, slo
     run_batch(shared, nq, nk, heads, kv, dim, dtype, n=n, causal=True, softcap=softcap, slope=slope)
 
 
+@pytest.mark.parametrize("softcap,causal", [(0.0, True), (0.0, False), (20.0, True)])
+@pytest.mark.parametrize("shared,n,nq,nk,heads,kv,dim,dtype",
+                         [(1030, 40, 9, 40, 32, 8, 128, BF16), (600, 70, 20, 20, 8, 4, 64, F16),
+                          (777, 50, 12, 33, 18, 6, 72, BF16), (520, 33, 33, 260, 32, 8, 128, F16)])
+def test_batches_of_few_tiles(shared, n, nq, nk, heads, kv, dim, dtype, softcap, causal):
+    """All rows of a padded batch together against the shared keys; lengths down to none."""
+    qn = [nq if s % 3 == 0 else s * 7 % (nq + 1) for s in range(n)]
+    kn = [min(nk, qn[s] + s % 5) for s in range(n)]
+    run_batch(shared, nq, nk, heads, kv, dim, dtype, causal=causal, softcap=softcap, qn=qn, kn=kn)
+
+
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (F16, 72)])
 @pytest.mark.parametrize("softcap,slope", [(0.0, True), (30.0, False), (5.0, True)])
 @pytest.mark.parametrize("shared,n,nq,nk,causal", [(500, 6, 1, 60, True), (129, 3, 3, 9, False), (200, 2, 200, 200, True),
