@@ -20,7 +20,7 @@ _FILL = 16  # ranks are filled up to multiples of this
 
 
 class LoraAdapters:
-    """A set of adapters for one projection, laid out once.
+    """A set of adapters for one projection, laid out once, a copy outside any autograd graph.
 
     ``pairs``: (A [rank, K], B [N, rank]) of every adapter, bfloat16 or float16 on one device,
     ranks from 1 to 256, not all alike if they are not; ``scales``: a factor each (alpha / rank),
@@ -30,6 +30,7 @@ class LoraAdapters:
     of 16.  In float16 B is held with its largest element between 1 and 2 (a power of two, which
     ``scales`` takes back), so that the products between A and B keep that type's range."""
 
+    @torch.no_grad()  # parameters would otherwise stay referenced by the copies
     def __init__(self, pairs: Sequence[tuple[torch.Tensor, torch.Tensor]],
                  scales: float | Sequence[float] | None = None):
         pairs = [tuple(p) for p in pairs]
