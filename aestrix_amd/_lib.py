@@ -54,7 +54,7 @@ class Lora(ctypes.Structure):
     """imq_lora."""
     _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("first", ctypes.c_void_p),
                 ("scale", ctypes.c_void_p), ("count", ctypes.c_int), ("rows", ctypes.c_int),
-                ("max_rank", ctypes.c_int)]
+                ("max_rank", ctypes.c_int), ("rank_scales", ctypes.c_int)]
 
 
 IMQ_ENTRY_QMM_T, IMQ_ENTRY_QGEMM, IMQ_ENTRY_QGEMV, IMQ_ENTRY_FUSED, IMQ_ENTRY_SWIGLU = 0, 1, 2, 3, 4

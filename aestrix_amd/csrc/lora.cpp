@@ -25,6 +25,8 @@ int check_lora(imq_ctx* ctx, const char* fn, const imq_lora* l, int k, int n, in
   if (l->max_rank > imq::kLoraMaxRank)
     return fail(ctx, IMQ_EUNSUPPORTED, "%s: rank %d (up to %d are provided)", fn, l->max_rank,
                 imq::kLoraMaxRank);
+  if (l->rank_scales != 0 && l->rank_scales != 1)
+    return fail(ctx, IMQ_EINVAL, "%s: rank_scales %d (0 or 1)", fn, l->rank_scales);
   if (!l->a || !l->b || !l->first || !l->scale)
     return fail(ctx, IMQ_EINVAL, "%s: null device pointer (a=%p b=%p first=%p scale=%p)", fn, l->a, l->b,
                 (const void*)l->first, (const void*)l->scale);
@@ -71,7 +73,7 @@ int imq_qmm_lora(imq_ctx* ctx, const uint32_t* w, const void* scales, const void
   if ((rc = bind_device(ctx)) != IMQ_OK) return rc;
   imq::LoraArgs l{static_cast<const uint16_t*>(lora->a), static_cast<const uint16_t*>(lora->b),
                         lora->first, lora->scale, which, static_cast<uint16_t*>(ws),
-                        lora->count, lora->rows, lora->max_rank, nullptr};
+                        lora->count, lora->rows, lora->max_rank, lora->rank_scales, nullptr};
   char* rest = static_cast<char*>(ws) + imq::lora_u_bytes(m, lora->max_rank);
   auto* part = reinterpret_cast<float*>(rest);
   const auto st = static_cast<hipStream_t>(stream);

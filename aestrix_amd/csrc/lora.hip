@@ -125,7 +125,8 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
       __builtin_amdgcn_sched_barrier(0);
       IMQ_WAIT_LGKM_0();  // and has been read
     }
-    const float scale = l.scale[i];
+    const int rank = r0 + (threadIdx.x & 31);  // of this thread's sums below
+    const float scale = lora_scale(l, i, at.row + min(rank, at.rank - 1));
     __builtin_amdgcn_sched_barrier(0);
     IMQ_WAIT_VMCNT(0);
     __syncthreads();  // every wave's pieces have landed and been read
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
     __syncthreads();
 #pragma unroll
     for (int o = threadIdx.x; o < 32 * 32; o += kShrinkWaves * 64) {
-      const int of = o >> 5, rank = r0 + (o & 31);
+      const int of = o >> 5;
       float u = 0.f;
 #pragma unroll
       for (int v = 0; v < kShrinkWaves; ++v) u += lds.sums[v][o];

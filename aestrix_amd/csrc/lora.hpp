@@ -17,11 +17,12 @@ struct LoraArgs {
   const int32_t* first;
   const float* scale;
   const int32_t* which;
-  // u = scale * A x of each row's adapter, as operand fragments of the second product:
+  // u = scale * A x of each row's adapter and rank, as operand fragments of the second product:
   // [32 rows][16 ranks][upper halves, what they leave][64 lanes][8], lane r + 32 h row r's
   // ranks 8 h to 8 h + 8.  Ranks past a row's adapter's are not written.
   uint16_t* u;
   int count, rows, max_rank;
+  int rank_scales;  // scale is by rows of A, not by adapters
   // Rows grouped by their adapters (launch_lora_order), or NULL: as they are.  `which` is then
   // the places' (in the workspace), and u stands by places too.
   const int32_t* order;

@@ -25,6 +25,11 @@ __device__ __forceinline__ int lora_of(const LoraArgs& l, int row) {
   return (unsigned)i < (unsigned)l.count ? i : -1;
 }
 
+// What A's row `row`, one of adapter i's, is multiplied by.
+__device__ __forceinline__ float lora_scale(const LoraArgs& l, int i, int row) {
+  return l.scale[l.rank_scales ? row : i];
+}
+
 // u of row `row` and rank `rank` to its place: the upper half, and what it leaves (nothing where
 // it is infinite).
 template <int T>
@@ -72,7 +77,7 @@ __device__ __forceinline__ void lora_dot(const LoraArgs& l, const uint16_t* x, i
   float u = sum[0] + sum[1];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) u += __shfl_xor(u, off, 64);
-  if (lane == 0) lora_put<T>(l, row, r, u * l.scale[i]);
+  if (lane == 0) lora_put<T>(l, row, r, u * lora_scale(l, i, to.row + r));
 }
 
 // u's fragment of 32 rows (tile), 16 ranks (chunk) and upper halves or what they leave (part)

@@ -19,6 +19,16 @@ _MAX_RANK = 256
 _FILL = 16  # ranks are filled up to multiples of this
 
 
+def _ups(b: torch.Tensor) -> torch.Tensor:
+    """Exponents [sets, rank] for float16 B [sets, N, rank]: of the powers of two that bring the columns'
+    largest finite elements to [1, 2), but no element's lowest bit under float16's, 2^-24."""
+    units = (torch.where(torch.isfinite(b), b, 0).double() * 2.0 ** 24).long()  # whole numbers
+    top, low = units.abs().amax(1), units & -units
+    low = low.masked_fill(low == 0, 1 << 62).amin(1)
+    at = lambda v: torch.frexp(v.double()).exponent - 1  # of the highest bit
+    return torch.where(top > 0, torch.maximum(24 - at(top), -at(low)), 0)
+
+
 class LoraAdapters:
     """A set of adapters for one projection, laid out once, a copy outside any autograd graph.
 
@@ -27,8 +37,9 @@ class LoraAdapters:
     one for all, or none.  Adapter i adds ``scales[i] * (x . A^T) . B^T``.
 
     The tensors are copied: in bytes about what the adapters have, ranks filled up to multiples
-    of 16.  In float16 B is held with its largest element between 1 and 2 (a power of two, which
-    ``scales`` takes back), so that the products between A and B keep that type's range."""
+    of 16.  In float16 each column of B is multiplied by a power of two, which its rank's scale takes
+    back, so that the products between A and B, which have that type's range, leave it only where one
+    of them times its element of B does."""
 
     @torch.no_grad()  # parameters would otherwise stay referenced by the copies
     def __init__(self, pairs: Sequence[tuple[torch.Tensor, torch.Tensor]],
@@ -60,24 +71,37 @@ class LoraAdapters:
         self.max_rank = max(q - p for p, q in zip(first, first[1:]))
         self.a = torch.zeros((self.rows, self.k), dtype=self.dtype, device=self.device)
         self.b = torch.zeros(self.rows * self.n, dtype=self.dtype, device=self.device)
-        self.scale = torch.tensor(scales, dtype=torch.float32, device=self.device)
+        by_rank = self.dtype == torch.float16
+        self.scale = torch.tensor([s for s, p, q in zip(scales, first, first[1:]) for _ in range(q - p)]
+                                  if by_rank else scales, dtype=torch.float32, device=self.device)
         self.first = torch.tensor(first, dtype=torch.int32, device=self.device)
         for i, (a, b) in enumerate(pairs):
             rank = a.shape[0]
             self.a[first[i]:first[i] + rank] = a
             at = self.b[first[i] * self.n:first[i + 1] * self.n].view(self.n, -1)[:, :rank]
-            if self.dtype == torch.float16:
-                # 2^up brings the largest element to [1, 2) (none, or not finite: as it is).
-                top = b.abs().max().float()
-                up = torch.where((top > 0) & torch.isfinite(top), 1 - torch.frexp(top).exponent, 0)
-                at.copy_(torch.ldexp(b.float(), up))
-                self.scale[i] = torch.ldexp(self.scale[i], -up)
-            else:
-                at.copy_(b)
+            at.copy_(b)
+        if by_rank:
+            self._bring_up(first)
         self._c = _lib.Lora(self.a.data_ptr(), self.b.data_ptr(), self.first.data_ptr(), self.scale.data_ptr(),
-                            self.count, self.rows, self.max_rank)
+                            self.count, self.rows, self.max_rank, int(by_rank))
         self._p = ctypes.addressof(self._c)
         self._bytes: dict[int, int] = {}  # of the workspace, by a call's rows
+
+    def _bring_up(self, first: list[int]) -> None:
+        """B's columns multiplied by 2^up each, the ranks' scales divided by it; adapters of one rank together."""
+        i = 0
+        while i < self.count:
+            fill = first[i + 1] - first[i]
+            end = i + 1
+            while end < self.count and first[end + 1] - first[end] == fill and (end + 1 - i) * self.n * fill <= 1 << 24:
+                end += 1
+            b = self.b[first[i] * self.n:first[end] * self.n].view(end - i, self.n, fill)
+            scale = self.scale[first[i]:first[end]].view(end - i, fill)
+            up = _ups(b)
+            b.copy_(torch.ldexp(b.float(), up[:, None]))
+            # (A product that is zero stays zero where this would leave float32.)
+            scale.copy_(torch.ldexp(scale, -up).clamp(-3.4e38, 3.4e38))
+            i = end
 
 
 def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,

@@ -8,10 +8,10 @@
  *   u[row] = scale[i] * A_i x[row]                       A_i [r_i, k]
  *   y[row] = T( deq(W) x[row] + B_i u[row] )             B_i [n, r_i]
  *
- * with one rounding to T at the end: sums and u are held in fp32, and the second
- * product takes u as two values of T, its upper half and what that leaves (16 bits
- * together in bf16, 22 in f16).  No counterpart in the reference, which has no
- * adapters.
+ * with one rounding to T at the end: sums are held in fp32, and the second product
+ * takes u as two values of T, its upper half and what that leaves (16 bits together
+ * in bf16; in f16 22, none below 2^-24).  No counterpart in the reference, which has
+ * no adapters.
  *
  * Conventions as in imq.h: an imq_status is returned, nothing throws, calls are
  * asynchronous on the given stream and may be captured into a graph, inputs are
@@ -31,17 +31,22 @@ extern "C" {
  *   a      T [rows, k]   adapter i in rows first[i] to first[i + 1]
  *   b      T             adapter i [n, first[i + 1] - first[i]] from element first[i] * n on
  *   first  int32 [count + 1], multiples of 16, rising from 0 to rows
- *   scale  fp32 [count]
+ *   scale  fp32 [count], an adapter's, or with rank_scales 1 fp32 [rows], one for each
+ *          row of A
  * all in device memory; a and b 16-byte aligned.  max_rank: the largest filled-up
- * rank, 16 to 256.  In f16 u has f16's range: with B_i multiplied by a power of two
- * that brings its largest element to between 1 and 2, and scale[i] divided by it,
- * u leaves that range only where y does. */
+ * rank, 16 to 256.
+ * In f16 u has f16's range: a row with a u[r] past it has no finite output, and what
+ * u's values lose below 2^-24 is up to 2^-25 |B_i[n, r]| of y[n].  So multiply every
+ * column of B by the power of two that brings its largest element to between 1 and 2
+ * (less, if smaller elements of the column would lose bits), and divide that rank's
+ * scale by it: then u[r] is out of range only where B_i[n, r] u[r] is for some n. */
 typedef struct imq_lora {
   const void* a;
   const void* b;
   const int32_t* first;
   const float* scale;
   int count, rows, max_rank;
+  int rank_scales; /* 0 or 1 */
 } imq_lora;
 
 /* Bytes of the workspace of an imq_qmm_lora call of these sizes (16 or more). */
