@@ -67,6 +67,16 @@ int imq_attention_shared_plan(imq_ctx* ctx, const imq_attention_args* args, cons
   int rc = check_attention(ctx, fn, args, &a);
   if (rc != IMQ_OK || (rc = check_shared(ctx, fn, args, shared, &sh)) != IMQ_OK) return rc;
   if (!out) return fail(ctx, IMQ_EINVAL, "%s: null output", fn);
+  if (sh.rows == 0) {
+    const imq::AttnPlan p = imq::attention_plan(a, ctx->cus);
+    const bool few = p.kernel == IMQ_ATTENTION_FEW;
+    out->kernel = few ? IMQ_SHARED_STREAM : p.kernel == IMQ_ATTENTION_TILES ? IMQ_SHARED_TILES : IMQ_SHARED_ROWS;
+    out->tile_rows = p.tile_rows;
+    out->splits = few ? 0 : p.splits;
+    out->own_splits = few ? p.splits : 0;
+    out->workspace_bytes = p.bytes;
+    return IMQ_OK;
+  }
   const imq::SharedPlan p = imq::attention_shared_plan(a, sh, ctx->cus, true);
   out->kernel = p.kernel;
   const bool apart = p.kernel == IMQ_SHARED_STREAM || p.kernel == IMQ_SHARED_PACKED;

@@ -209,7 +209,8 @@ typedef struct imq_shared_plan_info {
   size_t workspace_bytes;
 } imq_shared_plan_info;
 
-/* What imq_attention_shared would run, as imq_attention_plan. */
+/* What imq_attention_shared would run, as imq_attention_plan.  Of no shared keys imq_attention's
+ * plan, whose few rows are IMQ_SHARED_STREAM without a range of those. */
 int imq_attention_shared_plan(imq_ctx* ctx, const imq_attention_args* args,
                               const imq_shared_keys* shared, imq_shared_plan_info* out);
 
