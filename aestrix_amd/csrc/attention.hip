@@ -21,7 +21,7 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnArgs a) {
     const int t = (int)(row % a.max_q);
     const AttnSeq s = attn_seq(a, (int)(row / a.max_q));
     if (t >= s.nq) continue;
-    attn_row<T, kCap, kSlope>(a, s, head, t, attn_seen(a, s, t), qs[wave]);
+    attn_row<T, kCap, kSlope, unsigned>(a, s, head, t, attn_seen(a, s, t), qs[wave]);
   }
 }
 

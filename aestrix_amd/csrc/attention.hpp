@@ -83,8 +83,9 @@ struct AttnScore {
 // a key per lane for the scores, `dim` elements over the lanes for the product
 // with v, the running maximum and sum rescaled per 64 keys.  Only keys below
 // `seen` are read, so nothing that a mask hides can reach the output.
-// qs: dim floats of LDS of this wave's own.
-template <int T, bool kCap, bool kSlope>
+// qs: dim floats of LDS of this wave's own.  J counts the keys: unsigned where there may be more than
+// 2^31 - 64 of them, past which the last step leaves an int.
+template <int T, bool kCap, bool kSlope, class J = int>
 __device__ void attn_row(const AttnArgs& a, const AttnSeq& s, int head, int t, int seen,
                          float* qs) {
   using S = typename Elem<T>::S;
@@ -99,8 +100,8 @@ __device__ void attn_row(const AttnArgs& a, const AttnSeq& s, int head, int t, i
   __builtin_amdgcn_wave_barrier();
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
   const int p = t + s.nk - s.nq;
-  for (int j0 = 0; j0 < seen; j0 += 64) {
-    const int j = j0 + lane;
+  for (J at = 0; at < (J)seen; at += 64) {
+    const int j0 = (int)at, j = j0 + lane;
     float e = -INFINITY;
     if (j < seen) {
       const S* kr = k + (int64_t)j * a.k_row;
@@ -150,7 +151,7 @@ struct AttnRowSums {
 
 // The first n keys at k and v (rows k_row and v_row apart), key j at p - j from the query.
 // Weights are 2^-32 of what they are, so that the largest bf16 values of 2^32 keys add up in fp32.
-template <int T, bool kCap, bool kSlope>
+template <int T, class J, bool kCap, bool kSlope>
 __device__ __forceinline__ void attn_row_keys(const AttnArgs& a, const typename Elem<T>::S* k,
                                               const typename Elem<T>::S* v, int64_t k_row,
                                               int64_t v_row, int n_keys, int p,
@@ -158,8 +159,8 @@ __device__ __forceinline__ void attn_row_keys(const AttnArgs& a, const typename 
                                               const float* qs, AttnRowSums& r) {
   using S = typename Elem<T>::S;
   const int lane = threadIdx.x & 63;
-  for (int j0 = 0; j0 < n_keys; j0 += 64) {
-    const int j = j0 + lane;
+  for (J at = 0; at < (J)n_keys; at += 64) {
+    const int j0 = (int)at, j = j0 + lane;
     float e = -INFINITY;
     if (j < n_keys) {
       const S* kr = k + (int64_t)j * k_row;
@@ -195,7 +196,7 @@ __device__ __forceinline__ void attn_row_keys(const AttnArgs& a, const typename 
   }
 }
 
-template <int T, bool kCap, bool kSlope>
+template <int T, bool kCap, bool kSlope, class J = int>
 __device__ void attn_row_shared(const AttnArgs& a, const AttnShared& sh, const AttnSeq& s, int head, int t,
                                 int seen, float* qs) {
   using S = typename Elem<T>::S;
@@ -210,10 +211,10 @@ __device__ void attn_row_shared(const AttnArgs& a, const AttnShared& sh, const A
   __builtin_amdgcn_wave_barrier();
   AttnRowSums r;
   const int p = t + s.nk - s.nq;
-  attn_row_keys<T>(a, static_cast<const S*>(sh.k) + kh * sh.k_head,
+  attn_row_keys<T, J>(a, static_cast<const S*>(sh.k) + kh * sh.k_head,
                    static_cast<const S*>(sh.v) + kh * sh.v_head, sh.k_row, sh.v_row, sh.rows, sh.rows + p,
                    score, qs, r);
-  attn_row_keys<T>(a, k, v, a.k_row, a.v_row, seen, p, score, qs, r);
+  attn_row_keys<T, J>(a, k, v, a.k_row, a.v_row, seen, p, score, qs, r);
   const float inv = seen > 0 || sh.rows > 0 ? 1.f / r.sum : 0.f;
 #pragma unroll
   for (int c = 0; c < 4; ++c)

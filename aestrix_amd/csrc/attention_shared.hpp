@@ -332,7 +332,7 @@ __global__ __launch_bounds__(256) void attn_shared_rows_kernel(AttnArgs a, AttnS
     const int t = (int)(row % a.max_q);
     const AttnSeq s = attn_seq(a, (int)(row / a.max_q));
     if (t >= s.nq) continue;
-    attn_row_shared<T, kCap, kSlope>(a, sh, s, head, t, attn_seen(a, s, t), qs[wave]);
+    attn_row_shared<T, kCap, kSlope, unsigned>(a, sh, s, head, t, attn_seen(a, s, t), qs[wave]);
   }
 }
 
