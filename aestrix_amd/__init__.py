@@ -29,7 +29,7 @@ from .core import (  # noqa: F401
     rope,
     rope_frequencies,
 )
-from .lora import LoraAdapters, quantized_matmul_lora  # noqa: F401
+from .lora import LoraAdapters, quantized_matmul_lora, quantized_matmul_lora_plan  # noqa: F401
 from .ops import (  # noqa: F401
     BITS,
     GROUP_SIZE,

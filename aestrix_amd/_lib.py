@@ -57,6 +57,13 @@ class Lora(ctypes.Structure):
                 ("max_rank", ctypes.c_int), ("rank_scales", ctypes.c_int)]
 
 
+class LoraPlanInfo(ctypes.Structure):
+    """imq_lora_plan_info."""
+    _fields_ = [("kernel", ctypes.c_int), ("tile_rows", ctypes.c_int), ("splits", ctypes.c_int),
+                ("u_rows", ctypes.c_int), ("grouped", ctypes.c_int), ("join_tiles", ctypes.c_int),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 IMQ_ENTRY_QMM_T, IMQ_ENTRY_QGEMM, IMQ_ENTRY_QGEMV, IMQ_ENTRY_FUSED, IMQ_ENTRY_SWIGLU = 0, 1, 2, 3, 4
 DIT_GROUPS = {"qkv": 0, "attn_out": 1, "mlp_in": 2, "mlp_out": 3}
 KERNEL_NAMES = {0: "qgemv", 1: "few_row", 2: "tile", 3: "tile_reg"}
@@ -161,6 +168,7 @@ SIGNATURES = {
     "imq_attention_shared": ([_p, _p, _p, _p], _i),
     "imq_attention_shared_plan": ([_p, _p, _p, _p], _i),
     "imq_qmm_lora_workspace": ([_p, _p, _i, _i, _i, _i, _p], _i),
+    "imq_qmm_lora_plan": ([_p, _p, _i, _i, _i, _i, _p], _i),
     "imq_qmm_lora": ([_p] * 8 + [_i, _i, _i, _i, _i, _i, _p, ctypes.c_size_t, _p], _i),
 }
 

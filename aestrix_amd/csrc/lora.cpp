@@ -6,10 +6,8 @@
 
 using namespace imq::detail;
 
-namespace {
-
-// Everything but the device pointers of a call's x, y and workspace.
-int check_lora(imq_ctx* ctx, const char* fn, const imq_lora* l, int k, int n, int m, imq_dtype dtype) {
+int imq::detail::check_lora(imq_ctx* ctx, const char* fn, const imq_lora* l, int k, int n, int m,
+                            imq_dtype dtype) {
   if (!ctx) return fail(nullptr, IMQ_EINVAL, "%s: null context", fn);
   if (!l) return fail(ctx, IMQ_EINVAL, "%s: null adapters", fn);
   if (dtype != IMQ_BF16 && dtype != IMQ_F16)
@@ -34,6 +32,8 @@ int check_lora(imq_ctx* ctx, const char* fn, const imq_lora* l, int k, int n, in
     return fail(ctx, IMQ_EINVAL, "%s: a and b must be 16-byte, first and scale 4-byte aligned", fn);
   return IMQ_OK;
 }
+
+namespace {
 
 // u, then the partial sums or the order and the adapters of the places.
 size_t workspace(const imq_lora* l, const imq::LoraPlan& p, int m) {

@@ -336,21 +336,17 @@ hipError_t launch_lora_order(const LoraArgs& l, int32_t* order, int32_t* which_a
   return hipGetLastError();
 }
 
-namespace {
-
-// Whether u is made a wave a row and rank: by the times of both in us.  That one reads A's and x's
+// By the times of both in us.  That one reads A's and x's
 // rows out of the caches, some 30 TB/s, whatever adapters the rows name; a tile of 32 rows
 // takes its adapters two at a time, as many as it may have (all, or after grouping its share), 6 us
 // of K = 2560 and 12 of 9728 each turn.  160 rows of 24 adapters of rank 16 in turn against K = 9728
 // and N = 2560 30.8 us so, 168 by tiles; 64 rows of one adapter of rank 256 and K = 2560 44.7 and
 // 41.4; 512 rows of 32 adapters of rank 64, grouped, 74.8 and 64.4.
-bool lora_by_rows(const LoraArgs& l, int k, int m) {
-  const double rows_us = 2 + 4. * m * l.max_rank * k / 30e6;
-  const int most = std::min(std::min(l.count, m), l.order ? 1 + (int)((int64_t)l.count * 32 / m) : 32);
-  return rows_us <= (most + 1) / 2 * (3.5 + k * 0.0009) && (int64_t)m * l.max_rank < 1 << 24;
+bool lora_by_rows(int count, int max_rank, bool grouped, int k, int m) {
+  const double rows_us = 2 + 4. * m * max_rank * k / 30e6;
+  const int most = std::min(std::min(count, m), grouped ? 1 + (int)((int64_t)count * 32 / m) : 32);
+  return rows_us <= (most + 1) / 2 * (3.5 + k * 0.0009) && (int64_t)m * max_rank < 1 << 24;
 }
-
-}  // namespace
 
 double lora_join_few_us(int n, int m, int max_rank) { return 2. * m * n * max_rank / 10e6; }
 double lora_join_tiles_us(int n, int m, int count, int max_rank) {
@@ -359,10 +355,14 @@ double lora_join_tiles_us(int n, int m, int count, int max_rank) {
   return 1.5 + (1.2 + 0.27 * most) * ((n + 31) / 32) * rows / 256 + 2. * rows * most * n * max_rank / 3e6;
 }
 
+bool lora_join_few(int n, int m, int count, int max_rank) {
+  return m <= 65535 && lora_join_few_us(n, m, max_rank) <= lora_join_tiles_us(n, m, count, max_rank);
+}
+
 hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, int dtype,
                               hipStream_t stream) {
   const auto* xx = static_cast<const uint16_t*>(x);
-  if (lora_by_rows(l, k, m)) {
+  if (lora_by_rows(l.count, l.max_rank, l.order != nullptr, k, m)) {
     const dim3 grid((unsigned)((m * l.max_rank + kDotWaves - 1) / kDotWaves)), block(kDotWaves * 64);
     // Rows of more than 8 KB: 20 pieces at a time, of which shorter rows would have too few.
     if (k > 4096) {
@@ -390,7 +390,7 @@ hipError_t launch_lora_shrink(const LoraArgs& l, const void* x, int k, int m, in
 hipError_t launch_lora_join(const LoraArgs& l, const float* part, int splits, void* y, int n, int m,
                             int dtype, hipStream_t stream) {
   auto* yy = static_cast<uint16_t*>(y);
-  if (m <= 65535 && lora_join_few_us(n, m, l.max_rank) <= lora_join_tiles_us(n, m, l.count, l.max_rank)) {
+  if (lora_join_few(n, m, l.count, l.max_rank)) {
     const dim3 grid((unsigned)((n + 255) / 256), (unsigned)m);
     if (dtype == kBf16)
       hipLaunchKernelGGL((lora_join_few_kernel<kBf16>), grid, dim3(256), 0, stream, l, part, splits, yy, n, m);

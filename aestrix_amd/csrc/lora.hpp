@@ -6,7 +6,15 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "ctx.hpp"
+#include "imq_lora.h"
+
 namespace imq {
+
+namespace detail {
+// Everything but the device pointers of a call's x, y and workspace (lora.cpp).
+int check_lora(imq_ctx* ctx, const char* fn, const imq_lora* l, int k, int n, int m, imq_dtype dtype);
+}  // namespace detail
 
 constexpr int kLoraMaxRank = 256;
 
@@ -48,6 +56,9 @@ LoraPlan lora_plan(int k, int n, int m, int count, int max_rank, int dtype);
 // with one of rank 256 44.6 and 32.9.
 double lora_join_few_us(int n, int m, int max_rank);
 double lora_join_tiles_us(int n, int m, int count, int max_rank);
+// Whether u is made a wave a row and rank, and whether the join has a thread an output (lora.hip).
+bool lora_by_rows(int count, int max_rank, bool grouped, int k, int m);
+bool lora_join_few(int n, int m, int count, int max_rank);
 
 // Groups the rows by their adapters, those without one last, each group in its rows' order:
 // order [m] the row at a place, which_at [m] its adapter (lora.hip).

@@ -144,3 +144,19 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     if rc:
         _lib.check(rc, ctx)
     return out
+
+
+LORA_KERNELS = {0: "few", 1: "split", 2: "tiles", 3: "tiles_reg"}
+
+
+def quantized_matmul_lora_plan(adapters: LoraAdapters, m: int) -> dict:
+    """The kernel, tile height, ranges of K, way to u ("rows", "tiles"), grouping, join ("outputs", "tiles" or
+    None) and workspace that ``quantized_matmul_lora`` would use for m rows."""
+    ctx = context(adapters.device.index)
+    p = _lib.LoraPlanInfo()
+    _lib.check(_lib.load().imq_qmm_lora_plan(ctx, adapters._p, adapters.k, adapters.n, m, _DTYPES[adapters.dtype],
+                                             ctypes.byref(p)), ctx)
+    kernel = LORA_KERNELS[p.kernel]
+    join = ("tiles" if p.join_tiles else "outputs") if kernel in ("few", "split") else None
+    return {"kernel": kernel, "tile_rows": p.tile_rows, "splits": p.splits, "u": "rows" if p.u_rows else "tiles",
+            "grouped": bool(p.grouped), "join": join, "workspace_bytes": p.workspace_bytes}

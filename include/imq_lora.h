@@ -65,6 +65,27 @@ int imq_qmm_lora(imq_ctx* ctx, const uint32_t* w, const void* scales, const void
                  int m, int group_size, int bits, imq_dtype dtype, void* ws, size_t ws_bytes,
                  imq_stream stream);
 
+typedef enum imq_lora_kernel {
+  IMQ_LORA_FEW = 0,      /* up to 32 rows: partial sums of K, u beside them in the same launch, a join */
+  IMQ_LORA_SPLIT = 1,    /* u, tiles' partial sums (of all of K: splits 1), a join */
+  IMQ_LORA_TILES = 2,    /* u, tiles that add B u to their sums */
+  IMQ_LORA_TILES_REG = 3 /* the same on the register-staged tiles */
+} imq_lora_kernel;
+
+typedef struct imq_lora_plan_info {
+  int kernel;     /* an imq_lora_kernel */
+  int tile_rows;  /* of the projection's tiles; 0: not in the plan (IMQ_LORA_FEW, _TILES_REG) */
+  int splits;     /* ranges of K */
+  int u_rows;     /* 1: u a wave for each row and rank; 0: by tiles of 32 rows */
+  int grouped;    /* 1: rows are grouped by adapter first (as they are, of more than 1023 adapters) */
+  int join_tiles; /* of a join, 1: by tiles of 32 x 32; 0: a thread an output */
+  size_t workspace_bytes;
+} imq_lora_plan_info;
+
+/* What imq_qmm_lora would run for these sizes, without launching anything. */
+int imq_qmm_lora_plan(imq_ctx* ctx, const imq_lora* lora, int k, int n, int m, imq_dtype dtype,
+                      imq_lora_plan_info* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,8 +13,9 @@ pytestmark = pytest.mark.gpu
 
 F16 = torch.float16
 NAN, INF = float("nan"), float("inf")
-# Rows that the few-row kernel, partial sums of split tiles and the tiles themselves take.
-ROWS = [1, 5, 40, 70, 300]
+# (rows, K, N): the few-row kernel, partial sums and either join, the register-staged and the other
+# tiles, u by rows and by tiles (test_the_ways_there).
+SHAPES = [(1, 2560, 300), (5, 2560, 500), (40, 256, 300), (300, 256, 300), (70, 64, 300), (64, 2560, 6144), (1000, 512, 4100)]
 
 
 @pytest.fixture(autouse=True)
@@ -70,8 +71,9 @@ def wanted(x, proj, ab, c, ids):
     return y, half_step(F16) * y.abs() + 1.02 * err + least(F16)
 
 
-def run(ab, m, k=256, n=300, c=None, seed=0):
-    g = gen(seed + m)
+def run(ab, shape, c=None):
+    m, k, n = shape
+    g = gen(m)
     proj, x = projection(g, n, k), randn(g, m, k).half()
     c = [1.0] * len(ab) if c is None else c
     ids = torch.tensor([-1 if r % 7 == 6 else r % len(ab) for r in range(m)], dtype=torch.int32, device="cuda")
@@ -96,44 +98,59 @@ def test_what_is_held():
     assert torch.equal(at[:, :24].double().abs().nan_to_num(0.0, 0.0, 0.0), held(b))
 
 
-@pytest.mark.parametrize("m", ROWS)
-@pytest.mark.parametrize("rank", [2, 24, 64])
-def test_ranks_of_mixed_size(m, rank):
+def test_the_ways_there():
+    g = gen(2)
+    seen = []
+    for m, k, n in SHAPES:
+        for rank in (16, 64, 256):
+            plan = imq.quantized_matmul_lora_plan(imq.LoraAdapters([(randn(g, rank, k).half(), randn(g, n, rank).half())] * 2), m)
+            seen.append((plan["kernel"], plan["u"], plan["join"]))
+    assert {("few", "rows", "outputs"), ("split", "rows", "outputs"), ("split", "tiles", "tiles"), ("tiles", "tiles", None),
+            ("tiles_reg", "rows", None)} <= set(seen), seen
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("rank", [2, 24, 64, 256])
+def test_ranks_of_mixed_size(shape, rank):
     """Large rows of A before small columns of B, up to A x of some 2^26, and the other way round."""
     g = gen(rank)
     s = torch.arange(rank, device="cuda") % 27 - 13.0
-    ab = [((randn(g, rank, 256) * 0.06 * torch.exp2(s if i else -s)[:, None]).half(),
-           (randn(g, 300, rank) * torch.exp2(-s if i else s)).half()) for i in range(3)]
-    run(ab, m, c=[1.0, -2.0, 16.0])
+    _, k, n = shape
+    ab = [((randn(g, rank, k) / k ** 0.5 * torch.exp2(s if i else -s)[:, None]).half(),
+           (randn(g, n, rank) * torch.exp2(-s if i else s)).half()) for i in range(2)]
+    run(ab, shape, c=[-2.0, 16.0])
 
 
-@pytest.mark.parametrize("m", ROWS)
-def test_one_ordinary_rank_and_one_of_large_a(m):
+@pytest.mark.parametrize("shape", SHAPES)
+def test_one_ordinary_rank_and_one_of_large_a(shape):
     """A x of 2e5 and more in one rank times elements of 2^-14, beside a rank of B of about 1."""
     g = gen(3)
-    a = torch.stack([randn(g, 256) / 16, 12000.0 * randn(g, 256)]).half()
-    b = torch.stack([randn(g, 300), 2.0 ** -14 * randn(g, 300)], 1).half()
+    _, k, n = shape
+    a = torch.stack([randn(g, k) / 16, 12000.0 * randn(g, k)]).half()
+    b = torch.stack([randn(g, n), 2.0 ** -14 * randn(g, n)], 1).half()
     b[::9, 1] = 0.0
-    run([(a, b)], m)
+    run([(a, b)], shape)
 
 
-@pytest.mark.parametrize("m", ROWS)
-def test_rows_of_b_of_mixed_size(m):
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rows_of_b_of_mixed_size(shape):
     """Elements of 2^-12 to 2^10 in every column; one of 1000 among others of 0.01."""
     g = gen(4)
-    rows = torch.exp2(10.0 - torch.arange(300, device="cuda") % 23)
-    mixed = ((randn(g, 16, 256) / 64).half(), (randn(g, 300, 16) * rows[:, None]).half())
-    one = ((randn(g, 16, 256) / 64).half(), (0.01 * randn(g, 300, 16)).half())
+    _, k, n = shape
+    rows = torch.exp2(10.0 - torch.arange(n, device="cuda") % 23)
+    mixed = ((randn(g, 16, k) / 4 / k ** 0.5).half(), (randn(g, n, 16) * rows[:, None]).half())
+    one = ((randn(g, 16, k) / 4 / k ** 0.5).half(), (0.01 * randn(g, n, 16)).half())
     one[1][17] = 1000.0
-    run([mixed, one], m)
+    run([mixed, one], shape)
 
 
-@pytest.mark.parametrize("m", ROWS)
-def test_an_element_that_is_not_finite_leaves_its_column_in_range(m):
+@pytest.mark.parametrize("shape", SHAPES)
+def test_an_element_that_is_not_finite_leaves_its_column_in_range(shape):
     """NaN or infinite in one output; the others of that adapter have a large A before a small B."""
     g = gen(5)
-    proj, x = projection(g, 300, 256), randn(g, m, 256).half()
-    a, b = (3000 * randn(g, 16, 256)).half(), (2.0 ** -18 * randn(g, 300, 16)).half()
+    m, k, n = shape
+    proj, x = projection(g, n, k), randn(g, m, k).half()
+    a, b = (3000 * randn(g, 16, k)).half(), (2.0 ** -18 * randn(g, n, 16)).half()
     ids = torch.tensor([r % 2 - 1 for r in range(m)], dtype=torch.int32, device="cuda")
     ids[0] = 0
     want, bound = wanted(x, proj, [(a, b)], [1.0], ids)
@@ -154,14 +171,15 @@ def test_a_factor_that_ends_the_range_of_fp32():
     assert torch.equal(got, imq.quantized_matmul_lora(x, *proj, imq.LoraAdapters(ab, 2.9e38), ids - 1))
 
 
-@pytest.mark.parametrize("m", ROWS)
-def test_small_a_and_x(m):
+@pytest.mark.parametrize("shape", SHAPES)
+def test_small_a_and_x(shape):
     """A and x under f16's smallest normal value, whose bits count behind a large factor."""
     g = gen(7)
-    ab = [((2.0 ** -17 * randn(g, 24, 256)).half(), randn(g, 300, 24).half())]
-    run(ab, m, c=[2.0 ** 13])
-    proj, x = projection(g, 300, 256), (2.0 ** -17 * randn(g, m, 256)).half()
-    ab = [((64 * randn(g, 24, 256)).half(), randn(g, 300, 24).half())]
+    m, k, n = shape
+    ab = [((2.0 ** -17 * randn(g, 24, k)).half(), randn(g, n, 24).half())]
+    run(ab, shape, c=[2.0 ** 13])
+    proj, x = projection(g, n, k), (2.0 ** -17 * randn(g, m, k)).half()
+    ab = [((64 * randn(g, 24, k)).half(), randn(g, n, 24).half())]
     ids = torch.zeros(m, dtype=torch.int32, device="cuda")
     got = imq.quantized_matmul_lora(x, *proj, imq.LoraAdapters(ab, 8.0), ids)
     check(got, *wanted(x, proj, ab, [8.0], ids), f"small x, {m} rows")
