@@ -223,9 +223,10 @@ struct EpSwiGLU {
   }
 };
 
-// Stages with sums of their own behind the K loop: add_sums(acc, lds, m0, n0, M, N), with
-// 256 bytes of LDS a row that the K loop has left, adds them to a wave's 32 x 32 accumulators of the rows from m0 and the columns from n0 on.  Their rows
-// may stand in another order: row_at(i) is the row of x at i (the buffer-load kernel's).
+// Stages with sums of their own behind the K loop: add_sums(acc, lds, m0, n0, M, N), with 256 bytes
+// of LDS a row that the K loop has left, adds them to a wave's 32 x 32 accumulators of the rows from m0
+// and the columns from n0 on.  Their rows may stand in another order: row_at(i) is the row of x at i
+// (the buffer-load kernel's).
 template <class EP>
 constexpr bool adds_sums = false;
 

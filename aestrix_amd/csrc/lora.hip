@@ -312,12 +312,11 @@ __global__ __launch_bounds__(kJoinWaves * 64, 8) void lora_join_kernel(LoraArgs 
   uint32_t rows;
   LoraAt at;
   for (int j = wave; of_tile.nth(j, rows, at) >= 0; j += kJoinWaves) {
-    f32x16_t c[1];
-    lora_product<T, 1>(l, at, tile, n0, n, c);
+    const f32x16_t c = lora_product<T>(l, at, tile, n0, n);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int r = 8 * (e >> 2) + 4 * h + (e & 3);
-      if (rows >> r & 1u) add[r * 32 + r32] = c[0][e];
+      if (rows >> r & 1u) add[r * 32 + r32] = c[e];
     }
   }
   float sum = v[0];

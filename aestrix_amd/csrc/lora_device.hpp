@@ -80,11 +80,9 @@ __device__ __forceinline__ void lora_dot(const LoraArgs& l, const uint16_t* x, i
   if (lane == 0) lora_put<T>(l, row, r, u * lora_scale(l, i, to.row + r));
 }
 
-// u's fragment of 32 rows (tile), 16 ranks (chunk) and upper halves or what they leave (part)
-// for this lane.
-__device__ __forceinline__ const u32x4_t* lora_u(const LoraArgs& l, int tile, int chunk, int part) {
-  return reinterpret_cast<const u32x4_t*>(l.u) +
-         (((size_t)tile * (l.max_rank / 16) + chunk) * 2 + part) * 64 + (threadIdx.x & 63);
+// u's first fragment of 32 rows (tile) for this lane: the first 16 ranks' upper halves.
+__device__ __forceinline__ const u32x4_t* lora_u(const LoraArgs& l, int tile) {
+  return reinterpret_cast<const u32x4_t*>(l.u) + (size_t)tile * (l.max_rank / 16) * 128 + (threadIdx.x & 63);
 }
 
 template <int T>
@@ -97,31 +95,24 @@ __device__ __forceinline__ f32x16_t lora_mfma(u32x4_t a, u32x4_t b, f32x16_t c) 
                                                   __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// c[nt] = B_i u of 32 rows (tile) and 32 NT columns from n0 on, in the accumulators' layout.
+// c = B_i u of 32 rows (tile) and 32 columns from n0 on, in the accumulators' layout.
 // B's rows come straight from memory in operand layout: a lane's column and eight ranks are 16
 // bytes.
-template <int T, int NT>
-__device__ __forceinline__ void lora_product(const LoraArgs& l, const LoraAt& at, int tile, int n0, int N,
-                                             f32x16_t (&c)[NT]) {
+template <int T>
+__device__ __forceinline__ f32x16_t lora_product(const LoraArgs& l, const LoraAt& at, int tile, int n0, int N) {
   const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
-  const u32x4_t* b[NT];
+  const u32x4_t* b = reinterpret_cast<const u32x4_t*>(l.b + (size_t)at.row * N +
+                                                      (size_t)min(n0 + r32, N - 1) * at.rank) + h;
+  f32x16_t c;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    b[nt] = reinterpret_cast<const u32x4_t*>(l.b + (size_t)at.row * N +
-                                             (size_t)min(n0 + nt * 32 + r32, N - 1) * at.rank) + h;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) c[nt][e] = 0.f;
-  }
-  const u32x4_t* u = lora_u(l, tile, 0, 0);
+  for (int e = 0; e < 16; ++e) c[e] = 0.f;
+  const u32x4_t* u = lora_u(l, tile);
   for (int r = 0; r < at.rank / 16; ++r) {
-    const u32x4_t hi = u[r * 128], lo = u[r * 128 + 64];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const u32x4_t bv = b[nt][2 * r];
-      c[nt] = lora_mfma<T>(hi, bv, c[nt]);
-      c[nt] = lora_mfma<T>(lo, bv, c[nt]);
-    }
+    const u32x4_t hi = u[r * 128], lo = u[r * 128 + 64], bv = b[2 * r];
+    c = lora_mfma<T>(hi, bv, c);
+    c = lora_mfma<T>(lo, bv, c);
   }
+  return c;
 }
 
 // The smallest of the wave's values.

@@ -179,7 +179,9 @@ int imq_attention_plan(imq_ctx* ctx, const imq_attention_args* args, imq_attenti
  * to own key, and to the shared key j as to an own key at j - rows.
  * No own keys (max_k 0 or n_k 0) and no shared ones (rows 0) are allowed; a query
  * that sees neither gives zeros.  rows + max_k stays under 2^31.
- * Types, sizes, alignment, workspace and what spoilt keys do are imq_attention's.
+ * Types, sizes, alignment, workspace and what spoilt keys do are imq_attention's, and
+ * the weights' rounding to T: in tiles (IMQ_SHARED_TILES, _PACKED) once, of streams in
+ * bf16 as two bf16 each, by rows not.
  * shared: k and v of T, element (j, h, d) at j * row + h * head + d, kv_heads heads of
  * dim; out is none of them. */
 typedef struct imq_shared_keys {
