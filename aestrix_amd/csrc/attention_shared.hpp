@@ -5,7 +5,8 @@
 // Sequences with many rows (queries times the heads of a key head) run the tiles of
 // attention_walk.hpp, whose walk goes over the shared keys and then the own ones: the
 // matrix cores bind there, and the shared keys come out of the caches (4 x up to 2048 rows of
-// 32 / 8 heads of 128 behind 8192 keys, with slopes, 848 us, 966 TFLOP/s).  Sequences that
+// 32 / 8 heads of 128 behind 8192 keys, with slopes, 848-872 us, 940-966 TFLOP/s; of 6.0 GB of requests
+// 0.18 pass the L2s).  Sequences that
 // fill little of their tiles: all rows in one stretch against the shared keys first (launch_packed; 61
 // documents of up to 154 rows, capped, behind 3001 keys 76 us, 119 in tiles of their own; 64 x 36 rows
 // behind 8192 124 and 213).
@@ -14,9 +15,10 @@
 // shared ones are read once for the batch, the rows of all sequences stand together
 // against them, 32 or 64 a workgroup, and each sequence's own rows against its own keys, as
 // workgroups of one launch (attn_stream_kernel); a second one joins the ranges.  Tokens of 32 / 8 heads
-// of 128, keys once each over the time: 16 behind 65536 keys 60 us and the join 6, 4.2 TB/s; 64 behind
-// 8192, with up to 1024 own ones, 54 and 5, 2.9 TB/s (the shared ones are read four times, three
-// out of the caches); 8 behind 512 7.5 and 4.5, the latency of a tile or two and of the join's loads.
+// of 128: 16 behind 65536 keys 60 us and the join 6, 286 MB past the L2s, 4.7 TB/s; 64 behind
+// 8192, with up to 1024 own ones, 54 and 5, 173 MB, 3.2 TB/s (the shared ones are read four times, three
+// of them out of the L2s: 280 MB of requests); 8 behind 512 7.5 and 4.5, the latency of a tile or two and of
+// the join's loads.
 #pragma once
 
 #include <type_traits>
